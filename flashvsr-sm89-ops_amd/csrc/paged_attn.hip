@@ -1,0 +1,863 @@
+// Attention over an 8-bit paged cache (kv_pages.h): codes go from memory to
+// the matrix cores as they are stored, never widened.
+//
+//   o[q] = sum_k w[k] v[k] / sum_k w[k],  w[k] = exp(sm_scale * q.k) over the keys q sees
+//
+// The matrix cores multiply e4m3 by e4m3 only, at twice the bf16 rate, so the
+// bf16 side of each product is split: a bf16 value (8 significant bits) is the
+// sum of two e4m3 values (4 bits each, signed remainder), an fp16 value (11) of
+// three, each term 32 times finer than the one before.  Two terms cost what one
+// bf16 product would, and K and V are neither converted nor read wider.
+//   S^T = K Q^T   K rows are operand A as stored; q's terms operand B
+//   O^T = V^T P^T V is stored [dim][token]: again operand A as stored; P's terms
+//                 come from the S^T accumulators in the lane that holds them: the
+//                 key order of S^T's rows is chosen so that a lane's accumulators are
+//                 its P operand in V's token order.
+// Powers of two are the instruction's own scale operands: a page's K and V
+// scales, a query's scale, and, for P, the softmax's reference.  Weights are
+// w = 2^(x - E + 8), x the logit in log2 units and E the least integer above the row's
+// largest x among the keys at hand, so w lies in (0, 256] whatever its row's running
+// maximum is; their operand's scale is 2^(E - 8 - M).  M, the row's reference,
+// may therefore be any power of two near the maximum: it moves only when E exceeds
+// it by 64, which rescales O and the sum exactly and happens at a row's first keys
+// and hardly ever again.  Remainders keep w's error below 2^-8 (bf16) or
+// 2^-12 (fp16) of itself, or 2^-22 of the largest; sums are fp32 of the unrounded w.
+//
+// Two kernels.  attend_few: up to 16 (query, head) rows of one key/value head
+// per workgroup, bound by the cache's bytes: 16x16x128 products, K and V loaded
+// straight into operand registers, pages shared out over waves and workgroups.
+// attend_tile: 128 rows, 32 a wave, bound by products and exponentials: 32x32x64
+// products from a double-buffered LDS stage.  Either splits a long axis over
+// workgroups where rows alone leave CUs idle; attend_join adds the pieces.
+#include <algorithm>
+
+#include "kv_pages.h"
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v2s __attribute__((ext_vector_type(2)));
+#define LDS_AS __attribute__((address_space(3)))
+
+constexpr int kThreads = 256;
+constexpr float kNothing = -1e30f;  // reference of a row that has seen no key (finite: no inf - inf)
+constexpr int kMaxSplits = 64;
+
+struct Args {
+  fvsr_kv_cache c;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_ts, q_hs, o_ts, o_hs;
+  const uint8_t* keep;
+  int64_t keep_q, keep_k;
+  float* part;       // splits > 1: O of (row, split), then (M, l)
+  float scale_log2;  // sm_scale * log2(e)
+  int T, q_heads, group, causal, splits, tiles, tail;
+};
+
+template <int DT>
+FVSR_DEV float to_f(uint16_t x) {
+  return DT == FVSR_DT_F16 ? (float)__builtin_bit_cast(_Float16, x) : bf2f(x);
+}
+template <int DT>
+FVSR_DEV uint32_t pack2(float a, float b) {
+  if (DT == FVSR_DT_F16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
+  }
+  return pack_bf16x2(a, b);
+}
+
+constexpr int terms(int dt) { return dt == FVSR_DT_F16 ? 3 : 2; }
+
+// Four values of magnitude at most 256 as N e4m3 terms: x = t0 + t1 / 32 + t2 / 1024.
+template <int N>
+FVSR_DEV void split4(float a, float b, float c, float d, uint32_t (&w)[N]) {
+  const uint32_t t0 = e4m3x4(a, b, c, d);
+  w[0] = t0;
+  if constexpr (N > 1) {
+    const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)t0, false);
+    const v2f hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)t0, true);
+    a -= lo[0], b -= lo[1], c -= hi[0], d -= hi[1];
+    v2s t = {};
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, a, b, 0x1p-5f, false);
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, c, d, 0x1p-5f, true);
+    w[1] = __builtin_bit_cast(uint32_t, t);
+  }
+  if constexpr (N > 2) {
+    const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], 0x1p-5f, false);
+    const v2f hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], 0x1p-5f, true);
+    v2s t = {};
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, a - lo[0], b - lo[1], 0x1p-10f, false);
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, c - hi[0], d - hi[1], 0x1p-10f, true);
+    w[2] = __builtin_bit_cast(uint32_t, t);
+  }
+}
+
+FVSR_DEV int e8m0(int e) { return min(max(e + 127, 0), 254); }
+
+// Exponent e with the row's largest magnitude in [2^7, 2^8) * 2^e.  A row
+// with an infinity or NaN keeps it in its codes: all its logits are NaN.
+FVSR_DEV int row_exp(uint32_t top) { return max((int)(top >> 23) - 127, -100) - 7; }
+
+FVSR_DEV uint32_t max_mag(uint32_t m, float x) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+
+// Whether any of a V operand's codes is NaN (0x7f with either sign).
+FVSR_DEV bool has_nan(const v8i& v) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) any |= ((uint32_t)v[i] & 0x7f7f7f7fu) + 0x01010101u;
+  return (any & 0x80808080u) != 0;
+}
+// Bytes 0x38 (1.0) where a code is NaN; `v` loses them.
+FVSR_DEV v8i take_nan(v8i& v) {
+  v8i ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t hit = (((uint32_t)v[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    const uint32_t mask = (hit >> 7) * 0xffu;
+    ones[i] = (int)(mask & 0x38383838u);
+    v[i] = (int)((uint32_t)v[i] & ~mask);
+  }
+  return ones;
+}
+
+FVSR_DEV v4f mfma(const v8i& a, const v8i& b, const v4f& c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+FVSR_DEV v16f mfma(const v8i& a, const v8i& b, const v16f& c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
+FVSR_DEV v8i join(u32x4_t a, u32x4_t b) {
+  return v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+// The softmax of one row's N logits at hand (in s; -inf: hidden): s becomes
+// the weights, E - 8 - M goes to `shift`, and the reference M moves if need be
+// (`rescale` then multiplies O).  Every lane of a row calls it with the row's largest logit.
+template <class Acc, int N, class Rescale>
+FVSR_DEV void weigh(Acc (&s)[N], float top, float c, float& m, float& l, int& shift,
+                    Rescale rescale) {
+  constexpr int E = sizeof(Acc) / 4;
+  const float e = fmaxf(__builtin_ceilf(top * c), kNothing);
+  if (__ballot(e > m + 64.0f) != 0) {
+    asm volatile("" :::);  // a branch: rare after a row's first keys
+    const float to = e > m + 64.0f ? e : m;
+    const float f = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= f;
+    rescale(f);
+  }
+  const float off = 8.0f - e;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      s[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], c, off));
+      sum += s[i][j];
+    }
+  shift = (int)fmaxf(e - m, -300.0f) - 8;
+  l += __builtin_ldexpf(sum, shift);
+}
+
+// Keys that row i of a sequence sees.
+FVSR_DEV int row_limit(const Args& a, const SeqPart& s, int i) {
+  const int64_t cap = a.c.table_pages * kPage;
+  const int lim = a.causal ? min(s.len, s.len - s.rows.n + i + 1) : s.len;
+  return (int)min((int64_t)max(lim, 0), cap);
+}
+
+FVSR_DEV int range_at(int pages, int s, int splits) { return (int)((int64_t)pages * s / splits); }
+
+// ---------------------------------------------------------------------------
+// attend_few.  Operand layout of v_mfma_scale_f32_16x16x128: lane (r, g) = (l %
+// 16, l / 16) holds positions 16 g .. and 64 + 16 g .. (16 each) of row r; the
+// scale of 32 positions 32 j .. of row r comes from lane (r, j); accumulator j
+// of lane (q, g) is row 4 g + j of column q.
+// ---------------------------------------------------------------------------
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
+  constexpr int N = terms(DT);
+  constexpr int W = D / 64;                    // 16-byte pieces of a K row per lane
+  constexpr int F = D == 128 ? N : (N + 1) / 2;  // Q operands (64 dims: two terms each)
+  constexpr int DT16 = D / 16;
+  constexpr int P = D + 4;
+  __shared__ __attribute__((aligned(16))) float lds_o[4 * 16 * P];
+  __shared__ float lds_ml[4][16][2];
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x, H = (int)a.c.heads;
+  const int h = blockIdx.y;
+  SeqPart s;
+  s.b = blockIdx.z;
+  s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
+  s.len = max(a.c.lengths[s.b], 0);
+  const int rows = s.rows.n * a.group, r = min(col, rows - 1);
+  const int qi = r / a.group, hq = h * a.group + r % a.group;
+  const int limit = row_limit(a, s, qi);
+  const int lim_lo = row_limit(a, s, 0);
+  const int lim_hi = row_limit(a, s, s.rows.n - 1);
+  const int pages = (lim_hi + kPage - 1) / kPage;
+  const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
+  const int32_t* const table = a.c.table + s.b * a.c.table_stride;
+
+  // Q^T's terms.
+  v8i qf[F];
+  int qs[F];
+  {
+    const uint16_t* qp = a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs + 16 * g;
+    u32x4_t raw[W][2];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      raw[w][0] = *(const u32x4_t*)(qp + 64 * w);
+      raw[w][1] = *(const u32x4_t*)(qp + 64 * w + 8);
+    }
+    const auto el = [&](int w, int i) {
+      const uint32_t u = raw[w][i >> 3][(i >> 1) & 3];
+      return to_f<DT>((uint16_t)(i & 1 ? u >> 16 : u & 0xffff));
+    };
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max_mag(top, el(w, i));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int e = row_exp(top);
+    const float f = __builtin_ldexpf(1.0f, -e);
+    uint32_t t[W][4][N];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        split4<N>(el(w, 4 * i) * f, el(w, 4 * i + 1) * f, el(w, 4 * i + 2) * f,
+                  el(w, 4 * i + 3) * f, t[w][i]);
+#pragma unroll
+    for (int k = 0; k < F; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (D == 128)
+          qf[k][i] = (int)t[i >> 2][i & 3][k];
+        else  // positions 0-63: term 2k, 64-127: term 2k + 1, of the same dims
+          qf[k][i] = 2 * k + (i >> 2) < N ? (int)t[0][i & 3][min(2 * k + (i >> 2), N - 1)] : 0;
+      }
+      qs[k] = e8m0(e - 5 * (D == 128 ? k : 2 * k + (g >> 1)));
+    }
+  }
+
+  v4f acc[DT16] = {};
+  float m = kNothing, l = 0.0f;
+  // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4, so
+  // that accumulator (t, j) of lane g is position 64 (t / 4) + 16 g + 4 (t % 4) + j.
+  const int k_off = (16 * (col >> 2) + (col & 3)) * D + 16 * g;
+  const int v_off = col * kPage + 16 * g;
+  for (int p = p0 + wave; p < p1; p += 4) {
+    const int64_t id = __builtin_amdgcn_readfirstlane(table[p]);
+    if (id < 0 || id >= a.c.pages) {  // no such page: the rows that would read it are NaN
+      if (p * kPage < limit) l = __builtin_nanf("");
+      continue;
+    }
+    const int64_t ph = id * H + h;
+    const uint8_t* kp = (const uint8_t*)a.c.k + ph * kPage * D + k_off;
+    const uint8_t* vp = (const uint8_t*)a.c.v + ph * kPage * D + v_off;
+    const int ks = ((const uint8_t*)a.c.k_scale)[ph], vs = ((const uint8_t*)a.c.v_scale)[ph];
+    v8i kf[8], vf[DT16];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const uint8_t* x = kp + ((t >> 2) * 64 + (t & 3) * 4) * D;
+      const u32x4_t u = *(const u32x4_t*)x;
+      kf[t] = join(u, D == 128 ? *(const u32x4_t*)(x + 64) : u);
+    }
+#pragma unroll
+    for (int d = 0; d < DT16; ++d) {
+      const uint8_t* x = vp + d * 16 * kPage;
+      vf[d] = join(*(const u32x4_t*)x, *(const u32x4_t*)(x + 64));
+    }
+    v4f sc[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const v4f z = {};
+      sc[t] = mfma(kf[t], qf[0], z, ks, qs[0]);
+#pragma unroll
+      for (int k = 1; k < F; ++k) sc[t] = mfma(kf[t], qf[k], sc[t], ks, qs[k]);
+    }
+    const bool masked = (p + 1) * kPage > lim_lo;
+    if (masked) {
+      const int at = p * kPage + 16 * g;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (at + (t >> 2) * 64 + (t & 3) * 4 + j >= limit) sc[t][j] = -__builtin_huge_valf();
+    }
+    float top = -__builtin_huge_valf();
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[t][j]);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    int shift;
+    weigh(sc, top, a.scale_log2, m, l, shift, [&](float f) {
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) acc[d] *= f;
+    });
+    v8i pf[N];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      uint32_t w[N];
+      split4<N>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) pf[k][t] = (int)w[k];
+    }
+    if (masked) {
+      // Hidden tokens weigh 0, which a NaN code would not survive: NaN codes
+      // leave the product and are counted for the rows that see them.
+      bool any = false;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) any |= has_nan(vf[d]);
+      if (__ballot(any) != 0) {
+        v8i seen;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          seen[t] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p * kPage + 16 * g + (t >> 2) * 64 + (t & 3) * 4 + j < limit)
+              seen[t] |= 0x38 << (8 * j);
+        }
+#pragma unroll
+        for (int d = 0; d < DT16; ++d) {
+          const v8i ones = take_nan(vf[d]);
+          const v4f z = {};
+          const v4f n = mfma(ones, seen, z, 127, 127);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n[j] > 0.0f) acc[d][j] = __builtin_nanf("");
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int ps = e8m0(shift - 5 * k);
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) acc[d] = mfma(vf[d], pf[k], acc[d], vs, ps);
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // The waves' parts of each row.
+#pragma unroll
+  for (int d = 0; d < DT16; ++d)
+    *(v4f*)&lds_o[(wave * 16 + col) * P + d * 16 + 4 * g] = acc[d];
+  if (g == 0) lds_ml[wave][col][0] = m, lds_ml[wave][col][1] = l;
+  __syncthreads();
+  constexpr int C = D / 8;  // threads of a row
+  const int row = threadIdx.x / C, d0 = threadIdx.x % C * 8;
+  if (row >= rows) return;
+  float top = lds_ml[0][row][0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_ml[w][row][0]);
+  float o[8] = {}, sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(lds_ml[w][row][0] - top);
+    sum += f * lds_ml[w][row][1];
+    const v4f x = *(const v4f*)&lds_o[(w * 16 + row) * P + d0];
+    const v4f y = *(const v4f*)&lds_o[(w * 16 + row) * P + d0 + 4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * x[e], o[4 + e] += f * y[e];
+  }
+  const int64_t token = s.rows.lo + row / a.group;
+  const int oh = h * a.group + row % a.group;
+  if (a.splits == 1) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    u32x2_t* op = (u32x2_t*)(a.out + token * a.o_ts + oh * a.o_hs + d0);
+    op[0] = u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+    op[1] = u32x2_t{pack2<DT>(o[4] * inv, o[5] * inv), pack2<DT>(o[6] * inv, o[7] * inv)};
+  } else {
+    const int64_t pr = (token * a.q_heads + oh) * a.splits + split;
+    v4f* po = (v4f*)(a.part + pr * D + d0);
+    po[0] = v4f{o[0], o[1], o[2], o[3]};
+    po[1] = v4f{o[4], o[5], o[6], o[7]};
+    if (d0 == 0) {
+      float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
+      ml[0] = top, ml[1] = sum;
+    }
+  }
+}
+
+// The pieces of a row, a wave each: 4 dims a lane, several pieces at once.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void attend_join(Args a) {
+  constexpr int L = D / 4, G = 64 / L;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t rows = (int64_t)a.T * a.q_heads;
+  if (row >= rows) return;
+  const int token = (int)(row / a.q_heads), oh = (int)(row % a.q_heads);
+  // Rows behind the last sequence have no pieces.
+  if (a.c.cu && token >= a.c.cu[a.c.sequences] && !a.tail) return;
+  const int lane = threadIdx.x & 63;
+  const float* ml = a.part + rows * a.splits * D + row * a.splits * 2;
+  const float m = lane < a.splits ? ml[2 * lane] : kNothing;
+  const float l = lane < a.splits ? ml[2 * lane + 1] : 0.0f;
+  const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
+  const float sum = wave_sum(f * l);
+  v4f o = {};
+  const float* po = a.part + row * a.splits * D + (lane % L) * 4;
+  // (Every lane takes every turn: a lane that has left could not lend its factor.)
+  for (int s0 = 0; s0 < a.splits; s0 += G) {
+    const int s = s0 + lane / L;
+    const float w = __shfl(f, s & 63);
+    if (s < a.splits) o += *(const v4f*)(po + (int64_t)s * D) * w;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int d = L; d < 64; d *= 2) o[e] += __shfl_xor(o[e], d);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (lane < L)
+    *(u32x2_t*)(a.out + (int64_t)token * a.o_ts + (int64_t)oh * a.o_hs + lane * 4) =
+        u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+}
+
+// ---------------------------------------------------------------------------
+// attend_tile.  v_mfma_scale_f32_32x32x64: lane (r, g) = (l % 32, l / 32) holds
+// positions 16 g .. and 32 + 16 g .. of row r; accumulator 4 i + j of lane (q, g) is row
+// 8 i + 4 g + j of column q.
+// ---------------------------------------------------------------------------
+
+// 16-byte pieces of a stage's rows are swapped about so that 16 lanes reading
+// one piece of 16 of the rows above touch every bank once: the rows of a K
+// operand differ in token bits 0, 1, 2 and 4 (128-byte rows: bit 0 is the bank
+// half, 64-byte rows: bits 0-1 the quarter), those of a V operand in dim bits 0-3.
+template <int D>
+FVSR_DEV int k_swap(int key) {
+  return D == 128 ? ((key >> 1) & 3) | ((key >> 2) & 4) : ((key >> 2) & 1) | ((key >> 3) & 2);
+}
+FVSR_DEV int v_swap(int d) { return (d >> 1) & 7; }
+
+template <int D>
+struct Stage {
+  static constexpr int kK = kPage * D, kBytes = 2 * kK;
+};
+
+struct PageRef {
+  int page;       // its number in the sequence; -1: none
+  int64_t ph;     // (page id, head); -1: no such page
+  int ks, vs;
+};
+
+// Streams a page's codes into a stage: segment s (1 KB) by wave s % 4, straight from
+// memory; the piece that a lane fetches is the one that belongs where it lands.
+template <int D>
+FVSR_DEV void stream_page(uint8_t LDS_AS* st, const Args& a, int64_t ph, int wave, int lane) {
+  constexpr int KR = D / 16, S = kPage * D / 1024;  // pieces of a K row; segments
+  const uint8_t* k = (const uint8_t*)a.c.k + ph * kPage * D;
+  const uint8_t* v = (const uint8_t*)a.c.v + ph * kPage * D;
+  const int kr = wave * (64 / KR) + lane / KR;  // K row within segments 0-3, V row likewise
+  const int vr = wave * 8 + lane / 8;
+  const int ko = (lane / KR) * D + ((lane % KR) ^ k_swap<D>(kr)) * 16;
+  const int vo = (lane / 8) * kPage + ((lane % 8) ^ v_swap(vr)) * 16;
+#pragma unroll
+  for (int t = 0; t < S / 4; ++t) {
+    const int s = wave + 4 * t;
+    __builtin_amdgcn_global_load_lds(k + s * 1024 + ko, (void LDS_AS*)(st + s * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds(v + s * 1024 + vo,
+                                     (void LDS_AS*)(st + Stage<D>::kK + s * 1024), 16, 0, 0);
+  }
+}
+
+// Pages p .. p1 - 1 that a block mask's row keeps (or all of them), one after another.
+struct PageList {
+  const uint8_t* keep;  // the row, or null
+  int kept;             // its entries
+  int base, p, p1;
+  uint64_t word;
+
+  __device__ __forceinline__ void load() {
+    const int i = base + (threadIdx.x & 63);
+    word = __ballot(i >= p && i < p1 && i < kept && keep[i] != 0);
+  }
+  __device__ __forceinline__ void start(const uint8_t* row, int n, int from, int to) {
+    keep = row, kept = n, p = from, p1 = to, base = from, word = 0;
+    if (keep && p < p1) load();
+  }
+  __device__ __forceinline__ int next() {
+    if (!keep) return p < p1 ? p++ : -1;
+    while (!word) {
+      base += 64;
+      if (base >= p1) return -1;
+      load();
+    }
+    const int i = __builtin_ctzll(word);
+    word &= word - 1;
+    return base + i;
+  }
+};
+
+struct Rows {
+  int limit, lim_lo, lim_hi;  // keys this lane's row sees; least and most of the wave
+};
+
+template <int DT, int D>
+FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Rows& rw, float c,
+                          const v8i (&qf)[D / 64][terms(DT)], int qe, v16f (&acc)[D / 32], float& m,
+                          float& l) {
+  constexpr int N = terms(DT);
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+  const int at = ref.page * kPage;
+  if (at >= rw.lim_hi) return;  // nothing of it is seen by this wave
+  if (ref.ph < 0) {             // no such page: the rows that would read it are NaN
+    if (at < rw.limit) l = __builtin_nanf("");
+    return;
+  }
+  const bool masked = at + kPage > rw.lim_lo;
+  const uint8_t LDS_AS* kt = st;
+  const uint8_t LDS_AS* vt = st + Stage<D>::kK;
+  // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
+  const int kr = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    v16f s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = half * 64 + u * 32 + kr, sw = k_swap<D>(key);
+      const v16f z = {};
+      s[u] = z;
+#pragma unroll
+      for (int w = 0; w < D / 64; ++w) {
+        const v8i kf = join(*(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + g) ^ sw) << 4)),
+                            *(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + 2 + g) ^ sw) << 4)));
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[u] = mfma(kf, qf[w][k], s[u], ref.ks, e8m0(qe - 5 * k));
+      }
+    }
+    v8i vf[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const int dim = d * 32 + r, sw = v_swap(dim);
+      vf[d] = join(*(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + g) ^ sw) << 4)),
+                   *(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + 2 + g) ^ sw) << 4)));
+    }
+    const int key0 = at + half * 64 + 16 * g;  // + 32 u + e: this lane's keys
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (key0 + 32 * u + e >= rw.limit) s[u][e] = -__builtin_huge_valf();
+    }
+    float top = -__builtin_huge_valf();
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
+                                                     false, false);
+    top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    int shift;
+    weigh(s, top, c, m, l, shift, [&](float f) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] *= f;
+    });
+    v8i pf[N];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[N];
+        split4<N>(s[u][4 * i], s[u][4 * i + 1], s[u][4 * i + 2], s[u][4 * i + 3], w);
+#pragma unroll
+        for (int k = 0; k < N; ++k) pf[k][u * 4 + i] = (int)w[k];
+      }
+    if (masked) {  // as in attend_few
+      bool any = false;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) any |= has_nan(vf[d]);
+      if (__ballot(any) != 0) {
+        v8i seen;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          seen[i] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (key0 + 32 * (i >> 2) + 4 * (i & 3) + j < rw.limit) seen[i] |= 0x38 << (8 * j);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          const v8i ones = take_nan(vf[d]);
+          const v16f z = {};
+          const v16f n = mfma(ones, seen, z, 127, 127);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int ps = e8m0(shift - 5 * k);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] = mfma(vf[d], pf[k], acc[d], ref.vs, ps);
+    }
+  }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
+  constexpr int N = terms(DT);
+  __shared__ __attribute__((aligned(1024))) uint8_t stage0[Stage<D>::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage1[Stage<D>::kBytes];
+  uint8_t LDS_AS* st0 = (uint8_t LDS_AS*)stage0;
+  uint8_t LDS_AS* st1 = (uint8_t LDS_AS*)stage1;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous
+  // range of (head, split, tile) units, whose neighbours read the same pages.
+  const int total = gridDim.x, per = total / 8, rem = total % 8;
+  const int xcd = blockIdx.x % 8, loc = blockIdx.x / 8;
+  const int unit = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+  // Without a block mask a tile's rows are (query, head of the group) pairs, so
+  // a group's heads read its pages once; with one, each head has its own pages.
+  const int pack = a.keep ? 1 : a.group, H = (int)a.c.heads;
+  const int tile_unit = unit % a.tiles, split = unit / a.tiles % a.splits;
+  const int head = unit / a.tiles / a.splits;
+  const int h = a.keep ? head / a.group : head;
+  SeqPart s;
+  const auto tiles_of = [&](int n, int) { return (n * pack + 127) / 128; };
+  if (a.c.cu) {
+    if (!find_part(a.c.cu, a.c.lengths, (int)a.c.sequences, a.T, tile_unit, a.tail != 0, tiles_of,
+                   s))
+      return;
+  } else {
+    const int each = a.tiles / (int)a.c.sequences;
+    s.b = tile_unit / each;
+    s.part = tile_unit % each;
+    s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
+    s.len = max(a.c.lengths[s.b], 0);
+  }
+  const int rows = s.rows.n * pack;
+  const int first = s.part * 128 + wave * 32;           // the wave's first row
+  const int r = min(first + r32, rows - 1), qi = r / pack;
+  const int hq = a.keep ? head : h * a.group + r % pack;
+  Rows rw;
+  rw.limit = row_limit(a, s, qi);
+  rw.lim_lo = row_limit(a, s, min(first, rows - 1) / pack);
+  rw.lim_hi = first < rows ? row_limit(a, s, min(first + 31, rows - 1) / pack) : 0;
+  const int last = row_limit(a, s, min(s.part * 128 + 127, rows - 1) / pack);
+  const int pages = (last + kPage - 1) / kPage;
+  const int32_t* const table = a.c.table + s.b * a.c.table_stride;
+  const uint8_t* keep = nullptr;
+  int kept = 0;
+  if (a.keep) {
+    keep = a.keep + (((int64_t)s.b * a.q_heads + head) * a.keep_q + s.part) * a.keep_k;
+    kept = s.part < a.keep_q && s.b < a.c.sequences ? (int)min(a.keep_k, (int64_t)0x7fffffff) : 0;
+  }
+  PageList list;
+  list.start(keep, kept, range_at(pages, split, a.splits), range_at(pages, split + 1, a.splits));
+
+  const auto look_up = [&](int page) {
+    PageRef f{page, -1, 0, 0};
+    if (page >= 0) {
+      const int64_t id = __builtin_amdgcn_readfirstlane(table[page]);
+      if (id >= 0 && id < a.c.pages) f.ph = id * H + h;
+    }
+    return f;
+  };
+  const auto fetch = [&](uint8_t LDS_AS* st, PageRef& f) {
+    if (f.ph < 0) return;
+    stream_page<D>(st, a, f.ph, wave, lane);
+    f.ks = ((const uint8_t*)a.c.k_scale)[f.ph];
+    f.vs = ((const uint8_t*)a.c.v_scale)[f.ph];
+  };
+  PageRef cur = look_up(list.next());
+  if (cur.page >= 0) fetch(st0, cur);
+  PageRef nxt = cur.page >= 0 ? look_up(list.next()) : PageRef{-1, -1, 0, 0};
+
+  v8i qf[D / 64][N];
+  int qe;
+  {
+    const uint16_t* qp =
+        a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs + 16 * g;
+    u32x4_t raw[D / 32][2];
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      raw[w][0] = *(const u32x4_t*)(qp + 32 * w);
+      raw[w][1] = *(const u32x4_t*)(qp + 32 * w + 8);
+    }
+    const auto el = [&](int w, int i) {
+      const uint32_t u = raw[w][i >> 3][(i >> 1) & 3];
+      return to_f<DT>((uint16_t)(i & 1 ? u >> 16 : u & 0xffff));
+    };
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max_mag(top, el(w, i));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    qe = row_exp(top);
+    const float f = __builtin_ldexpf(1.0f, -qe);
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t t[N];
+        split4<N>(el(w, 4 * i) * f, el(w, 4 * i + 1) * f, el(w, 4 * i + 2) * f,
+                  el(w, 4 * i + 3) * f, t);
+#pragma unroll
+        for (int k = 0; k < N; ++k) qf[w >> 1][k][(w & 1) * 4 + i] = (int)t[k];
+      }
+  }
+
+  v16f acc[D / 32] = {};
+  float m = kNothing, l = 0.0f;
+  // One page: wait for it, start the next one, then multiply.  The stages
+  // are distinct objects, so the loads into one do not wait for reads of the other.
+  const auto step = [&](uint8_t LDS_AS* st, uint8_t LDS_AS* other) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (nxt.page >= 0) fetch(other, nxt);
+    const PageRef after = nxt.page >= 0 ? look_up(list.next()) : PageRef{-1, -1, 0, 0};
+    attend_page<DT, D>(st, cur, rw, a.scale_log2, qf, qe, acc, m, l);
+    cur = nxt;
+    nxt = after;
+  };
+  while (cur.page >= 0) {
+    step(st0, st1);
+    if (cur.page < 0) break;
+    step(st1, st0);
+  }
+
+  l += __shfl_xor(l, 32);
+  if (first + r32 >= rows) return;
+  const int64_t token = s.rows.lo + qi;
+  if (a.splits == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* op = a.out + token * a.o_ts + (int64_t)hq * a.o_hs + 4 * g;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(u32x2_t*)(op + d * 32 + 8 * i) =
+            u32x2_t{pack2<DT>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
+                    pack2<DT>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
+  } else {
+    const int64_t pr = (token * a.q_heads + hq) * a.splits + split;
+    float* po = a.part + pr * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(v4f*)(po + d * 32 + 8 * i) =
+            v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+    if (g == 0) {
+      float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
+      ml[0] = m, ml[1] = l;
+    }
+  }
+}
+
+// How a call is cut up: a function of its sizes only.
+struct Plan {
+  bool few;
+  int64_t tiles;  // per head: row tiles over all sequences
+  int64_t heads;  // units' heads
+  int splits;
+  int64_t floats(int64_t T, int64_t q_heads, int64_t D) const {
+    return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
+  }
+};
+
+Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
+  Plan p{};
+  const int64_t group = q_heads / c->heads, B = c->sequences;
+  const int64_t rows = T / B * group;  // of a sequence and key/value head, if all are alike
+  p.few = !c->cu && !keep && rows <= 16;
+  const int64_t pack = keep ? 1 : group;
+  p.heads = keep ? q_heads : c->heads;
+  if (p.few)
+    p.tiles = B;
+  else if (c->cu)  // at most this many over any counts that add up to T, the rows behind included
+    p.tiles = T * pack / 128 + B + 1;
+  else
+    p.tiles = B * ((T / B * pack + 127) / 128);
+  const int64_t units = p.tiles * p.heads, want = p.few ? 1024 : 512;
+  const int64_t most = std::max<int64_t>(1, c->table_pages / (p.few ? 4 : 2));
+  p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, want / units), most, kMaxSplits});
+  return p;
+}
+
+template <int DT, int D>
+void launch(const Args& a, const Plan& p, hipStream_t st) {
+  if (p.few)
+    hipLaunchKernelGGL((attend_few<DT, D>), dim3((unsigned)a.splits, (unsigned)a.c.heads,
+                                                 (unsigned)a.c.sequences),
+                       dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((attend_tile<DT, D>), dim3((unsigned)(p.tiles * p.heads * p.splits)),
+                       dim3(kThreads), 0, st, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((attend_join<DT, D>), dim3((unsigned)(((int64_t)a.T * a.q_heads + 3) / 4)),
+                       dim3(kThreads), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int64_t fvsr_paged_attn_workspace_floats(const fvsr_kv_cache* cache, int64_t T,
+                                                    int64_t q_heads, int has_keep) {
+  if (kv_cache_ok(cache, T) != FVSR_OK || T == 0 || cache->sequences == 0 || q_heads <= 0 ||
+      q_heads % cache->heads)
+    return 0;
+  return plan_attn(cache, T, q_heads, has_keep != 0).floats(T, q_heads, cache->head_dim);
+}
+
+extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_stride,
+                               int64_t q_head_stride, int64_t q_heads, void* out,
+                               int64_t o_tok_stride, int64_t o_head_stride, int dtype, int64_t T,
+                               int causal, const uint8_t* keep, int64_t keep_q, int64_t keep_k,
+                               float sm_scale, int fill_tail, float* workspace,
+                               int64_t workspace_floats, void* stream) {
+  const int rc = kv_cache_ok(cache, T);
+  if (rc != FVSR_OK) return rc;
+  if (dtype != FVSR_DT_BF16 && dtype != FVSR_DT_F16) return FVSR_EINVAL;
+  if (q_heads <= 0 || q_heads % cache->heads || !(sm_scale > 0.0f) || sm_scale > 3e38f)
+    return FVSR_EINVAL;
+  if (keep && (keep_q < 0 || keep_k < 0)) return FVSR_EINVAL;
+  if (T == 0 || cache->sequences == 0) return FVSR_OK;
+  if (!q || !out) return FVSR_EINVAL;
+  if ((((uintptr_t)q) | (uint64_t)(q_tok_stride * 2) | (uint64_t)(q_head_stride * 2)) & 15)
+    return FVSR_EUNSUPPORTED;
+  if ((((uintptr_t)out) | (uint64_t)(o_tok_stride * 2) | (uint64_t)(o_head_stride * 2)) & 7)
+    return FVSR_EUNSUPPORTED;
+  if (T * q_heads > 0x7fffffff - 256) return FVSR_EUNSUPPORTED;
+  const Plan p = plan_attn(cache, T, q_heads, keep != nullptr);
+  if (p.tiles * p.heads * p.splits > 0x7fffffff || cache->heads > 65535 ||
+      (p.few && cache->sequences > 65535))
+    return FVSR_EUNSUPPORTED;
+  const int64_t need = p.floats(T, q_heads, cache->head_dim);
+  if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;
+  if (need && ((uintptr_t)workspace & 15)) return FVSR_EUNSUPPORTED;
+  Args a{};
+  a.c = *cache;
+  a.q = (const uint16_t*)q, a.out = (uint16_t*)out;
+  a.q_ts = q_tok_stride, a.q_hs = q_head_stride, a.o_ts = o_tok_stride, a.o_hs = o_head_stride;
+  a.keep = keep, a.keep_q = keep_q, a.keep_k = keep_k;
+  a.part = workspace;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / cache->heads);
+  a.causal = causal != 0, a.splits = p.splits, a.tiles = (int)p.tiles, a.tail = fill_tail != 0;
+  const hipStream_t st = (hipStream_t)stream;
+  const bool half = dtype == FVSR_DT_F16;
+  if (cache->head_dim == 128)
+    half ? launch<FVSR_DT_F16, 128>(a, p, st) : launch<FVSR_DT_BF16, 128>(a, p, st);
+  else
+    half ? launch<FVSR_DT_F16, 64>(a, p, st) : launch<FVSR_DT_BF16, 64>(a, p, st);
+  return fvsr_launch_status();
+}

@@ -34,6 +34,7 @@ from .fp8_ffn import FP8FFN, convert_ffn_fp8, fused_gelu_quant_fp8  # noqa: E402
 from .integrate import enable  # noqa: E402
 from .lcsa import block_sparse_attention, build_csr, draft_block_mask  # noqa: E402
 from .cross_attn import cross_attention, cross_attention_residual  # noqa: E402
+from .paged_kv import KVPages, append_kv, kv_pages, paged_attention  # noqa: E402
 
 __version__ = "0.1.0"
 
@@ -62,6 +63,10 @@ __all__ = [
     "draft_block_mask",
     "cross_attention",
     "cross_attention_residual",
+    "KVPages",
+    "kv_pages",
+    "append_kv",
+    "paged_attention",
     "active_backend",
     "ensure_bsa_available",
 ]

@@ -22,6 +22,7 @@ FVSR_OK, FVSR_EINVAL, FVSR_EHIP, FVSR_EUNSUPPORTED, FVSR_EWORKSPACE = 0, -1, -2,
 SCALE_TENSOR, SCALE_ROW = 0, 1
 EPI_BIAS, EPI_ROWMAX, EPI_GATE_ADD = 0, 1, 2
 DT_BF16, DT_F16, DT_F32 = 0, 1, 2
+NORM_NONE, NORM_HEAD, NORM_ROW = 0, 1, 2
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 
 _ERR = {
@@ -82,6 +83,12 @@ _SIGS = {
                          _I64, _F, _P], _I),
     "fvsr_bsa_fwd_window": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64,
                              _I64, _I64, _I64, _I64, _F, _I64, _I64, _I64, _I, _P], _I),
+    "fvsr_kv_append_workspace_floats": ([_I64, _I], _I64),
+    "fvsr_kv_append": ([_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I, _I64, _P,
+                        _I, _P, _I, _I, _F, _P, _I64, _P, _P, _I64, _P], _I),
+    "fvsr_paged_attn_workspace_floats": ([_P, _I64, _I64, _I], _I64),
+    "fvsr_paged_attn": ([_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I, _I64, _I, _P, _I64, _I64, _F,
+                         _I, _P, _I64, _P], _I),
 }
 
 _lib = None

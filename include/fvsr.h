@@ -430,6 +430,96 @@ int fvsr_attn_dense(const void* q, const void* k, const void* v, void* o, int64_
                     int64_t o_tok_stride, int64_t o_head_stride, int64_t H, int64_t NQ,
                     int64_t NK, int64_t head_dim, float sm_scale, void* stream);
 
+/*
+ * 8-bit K/V cache in pages of FVSR_PAGE tokens (the attention's key block).
+ * No counterpart in the reference, whose self-attention keeps the cached
+ * windows' keys and values in bf16 (integrate.py:59-83).
+ *
+ *   k        [pages, heads, FVSR_PAGE, head_dim] e4m3
+ *   v        [pages, heads, head_dim, FVSR_PAGE] e4m3 (both as the matrix
+ *            cores take them: no value moves between memory and an operand)
+ *   k_scale, v_scale  [pages, heads] e8m0 (byte b stands for 2^(b - 127)): one
+ *            power of two for a page and head; value = code * scale
+ *   table    [sequences, table_stride] int32, its first table_pages columns
+ *            used: page of a sequence's tokens 128 j .. 128 j + 127
+ *   lengths  [sequences] int32: tokens, those of this call included
+ *   cu       [sequences + 1] int32, from 0: rows cu[b] .. cu[b + 1] - 1 of the call belong
+ *            to sequence b; NULL: T / sequences rows each, in order
+ *
+ * The n rows of sequence b stand at positions lengths[b] - n .. lengths[b] - 1.
+ * Table, lengths and cu are device memory and cannot be checked on the host;
+ * whatever they hold, no kernel reaches outside the tensors: positions below 0
+ * or past the table are not stored, a page id outside 0 .. pages - 1 is not written
+ * and turns the rows that read it NaN.  Rows behind cu[sequences] belong to
+ * nobody.  head_dim 64 or 128.  k and v are 16-byte aligned.
+ */
+enum { FVSR_PAGE = 128 };
+typedef struct {
+  void *k, *v, *k_scale, *v_scale;
+  int64_t pages, heads, head_dim;
+  const int32_t* table;
+  int64_t table_stride, table_pages;
+  const int32_t *lengths, *cu;
+  int64_t sequences;
+} fvsr_kv_cache;
+
+/* RMSNorm of fvsr_kv_append: over each head (weight [head_dim]) or the whole
+ * row (weight [heads * head_dim]). */
+enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
+
+/*
+ * Append T rows of keys and values to the cache.  k and v [T, heads, head_dim]
+ * and, if given, q [T, q_heads, head_dim] in `dtype`, heads contiguous, token
+ * and head strides in elements (multiples of 16 bytes; bases too).
+ *   k, q   normalised (k_norm, q_norm; weights in weight_dtype), then pairs
+ *          (2i, 2i + 1) rotated by row positions[t] (NULL: row t) of cs, fp32
+ *          [cs_rows, head_dim / 2, 2] of (cos, sin) (NULL: not rotated); a position outside
+ *          the table gives NaN
+ *   q_out  [T, q_heads, head_dim] in dtype, every row of it written
+ * fp32 from the loads to the one rounding.  A page's scale is the least 2^e, e
+ * >= -126, with every finite new magnitude at most 448 * 2^e; where the page
+ * holds tokens before the new ones, not below its old one, and their codes are
+ * rounded again if it grows.  Infinities and NaN are stored as NaN.  Slots
+ * behind the last new token keep their bytes.  Sequences that append must not
+ * share the pages they append to.
+ *   workspace  fvsr_kv_append_workspace_floats(T, k_norm) floats (0: NULL is
+ *              fine), used until the call's kernels have run
+ */
+int64_t fvsr_kv_append_workspace_floats(int64_t T, int k_norm);
+int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stride,
+                   int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                   int64_t v_head_stride, const void* q, int64_t q_tok_stride,
+                   int64_t q_head_stride, int64_t q_heads, void* q_out, int dtype, int64_t T,
+                   const void* k_weight, int k_norm, const void* q_weight, int q_norm,
+                   int weight_dtype, float eps, const float* cs, int64_t cs_rows,
+                   const int32_t* positions, float* workspace, int64_t workspace_floats,
+                   void* stream);
+
+/*
+ * softmax(q k^T * sm_scale) v over a paged cache: q and out [T, q_heads, head_dim]
+ * in `dtype` (FVSR_DT_BF16 or FVSR_DT_F16), heads contiguous, strides in elements
+ * (q: multiples of 8, 16-byte aligned; out: multiples of 4, 8-byte aligned);
+ * query head h reads key/value head h / (q_heads / heads).
+ *   causal  a query at position p sees the positions 0 .. p, otherwise every
+ *           token of its sequence
+ *   keep    bytes [sequences, q_heads, keep_q, keep_k] or NULL: queries 128 i ..
+ *           128 i + 127 of a sequence's rows see page j only where entry (i, j) is
+ *           nonzero; blocks outside keep_q x keep_k are not kept
+ *   out     rows that see nothing are zeros; rows behind cu[sequences] are zeros
+ *           if fill_tail, else left as they are
+ * Logits and sums in fp32.  What a mask hides does not count, whatever it holds
+ * (NaN included).  sm_scale positive.
+ *   workspace  fvsr_paged_attn_workspace_floats(...) floats, 16-byte aligned
+ *              (0: NULL is fine), used until the call's kernels have run
+ */
+int64_t fvsr_paged_attn_workspace_floats(const fvsr_kv_cache* cache, int64_t T, int64_t q_heads,
+                                         int has_keep);
+int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_stride,
+                    int64_t q_head_stride, int64_t q_heads, void* out, int64_t o_tok_stride,
+                    int64_t o_head_stride, int dtype, int64_t T, int causal, const uint8_t* keep,
+                    int64_t keep_q, int64_t keep_k, float sm_scale, int fill_tail,
+                    float* workspace, int64_t workspace_floats, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
