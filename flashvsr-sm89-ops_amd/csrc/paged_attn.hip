@@ -448,19 +448,12 @@ struct Stage {
   static constexpr int kK = kPage * D, kBytes = 2 * kK;
 };
 
-struct PageRef {
-  int page;       // its number in the sequence; -1: none
-  int64_t ph;     // (page id, head); -1: no such page
-  int ks, vs;
-};
-
 // Streams a page's codes into a stage: segment s (1 KB) by wave s % 4, straight from
 // memory; the piece that a lane fetches is the one that belongs where it lands.
 template <int D>
-FVSR_DEV void stream_page(uint8_t LDS_AS* st, const Args& a, int64_t ph, int wave, int lane) {
+FVSR_DEV void stream_page(uint8_t LDS_AS* st, const uint8_t* k, const uint8_t* v, int wave,
+                          int lane) {
   constexpr int KR = D / 16, S = kPage * D / 1024;  // pieces of a K row; segments
-  const uint8_t* k = (const uint8_t*)a.c.k + ph * kPage * D;
-  const uint8_t* v = (const uint8_t*)a.c.v + ph * kPage * D;
   const int kr = wave * (64 / KR) + lane / KR;  // K row within segments 0-3, V row likewise
   const int vr = wave * 8 + lane / 8;
   const int ko = (lane / KR) * D + ((lane % KR) ^ k_swap<D>(kr)) * 16;
@@ -474,47 +467,52 @@ FVSR_DEV void stream_page(uint8_t LDS_AS* st, const Args& a, int64_t ph, int wav
   }
 }
 
-// Pages p .. p1 - 1 that a block mask's row keeps (or all of them), one after another.
-struct PageList {
-  const uint8_t* keep;  // the row, or null
-  int kept;             // its entries
-  int base, p, p1;
-  uint64_t word;
+// The pages ahead, looked up kList at a time: number in the sequence, id (-1:
+// no such page), K scale | V scale << 8.
+constexpr int kList = 512;
+typedef int v4i __attribute__((ext_vector_type(4)));
 
-  __device__ __forceinline__ void load() {
-    const int i = base + (threadIdx.x & 63);
-    word = __ballot(i >= p && i < p1 && i < kept && keep[i] != 0);
-  }
-  __device__ __forceinline__ void start(const uint8_t* row, int n, int from, int to) {
-    keep = row, kept = n, p = from, p1 = to, base = from, word = 0;
-    if (keep && p < p1) load();
-  }
-  __device__ __forceinline__ int next() {
-    if (!keep) return p < p1 ? p++ : -1;
-    while (!word) {
-      base += 64;
-      if (base >= p1) return -1;
-      load();
+// Entries of pages from .. from + kList - 1 below p1 that the block mask's row
+// keeps (null: all), in order; returns their number.  Every wave counts all of
+// them and writes its share.
+FVSR_DEV int list_pages(v4i LDS_AS* list, const Args& a, const int32_t* table, int h,
+                        const uint8_t* keep, int kept, int from, int p1, int wave) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+#pragma unroll 1
+  for (int g = 0; g < kList / 64 && from + g * 64 < p1; ++g) {
+    const int i = from + g * 64 + lane;
+    const bool in = i < p1 && (!keep || (i < kept && keep[i] != 0));
+    const uint64_t word = __ballot(in);
+    if (in && g % 4 == wave) {
+      const int id = table[i];
+      v4i e{i, -1, 0, 0};
+      if (id >= 0 && id < a.c.pages) {
+        const int64_t ph = (int64_t)id * a.c.heads + h;
+        e[1] = id;
+        e[2] = ((const uint8_t*)a.c.k_scale)[ph] | ((const uint8_t*)a.c.v_scale)[ph] << 8;
+      }
+      list[n + __popcll(word & ((1ull << lane) - 1))] = e;
     }
-    const int i = __builtin_ctzll(word);
-    word &= word - 1;
-    return base + i;
+    n += __popcll(word);
   }
-};
+  return n;
+}
 
 struct Rows {
   int limit, lim_lo, lim_hi;  // keys this lane's row sees; least and most of the wave
 };
 
 template <int DT, int D>
-FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Rows& rw, float c,
-                          const v8i (&qf)[D / 64][terms(DT)], int qe, v16f (&acc)[D / 32], float& m,
-                          float& l) {
+FVSR_DEV void attend_page(const uint8_t LDS_AS* st, int page, bool there, int ks, int vs,
+                          const Rows& rw, float c,
+                          const v8i (&qf)[D / 64][terms(DT)], const int (&qs)[terms(DT)],
+                          v16f (&acc)[D / 32], float& m, float& l) {
   constexpr int N = terms(DT);
   const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-  const int at = ref.page * kPage;
+  const int at = page * kPage;
   if (at >= rw.lim_hi) return;  // nothing of it is seen by this wave
-  if (ref.ph < 0) {             // no such page: the rows that would read it are NaN
+  if (!there) {                 // no such page: the rows that would read it are NaN
     if (at < rw.limit) l = __builtin_nanf("");
     return;
   }
@@ -523,7 +521,7 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
   const uint8_t LDS_AS* vt = st + Stage<D>::kK;
   // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
   const int kr = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
-#pragma unroll
+#pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     v16f s[2];
 #pragma unroll
@@ -536,7 +534,7 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
         const v8i kf = join(*(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + g) ^ sw) << 4)),
                             *(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + 2 + g) ^ sw) << 4)));
 #pragma unroll
-        for (int k = 0; k < N; ++k) s[u] = mfma(kf, qf[w][k], s[u], ref.ks, e8m0(qe - 5 * k));
+        for (int k = 0; k < N; ++k) s[u] = mfma(kf, qf[w][k], s[u], ks, qs[k]);
       }
     }
     v8i vf[D / 32];
@@ -546,13 +544,14 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
       vf[d] = join(*(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + g) ^ sw) << 4)),
                    *(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + 2 + g) ^ sw) << 4)));
     }
-    const int key0 = at + half * 64 + 16 * g;  // + 32 u + e: this lane's keys
+    const int room = rw.limit - (at + half * 64 + 16 * g);  // this lane's keys: 32 u + e < room
     if (masked) {
+      asm volatile("" :::);  // a branch: most pages are seen whole
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (key0 + 32 * u + e >= rw.limit) s[u][e] = -__builtin_huge_valf();
+          if (32 * u + e >= room) s[u][e] = -__builtin_huge_valf();
     }
     float top = -__builtin_huge_valf();
 #pragma unroll
@@ -578,6 +577,7 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
         for (int k = 0; k < N; ++k) pf[k][u * 4 + i] = (int)w[k];
       }
     if (masked) {  // as in attend_few
+      asm volatile("" :::);
       bool any = false;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) any |= has_nan(vf[d]);
@@ -588,7 +588,7 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
           seen[i] = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (key0 + 32 * (i >> 2) + 4 * (i & 3) + j < rw.limit) seen[i] |= 0x38 << (8 * j);
+            if (32 * (i >> 2) + 4 * (i & 3) + j < room) seen[i] |= 0x38 << (8 * j);
         }
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) {
@@ -605,7 +605,7 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, const PageRef& ref, const Ro
     for (int k = 0; k < N; ++k) {
       const int ps = e8m0(shift - 5 * k);
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] = mfma(vf[d], pf[k], acc[d], ref.vs, ps);
+      for (int d = 0; d < D / 32; ++d) acc[d] = mfma(vf[d], pf[k], acc[d], vs, ps);
     }
   }
 }
@@ -615,6 +615,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   constexpr int N = terms(DT);
   __shared__ __attribute__((aligned(1024))) uint8_t stage0[Stage<D>::kBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t stage1[Stage<D>::kBytes];
+  __shared__ v4i list[kList];
   uint8_t LDS_AS* st0 = (uint8_t LDS_AS*)stage0;
   uint8_t LDS_AS* st1 = (uint8_t LDS_AS*)stage1;
   const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
@@ -660,29 +661,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
     keep = a.keep + (((int64_t)s.b * a.q_heads + head) * a.keep_q + s.part) * a.keep_k;
     kept = s.part < a.keep_q && s.b < a.c.sequences ? (int)min(a.keep_k, (int64_t)0x7fffffff) : 0;
   }
-  PageList list;
-  list.start(keep, kept, range_at(pages, split, a.splits), range_at(pages, split + 1, a.splits));
-
-  const auto look_up = [&](int page) {
-    PageRef f{page, -1, 0, 0};
-    if (page >= 0) {
-      const int64_t id = __builtin_amdgcn_readfirstlane(table[page]);
-      if (id >= 0 && id < a.c.pages) f.ph = id * H + h;
-    }
-    return f;
-  };
-  const auto fetch = [&](uint8_t LDS_AS* st, PageRef& f) {
-    if (f.ph < 0) return;
-    stream_page<D>(st, a, f.ph, wave, lane);
-    f.ks = ((const uint8_t*)a.c.k_scale)[f.ph];
-    f.vs = ((const uint8_t*)a.c.v_scale)[f.ph];
-  };
-  PageRef cur = look_up(list.next());
-  if (cur.page >= 0) fetch(st0, cur);
-  PageRef nxt = cur.page >= 0 ? look_up(list.next()) : PageRef{-1, -1, 0, 0};
+  const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
 
   v8i qf[D / 64][N];
-  int qe;
+  int qs[N];
   {
     const uint16_t* qp =
         a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs + 16 * g;
@@ -702,8 +684,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = max_mag(top, el(w, i));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    qe = row_exp(top);
-    const float f = __builtin_ldexpf(1.0f, -qe);
+    const int e = row_exp(top);
+    const float f = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+    for (int k = 0; k < N; ++k) qs[k] = e8m0(e - 5 * k);
 #pragma unroll
     for (int w = 0; w < D / 32; ++w)
 #pragma unroll
@@ -718,21 +702,39 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
 
   v16f acc[D / 32] = {};
   float m = kNothing, l = 0.0f;
+  const uint8_t* const kb = (const uint8_t*)a.c.k + (int64_t)h * kPage * D;
+  const uint8_t* const vb = (const uint8_t*)a.c.v + (int64_t)h * kPage * D;
+  const int64_t stride = (int64_t)H * kPage * D;
+  int n = 0;
+  const auto entry = [&](int i) {
+    v4i e = ((const v4i LDS_AS*)list)[i];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) e[k] = __builtin_amdgcn_readfirstlane(e[k]);
+    return e;
+  };
+  const auto fetch = [&](uint8_t LDS_AS* st, int id) {
+    if (id >= 0) stream_page<D>(st, kb + id * stride, vb + id * stride, wave, lane);
+  };
   // One page: wait for it, start the next one, then multiply.  The stages
   // are distinct objects, so the loads into one do not wait for reads of the other.
-  const auto step = [&](uint8_t LDS_AS* st, uint8_t LDS_AS* other) {
+  const auto step = [&](uint8_t LDS_AS* st, uint8_t LDS_AS* other, int i) {
+    const v4i e = entry(i);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (nxt.page >= 0) fetch(other, nxt);
-    const PageRef after = nxt.page >= 0 ? look_up(list.next()) : PageRef{-1, -1, 0, 0};
-    attend_page<DT, D>(st, cur, rw, a.scale_log2, qf, qe, acc, m, l);
-    cur = nxt;
-    nxt = after;
+    if (i + 1 < n) fetch(other, entry(i + 1)[1]);
+    attend_page<DT, D>(st, e[0], e[1] >= 0, e[2] & 255, e[2] >> 8, rw, a.scale_log2, qf, qs, acc,
+                       m, l);
   };
-  while (cur.page >= 0) {
-    step(st0, st1);
-    if (cur.page < 0) break;
-    step(st1, st0);
+  for (int from = p0; from < p1; from += kList) {
+    __syncthreads();
+    n = list_pages((v4i LDS_AS*)list, a, table, h, keep, kept, from, p1, wave);
+    __syncthreads();
+    if (n == 0) continue;
+    fetch(st0, entry(0)[1]);
+    for (int i = 0; i < n; i += 2) {
+      step(st0, st1, i);
+      if (i + 1 < n) step(st1, st0, i + 1);
+    }
   }
 
   l += __shfl_xor(l, 32);
