@@ -122,15 +122,15 @@ def lib():
 class _GeneralPath:
     """Stands in for the extension where it cannot be used: every call is left
     to the Python path, which reaches the same kernels through ctypes."""
-    quantize = gemm = staticmethod(lambda *args: None)
+    quantize = gemm = append_kv = paged_attention = staticmethod(lambda *args: None)
 
 
 _host = None
 
 
 def host():
-    """The extension with the native host side of quantisation and GEMM
-    (csrc/host_ops.cpp), bound to the loaded library's functions.  It only
+    """The extension with the native host side of quantisation, GEMM and the
+    paged cache (csrc/host_ops.cpp), bound to the loaded library's functions.  It only
     saves host time, and unlike the library it is tied to the Python and torch
     it was built with: where it does not load or was built with another torch, a
     warning says why, once, and the calls take the Python path."""
@@ -157,6 +157,22 @@ def host():
                     h = _GeneralPath
                 _host = h
     return _host
+
+
+_paged_host = None
+
+
+def paged_host():
+    """host(), with the paged cache's functions bound too."""
+    global _paged_host
+    if _paged_host is None:
+        h, L = host(), lib()
+        if h is not _GeneralPath:
+            h.bind_paged(*(ctypes.cast(getattr(L, n), _P).value for n in (
+                "fvsr_kv_append_workspace_floats", "fvsr_kv_append",
+                "fvsr_paged_attn_workspace_floats", "fvsr_paged_attn")))
+        _paged_host = h
+    return _paged_host
 
 
 def check(rc: int, what: str):

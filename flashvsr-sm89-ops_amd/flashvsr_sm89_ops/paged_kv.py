@@ -165,6 +165,11 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     does not count); if the page already holds tokens, the scale never falls, and where it
     grows their codes are rounded again.  Sequences that append must not share the
     pages they append to."""
+    r = (_lib._paged_host or _lib.paged_host()).append_kv(
+        pages, k, v, page_table, lengths, cu_tokens, freqs_cis, positions, k_weight, q, q_weight,
+        eps)
+    if r is not None:
+        return None if r is True else r
     name = "append_kv"
     T = k.shape[0]
     H, D = _check_cache(name, pages, page_table, lengths, cu_tokens, T)
@@ -241,6 +246,11 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor,
     id outside the pool makes the rows that read it NaN; what a mask hides, or lies
     behind a length, does not count even if it is NaN.  Logits and sums are fp32;
     the weights count with q's precision."""
+    if out is None:
+        r = (_lib._paged_host or _lib.paged_host()).paged_attention(
+            q, pages, page_table, lengths, cu_tokens, causal, keep, sm_scale)
+        if r is not None:
+            return r
     name = "paged_attention"
     _check(q.dim() == 3, f"{name}: q must be [T, heads, head_dim], got {tuple(q.shape)}")
     T, Hq = q.shape[:2]
