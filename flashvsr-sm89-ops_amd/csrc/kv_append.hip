@@ -21,6 +21,7 @@
 // statistics come from a launch before (which also does q), or, for a few
 // tokens, each workgroup sums its own rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_pages.h"
 
@@ -37,27 +38,45 @@ struct Args {
   const int32_t* positions;  // row of cs for each token; null: the token's own number
   float* row_stat;           // 1/rms of each k row (row norm, from the launch before)
   int64_t k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, cs_rows;
-  int T, q_heads, k_norm, q_norm, w_dt, units_max, page_wgs;
+  int T, q_heads, k_norm, q_norm, w_dt, units, units_max, page_wgs;
   float eps;
 };
 
-// Eight consecutive elements as fp32 (16-byte aligned).
-FVSR_DEV void load8(const void* p, int dt, int64_t i, float (&x)[8]) {
-  if (dt == FVSR_DT_F32) {
-    const f32x4_t* s = (const f32x4_t*)((const float*)p + i);
-    const f32x4_t a = s[0], b = s[1];
+// Eight consecutive elements as they lie in memory (16-byte aligned).
+template <int DT>
+struct Raw8 {
+  u32x4_t w[DT == FVSR_DT_F32 ? 2 : 1];
+};
+template <int DT>
+FVSR_DEV Raw8<DT> load_raw(const void* p, int64_t i) {
+  const u32x4_t* s = (const u32x4_t*)((const uint8_t*)p + i * (DT == FVSR_DT_F32 ? 4 : 2));
+  Raw8<DT> r;
+  r.w[0] = s[0];
+  if constexpr (DT == FVSR_DT_F32) r.w[1] = s[1];
+  return r;
+}
+template <int DT>
+FVSR_DEV void widen(const Raw8<DT>& r, float (&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-  } else if (dt == FVSR_DT_F16) {
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    const h8 a = *(const h8*)((const _Float16*)p + i);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (float)a[e];
-  } else {
-    const u32x4_t a = *(const u32x4_t*)((const uint16_t*)p + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[2 * e] = bf_lo(a[e]), x[2 * e + 1] = bf_hi(a[e]);
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (DT == FVSR_DT_F32) {
+      x[e] = __uint_as_float(r.w[e >> 2][e & 3]);
+    } else {
+      const uint32_t u = r.w[0][e >> 1];
+      if constexpr (DT == FVSR_DT_F16)
+        x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? u >> 16 : u));
+      else
+        x[e] = e & 1 ? bf_hi(u) : bf_lo(u);
+    }
   }
+}
+FVSR_DEV void load8(const void* p, int dt, int64_t i, float (&x)[8]) {
+  if (dt == FVSR_DT_F32)
+    widen(load_raw<FVSR_DT_F32>(p, i), x);
+  else if (dt == FVSR_DT_F16)
+    widen(load_raw<FVSR_DT_F16>(p, i), x);
+  else
+    widen(load_raw<FVSR_DT_BF16>(p, i), x);
 }
 
 FVSR_DEV void store8(void* p, int dt, int64_t i, const float (&x)[8]) {
@@ -201,11 +220,8 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args a) {
 // 1.75 * 2^8, so a mantissa above 1.75 carries into the exponent.
 FVSR_DEV int scale_exp(uint32_t top) { return max((int)((top + 0x1fffffu) >> 23) - 135, -126); }
 
-FVSR_DEV uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-FVSR_DEV uint32_t finite_mag(float x) {
-  const uint32_t m = mag(x);
-  return m < 0x7f800000u ? m : 0u;
+FVSR_DEV float finite_abs(float x) {
+  return fabsf(x) < __builtin_huge_valf() ? fabsf(x) : 0.0f;  // infinity, NaN: 0
 }
 
 // Four held codes at another scale: exact but for results below 2^-6.
@@ -218,15 +234,28 @@ FVSR_DEV uint32_t rescale4(uint32_t w, float f) {
 
 FVSR_DEV float pow2(int e) { return __builtin_ldexpf(1.0f, e); }
 
+// Four values / f (a power of two) as e4m3; infinities and NaN give NaN.
+FVSR_DEV uint32_t codes4(float a, float b, float c, float d, float f) {
+  typedef short v2s __attribute__((ext_vector_type(2)));
+  v2s t = {};
+  t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, a, b, f, false);
+  t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, c, d, f, true);
+  return __builtin_bit_cast(uint32_t, t);
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   if ((int)blockIdx.x >= a.page_wgs) return q_rows<DT, D>(a, blockIdx.x - a.page_wgs);
   constexpr int C = D / 8;                  // threads of a token
   constexpr int R = kPage / (kThreads / C);  // tokens of a thread: 8 (D = 128) or 4
-  __shared__ uint8_t vt[D * kPage];          // v's codes, [dim][token]
+  __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
   __shared__ float stat[kPage];
-  __shared__ uint32_t tops[4][2];
-  const int H = (int)a.c.heads, h = blockIdx.x % H, unit = blockIdx.x / H;
+  __shared__ float tops[4][2];
+  // A page's heads share the rotations of its tokens: they take one XCD's
+  // L2 (workgroups go round robin over the 8).
+  const int H = (int)a.c.heads, turn = blockIdx.x / 8;
+  const int h = turn % H, unit = turn / H * 8 + blockIdx.x % 8;
+  if (unit >= a.units) return;
   const int tid = threadIdx.x, wave = tid >> 6;
 
   SeqPart s;
@@ -269,50 +298,87 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   float w[8] = {};
   if (a.k_norm == kHead) load8(a.k_weight, a.w_dt, d0, w);
   if (a.k_norm == kRow) load8(a.k_weight, a.w_dt, h * D + d0, w);
-  float x[R][8], y[R][8];
-  uint32_t kt = 0, vtop = 0;
+  float x[R][8];
+  Raw8<DT> raw[R];  // v
+  float kt = 0.0f, vtop = 0.0f;
+  const int64_t k0 = (int64_t)h * a.k_hs + d0, v0 = (int64_t)h * a.v_hs + d0;
+  const auto live = [&](int i) { return slot0 + i >= lo && slot0 + i < hi; };
+  // `full`: every slot is new, and all loads go out together.  Otherwise a
+  // wave passes over rows that none of its lanes has.
+  const auto take = [&](auto full) {
+    Raw8<DT> kr[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int slot = slot0 + i;
-    const bool live = slot >= lo && slot < hi;
-    const int t = row0 + (live ? slot : lo);  // others: a token that exists, as zeros
-    float cs[8] = {};
-    load8(a.k, DT, t * a.k_ts + h * a.k_hs + d0, x[i]);
-    load8(a.v, DT, t * a.v_ts + h * a.v_hs + d0, y[i]);
-    if (a.cs) load_turn<D>(a, t, d0, cs);
-    float r = 1.0f;
-    if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
-    if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - row0];
-    norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
-    if (!live) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = y[i][e] = 0.0f;
+    for (int i = 0; i < R; ++i) {
+      kr[i] = Raw8<DT>{}, raw[i] = Raw8<DT>{};
+      if (full || live(i)) {
+        kr[i] = load_raw<DT>(a.k, (int64_t)(row0 + slot0 + i) * a.k_ts + k0);
+        raw[i] = load_raw<DT>(a.v, (int64_t)(row0 + slot0 + i) * a.v_ts + v0);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      kt = max(kt, finite_mag(x[i][e]));
-      vtop = max(vtop, finite_mag(y[i][e]));
+    for (int i = 0; i < R; ++i) {
+      widen(kr[i], x[i]);
+      if (!full && __ballot(live(i)) == 0) continue;
+      const int t = row0 + (full || live(i) ? slot0 + i : lo);
+      float cs[8] = {};
+      if (a.cs) load_turn<D>(a, t, d0, cs);
+      float r = 1.0f;
+      if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
+      if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - row0];
+      norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
+      if (!full && !live(i)) {  // (a NaN position's turn of zeros, or nothing)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+      }
+      float y[8];
+      widen(raw[i], y);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        kt = max3_abs(kt, x[i][e], x[i][e + 1]);
+        vtop = max3_abs(vtop, y[e], y[e + 1]);
+      }
     }
+  };
+  if (lo == 0 && hi == kPage)
+    take(std::true_type{});
+  else
+    take(std::false_type{});
+  // The largest magnitudes (NaN passed over).  An infinity among them: again,
+  // over the finite ones.
+  const auto reduce = [&] {
+    kt = wave_max_abs(kt), vtop = wave_max_abs(vtop);
+    if ((tid & 63) == 0) tops[wave][0] = kt, tops[wave][1] = vtop;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kt = fmaxf(kt, tops[i][0]), vtop = fmaxf(vtop, tops[i][1]);
+  };
+  reduce();
+  if (__builtin_isinf(fmaxf(kt, vtop))) {
+    kt = vtop = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float y[8];
+      widen(raw[i], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        kt = fmaxf(kt, finite_abs(x[i][e])), vtop = fmaxf(vtop, finite_abs(y[e]));
+    }
+    __syncthreads();
+    reduce();
   }
-  kt = __float_as_uint(wave_max_abs(__uint_as_float(kt)));
-  vtop = __float_as_uint(wave_max_abs(__uint_as_float(vtop)));
-  if ((tid & 63) == 0) tops[wave][0] = kt, tops[wave][1] = vtop;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) kt = max(kt, tops[i][0]), vtop = max(vtop, tops[i][1]);
-  int ke = scale_exp(kt), ve = scale_exp(vtop);
+  int ke = scale_exp(__float_as_uint(kt)), ve = scale_exp(__float_as_uint(vtop));
   if (lo > 0) ke = max(ke, k_old), ve = max(ve, v_old);
   if (tid == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
 
   uint8_t* const kp = (uint8_t*)a.c.k + ph * kPage * D;
-  const float kf = pow2(-ke), vf = pow2(-ve);
+  const float kf = pow2(ke), vf = pow2(ve);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int slot = slot0 + i;
     u32x2_t* const p = (u32x2_t*)(kp + slot * D + d0);
     if (slot >= lo && slot < hi) {
-      *p = u32x2_t{e4m3x4(x[i][0] * kf, x[i][1] * kf, x[i][2] * kf, x[i][3] * kf),
-                   e4m3x4(x[i][4] * kf, x[i][5] * kf, x[i][6] * kf, x[i][7] * kf)};
+      *p = u32x2_t{codes4(x[i][0], x[i][1], x[i][2], x[i][3], kf),
+                   codes4(x[i][4], x[i][5], x[i][6], x[i][7], kf)};
     } else if (slot < lo && ke != k_old) {
       const u32x2_t c = *p;
       *p = u32x2_t{rescale4(c[0], pow2(k_old - ke)), rescale4(c[1], pow2(k_old - ke))};
@@ -323,13 +389,14 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   // over the banks.
   const auto vt_at = [&](int d, int u) { return vt + d * kPage + (u ^ ((d >> 3) & 15)) * R; };
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    uint32_t c[2];
+  for (int g = 0; g < R / 4; ++g) {
+    float y[4][8];
 #pragma unroll
-    for (int g = 0; g < R / 4; ++g)
-      c[g] = e4m3x4(y[4 * g][e] * vf, y[4 * g + 1][e] * vf, y[4 * g + 2][e] * vf,
-                    y[4 * g + 3][e] * vf);
-    __builtin_memcpy(__builtin_assume_aligned(vt_at(d0 + e, slot0 / R), R), c, R);
+    for (int i = 0; i < 4; ++i) widen(raw[4 * g + i], y[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *(uint32_t*)(vt_at(d0 + e, slot0 / R) + 4 * g) =
+          codes4(y[0][e], y[1][e], y[2][e], y[3][e], vf);
   }
   __syncthreads();
   uint8_t* const vp = (uint8_t*)a.c.v + ph * kPage * D;
@@ -371,13 +438,147 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   }
 }
 
+// Two neighbouring elements as fp32.
+template <int DT>
+FVSR_DEV void load2(const void* p, int64_t i, float (&x)[2]) {
+  if constexpr (DT == FVSR_DT_F32) {
+    const float* s = (const float*)p + i;
+    x[0] = s[0], x[1] = s[1];
+  } else {
+    const uint32_t u = *(const uint32_t*)((const uint16_t*)p + i);
+    if constexpr (DT == FVSR_DT_F16) {
+      x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+      x[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+    } else {
+      x[0] = bf_lo(u), x[1] = bf_hi(u);
+    }
+  }
+}
+
+// The step of one token per sequence: a wave per (sequence, head), of k and v
+// or of q, two dims a lane (64 dims: the upper lanes repeat the lower ones).  It is
+// all latency: the row, lengths and positions load at once, then the page id and
+// the rotation, then the page's scales; a norm over the row is summed by
+// every wave for itself.  A page whose scale grows (rare: a power of two) has its held
+// codes rounded again by the wave.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
+  const int lane = threadIdx.x & 63, d0 = lane * 2 % D;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int H = (int)a.c.heads, unit = blockIdx.x * 4 + wave;
+  if (unit >= a.T * (H + a.q_heads)) return;
+  const bool is_q = unit >= a.T * H;
+  const int heads = is_q ? a.q_heads : H, u = is_q ? unit - a.T * H : unit;
+  const int t = u / heads, h = u % heads;
+  const int len = is_q ? 0 : max(a.c.lengths[t], 0);
+  const int64_t ts = is_q ? a.q_ts : a.k_ts, hs = is_q ? a.q_hs : a.k_hs;
+  const void* const src = is_q ? a.q : a.k;
+  const int norm = is_q ? a.q_norm : a.k_norm;
+  float x[2], y[2] = {}, cs[2] = {1.0f, 0.0f};
+  load2<DT>(src, t * ts + h * hs + d0, x);
+  if (!is_q) load2<DT>(a.v, t * a.v_ts + h * a.v_hs + d0, y);
+  if (a.cs) {
+    const int64_t p = a.positions ? (int64_t)a.positions[t] : t;
+    if (p >= 0 && p < a.cs_rows)
+      cs[0] = a.cs[p * D + d0], cs[1] = a.cs[p * D + d0 + 1];
+    else
+      cs[0] = cs[1] = __builtin_nanf("");
+  }
+  if (norm != kNone) {
+    const void* const wp = is_q ? a.q_weight : a.k_weight;
+    const int64_t w0 = (norm == kRow ? h * D : 0) + d0;
+    const float sq = norm == kRow ? row_sq<DT, D>(src, t * ts, hs, heads)
+                                  : wave_sum(lane * 2 < D ? x[0] * x[0] + x[1] * x[1] : 0.0f);
+    const float r = inv_rms(sq, norm == kRow ? heads * D : D, a.eps);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = x[e] * r * ld_elem(wp, a.w_dt, w0 + e);
+  }
+  if (a.cs) {
+    const float b = x[0];
+    x[0] = __builtin_fmaf(b, cs[0], -(x[1] * cs[1]));
+    x[1] = __builtin_fmaf(b, cs[1], x[1] * cs[0]);
+  }
+  if (is_q) {
+    if (lane * 2 < D) {
+      const int64_t o = (int64_t)u * D + d0;
+      if constexpr (DT == FVSR_DT_F32) {
+        ((float*)a.q_out)[o] = x[0], ((float*)a.q_out)[o + 1] = x[1];
+      } else {
+        const uint32_t c =
+            DT == FVSR_DT_F16
+                ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[0]) |
+                      (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[1]) << 16
+                : pack_bf16x2(x[0], x[1]);
+        *(uint32_t*)((uint16_t*)a.q_out + o) = c;
+      }
+    }
+    return;
+  }
+  const int page = (len - 1) / kPage, slot = (len - 1) % kPage;
+  if (len == 0 || page >= a.c.table_pages) return;
+  const int64_t id = __builtin_amdgcn_readfirstlane(a.c.table[t * a.c.table_stride + page]);
+  if (id < 0 || id >= a.c.pages) return;
+  const int64_t ph = id * H + h;
+  uint8_t* const ksp = (uint8_t*)a.c.k_scale + ph;
+  uint8_t* const vsp = (uint8_t*)a.c.v_scale + ph;
+  const int k_old = *ksp - 127, v_old = *vsp - 127;
+  int ke = scale_exp(__float_as_uint(wave_max_abs(fmaxf(finite_abs(x[0]), finite_abs(x[1])))));
+  int ve = scale_exp(__float_as_uint(wave_max_abs(fmaxf(finite_abs(y[0]), finite_abs(y[1])))));
+  if (slot > 0) ke = max(ke, k_old), ve = max(ve, v_old);
+  uint8_t* const kp = (uint8_t*)a.c.k + ph * kPage * D;
+  uint8_t* const vp = (uint8_t*)a.c.v + ph * kPage * D;
+  if (slot > 0 && (ke != k_old || ve != v_old)) {
+    if (ke != k_old) {
+      const float f = pow2(k_old - ke);
+      for (int c = lane; c < slot * (D / 16); c += 64) {
+        u32x4_t* const p = (u32x4_t*)(kp + c * 16);
+        u32x4_t o = *p;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) o[g] = rescale4(o[g], f);
+        *p = o;
+      }
+    }
+    if (ve != v_old) {
+      const float f = pow2(v_old - ve);
+      const int per = (slot + 15) / 16;  // pieces of a dim with held tokens
+      for (int c = lane; c < D * per; c += 64) {
+        const int s0 = c % per * 16;
+        u32x4_t* const p = (u32x4_t*)(vp + c / per * kPage + s0);
+        u32x4_t o = *p;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int held = min(max(slot - s0 - 4 * g, 0), 4);  // of these four
+          const uint32_t m = held == 4 ? ~0u : (1u << (8 * held)) - 1;
+          o[g] = (rescale4(o[g], f) & m) | (o[g] & ~m);
+        }
+        *p = o;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // before the new token goes into the same pieces
+  }
+  if (lane * 2 < D) {
+    *(uint16_t*)(kp + slot * D + d0) = (uint16_t)codes4(x[0], x[1], 0.0f, 0.0f, pow2(ke));
+    const uint32_t c = codes4(y[0], y[1], 0.0f, 0.0f, pow2(ve));
+    vp[d0 * kPage + slot] = (uint8_t)c;
+    vp[(d0 + 1) * kPage + slot] = (uint8_t)(c >> 8);
+    if (lane == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
+  }
+}
+
 // Tokens up to which each workgroup sums its own rows for a row norm.
 constexpr int64_t kOwnStat = 64;
 
 template <int DT, int D>
 void launch(const Args& a, int64_t units, hipStream_t st) {
+  if (!a.c.cu && a.T == a.c.sequences) {
+    const int64_t waves = a.T * (a.c.heads + a.q_heads);
+    hipLaunchKernelGGL((kv_token_kernel<DT, D>), dim3((unsigned)((waves + 3) / 4)), dim3(kThreads),
+                       0, st, a);
+    return;
+  }
   Args b = a;
-  b.page_wgs = (int)(units * a.c.heads);
+  b.units = (int)units;
+  b.page_wgs = (int)((units + 7) / 8 * 8 * a.c.heads);
   const int64_t q_wgs = !a.q                ? 0
                         : a.q_norm == kRow ? (a.T + 3) / 4
                                            : ((int64_t)a.T * a.q_heads * (D / 8) + kThreads - 1) / kThreads;
@@ -436,13 +637,13 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   a.cs = cs, a.positions = positions, a.row_stat = need ? workspace : nullptr;
   a.k_ts = k_tok_stride, a.k_hs = k_head_stride, a.v_ts = v_tok_stride, a.v_hs = v_head_stride;
   a.q_ts = q_tok_stride, a.q_hs = q_head_stride, a.cs_rows = cs_rows;
-  a.T = (int)T, a.q_heads = (int)q_heads, a.k_norm = k_norm, a.q_norm = q_norm;
+  a.T = (int)T, a.q_heads = q ? (int)q_heads : 0, a.k_norm = k_norm, a.q_norm = q_norm;
   a.w_dt = weight_dtype, a.eps = eps;
   a.units_max = (int)most(T / B);
   // Packed rows: the sum of those bounds over any B counts that add up to T.
   const int64_t units = cache->cu ? std::min(T, (T + 126 * B) / kPage + B) : B * a.units_max;
   const int64_t q_wgs = q ? (T * q_heads * (D / 8)) / kThreads + T / 4 + 2 : 0;
-  if (units * cache->heads + q_wgs > 0x7fffffff || (q && T * q_heads > 0x7fffffff))
+  if ((units + 7) * cache->heads + q_wgs > 0x7fffffff || (q && T * (cache->heads + q_heads) > 0x7ffffff0))
     return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (D == 128) {

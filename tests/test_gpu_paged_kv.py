@@ -181,6 +181,94 @@ def test_append_tokens(D, H, norm):
         check_append(pages, before, k, v, table, now, None, None, None, kw)
 
 
+@pytest.mark.parametrize("D,Hq,H", [(64, 3, 3), (128, 6, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("norm", ["none", "head", "row"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_token_with_q(D, Hq, H, dtype, norm, packed):
+    """One token for each sequence with q, norms and a rotation, strided columns of one
+    projection; the same as a packed call; a length of 0, a page outside the pool and one
+    past the table."""
+    from flashvsr_sm89_ops import append_kv
+    lengths, g = [1, 128, 129, 77, 0, 200, 500], gen(D)
+    B = len(lengths)
+    table, N = tables(lengths, seed=1)
+    table = table[:, :3].contiguous()
+    table[5, 1] = N
+    pages = pool(N, H, D, seed=2)
+    before = O.from_pages(*pages)
+    qkv = torch.randn(B, Hq + 2 * H, D, generator=g).to(dtype)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + H], qkv[:, Hq + H:]
+    kw = qw = None
+    if norm != "none":
+        kw = 1 + 0.2 * torch.randn(D * (H if norm == "row" else 1), generator=g)
+        qw = 1 + 0.2 * torch.randn(D * (Hq if norm == "row" else 1), generator=g)
+    fr, pos = freqs_of(300, D), i32([0, 127, 128, 76, 5, -3, 300])
+    d = qkv.to(DEV)
+    cu = torch.arange(B + 1).int() if packed else None
+    out = append_kv(pages, d[:, Hq:Hq + H], d[:, Hq + H:], table.to(DEV), i32(lengths).to(DEV),
+                    None if cu is None else cu.to(DEV), freqs_cis=fr.to(DEV),
+                    positions=pos.to(DEV), k_weight=None if kw is None else kw.to(DEV),
+                    q=d[:, :Hq], q_weight=None if qw is None else qw.to(DEV))
+    check_q(out, q, fr, pos, qw)
+    check_append(pages, before, k, v, table, lengths, cu, fr, pos, kw)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_token_special_values(D):
+    """As test_append_special_values, a token at a time."""
+    from flashvsr_sm89_ops import append_kv
+    H, B = 4, 6
+    k, v = (torch.randn(B, H, D, generator=gen(i)) for i in range(2))
+    k[0, 0, 5], k[1, 0, 6], k[2, 0, 7] = math.inf, -math.inf, math.nan
+    k[:, 1] = 0.0
+    k[:, 2] *= 1e-38
+    k[:, 3] *= 1e37
+    v[0] = math.nan
+    v[1] = 0.0
+    v[1, 0, 0], v[1, 1, 1], v[1, 2, 2] = 448.0, 448.0 * (1 + 2.0 ** -23), 3.5 * 2.0 ** -130
+    lengths = [1, 129, 257, 2, 100, 128]
+    table, N = tables(lengths)
+    pages = pool(N, H, D)
+    before = O.from_pages(*pages)
+    append_kv(pages, k.to(DEV), v.to(DEV), table.to(DEV), i32(lengths).to(DEV))
+    check_append(pages, before, k, v, table, lengths, None, None, None, None)
+
+
+def test_native_and_general_path(monkeypatch):
+    """The native host path serves the calls above and gives what the general one does."""
+    from flashvsr_sm89_ops import _lib, append_kv, paged_attention
+    H, D, B = 2, 128, 3
+    table, N = tables([400] * B)
+    q, k, v = (torch.randn(B * 7, h, D, generator=gen(h + i)).bfloat16().to(DEV)
+               for i, h in enumerate((4, H, H)))
+    w = torch.ones(H * D, device=DEV)
+    fr, keep = freqs_of(30, D).to(DEV), torch.rand(B, 4, 1, 4, generator=gen(1)).lt(0.7).to(DEV)
+    host, got = _lib.paged_host(), []
+    assert host is not _lib._GeneralPath
+    for general in (False, True):
+        monkeypatch.setattr(_lib, "_paged_host", _lib._GeneralPath if general else host)
+        pages = pool(N, H, D)
+        t, n = table.to(DEV), i32([400, 300, 20]).to(DEV)
+        r = [append_kv(pages, k, v, t, n, freqs_cis=fr, k_weight=w, q=q)]
+        assert append_kv(pages, k, v, t, n) is None
+        r += [paged_attention(q, pages, t, n), paged_attention(q, pages, t, n, keep=keep),
+              paged_attention(q[:3], pages, t, n, causal=False, sm_scale=0.3)]
+        got.append([x.view(torch.uint8) for x in (*r, *pages)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    monkeypatch.setattr(_lib, "_paged_host", host)
+    c = (pages, k, v, t, n, None, fr, None, w, q, None, 1e-6)
+    assert host.append_kv(*c).shape == q.shape and host.append_kv(*c[:9], None, None, 1e-6) is True
+    assert host.paged_attention(q, pages, t, n, None, True, keep, None).shape == q.shape
+    for i, bad in ((1, k.float()), (2, v[:5]), (3, t.long()), (4, n[:2]), (6, fr[:5]), (6, fr.T),
+                   (7, n), (8, w[:5]), (9, q.half()), (0, pages[:3]), (1, k.cpu())):
+        assert host.append_kv(*c[:i], bad, *c[i + 1:]) is None, i
+    c = (q, pages, t, n, None, True, keep, None)
+    for i, bad in ((0, q.float()), (0, q[:, :, :64]), (2, t[:2]), (4, n), (6, keep[:2]),
+                   (6, keep.int()), (7, 0.0), (7, -1.0)):
+        assert host.paged_attention(*c[:i], bad, *c[i + 1:]) is None, i
+
+
 def test_append_long_row_norm():
     """Enough tokens that the rows' statistics have a launch of their own, without q; and
     no rotation of a table, row t of it by default."""
