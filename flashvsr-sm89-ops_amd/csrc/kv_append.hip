@@ -13,9 +13,9 @@
 // neighbours (2i, 2i + 1), as fvsr_rms_rope does, and nothing is rounded between
 // the norm and the code (q: the output).
 //
-// One workgroup per (page, head): a page's scale needs all of its new tokens at
-// once, and 128 x 128 values of k and v fit its registers, so k and v are read
-// once.  Thread t holds dims 8*(t % (D/8)).. of R consecutive tokens; v's codes
+// One workgroup per (page, head) and k or v: a page's scale needs all of its new
+// tokens at once, and 128 x 128 values fit a workgroup's registers, so they are
+// read once.  Thread t holds dims 8*(t % (D/8)).. of R consecutive tokens; v's codes
 // turn to [dim][token] through LDS.  The q rows are further workgroups of the
 // same launch.  An RMSNorm over whole rows needs other heads' values: the rows'
 // statistics come from a launch before (which also does q), or, for a few
@@ -243,20 +243,217 @@ FVSR_DEV uint32_t codes4(float a, float b, float c, float d, float f) {
   return __builtin_bit_cast(uint32_t, t);
 }
 
+// A page's new tokens: slots lo .. hi - 1, slot 0 being row row0 of the call; ph: (page id, head).
+struct Job {
+  int lo, hi, row0, h;
+  int64_t ph;
+};
+
+// Threads of a token, and consecutive tokens of a thread: 16 and 8, or 8 and 4.
+template <int D>
+constexpr int kLanes = D / 8;
+template <int D>
+constexpr int kTokens = kPage / (kThreads / kLanes<D>);
+
+// The largest of all threads' magnitudes (not NaN), as bits.  An infinity among
+// them: once more over the finite ones, of which again() gives a thread's largest.
+template <class Again>
+FVSR_DEV uint32_t page_top(float top, float (&lds)[4], Again again) {
+  const auto reduce = [&](float t) {
+    t = wave_max_abs(t);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = t;
+    __syncthreads();
+    return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  };
+  top = reduce(top);
+  if (__builtin_isinf(top)) {
+    __syncthreads();
+    top = reduce(again());
+  }
+  return __float_as_uint(top);
+}
+
+// Runs body(full): true if every slot of the page is new and its rows can load
+// together, else with a test of each row.
+template <class Body>
+FVSR_DEV void rows_of(const Job& j, Body body) {
+  if (j.lo == 0 && j.hi == kPage)
+    body(std::true_type{});
+  else
+    body(std::false_type{});
+}
+
+template <int DT, int D>
+FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float (&tops)[4]) {
+  constexpr int C = kLanes<D>, R = kTokens<D>;
+  const int tid = threadIdx.x, H = (int)a.c.heads;
+  uint8_t* const sp = (uint8_t*)a.c.k_scale + j.ph;
+  const int old = *sp - 127;
+  // Row norms that no launch before has summed: a wave per token.
+  if (a.k_norm == kRow && !a.row_stat) {
+    for (int i = j.lo + (tid >> 6); i < j.hi; i += 4) {
+      const float r = inv_rms(row_sq<DT, D>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
+      if ((tid & 63) == 0) stat[i] = r;
+    }
+    __syncthreads();
+  }
+  const int d0 = (tid % C) * 8, slot0 = tid / C * R;
+  float w[8] = {};
+  if (a.k_norm != kNone) load8(a.k_weight, a.w_dt, (a.k_norm == kRow ? j.h * D : 0) + d0, w);
+  float x[R][8];
+  float top = 0.0f;
+  rows_of(j, [&](auto full) {
+    const auto live = [&](int i) { return full || (slot0 + i >= j.lo && slot0 + i < j.hi); };
+    Raw8<DT> raw[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      raw[i] = Raw8<DT>{};
+      if (live(i))
+        raw[i] = load_raw<DT>(a.k, (int64_t)(j.row0 + slot0 + i) * a.k_ts + j.h * a.k_hs + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      widen(raw[i], x[i]);
+      if (!full && __ballot(live(i)) == 0) continue;
+      const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
+      float cs[8] = {};
+      if (a.cs) load_turn<D>(a, t, d0, cs);
+      float r = 1.0f;
+      if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
+      if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - j.row0];
+      norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
+      if (!live(i)) continue;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) top = max3_abs(top, x[i][e], x[i][e + 1]);
+    }
+  });
+  int e = scale_exp(page_top(top, tops, [&] {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (slot0 + i >= j.lo && slot0 + i < j.hi) t = fmaxf(t, finite_abs(x[i][k]));
+    return t;
+  }));
+  if (j.lo > 0) e = max(e, old);
+  if (tid == 0) *sp = (uint8_t)(e + 127);
+  uint8_t* const page = (uint8_t*)a.c.k + j.ph * kPage * D;
+  const float f = pow2(e);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int slot = slot0 + i;
+    u32x2_t* const p = (u32x2_t*)(page + slot * D + d0);
+    if (slot >= j.lo && slot < j.hi) {
+      *p = u32x2_t{codes4(x[i][0], x[i][1], x[i][2], x[i][3], f),
+                   codes4(x[i][4], x[i][5], x[i][6], x[i][7], f)};
+    } else if (slot < j.lo && e != old) {
+      const u32x2_t c = *p;
+      *p = u32x2_t{rescale4(c[0], pow2(old - e)), rescale4(c[1], pow2(old - e))};
+    }
+  }
+}
+
+template <int DT, int D>
+FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4]) {
+  constexpr int C = kLanes<D>, R = kTokens<D>;
+  const int tid = threadIdx.x;
+  uint8_t* const sp = (uint8_t*)a.c.v_scale + j.ph;
+  const int old = *sp - 127;
+  const int d0 = (tid % C) * 8, slot0 = tid / C * R;
+  Raw8<DT> raw[R];
+  float top = 0.0f;
+  rows_of(j, [&](auto full) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      raw[i] = Raw8<DT>{};
+      if (full || (slot0 + i >= j.lo && slot0 + i < j.hi))
+        raw[i] = load_raw<DT>(a.v, (int64_t)(j.row0 + slot0 + i) * a.v_ts + j.h * a.v_hs + d0);
+    }
+  });
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    float y[8];
+    widen(raw[i], y);
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) top = max3_abs(top, y[k], y[k + 1]);
+  }
+  int e = scale_exp(page_top(top, tops, [&] {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float y[8];
+      widen(raw[i], y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t = fmaxf(t, finite_abs(y[k]));
+    }
+    return t;
+  }));
+  if (j.lo > 0) e = max(e, old);
+  if (tid == 0) *sp = (uint8_t)(e + 127);
+  // [dim][token]: a thread's R tokens of a dim are one unit of R bytes; unit u
+  // of row d sits at u ^ (d / 8 % 16), so that the D/8 threads of a token spread
+  // over the banks.
+  const auto vt_at = [&](int d, int u) { return vt + d * kPage + (u ^ ((d >> 3) & 15)) * R; };
+  const float f = pow2(e);
+#pragma unroll
+  for (int g = 0; g < R / 4; ++g) {
+    float y[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) widen(raw[4 * g + i], y[i]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      *(uint32_t*)(vt_at(d0 + k, slot0 / R) + 4 * g) =
+          codes4(y[0][k], y[1][k], y[2][k], y[3][k], f);
+  }
+  __syncthreads();
+  uint8_t* const page = (uint8_t*)a.c.v + j.ph * kPage * D;
+#pragma unroll
+  for (int it = 0; it < D * (kPage / 16) / kThreads; ++it) {
+    const int idx = it * kThreads + tid, d = idx / (kPage / 16), s0 = idx % (kPage / 16) * 16;
+    const bool grow = s0 < j.lo && e != old;  // held codes to round again
+    if ((s0 + 16 <= j.lo && !grow) || s0 >= j.hi) continue;
+    u32x4_t c;
+#pragma unroll
+    for (int g = 0; g < 16 / R; ++g)
+      __builtin_memcpy((uint8_t*)&c + g * R,
+                       __builtin_assume_aligned(vt_at(d, s0 / R + g), R), R);
+    uint8_t* const p = page + d * kPage + s0;
+    if (s0 >= j.lo && s0 + 16 <= j.hi) {
+      *(u32x4_t*)p = c;
+    } else if (grow) {
+      u32x4_t o = *(const u32x4_t*)p;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t n = rescale4(o[g], pow2(old - e));
+        uint32_t m = 0, keep = 0;  // bytes of new tokens; bytes behind them
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int slot = s0 + 4 * g + k;
+          if (slot >= j.hi) keep |= 0xffu << (8 * k);
+          else if (slot >= j.lo) m |= 0xffu << (8 * k);
+        }
+        o[g] = (c[g] & m) | (o[g] & keep) | (n & ~(m | keep));
+      }
+      *(u32x4_t*)p = o;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (s0 + k >= j.lo && s0 + k < j.hi) p[k] = (uint8_t)(c[k >> 2] >> (8 * (k & 3)));
+    }
+  }
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   if ((int)blockIdx.x >= a.page_wgs) return q_rows<DT, D>(a, blockIdx.x - a.page_wgs);
-  constexpr int C = D / 8;                  // threads of a token
-  constexpr int R = kPage / (kThreads / C);  // tokens of a thread: 8 (D = 128) or 4
   __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
-  __shared__ float stat[kPage];
-  __shared__ float tops[4][2];
+  __shared__ float stat[kPage], tops[4];
   // A page's heads share the rotations of its tokens: they take one XCD's
   // L2 (workgroups go round robin over the 8).
   const int H = (int)a.c.heads, turn = blockIdx.x / 8;
-  const int h = turn % H, unit = turn / H * 8 + blockIdx.x % 8;
+  const int part = turn % (2 * H), unit = turn / (2 * H) * 8 + blockIdx.x % 8;
   if (unit >= a.units) return;
-  const int tid = threadIdx.x, wave = tid >> 6;
 
   SeqPart s;
   const auto pages_of = [](int n, int len) {
@@ -272,170 +469,21 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
     s.len = max(a.c.lengths[s.b], 0);
     if (s.part >= pages_of(s.rows.n, s.len)) return;
   }
-  const int at = s.len - s.rows.n;                  // position of the sequence's first new token
+  const int at = s.len - s.rows.n;          // position of the sequence's first new token
   const int page = max(at, 0) / kPage + s.part;
-  if (page >= a.c.table_pages) return;              // past the table: dropped
-  const int lo = max(max(at, 0), page * kPage) - page * kPage;
-  const int hi = min(s.len - page * kPage, kPage);  // new tokens: slots lo .. hi - 1
+  if (page >= a.c.table_pages) return;      // past the table: dropped
   const int64_t id = a.c.table[s.b * a.c.table_stride + page];
-  if (id < 0 || id >= a.c.pages) return;            // no such page: dropped
-  const int row0 = s.rows.lo + page * kPage - at;   // token of slot 0
-  const int64_t ph = id * H + h;
-  uint8_t* const ksp = (uint8_t*)a.c.k_scale + ph;
-  uint8_t* const vsp = (uint8_t*)a.c.v_scale + ph;
-  const int k_old = *ksp - 127, v_old = *vsp - 127;
-
-  // Row norms that no launch before has summed: a wave per token.
-  if (a.k_norm == kRow && !a.row_stat) {
-    for (int i = lo + wave; i < hi; i += 4) {
-      const float r = inv_rms(row_sq<DT, D>(a.k, (row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
-      if ((tid & 63) == 0) stat[i] = r;
-    }
-    __syncthreads();
-  }
-
-  const int d0 = (tid % C) * 8, slot0 = tid / C * R;
-  float w[8] = {};
-  if (a.k_norm == kHead) load8(a.k_weight, a.w_dt, d0, w);
-  if (a.k_norm == kRow) load8(a.k_weight, a.w_dt, h * D + d0, w);
-  float x[R][8];
-  Raw8<DT> raw[R];  // v
-  float kt = 0.0f, vtop = 0.0f;
-  const int64_t k0 = (int64_t)h * a.k_hs + d0, v0 = (int64_t)h * a.v_hs + d0;
-  const auto live = [&](int i) { return slot0 + i >= lo && slot0 + i < hi; };
-  // `full`: every slot is new, and all loads go out together.  Otherwise a
-  // wave passes over rows that none of its lanes has.
-  const auto take = [&](auto full) {
-    Raw8<DT> kr[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      kr[i] = Raw8<DT>{}, raw[i] = Raw8<DT>{};
-      if (full || live(i)) {
-        kr[i] = load_raw<DT>(a.k, (int64_t)(row0 + slot0 + i) * a.k_ts + k0);
-        raw[i] = load_raw<DT>(a.v, (int64_t)(row0 + slot0 + i) * a.v_ts + v0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      widen(kr[i], x[i]);
-      if (!full && __ballot(live(i)) == 0) continue;
-      const int t = row0 + (full || live(i) ? slot0 + i : lo);
-      float cs[8] = {};
-      if (a.cs) load_turn<D>(a, t, d0, cs);
-      float r = 1.0f;
-      if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
-      if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - row0];
-      norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
-      if (!full && !live(i)) {  // (a NaN position's turn of zeros, or nothing)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-      }
-      float y[8];
-      widen(raw[i], y);
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        kt = max3_abs(kt, x[i][e], x[i][e + 1]);
-        vtop = max3_abs(vtop, y[e], y[e + 1]);
-      }
-    }
-  };
-  if (lo == 0 && hi == kPage)
-    take(std::true_type{});
+  if (id < 0 || id >= a.c.pages) return;    // no such page: dropped
+  Job j;
+  j.lo = max(max(at, 0), page * kPage) - page * kPage;
+  j.hi = min(s.len - page * kPage, kPage);
+  j.row0 = s.rows.lo + page * kPage - at;
+  j.h = part >> 1;
+  j.ph = id * H + j.h;
+  if (part & 1)
+    append_v<DT, D>(a, j, vt, tops);
   else
-    take(std::false_type{});
-  // The largest magnitudes (NaN passed over).  An infinity among them: again,
-  // over the finite ones.
-  const auto reduce = [&] {
-    kt = wave_max_abs(kt), vtop = wave_max_abs(vtop);
-    if ((tid & 63) == 0) tops[wave][0] = kt, tops[wave][1] = vtop;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) kt = fmaxf(kt, tops[i][0]), vtop = fmaxf(vtop, tops[i][1]);
-  };
-  reduce();
-  if (__builtin_isinf(fmaxf(kt, vtop))) {
-    kt = vtop = 0.0f;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float y[8];
-      widen(raw[i], y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        kt = fmaxf(kt, finite_abs(x[i][e])), vtop = fmaxf(vtop, finite_abs(y[e]));
-    }
-    __syncthreads();
-    reduce();
-  }
-  int ke = scale_exp(__float_as_uint(kt)), ve = scale_exp(__float_as_uint(vtop));
-  if (lo > 0) ke = max(ke, k_old), ve = max(ve, v_old);
-  if (tid == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
-
-  uint8_t* const kp = (uint8_t*)a.c.k + ph * kPage * D;
-  const float kf = pow2(ke), vf = pow2(ve);
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int slot = slot0 + i;
-    u32x2_t* const p = (u32x2_t*)(kp + slot * D + d0);
-    if (slot >= lo && slot < hi) {
-      *p = u32x2_t{codes4(x[i][0], x[i][1], x[i][2], x[i][3], kf),
-                   codes4(x[i][4], x[i][5], x[i][6], x[i][7], kf)};
-    } else if (slot < lo && ke != k_old) {
-      const u32x2_t c = *p;
-      *p = u32x2_t{rescale4(c[0], pow2(k_old - ke)), rescale4(c[1], pow2(k_old - ke))};
-    }
-  }
-  // [dim][token]: a thread's R tokens of a dim are one unit of R bytes; unit u
-  // of row d sits at u ^ (d / 8 % 16), so that the D/8 threads of a token spread
-  // over the banks.
-  const auto vt_at = [&](int d, int u) { return vt + d * kPage + (u ^ ((d >> 3) & 15)) * R; };
-#pragma unroll
-  for (int g = 0; g < R / 4; ++g) {
-    float y[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) widen(raw[4 * g + i], y[i]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      *(uint32_t*)(vt_at(d0 + e, slot0 / R) + 4 * g) =
-          codes4(y[0][e], y[1][e], y[2][e], y[3][e], vf);
-  }
-  __syncthreads();
-  uint8_t* const vp = (uint8_t*)a.c.v + ph * kPage * D;
-#pragma unroll
-  for (int it = 0; it < D * (kPage / 16) / kThreads; ++it) {
-    const int idx = it * kThreads + tid, d = idx / (kPage / 16), s0 = idx % (kPage / 16) * 16;
-    const bool grow = s0 < lo && ve != v_old;  // held codes to round again
-    if ((s0 + 16 <= lo && !grow) || s0 >= hi) continue;
-    u32x4_t c;
-#pragma unroll
-    for (int g = 0; g < 16 / R; ++g)
-      __builtin_memcpy((uint8_t*)&c + g * R,
-                       __builtin_assume_aligned(vt_at(d, s0 / R + g), R), R);
-    uint8_t* const p = vp + d * kPage + s0;
-    if (s0 >= lo && s0 + 16 <= hi) {
-      *(u32x4_t*)p = c;
-      continue;
-    }
-    if (grow) {
-      u32x4_t o = *(const u32x4_t*)p;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t n = rescale4(o[g], pow2(v_old - ve));
-        uint32_t m = 0, keep = 0;  // bytes of new tokens; bytes behind them
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = s0 + 4 * g + e;
-          if (slot >= hi) keep |= 0xffu << (8 * e);
-          else if (slot >= lo) m |= 0xffu << (8 * e);
-        }
-        o[g] = (c[g] & m) | (o[g] & keep) | (n & ~(m | keep));
-      }
-      *(u32x4_t*)p = o;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (s0 + e >= lo && s0 + e < hi) p[e] = (uint8_t)(c[e >> 2] >> (8 * (e & 3)));
-    }
-  }
+    append_k<DT, D>(a, j, stat, tops);
 }
 
 // Two neighbouring elements as fp32.
@@ -578,7 +626,7 @@ void launch(const Args& a, int64_t units, hipStream_t st) {
   }
   Args b = a;
   b.units = (int)units;
-  b.page_wgs = (int)((units + 7) / 8 * 8 * a.c.heads);
+  b.page_wgs = (int)((units + 7) / 8 * 8 * 2 * a.c.heads);
   const int64_t q_wgs = !a.q                ? 0
                         : a.q_norm == kRow ? (a.T + 3) / 4
                                            : ((int64_t)a.T * a.q_heads * (D / 8) + kThreads - 1) / kThreads;
@@ -643,7 +691,7 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   // Packed rows: the sum of those bounds over any B counts that add up to T.
   const int64_t units = cache->cu ? std::min(T, (T + 126 * B) / kPage + B) : B * a.units_max;
   const int64_t q_wgs = q ? (T * q_heads * (D / 8)) / kThreads + T / 4 + 2 : 0;
-  if ((units + 7) * cache->heads + q_wgs > 0x7fffffff || (q && T * (cache->heads + q_heads) > 0x7ffffff0))
+  if ((units + 7) * 2 * cache->heads + q_wgs > 0x7fffffff || (q && T * (cache->heads + q_heads) > 0x7ffffff0))
     return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (D == 128) {
