@@ -127,17 +127,19 @@ FVSR_DEV float row_sq(const void* x, int64_t row, int64_t hs, int H) {
   return wave_sum(s);
 }
 
-// cos and sin of dims d0..d0+7 of token t.  A position outside the table
-// gives NaN instead of a read outside it.
+// A position outside the table gives NaN (every result has a cosine in it).
+FVSR_DEV void outside(int p, int64_t rows, float (&cs)[8]) {
+  const bool in = p >= 0 && p < rows;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) cs[e] = in ? cs[e] : __builtin_nanf("");
+}
+
+// cos and sin of dims d0..d0+7 of token t.
 template <int D>
 FVSR_DEV void load_turn(const Args& a, int t, int d0, float (&cs)[8]) {
-  const int64_t p = a.positions ? (int64_t)a.positions[t] : t;
-  const bool in = p >= 0 && p < a.cs_rows;
-  load8(a.cs, FVSR_DT_F32, (in ? p : 0) * D + d0, cs);
-  if (!in) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) cs[e] = __builtin_nanf("");
-  }
+  const int p = a.positions ? a.positions[t] : t;
+  load8(a.cs, FVSR_DT_F32, (int64_t)(p >= 0 && p < a.cs_rows ? p : 0) * D + d0, cs);
+  outside(p, a.cs_rows, cs);
 }
 
 // x * r * w, then the rotation of its four pairs.
@@ -201,19 +203,6 @@ FVSR_DEV void q_rows(const Args& a, int64_t wg) {
     q_row<DT, D>(a, (int)(wg * 4 + (threadIdx.x >> 6)));
   else
     q_chunk<DT, D>(a, wg * kThreads + threadIdx.x);
-}
-
-// The launch before, for row norms of many tokens: workgroups 0.. the k rows'
-// 1/rms, the rest the q rows.
-template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args a) {
-  const int stat_wgs = (a.T + 3) / 4;
-  if ((int)blockIdx.x >= stat_wgs) return q_rows<DT, D>(a, blockIdx.x - stat_wgs);
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= a.T) return;
-  const int H = (int)a.c.heads;
-  const float r = inv_rms(row_sq<DT, D>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
-  if ((threadIdx.x & 63) == 0) a.row_stat[t] = r;
 }
 
 // Scale exponent of a largest magnitude, given as its (finite) bits: 448 =
@@ -304,7 +293,17 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
   float top = 0.0f;
   rows_of(j, [&](auto full) {
     const auto live = [&](int i) { return full || (slot0 + i >= j.lo && slot0 + i < j.hi); };
+    // All positions and rows go out together, then all rotations: a load
+    // behind a load eight times over took 22 of a 57 us call (16896 tokens x 12 heads).
     Raw8<DT> raw[R];
+    constexpr int Q = 4;  // rotations in flight
+    Raw8<FVSR_DT_F32> turn[Q];
+    int pos[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
+      pos[i] = a.positions ? a.positions[t] : t;
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       raw[i] = Raw8<DT>{};
@@ -313,11 +312,22 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
+      if (a.cs && i % Q == 0) {
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+          const int p = pos[i + k];
+          turn[k] = load_raw<FVSR_DT_F32>(
+              a.cs, (int64_t)(p >= 0 && p < a.cs_rows ? p : 0) * D + d0);
+        }
+      }
       widen(raw[i], x[i]);
       if (!full && __ballot(live(i)) == 0) continue;
       const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
       float cs[8] = {};
-      if (a.cs) load_turn<D>(a, t, d0, cs);
+      if (a.cs) {
+        widen(turn[i % Q], cs);
+        outside(pos[i], a.cs_rows, cs);
+      }
       float r = 1.0f;
       if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
       if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - j.row0];
@@ -444,15 +454,15 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
   }
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
-  if ((int)blockIdx.x >= a.page_wgs) return q_rows<DT, D>(a, blockIdx.x - a.page_wgs);
-  __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
-  __shared__ float stat[kPage], tops[4];
+// Workgroup wg's part of a page: units * heads workgroups, for k and v each if both.
+enum { kKeys = 1, kValues = 2 };
+template <int DT, int D, int KINDS>
+FVSR_DEV void page_part(const Args& a, int wg) {
+  constexpr int n = KINDS == (kKeys | kValues) ? 2 : 1;
   // A page's heads share the rotations of its tokens: they take one XCD's
   // L2 (workgroups go round robin over the 8).
-  const int H = (int)a.c.heads, turn = blockIdx.x / 8;
-  const int part = turn % (2 * H), unit = turn / (2 * H) * 8 + blockIdx.x % 8;
+  const int H = (int)a.c.heads, turn = wg / 8;
+  const int part = turn % (n * H), unit = turn / (n * H) * 8 + wg % 8;
   if (unit >= a.units) return;
 
   SeqPart s;
@@ -478,12 +488,46 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
   j.lo = max(max(at, 0), page * kPage) - page * kPage;
   j.hi = min(s.len - page * kPage, kPage);
   j.row0 = s.rows.lo + page * kPage - at;
-  j.h = part >> 1;
+  j.h = part / n;
   j.ph = id * H + j.h;
-  if (part & 1)
-    append_v<DT, D>(a, j, vt, tops);
-  else
+  __shared__ float tops[4];
+  if constexpr ((KINDS & kValues) != 0) {
+    __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
+    if (n == 1 || part % n) return append_v<DT, D>(a, j, vt, tops);
+  }
+  if constexpr ((KINDS & kKeys) != 0) {
+    __shared__ float stat[kPage];
     append_k<DT, D>(a, j, stat, tops);
+  }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
+  if ((int)blockIdx.x < a.page_wgs)
+    page_part<DT, D, kKeys | kValues>(a, blockIdx.x);
+  else
+    q_rows<DT, D>(a, blockIdx.x - a.page_wgs);
+}
+
+// Row norms of many tokens take two launches: what needs no k statistics (v,
+// the q rows) beside the statistics, then k, read again.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args a) {
+  const int stat_wgs = (a.T + 3) / 4;
+  int wg = blockIdx.x;
+  if (wg < a.page_wgs) return page_part<DT, D, kValues>(a, wg);
+  wg -= a.page_wgs;
+  if (wg >= stat_wgs) return q_rows<DT, D>(a, wg - stat_wgs);
+  const int t = wg * 4 + (threadIdx.x >> 6);
+  if (t >= a.T) return;
+  const int H = (int)a.c.heads;
+  const float r = inv_rms(row_sq<DT, D>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
+  if ((threadIdx.x & 63) == 0) a.row_stat[t] = r;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_keys_kernel(Args a) {
+  page_part<DT, D, kKeys>(a, blockIdx.x);
 }
 
 // Two neighbouring elements as fp32.
@@ -626,18 +670,19 @@ void launch(const Args& a, int64_t units, hipStream_t st) {
   }
   Args b = a;
   b.units = (int)units;
-  b.page_wgs = (int)((units + 7) / 8 * 8 * 2 * a.c.heads);
-  const int64_t q_wgs = !a.q                ? 0
-                        : a.q_norm == kRow ? (a.T + 3) / 4
-                                           : ((int64_t)a.T * a.q_heads * (D / 8) + kThreads - 1) / kThreads;
+  b.page_wgs = (int)((units + 7) / 8 * 8 * a.c.heads) * (a.row_stat ? 1 : 2);
+  const int64_t q_wgs =
+      !a.q                ? 0
+      : a.q_norm == kRow ? (a.T + 3) / 4
+                         : ((int64_t)a.T * a.q_heads * (D / 8) + kThreads - 1) / kThreads;
+  const dim3 block(kThreads);
   if (a.row_stat) {
-    hipLaunchKernelGGL((kv_rows_kernel<DT, D>), dim3((unsigned)((a.T + 3) / 4 + q_wgs)),
-                       dim3(kThreads), 0, st, b);
-    hipLaunchKernelGGL((kv_append_kernel<DT, D>), dim3((unsigned)b.page_wgs), dim3(kThreads), 0,
-                       st, b);
+    hipLaunchKernelGGL((kv_rows_kernel<DT, D>),
+                       dim3((unsigned)(b.page_wgs + (a.T + 3) / 4 + q_wgs)), block, 0, st, b);
+    hipLaunchKernelGGL((kv_keys_kernel<DT, D>), dim3((unsigned)b.page_wgs), block, 0, st, b);
   } else {
-    hipLaunchKernelGGL((kv_append_kernel<DT, D>), dim3((unsigned)(b.page_wgs + q_wgs)),
-                       dim3(kThreads), 0, st, b);
+    hipLaunchKernelGGL((kv_append_kernel<DT, D>), dim3((unsigned)(b.page_wgs + q_wgs)), block, 0,
+                       st, b);
   }
 }
 
