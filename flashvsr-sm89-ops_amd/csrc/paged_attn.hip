@@ -443,116 +443,148 @@ FVSR_DEV int k_swap(int key) {
 }
 FVSR_DEV int v_swap(int d) { return (d >> 1) & 7; }
 
+// A page's K or V codes go into LDS straight from memory, segment s (1 KB) by wave
+// s % 4; the piece that a lane fetches is the one that belongs where it lands.  Offset of a
+// lane's piece in its wave's first segment:
 template <int D>
-struct Stage {
-  static constexpr int kK = kPage * D, kBytes = 2 * kK;
-};
-
-// Streams a page's codes into a stage: segment s (1 KB) by wave s % 4, straight from
-// memory; the piece that a lane fetches is the one that belongs where it lands.
+FVSR_DEV int k_piece(int wave, int lane) {
+  constexpr int KR = D / 16;  // pieces of a row
+  return wave * 1024 + lane / KR * D +
+         ((lane % KR) ^ k_swap<D>(wave * (64 / KR) + lane / KR)) * 16;
+}
+FVSR_DEV int v_piece(int wave, int lane) {
+  return wave * 1024 + lane / 8 * kPage + ((lane % 8) ^ v_swap(wave * 8 + lane / 8)) * 16;
+}
 template <int D>
-FVSR_DEV void stream_page(uint8_t LDS_AS* st, const uint8_t* k, const uint8_t* v, int wave,
-                          int lane) {
-  constexpr int KR = D / 16, S = kPage * D / 1024;  // pieces of a K row; segments
-  const int kr = wave * (64 / KR) + lane / KR;  // K row within segments 0-3, V row likewise
-  const int vr = wave * 8 + lane / 8;
-  const int ko = (lane / KR) * D + ((lane % KR) ^ k_swap<D>(kr)) * 16;
-  const int vo = (lane / 8) * kPage + ((lane % 8) ^ v_swap(vr)) * 16;
+FVSR_DEV void stream(uint8_t LDS_AS* to, const uint8_t* from, int wave, int& piece) {
+  // (Opaque, so that no sum with it is kept in registers from page to page.)
+  asm volatile("" : "+v"(piece));
 #pragma unroll
-  for (int t = 0; t < S / 4; ++t) {
-    const int s = wave + 4 * t;
-    __builtin_amdgcn_global_load_lds(k + s * 1024 + ko, (void LDS_AS*)(st + s * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds(v + s * 1024 + vo,
-                                     (void LDS_AS*)(st + Stage<D>::kK + s * 1024), 16, 0, 0);
-  }
+  for (int t = 0; t < kPage * D / 4096; ++t)
+    __builtin_amdgcn_global_load_lds(from + t * 4096 + piece,
+                                     (void LDS_AS*)(to + wave * 1024 + t * 4096), 16, 0, 0);
 }
 
-// The pages ahead, looked up kList at a time: number in the sequence, id (-1:
-// no such page), K scale | V scale << 8.
+// The pages ahead, looked up kList at a time: first position, id, K scale | V
+// scale << 8.
 constexpr int kList = 512;
 typedef int v4i __attribute__((ext_vector_type(4)));
+struct Listed {
+  int n, whole;  // entries; those that every row of the tile sees whole (the first ones)
+};
 
 // Entries of pages from .. from + kList - 1 below p1 that the block mask's row
-// keeps (null: all), in order; returns their number.  Every wave counts all of
-// them and writes its share.
-FVSR_DEV int list_pages(v4i LDS_AS* list, const Args& a, const int32_t* table, int h,
-                        const uint8_t* keep, int kept, int from, int p1, int wave) {
+// keeps (null: all), in order.  A page id outside the pool has no entry: `bad` is the
+// first position of any.  Every wave counts all pages and writes its share.
+FVSR_DEV Listed list_pages(v4i LDS_AS* list, const Args& a, const int32_t* table, int h,
+                           const uint8_t* keep, int kept, int from, int p1, int seen, int wave,
+                           int& bad) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
+  Listed c{0, 0};
 #pragma unroll 1
   for (int g = 0; g < kList / 64 && from + g * 64 < p1; ++g) {
     const int i = from + g * 64 + lane;
     const bool in = i < p1 && (!keep || (i < kept && keep[i] != 0));
-    const uint64_t word = __ballot(in);
-    if (in && g % 4 == wave) {
-      const int id = table[i];
-      v4i e{i, -1, 0, 0};
-      if (id >= 0 && id < a.c.pages) {
-        const int64_t ph = (int64_t)id * a.c.heads + h;
-        e[1] = id;
-        e[2] = ((const uint8_t*)a.c.k_scale)[ph] | ((const uint8_t*)a.c.v_scale)[ph] << 8;
-      }
-      list[n + __popcll(word & ((1ull << lane) - 1))] = e;
+    const int id = in ? table[i] : 0;
+    const bool there = in && id >= 0 && id < a.c.pages;
+    const uint64_t word = __ballot(there), wrong = __ballot(in && !there);
+    if (wrong) bad = min(bad, (from + g * 64 + __builtin_ctzll(wrong)) * kPage);
+    if (there && g % 4 == wave) {
+      const int64_t ph = (int64_t)id * a.c.heads + h;
+      list[c.n + __popcll(word & ((1ull << lane) - 1))] =
+          v4i{i * kPage, id,
+              ((const uint8_t*)a.c.k_scale)[ph] | ((const uint8_t*)a.c.v_scale)[ph] << 8, 0};
     }
-    n += __popcll(word);
+    c.n += __popcll(word);
+    c.whole += __popcll(__ballot(there && (i + 1) * kPage <= seen));
   }
-  return n;
+  return c;
 }
 
-struct Rows {
-  int limit, lim_lo, lim_hi;  // keys this lane's row sees; least and most of the wave
-};
-
+// One wave's 32 rows.
+//
+// step(): pages that every row sees whole, in a pipeline of half pages (64 keys).
+// Step t turns the logits S of half t into weights P while the matrix cores do O +=
+// V P of half t - 1 and S of half t + 1, so that neither waits for the other even
+// within a wave.  Its steps are one straight block, which is what lets the compiler
+// keep to their order: the reference M stays that of the first half page, and a row that
+// would have to move it is noted (`lost`).  The tile is then done again without the
+// pipeline; it takes a logit 44 above all of that half page's.
+// one(): any page, half by half, with masks, a moving M and NaN codes.
 template <int DT, int D>
-FVSR_DEV void attend_page(const uint8_t LDS_AS* st, int page, bool there, int ks, int vs,
-                          const Rows& rw, float c,
-                          const v8i (&qf)[D / 64][terms(DT)], const int (&qs)[terms(DT)],
-                          v16f (&acc)[D / 32], float& m, float& l) {
-  constexpr int N = terms(DT);
-  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-  const int at = page * kPage;
-  if (at >= rw.lim_hi) return;  // nothing of it is seen by this wave
-  if (!there) {                 // no such page: the rows that would read it are NaN
-    if (at < rw.limit) l = __builtin_nanf("");
-    return;
+struct RowTile {
+  static constexpr int N = terms(DT);
+  v8i qf[D / 64][N];
+  int qs[N];
+  v16f acc[D / 32] = {};
+  float m = kNothing, l = 0.0f;
+  v8i pf[N];       // weights of the half before, and their scale
+  int shift = 0;
+  bool lost = false;
+  int limit, lim_lo;  // keys this lane's row sees; least of the wave
+  float c;
+  int k_at[D / 32], v_at[2];  // this lane's pieces of an operand, half 0
+
+  __device__ __forceinline__ void place() {
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+    // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
+    const int kr = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) k_at[w] = kr * D + (((2 * w + g) ^ k_swap<D>(kr)) << 4);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) v_at[w] = r * kPage + (((2 * w + g) ^ v_swap(r)) << 4);
   }
-  const bool masked = at + kPage > rw.lim_lo;
-  const uint8_t LDS_AS* kt = st;
-  const uint8_t LDS_AS* vt = st + Stage<D>::kK;
-  // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
-  const int kr = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
-#pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    v16f s[2];
+  // Makes the addresses unknown, as in stream().
+  __device__ __forceinline__ void fresh() {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int key = half * 64 + u * 32 + kr, sw = k_swap<D>(key);
-      const v16f z = {};
-      s[u] = z;
+    for (int w = 0; w < D / 32; ++w) asm volatile("" : "+v"(k_at[w]));
+    asm volatile("" : "+v"(v_at[0]), "+v"(v_at[1]));
+  }
+  __device__ __forceinline__ v8i k_operand(const uint8_t LDS_AS* k, int half, int u, int w) const {
+    const uint8_t LDS_AS* p = k + (half * 64 + u * 32) * D;
+    return join(*(const u32x4_t LDS_AS*)(p + k_at[2 * w]),
+                *(const u32x4_t LDS_AS*)(p + k_at[2 * w + 1]));
+  }
+  __device__ __forceinline__ v8i v_operand(const uint8_t LDS_AS* v, int half, int d) const {
+    const uint8_t LDS_AS* p = v + d * 32 * kPage;  // (half 1: piece ^ 4)
+    return join(*(const u32x4_t LDS_AS*)(p + (v_at[0] ^ (half * 64))),
+                *(const u32x4_t LDS_AS*)(p + (v_at[1] ^ (half * 64))));
+  }
+  __device__ __forceinline__ void logits(v16f (&s)[2], const uint8_t LDS_AS* k, int half, int ks) {
 #pragma unroll
-      for (int w = 0; w < D / 64; ++w) {
-        const v8i kf = join(*(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + g) ^ sw) << 4)),
-                            *(const u32x4_t LDS_AS*)(kt + key * D + (((4 * w + 2 + g) ^ sw) << 4)));
+    for (int u = 0; u < 2; ++u) s[u] = v16f{};
 #pragma unroll
-        for (int k = 0; k < N; ++k) s[u] = mfma(kf, qf[w][k], s[u], ks, qs[k]);
+    for (int w = 0; w < D / 64; ++w)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const v8i kf = k_operand(k, half, u, w);
+#pragma unroll
+        for (int t = 0; t < N; ++t) s[u] = mfma(kf, qf[w][t], s[u], ks, qs[t]);
       }
-    }
-    v8i vf[D / 32];
+  }
+  __device__ __forceinline__ void add_values(const uint8_t LDS_AS* v, int half, int vs) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-      const int dim = d * 32 + r, sw = v_swap(dim);
-      vf[d] = join(*(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + g) ^ sw) << 4)),
-                   *(const u32x4_t LDS_AS*)(vt + dim * kPage + (((4 * half + 2 + g) ^ sw) << 4)));
-    }
-    const int room = rw.limit - (at + half * 64 + 16 * g);  // this lane's keys: 32 u + e < room
-    if (masked) {
-      asm volatile("" :::);  // a branch: most pages are seen whole
+      const v8i vf = v_operand(v, half, d);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * u + e >= room) s[u][e] = -__builtin_huge_valf();
+      for (int t = 0; t < N; ++t) acc[d] = mfma(vf, pf[t], acc[d], vs, e8m0(shift - 5 * t));
     }
+  }
+  // The order of a phase with n products: after each its share of exponentials
+  // and of other arithmetic; two LDS reads before each operand's first product.
+  template <bool EXP, bool MFMA, int TRANS, int VALU>
+  static __device__ __forceinline__ void order(int n) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      if (MFMA) {
+        if (i % N == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      if (EXP) __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+    }
+  }
+  static __device__ __forceinline__ float top_of(const v16f (&s)[2]) {
     float top = -__builtin_huge_valf();
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -560,64 +592,147 @@ FVSR_DEV void attend_page(const uint8_t LDS_AS* st, int page, bool there, int ks
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
                                                      false, false);
-    top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    int shift;
-    weigh(s, top, c, m, l, shift, [&](float f) {
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+  }
+  // E of the logits at hand.
+  __device__ __forceinline__ float exponent(const v16f (&s)[2]) const {
+    return fmaxf(__builtin_ceilf(top_of(s) * c), kNothing);
+  }
+  // Step of the half whose logits are s: PV: with the half before (its V in v,
+  // half pv_half), QK: with the logits of the half behind (into next).
+  template <bool PV, bool QK>
+  __device__ __forceinline__ void step(v16f (&s)[2], v16f (&next)[2], const uint8_t LDS_AS* v,
+                                       int pv_half, int vs, const uint8_t LDS_AS* k, int qk_half,
+                                       int ks) {
+    const float e = exponent(s);
+    lost |= e > m + 64.0f;
+    // Each product is followed by its share of the arithmetic, which it runs
+    // beside; operands are read from LDS one product ahead.
+    const float off = 8.0f - e;
+    float sum = 0.0f;
+    v8i f{}, ahead{};
+    constexpr int P1 = D / 32 * N;  // products of O
+    if constexpr (PV) ahead = v_operand(v, pv_half, 0);
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] *= f;
-    });
-    v8i pf[N];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[N];
-        split4<N>(s[u][4 * i], s[u][4 * i + 1], s[u][4 * i + 2], s[u][4 * i + 3], w);
-#pragma unroll
-        for (int k = 0; k < N; ++k) pf[k][u * 4 + i] = (int)w[k];
+    for (int i = 0; i < P1; ++i) {
+      const int d = i / N, t = i % N;
+      if (t == 0) {
+        f = ahead;
+        if (d + 1 < D / 32) {
+          if constexpr (PV) ahead = v_operand(v, pv_half, d + 1);
+        } else {
+          if constexpr (QK) ahead = k_operand(k, qk_half, 0, 0);
+        }
       }
-    if (masked) {  // as in attend_few
-      asm volatile("" :::);
-      bool any = false;
+      if constexpr (PV) acc[d] = mfma(f, pf[t], acc[d], vs, e8m0(shift - 5 * t));
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) any |= has_nan(vf[d]);
-      if (__ballot(any) != 0) {
-        v8i seen;
+      for (int x = 32 * i / P1; x < 32 * (i + 1) / P1; ++x) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x >> 4][x & 15], c, off));
+        s[x >> 4][x & 15] = p;
+        sum += p;
+      }
+    }
+    order<true, PV, (32 + P1 - 1) / P1, (64 + P1 - 1) / P1 + 1>(P1);
+    __builtin_amdgcn_sched_barrier(0);
+    shift = (int)fmaxf(e - m, -300.0f) - 8;
+    l += __builtin_ldexpf(sum, shift);
+    constexpr int P2 = D / 64 * 2 * N;  // products of the next S
+    if constexpr (QK) next[0] = next[1] = v16f{};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          seen[i] = 0;
+    for (int i = 0; i < P2; ++i) {
+      const int x = i / N, t = i % N, u = x & 1, w = x >> 1;
+      if constexpr (QK) {
+        if (t == 0) {
+          f = ahead;
+          if (x + 1 < P2 / N) ahead = k_operand(k, qk_half, (x + 1) & 1, (x + 1) >> 1);
+        }
+        next[u] = mfma(f, qf[w][t], next[u], ks, qs[t]);
+      }
+#pragma unroll
+      for (int g = 8 * i / P2; g < 8 * (i + 1) / P2; ++g) {
+        uint32_t o[N];
+        const v16f& sg = s[g >> 2];
+        const int b = 4 * (g & 3);
+        split4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o);
+#pragma unroll
+        for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
+      }
+    }
+    order<false, QK, 0, (10 * N * 4 + P2 - 1) / P2>(P2);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // A page at position `at`.
+  __device__ __forceinline__ void one(const uint8_t LDS_AS* k, const uint8_t LDS_AS* v, int at,
+                                      int ks, int vs) {
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      fresh();
+      v16f s[2];
+      logits(s, k, half, ks);
+      const int room = limit - at - half * 64 - 16 * ((threadIdx.x >> 5) & 1);  // 32 u + e < it
+      const bool masked = at + half * 64 + 64 > lim_lo;
+      if (masked) {
+        asm volatile("" :::);  // a branch: most pages are seen whole
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * u + e >= room) s[u][e] = -__builtin_huge_valf();
+      }
+      weigh(s, top_of(s), c, m, l, shift, [&](float f) {
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
+      });
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        uint32_t o[N];
+        const v16f& sg = s[g >> 2];
+        const int b = 4 * (g & 3);
+        split4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o);
+#pragma unroll
+        for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
+      }
+      v8i seen{};  // 1.0 where this lane's row sees a token (masked halves)
+      if (masked) {
+        asm volatile("" :::);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (32 * (i >> 2) + 4 * (i & 3) + j < room) seen[i] |= 0x38 << (8 * j);
-        }
+      }
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-          const v8i ones = take_nan(vf[d]);
+      for (int d = 0; d < D / 32; ++d) {
+        v8i f = v_operand(v, half, d);
+        if (masked && __ballot(has_nan(f)) != 0) {  // as in attend_few
+          const v8i ones = take_nan(f);
           const v16f z = {};
           const v16f n = mfma(ones, seen, z, 127, 127);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
         }
+#pragma unroll
+        for (int t = 0; t < N; ++t) acc[d] = mfma(f, pf[t], acc[d], vs, e8m0(shift - 5 * t));
       }
     }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int ps = e8m0(shift - 5 * k);
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] = mfma(vf[d], pf[k], acc[d], vs, ps);
-    }
   }
-}
+};
 
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   constexpr int N = terms(DT);
-  __shared__ __attribute__((aligned(1024))) uint8_t stage0[Stage<D>::kBytes];
-  __shared__ __attribute__((aligned(1024))) uint8_t stage1[Stage<D>::kBytes];
+  // Two pages' K and V: page i of the list in the even or odd ones.  Distinct
+  // objects, so that the compiler can tell the loads into one from the reads of
+  // another and does not wait for them.
+  __shared__ __attribute__((aligned(1024))) uint8_t k_even[kPage * D], k_odd[kPage * D];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_even[kPage * D], v_odd[kPage * D];
   __shared__ v4i list[kList];
-  uint8_t LDS_AS* st0 = (uint8_t LDS_AS*)stage0;
-  uint8_t LDS_AS* st1 = (uint8_t LDS_AS*)stage1;
+  __shared__ int again;
+  uint8_t LDS_AS* const k0 = (uint8_t LDS_AS*)k_even;
+  uint8_t LDS_AS* const k1 = (uint8_t LDS_AS*)k_odd;
+  uint8_t LDS_AS* const v0 = (uint8_t LDS_AS*)v_even;
+  uint8_t LDS_AS* const v1 = (uint8_t LDS_AS*)v_odd;
   const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous
@@ -648,10 +763,12 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   const int first = s.part * 128 + wave * 32;           // the wave's first row
   const int r = min(first + r32, rows - 1), qi = r / pack;
   const int hq = a.keep ? head : h * a.group + r % pack;
-  Rows rw;
-  rw.limit = row_limit(a, s, qi);
-  rw.lim_lo = row_limit(a, s, min(first, rows - 1) / pack);
-  rw.lim_hi = first < rows ? row_limit(a, s, min(first + 31, rows - 1) / pack) : 0;
+  RowTile<DT, D> w;
+  w.limit = row_limit(a, s, qi);
+  w.lim_lo = row_limit(a, s, min(first, rows - 1) / pack);
+  w.c = a.scale_log2;
+  w.place();
+  const int tile_lo = row_limit(a, s, min(s.part * 128, rows - 1) / pack);
   const int last = row_limit(a, s, min(s.part * 128 + 127, rows - 1) / pack);
   const int pages = (last + kPage - 1) / kPage;
   const int32_t* const table = a.c.table + s.b * a.c.table_stride;
@@ -663,8 +780,6 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   }
   const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
 
-  v8i qf[D / 64][N];
-  int qs[N];
   {
     const uint16_t* qp =
         a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs + 16 * g;
@@ -687,57 +802,114 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
     const int e = row_exp(top);
     const float f = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-    for (int k = 0; k < N; ++k) qs[k] = e8m0(e - 5 * k);
+    for (int k = 0; k < N; ++k) w.qs[k] = e8m0(e - 5 * k);
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w)
+    for (int x = 0; x < D / 32; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t t[N];
-        split4<N>(el(w, 4 * i) * f, el(w, 4 * i + 1) * f, el(w, 4 * i + 2) * f,
-                  el(w, 4 * i + 3) * f, t);
+        split4<N>(el(x, 4 * i) * f, el(x, 4 * i + 1) * f, el(x, 4 * i + 2) * f,
+                  el(x, 4 * i + 3) * f, t);
 #pragma unroll
-        for (int k = 0; k < N; ++k) qf[w >> 1][k][(w & 1) * 4 + i] = (int)t[k];
+        for (int k = 0; k < N; ++k) w.qf[x >> 1][k][(x & 1) * 4 + i] = (int)t[k];
       }
   }
 
-  v16f acc[D / 32] = {};
-  float m = kNothing, l = 0.0f;
   const uint8_t* const kb = (const uint8_t*)a.c.k + (int64_t)h * kPage * D;
   const uint8_t* const vb = (const uint8_t*)a.c.v + (int64_t)h * kPage * D;
   const int64_t stride = (int64_t)H * kPage * D;
-  int n = 0;
   const auto entry = [&](int i) {
     v4i e = ((const v4i LDS_AS*)list)[i];
 #pragma unroll
     for (int k = 0; k < 3; ++k) e[k] = __builtin_amdgcn_readfirstlane(e[k]);
     return e;
   };
-  const auto fetch = [&](uint8_t LDS_AS* st, int id) {
-    if (id >= 0) stream_page<D>(st, kb + id * stride, vb + id * stride, wave, lane);
+  const auto wait_all = [] {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's loads
+    __syncthreads();                // ... and everyone's
   };
-  // One page: wait for it, start the next one, then multiply.  The stages
-  // are distinct objects, so the loads into one do not wait for reads of the other.
-  const auto step = [&](uint8_t LDS_AS* st, uint8_t LDS_AS* other, int i) {
-    const v4i e = entry(i);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (i + 1 < n) fetch(other, entry(i + 1)[1]);
-    attend_page<DT, D>(st, e[0], e[1] >= 0, e[2] & 255, e[2] >> 8, rw, a.scale_log2, qf, qs, acc,
-                       m, l);
-  };
-  for (int from = p0; from < p1; from += kList) {
-    __syncthreads();
-    n = list_pages((v4i LDS_AS*)list, a, table, h, keep, kept, from, p1, wave);
-    __syncthreads();
-    if (n == 0) continue;
-    fetch(st0, entry(0)[1]);
-    for (int i = 0; i < n; i += 2) {
-      step(st0, st1, i);
-      if (i + 1 < n) step(st1, st0, i + 1);
+  int kp = k_piece<D>(wave, lane), vp = v_piece(wave, lane);
+  int bad = 0x7fffffff;
+  const auto k_of = [&](const v4i& e) { return kb + e[1] * stride; };
+  const auto v_of = [&](const v4i& e) { return vb + e[1] * stride; };
+  if (threadIdx.x == 0) again = 0;
+  for (bool piped = true;; piped = false) {
+    for (int from = p0; from < p1; from += kList) {
+      __syncthreads();
+      const Listed c = list_pages((v4i LDS_AS*)list, a, table, h, keep, kept, from, p1, tile_lo,
+                                  wave, bad);
+      const int n = c.n;
+      __syncthreads();
+      if (n == 0) continue;
+      v4i cur = entry(0), nxt = n > 1 ? entry(1) : cur;
+      stream<D>(k0, k_of(cur), wave, kp);
+      stream<D>(v0, v_of(cur), wave, vp);
+      int i = 0;
+      // The pipeline's pages: the first `e`, an odd number of them (a branch between
+      // two pages makes the compiler spill).
+      const int e = piped && c.whole > 2 ? (c.whole - 1) | 1 : 0;
+      if (e > 0) {
+        v16f sa[2], sb[2];
+        // Page i's second half and the first of page i + 1.
+        const auto pair = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
+                              uint8_t LDS_AS* v_next) {
+          wait_all();
+          const v4i behind = entry(min(i + 2, n - 1));  // (the last one again: no branch)
+          stream<D>(k, k_of(behind), wave, kp);
+          stream<D>(v_next, v_of(nxt), wave, vp);
+          const int vs = cur[2] >> 8, ks = nxt[2] & 255;
+          w.fresh();
+          w.template step<true, true>(sb, sa, v, 0, vs, k_next, 0, ks);
+          w.template step<true, true>(sa, sb, v, 1, vs, k_next, 1, ks);
+          cur = nxt;
+          nxt = behind;
+          ++i;
+        };
+        wait_all();
+        stream<D>(k1, k_of(nxt), wave, kp);
+        w.logits(sa, k0, 0, cur[2] & 255);
+        if (w.m == kNothing) w.m = w.exponent(sa);
+        w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
+        while (i + 1 < e) {
+          pair(k0, v0, k1, v1);
+          pair(k1, v1, k0, v0);
+        }
+        wait_all();
+        if (i + 1 < n) stream<D>(v1, v_of(nxt), wave, vp);
+        w.template step<true, false>(sb, sa, v0, 0, cur[2] >> 8, nullptr, 0, 0);
+        w.add_values(v0, 1, cur[2] >> 8);
+        cur = nxt;
+        ++i;
+      }
+      // Page i alone, its codes being on their way to k and v.
+      const auto single = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
+                              uint8_t LDS_AS* v_next) {
+        wait_all();
+        if (i + 1 < n) {
+          nxt = entry(i + 1);
+          stream<D>(k_next, k_of(nxt), wave, kp);
+          stream<D>(v_next, v_of(nxt), wave, vp);
+        }
+        w.one(k, v, cur[0], cur[2] & 255, cur[2] >> 8);
+        cur = nxt;
+        ++i;
+      };
+      while (i < n) {
+        if (!(i & 1)) single(k0, v0, k1, v1);
+        if (i < n) single(k1, v1, k0, v0);
+      }
     }
+    if (!piped || p0 >= p1) break;
+    if (__ballot(w.lost) != 0) again = 1;
+    __syncthreads();
+    if (!again) break;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) w.acc[d] = v16f{};
+    w.m = kNothing, w.l = 0.0f;
   }
 
-  l += __shfl_xor(l, 32);
+  float l = w.l + __shfl_xor(w.l, 32);
+  if (w.limit > bad) l = __builtin_nanf("");  // the row reads a page that does not exist
   if (first + r32 >= rows) return;
   const int64_t token = s.rows.lo + qi;
   if (a.splits == 1) {
@@ -748,8 +920,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *(u32x2_t*)(op + d * 32 + 8 * i) =
-            u32x2_t{pack2<DT>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
-                    pack2<DT>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)};
+            u32x2_t{pack2<DT>(w.acc[d][4 * i] * inv, w.acc[d][4 * i + 1] * inv),
+                    pack2<DT>(w.acc[d][4 * i + 2] * inv, w.acc[d][4 * i + 3] * inv)};
   } else {
     const int64_t pr = (token * a.q_heads + hq) * a.splits + split;
     float* po = a.part + pr * D + 4 * g;
@@ -758,10 +930,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *(v4f*)(po + d * 32 + 8 * i) =
-            v4f{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+            v4f{w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]};
     if (g == 0) {
       float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
-      ml[0] = m, ml[1] = l;
+      ml[0] = w.m, ml[1] = l;
     }
   }
 }
