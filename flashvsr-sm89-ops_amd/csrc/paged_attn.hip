@@ -28,8 +28,9 @@
 // straight into operand registers, pages shared out over waves and workgroups.
 // attend_tile: 128 rows, 32 a wave, bound by products and exponentials: 32x32x64
 // products from a double-buffered LDS stage.  Either splits a long axis over
-// workgroups where rows alone leave CUs idle; attend_join adds the pieces.
+// workgroups where rows alone leave CUs idle; join_few and join_tile add the pieces.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_pages.h"
 
@@ -53,9 +54,10 @@ struct Args {
   int64_t q_ts, q_hs, o_ts, o_hs;
   const uint8_t* keep;
   int64_t keep_q, keep_k;
-  float* part;       // splits > 1: O of (row, split), then (M, l)
+  float* part;       // splits > 1: O of each row of each piece, then (M, l)
   float scale_log2;  // sm_scale * log2(e)
   int T, q_heads, group, causal, splits, tiles, tail;
+  int whole, pieces;  // attend_tile: units done by one workgroup; workgroups of a later one
 };
 
 template <int DT>
@@ -393,29 +395,23 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   }
 }
 
-// The pieces of a row, a wave each: 4 dims a lane, several pieces at once.
+// One wave adds the n pieces of a row: O at o + k * o_step, (M, l) at ml + k * ml_step;
+// 4 dims a lane, several pieces at once.
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void attend_join(Args a) {
+FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t ml_step, int n,
+                       uint16_t* out) {
   constexpr int L = D / 4, G = 64 / L;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t rows = (int64_t)a.T * a.q_heads;
-  if (row >= rows) return;
-  const int token = (int)(row / a.q_heads), oh = (int)(row % a.q_heads);
-  // Rows behind the last sequence have no pieces.
-  if (a.c.cu && token >= a.c.cu[a.c.sequences] && !a.tail) return;
   const int lane = threadIdx.x & 63;
-  const float* ml = a.part + rows * a.splits * D + row * a.splits * 2;
-  const float m = lane < a.splits ? ml[2 * lane] : kNothing;
-  const float l = lane < a.splits ? ml[2 * lane + 1] : 0.0f;
+  const float m = lane < n ? ml[lane * ml_step] : kNothing;
+  const float l = lane < n ? ml[lane * ml_step + 1] : 0.0f;
   const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
   const float sum = wave_sum(f * l);
   v4f o = {};
-  const float* po = a.part + row * a.splits * D + (lane % L) * 4;
   // (Every lane takes every turn: a lane that has left could not lend its factor.)
-  for (int s0 = 0; s0 < a.splits; s0 += G) {
+  for (int s0 = 0; s0 < n; s0 += G) {
     const int s = s0 + lane / L;
     const float w = __shfl(f, s & 63);
-    if (s < a.splits) o += *(const v4f*)(po + (int64_t)s * D) * w;
+    if (s < n) o += *(const v4f*)(po + s * o_step + (lane % L) * 4) * w;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -423,8 +419,18 @@ __global__ __launch_bounds__(kThreads) void attend_join(Args a) {
     for (int d = L; d < 64; d *= 2) o[e] += __shfl_xor(o[e], d);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (lane < L)
-    *(u32x2_t*)(a.out + (int64_t)token * a.o_ts + (int64_t)oh * a.o_hs + lane * 4) =
+    *(u32x2_t*)(out + lane * 4) =
         u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void join_few(Args a) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t rows = (int64_t)a.T * a.q_heads;
+  if (row >= rows) return;
+  join_row<DT, D>(a.part + row * a.splits * D, D,
+                  a.part + rows * a.splits * D + row * a.splits * 2, 2, a.splits,
+                  a.out + row / a.q_heads * a.o_ts + row % a.q_heads * a.o_hs);
 }
 
 // ---------------------------------------------------------------------------
@@ -719,6 +725,60 @@ struct RowTile {
   }
 };
 
+// Unit u of a call: a head (of the queries with a block mask, else of the keys)
+// and 128 rows of one sequence.  Without a mask a tile's rows are (query, head of the
+// group) pairs, so a group's heads read its pages once; with one, each head has
+// its own pages.
+struct TileUnit {
+  SeqPart s;
+  int head, h, pack, rows;  // h: key/value head; rows: of the sequence
+  __device__ __forceinline__ int query(int r) const { return r / pack; }
+  __device__ __forceinline__ int q_head(const Args& a, int r) const { return a.keep ? head : h * a.group + r % pack; }
+};
+FVSR_DEV bool unit_of(const Args& a, int u, TileUnit& t) {
+  t.pack = a.keep ? 1 : a.group;
+  t.head = u / a.tiles;
+  t.h = a.keep ? t.head / a.group : t.head;
+  // Under a causal mask later tiles see more: they go first.
+  const int tile = a.causal ? a.tiles - 1 - u % a.tiles : u % a.tiles;
+  const int pack = t.pack;
+  const auto tiles_of = [pack](int n, int) { return (n * pack + 127) / 128; };
+  if (a.c.cu) {
+    if (!find_part(a.c.cu, a.c.lengths, (int)a.c.sequences, a.T, tile, a.tail != 0, tiles_of, t.s))
+      return false;
+  } else {
+    const int each = a.tiles / (int)a.c.sequences;
+    t.s.b = tile / each;
+    t.s.part = tile % each;
+    t.s.rows = seq_rows(nullptr, t.s.b, (int)a.c.sequences, a.T);
+    t.s.len = max(a.c.lengths[t.s.b], 0);
+  }
+  t.rows = t.s.rows.n * pack;
+  return true;
+}
+
+// Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous range of
+// `total` units, whose neighbours read the same pages.
+FVSR_DEV int xcd_order(int wg, int total) {
+  const int per = total / 8, rem = total % 8, xcd = wg % 8, loc = wg / 8;
+  return xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void join_tile(Args a) {
+  const int cut = blockIdx.x / 32, r = blockIdx.x % 32 * 4 + (threadIdx.x >> 6);
+  const int64_t cuts = gridDim.x / 32;
+  TileUnit t;
+  if (!unit_of(a, a.whole + cut, t)) return;
+  const int row = t.s.part * 128 + r;
+  if (row >= t.rows) return;
+  const int64_t at = (int64_t)cut * a.pieces * 128 + r;
+  join_row<DT, D>(a.part + at * D, 128 * D, a.part + cuts * a.pieces * 128 * D + at * 2, 128 * 2,
+                  a.pieces,
+                  a.out + (int64_t)(t.s.rows.lo + t.query(row)) * a.o_ts +
+                      (int64_t)t.q_head(a, row) * a.o_hs);
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   constexpr int N = terms(DT);
@@ -735,50 +795,32 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   uint8_t LDS_AS* const v1 = (uint8_t LDS_AS*)v_odd;
   const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous
-  // range of (head, split, tile) units, whose neighbours read the same pages.
-  const int total = gridDim.x, per = total / 8, rem = total % 8;
-  const int xcd = blockIdx.x % 8, loc = blockIdx.x / 8;
-  const int unit = xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
-  // Without a block mask a tile's rows are (query, head of the group) pairs, so
-  // a group's heads read its pages once; with one, each head has its own pages.
-  const int pack = a.keep ? 1 : a.group, H = (int)a.c.heads;
-  const int tile_unit = unit % a.tiles, split = unit / a.tiles % a.splits;
-  const int head = unit / a.tiles / a.splits;
-  const int h = a.keep ? head / a.group : head;
-  SeqPart s;
-  const auto tiles_of = [&](int n, int) { return (n * pack + 127) / 128; };
-  if (a.c.cu) {
-    if (!find_part(a.c.cu, a.c.lengths, (int)a.c.sequences, a.T, tile_unit, a.tail != 0, tiles_of,
-                   s))
-      return;
-  } else {
-    const int each = a.tiles / (int)a.c.sequences;
-    s.b = tile_unit / each;
-    s.part = tile_unit % each;
-    s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
-    s.len = max(a.c.lengths[s.b], 0);
-  }
-  const int rows = s.rows.n * pack;
-  const int first = s.part * 128 + wave * 32;           // the wave's first row
-  const int r = min(first + r32, rows - 1), qi = r / pack;
-  const int hq = a.keep ? head : h * a.group + r % pack;
+  const int wg = blockIdx.x;
+  const bool cut = wg >= a.whole;  // a piece of a unit
+  const int cut_at = cut ? xcd_order(wg - a.whole, (int)gridDim.x - a.whole) : 0;
+  const int piece = cut ? cut_at % a.pieces : 0, pieces = cut ? a.pieces : 1;
+  TileUnit t;
+  if (!unit_of(a, cut ? a.whole + cut_at / a.pieces : xcd_order(wg, a.whole), t)) return;
+  const SeqPart& s = t.s;
+  const int H = (int)a.c.heads, h = t.h, rows = t.rows;
+  const int first = s.part * 128 + wave * 32;  // the wave's first row
+  const int r = min(first + r32, rows - 1), qi = t.query(r), hq = t.q_head(a, r);
   RowTile<DT, D> w;
   w.limit = row_limit(a, s, qi);
-  w.lim_lo = row_limit(a, s, min(first, rows - 1) / pack);
+  w.lim_lo = row_limit(a, s, t.query(min(first, rows - 1)));
   w.c = a.scale_log2;
   w.place();
-  const int tile_lo = row_limit(a, s, min(s.part * 128, rows - 1) / pack);
-  const int last = row_limit(a, s, min(s.part * 128 + 127, rows - 1) / pack);
+  const int tile_lo = row_limit(a, s, t.query(s.part * 128));
+  const int last = row_limit(a, s, t.query(min(s.part * 128 + 127, rows - 1)));
   const int pages = (last + kPage - 1) / kPage;
   const int32_t* const table = a.c.table + s.b * a.c.table_stride;
   const uint8_t* keep = nullptr;
   int kept = 0;
   if (a.keep) {
-    keep = a.keep + (((int64_t)s.b * a.q_heads + head) * a.keep_q + s.part) * a.keep_k;
+    keep = a.keep + (((int64_t)s.b * a.q_heads + t.head) * a.keep_q + s.part) * a.keep_k;
     kept = s.part < a.keep_q && s.b < a.c.sequences ? (int)min(a.keep_k, (int64_t)0x7fffffff) : 0;
   }
-  const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
+  const int p0 = range_at(pages, piece, pieces), p1 = range_at(pages, piece + 1, pieces);
 
   {
     const uint16_t* qp =
@@ -833,6 +875,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   const auto k_of = [&](const v4i& e) { return kb + e[1] * stride; };
   const auto v_of = [&](const v4i& e) { return vb + e[1] * stride; };
   if (threadIdx.x == 0) again = 0;
+  // A wave without rows (`live` false) only streams and waits with the others.
+  const auto all_pages = [&](auto live) {
   for (bool piped = true;; piped = false) {
     for (int from = p0; from < p1; from += kList) {
       __syncthreads();
@@ -857,27 +901,33 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
           const v4i behind = entry(min(i + 2, n - 1));  // (the last one again: no branch)
           stream<D>(k, k_of(behind), wave, kp);
           stream<D>(v_next, v_of(nxt), wave, vp);
-          const int vs = cur[2] >> 8, ks = nxt[2] & 255;
-          w.fresh();
-          w.template step<true, true>(sb, sa, v, 0, vs, k_next, 0, ks);
-          w.template step<true, true>(sa, sb, v, 1, vs, k_next, 1, ks);
+          if constexpr (live) {
+            const int vs = cur[2] >> 8, ks = nxt[2] & 255;
+            w.fresh();
+            w.template step<true, true>(sb, sa, v, 0, vs, k_next, 0, ks);
+            w.template step<true, true>(sa, sb, v, 1, vs, k_next, 1, ks);
+          }
           cur = nxt;
           nxt = behind;
           ++i;
         };
         wait_all();
         stream<D>(k1, k_of(nxt), wave, kp);
-        w.logits(sa, k0, 0, cur[2] & 255);
-        if (w.m == kNothing) w.m = w.exponent(sa);
-        w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
+        if constexpr (live) {
+          w.logits(sa, k0, 0, cur[2] & 255);
+          if (w.m == kNothing) w.m = w.exponent(sa);
+          w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
+        }
         while (i + 1 < e) {
           pair(k0, v0, k1, v1);
           pair(k1, v1, k0, v0);
         }
         wait_all();
         if (i + 1 < n) stream<D>(v1, v_of(nxt), wave, vp);
-        w.template step<true, false>(sb, sa, v0, 0, cur[2] >> 8, nullptr, 0, 0);
-        w.add_values(v0, 1, cur[2] >> 8);
+        if constexpr (live) {
+          w.template step<true, false>(sb, sa, v0, 0, cur[2] >> 8, nullptr, 0, 0);
+          w.add_values(v0, 1, cur[2] >> 8);
+        }
         cur = nxt;
         ++i;
       }
@@ -890,7 +940,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
           stream<D>(k_next, k_of(nxt), wave, kp);
           stream<D>(v_next, v_of(nxt), wave, vp);
         }
-        w.one(k, v, cur[0], cur[2] & 255, cur[2] >> 8);
+        if constexpr (live) w.one(k, v, cur[0], cur[2] & 255, cur[2] >> 8);
         cur = nxt;
         ++i;
       };
@@ -907,14 +957,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
     for (int d = 0; d < D / 32; ++d) w.acc[d] = v16f{};
     w.m = kNothing, w.l = 0.0f;
   }
+  };
+  if (first < rows)
+    all_pages(std::true_type{});
+  else
+    all_pages(std::false_type{});
 
   float l = w.l + __shfl_xor(w.l, 32);
   if (w.limit > bad) l = __builtin_nanf("");  // the row reads a page that does not exist
   if (first + r32 >= rows) return;
-  const int64_t token = s.rows.lo + qi;
-  if (a.splits == 1) {
+  if (!cut) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* op = a.out + token * a.o_ts + (int64_t)hq * a.o_hs + 4 * g;
+    uint16_t* op = a.out + (int64_t)(s.rows.lo + qi) * a.o_ts + (int64_t)hq * a.o_hs + 4 * g;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -923,8 +977,9 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
             u32x2_t{pack2<DT>(w.acc[d][4 * i] * inv, w.acc[d][4 * i + 1] * inv),
                     pack2<DT>(w.acc[d][4 * i + 2] * inv, w.acc[d][4 * i + 3] * inv)};
   } else {
-    const int64_t pr = (token * a.q_heads + hq) * a.splits + split;
-    float* po = a.part + pr * D + 4 * g;
+    const int64_t total = (int64_t)((int)gridDim.x - a.whole);  // pieces of the call
+    const int64_t at = (int64_t)cut_at * 128 + wave * 32 + r32;
+    float* po = a.part + at * D + 4 * g;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -932,54 +987,84 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
         *(v4f*)(po + d * 32 + 8 * i) =
             v4f{w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]};
     if (g == 0) {
-      float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
+      float* ml = a.part + total * 128 * D + at * 2;
       ml[0] = w.m, ml[1] = l;
     }
   }
 }
 
-// How a call is cut up: a function of its sizes only.
+int64_t cu_count() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus < 8)
+    cus = 256;
+  return cus & ~7;
+}
+
+// How a call is cut up: a function of its sizes (and the CUs) only.
 struct Plan {
   bool few;
-  int64_t tiles;  // per head: row tiles over all sequences
-  int64_t heads;  // units' heads
-  int splits;
+  int64_t tiles;   // of 128 rows, per head, over all sequences
+  int64_t units;   // tiles of all heads
+  int64_t whole;   // units done by one workgroup each; the others by `pieces` each
+  int pieces;
+  int splits;      // attend_few: workgroups of a sequence and head
   int64_t floats(int64_t T, int64_t q_heads, int64_t D) const {
-    return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
+    if (few) return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
+    return (units - whole) * pieces * 128 * (D + 2);
   }
 };
 
 Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   Plan p{};
-  const int64_t group = q_heads / c->heads, B = c->sequences;
-  const int64_t rows = T / B * group;  // of a sequence and key/value head, if all are alike
-  p.few = !c->cu && !keep && rows <= 16;
+  const int64_t group = q_heads / c->heads, B = c->sequences, cus = cu_count();
+  p.few = !c->cu && !keep && T / B * group <= 16;
+  if (p.few) {
+    const int64_t units = B * c->heads;
+    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 4 * cus / units),
+                                       std::max<int64_t>(1, c->table_pages / 4), kMaxSplits});
+    return p;
+  }
   const int64_t pack = keep ? 1 : group;
-  p.heads = keep ? q_heads : c->heads;
-  if (p.few)
-    p.tiles = B;
-  else if (c->cu)  // at most this many over any counts that add up to T, the rows behind included
-    p.tiles = T * pack / 128 + B + 1;
-  else
-    p.tiles = B * ((T / B * pack + 127) / 128);
-  const int64_t units = p.tiles * p.heads, want = p.few ? 1024 : 512;
-  const int64_t most = std::max<int64_t>(1, c->table_pages / (p.few ? 4 : 2));
-  p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, want / units), most, kMaxSplits});
+  // Packed rows: at most this many tiles over any counts that add up to T, the
+  // rows behind the last sequence included.
+  p.tiles = c->cu ? T * pack / 128 + B + 1 : B * ((T / B * pack + 127) / 128);
+  p.units = p.whole = p.tiles * (keep ? q_heads : c->heads);
+  p.pieces = 1;
+  // A CU is nearly as fast with one workgroup as with two, so it is whole units
+  // per CU that must come out even: the units past a multiple of the CUs are cut into
+  // pieces, as many as two per CU take at once.  A page costs a workgroup 1.8 us; a
+  // piece 132 KB written and read again (0.04 us of the GPU's time), and all of them
+  // the joining launch.
+  const int64_t rest = p.units % cus;
+  if (rest == 0) return p;
+  const int64_t pieces = std::min<int64_t>({2 * cus / rest, c->table_pages / 4, 16});
+  if (pieces < 2) return p;
+  const int64_t saved = c->table_pages - c->table_pages / pieces;
+  if (18 * saved < 80 + rest * pieces * 4 / 10) return p;
+  p.pieces = (int)pieces;
+  p.whole = p.units - rest;
   return p;
 }
 
 template <int DT, int D>
 void launch(const Args& a, const Plan& p, hipStream_t st) {
-  if (p.few)
-    hipLaunchKernelGGL((attend_few<DT, D>), dim3((unsigned)a.splits, (unsigned)a.c.heads,
-                                                 (unsigned)a.c.sequences),
-                       dim3(kThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((attend_tile<DT, D>), dim3((unsigned)(p.tiles * p.heads * p.splits)),
-                       dim3(kThreads), 0, st, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((attend_join<DT, D>), dim3((unsigned)(((int64_t)a.T * a.q_heads + 3) / 4)),
-                       dim3(kThreads), 0, st, a);
+  const dim3 block(kThreads);
+  if (p.few) {
+    hipLaunchKernelGGL((attend_few<DT, D>),
+                       dim3((unsigned)a.splits, (unsigned)a.c.heads, (unsigned)a.c.sequences),
+                       block, 0, st, a);
+    if (p.splits > 1)
+      hipLaunchKernelGGL((join_few<DT, D>), dim3((unsigned)(((int64_t)a.T * a.q_heads + 3) / 4)),
+                         block, 0, st, a);
+    return;
+  }
+  const int64_t cut = p.units - p.whole;
+  hipLaunchKernelGGL((attend_tile<DT, D>), dim3((unsigned)(p.whole + cut * p.pieces)), block, 0, st,
+                     a);
+  if (cut > 0)
+    hipLaunchKernelGGL((join_tile<DT, D>), dim3((unsigned)(cut * 32)), block, 0, st, a);
 }
 
 }  // namespace
@@ -1012,8 +1097,7 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
     return FVSR_EUNSUPPORTED;
   if (T * q_heads > 0x7fffffff - 256) return FVSR_EUNSUPPORTED;
   const Plan p = plan_attn(cache, T, q_heads, keep != nullptr);
-  if (p.tiles * p.heads * p.splits > 0x7fffffff || cache->heads > 65535 ||
-      (p.few && cache->sequences > 65535))
+  if (p.units > 0x3fffffff || (p.few && (cache->heads > 65535 || cache->sequences > 65535)))
     return FVSR_EUNSUPPORTED;
   const int64_t need = p.floats(T, q_heads, cache->head_dim);
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;
@@ -1027,6 +1111,7 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / cache->heads);
   a.causal = causal != 0, a.splits = p.splits, a.tiles = (int)p.tiles, a.tail = fill_tail != 0;
+  a.whole = (int)p.whole, a.pieces = p.pieces;
   const hipStream_t st = (hipStream_t)stream;
   const bool half = dtype == FVSR_DT_F16;
   if (cache->head_dim == 128)
