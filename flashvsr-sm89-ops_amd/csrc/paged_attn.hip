@@ -258,8 +258,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   // that accumulator (t, j) of lane g is position 64 (t / 4) + 16 g + 4 (t % 4) + j.
   const int k_off = (16 * (col >> 2) + (col & 3)) * D + 16 * g;
   const int v_off = col * kPage + 16 * g;
+  int ahead = p0 + wave < p1 ? table[p0 + wave] : 0;
   for (int p = p0 + wave; p < p1; p += 4) {
-    const int64_t id = __builtin_amdgcn_readfirstlane(table[p]);
+    const int64_t id = __builtin_amdgcn_readfirstlane(ahead);
+    if (p + 4 < p1) ahead = table[p + 4];
     if (id < 0 || id >= a.c.pages) {  // no such page: the rows that would read it are NaN
       if (p * kPage < limit) l = __builtin_nanf("");
       continue;
@@ -395,13 +397,14 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   }
 }
 
-// One wave adds the n pieces of a row: O at o + k * o_step, (M, l) at ml + k * ml_step;
-// 4 dims a lane, several pieces at once.
+// A workgroup adds the n pieces of a row: O at o + k * o_step, (M, l) at ml + k *
+// ml_step; 4 dims a thread, 8 or 16 pieces at once.
 template <int DT, int D>
 FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t ml_step, int n,
                        uint16_t* out) {
-  constexpr int L = D / 4, G = 64 / L;
-  const int lane = threadIdx.x & 63;
+  constexpr int L = D / 4, G = kThreads / L;
+  __shared__ __attribute__((aligned(16))) float part[kThreads / 64][D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x / L;
   const float m = lane < n ? ml[lane * ml_step] : kNothing;
   const float l = lane < n ? ml[lane * ml_step + 1] : 0.0f;
   const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
@@ -409,7 +412,7 @@ FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t
   v4f o = {};
   // (Every lane takes every turn: a lane that has left could not lend its factor.)
   for (int s0 = 0; s0 < n; s0 += G) {
-    const int s = s0 + lane / L;
+    const int s = s0 + group;
     const float w = __shfl(f, s & 63);
     if (s < n) o += *(const v4f*)(po + s * o_step + (lane % L) * 4) * w;
   }
@@ -417,17 +420,19 @@ FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int d = L; d < 64; d *= 2) o[e] += __shfl_xor(o[e], d);
+  if (lane < L) *(v4f*)&part[wave][lane * 4] = o;
+  __syncthreads();
+  if (threadIdx.x >= L) return;
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; ++w) o += *(const v4f*)&part[w][lane * 4];
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (lane < L)
-    *(u32x2_t*)(out + lane * 4) =
-        u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+  *(u32x2_t*)(out + lane * 4) =
+      u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void join_few(Args a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t rows = (int64_t)a.T * a.q_heads;
-  if (row >= rows) return;
+  const int64_t row = blockIdx.x, rows = (int64_t)a.T * a.q_heads;
   join_row<DT, D>(a.part + row * a.splits * D, D,
                   a.part + rows * a.splits * D + row * a.splits * 2, 2, a.splits,
                   a.out + row / a.q_heads * a.o_ts + row % a.q_heads * a.o_hs);
@@ -766,8 +771,8 @@ FVSR_DEV int xcd_order(int wg, int total) {
 
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void join_tile(Args a) {
-  const int cut = blockIdx.x / 32, r = blockIdx.x % 32 * 4 + (threadIdx.x >> 6);
-  const int64_t cuts = gridDim.x / 32;
+  const int cut = blockIdx.x / 128, r = blockIdx.x % 128;
+  const int64_t cuts = gridDim.x / 128;
   TileUnit t;
   if (!unit_of(a, a.whole + cut, t)) return;
   const int row = t.s.part * 128 + r;
@@ -1021,9 +1026,14 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   const int64_t group = q_heads / c->heads, B = c->sequences, cus = cu_count();
   p.few = !c->cu && !keep && T / B * group <= 16;
   if (p.few) {
-    const int64_t units = B * c->heads;
-    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 4 * cus / units),
-                                       std::max<int64_t>(1, c->table_pages / 4), kMaxSplits});
+    // Sequences may be of any lengths: 16 workgroups per CU even them out (128
+    // ragged sequences of up to 16000 tokens, us at 4 / 8 / 16 / 32: 390, 376, 364, 374).
+    // Two pages to a wave, or one where that would leave CUs idle (20000 tokens x 12
+    // heads 20.5 against 23.8 us; 4 sequences of 5000 x 2 heads 14.6 against 12.1).
+    const int64_t units = B * c->heads, pages = c->table_pages;
+    const int64_t each = units * (pages / 8) * 2 < cus ? 4 : 8;
+    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 16 * cus / units),
+                                       std::max<int64_t>(1, pages / each), kMaxSplits});
     return p;
   }
   const int64_t pack = keep ? 1 : group;
@@ -1056,15 +1066,15 @@ void launch(const Args& a, const Plan& p, hipStream_t st) {
                        dim3((unsigned)a.splits, (unsigned)a.c.heads, (unsigned)a.c.sequences),
                        block, 0, st, a);
     if (p.splits > 1)
-      hipLaunchKernelGGL((join_few<DT, D>), dim3((unsigned)(((int64_t)a.T * a.q_heads + 3) / 4)),
-                         block, 0, st, a);
+      hipLaunchKernelGGL((join_few<DT, D>), dim3((unsigned)((int64_t)a.T * a.q_heads)), block,
+                         0, st, a);
     return;
   }
   const int64_t cut = p.units - p.whole;
   hipLaunchKernelGGL((attend_tile<DT, D>), dim3((unsigned)(p.whole + cut * p.pieces)), block, 0, st,
                      a);
   if (cut > 0)
-    hipLaunchKernelGGL((join_tile<DT, D>), dim3((unsigned)(cut * 32)), block, 0, st, a);
+    hipLaunchKernelGGL((join_tile<DT, D>), dim3((unsigned)(cut * 128)), block, 0, st, a);
 }
 
 }  // namespace
