@@ -736,7 +736,8 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   // Packed rows: the sum of those bounds over any B counts that add up to T.
   const int64_t units = cache->cu ? std::min(T, (T + 126 * B) / kPage + B) : B * a.units_max;
   const int64_t q_wgs = q ? (T * q_heads * (D / 8)) / kThreads + T / 4 + 2 : 0;
-  if ((units + 7) * 2 * cache->heads + q_wgs > 0x7fffffff || (q && T * (cache->heads + q_heads) > 0x7ffffff0))
+  if ((q && q_heads > kMaxBlocks) || (units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks ||
+      T * (cache->heads + a.q_heads) > kMaxBlocks * 64)
     return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (D == 128) {

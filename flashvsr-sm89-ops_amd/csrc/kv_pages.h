@@ -5,6 +5,7 @@
 #include "common.h"
 
 constexpr int kPage = FVSR_PAGE;  // tokens of a page
+constexpr int64_t kMaxBlocks = 0xffffff;  // workgroups of a launch: 2^32 threads, 256 each
 
 // Rows of a call that belong to sequence b: T rows packed at cu[0..B], or
 // the same number each.  Clamped, so that no offsets reach outside the T rows.
@@ -71,15 +72,15 @@ FVSR_DEV bool find_part(const int32_t* cu, const int32_t* lengths, int B, int T,
   return false;
 }
 
-// What both entry points check of the cache and the call's rows; T * heads
-// of either kind stays below 2^31 (row and unit counts are 32-bit).
+// What both entry points check of the cache and the call's rows (rows and units
+// are counted in 32 bits).
 static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T) {
   if (!c) return FVSR_EINVAL;
   if (c->pages < 0 || c->heads <= 0 || c->sequences < 0 || c->table_pages < 0 || T < 0 ||
       c->table_stride < c->table_pages)
     return FVSR_EINVAL;
   if (c->head_dim != 64 && c->head_dim != 128) return FVSR_EUNSUPPORTED;
-  if (T > 0x3fffffff || T * c->heads > 0x7fffffff || c->sequences > 0x3fffff ||
+  if (T > 0x3fffffff || T * c->heads > kMaxBlocks * 64 || c->sequences > 0x3fffff ||
       c->pages > 0x7fffffff || c->table_pages > 0xffffff)
     return FVSR_EUNSUPPORTED;
   if (T == 0 || c->sequences == 0) return FVSR_OK;

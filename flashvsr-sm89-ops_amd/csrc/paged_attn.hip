@@ -44,7 +44,7 @@ typedef short v2s __attribute__((ext_vector_type(2)));
 #define LDS_AS __attribute__((address_space(3)))
 
 constexpr int kThreads = 256;
-constexpr float kNothing = -1e30f;  // reference of a row that has seen no key (finite: no inf - inf)
+constexpr float kNothing = -1e30f;  // reference of a row that has seen no key (finite)
 constexpr int kMaxSplits = 64;
 
 struct Args {
@@ -58,6 +58,7 @@ struct Args {
   float scale_log2;  // sm_scale * log2(e)
   int T, q_heads, group, causal, splits, tiles, tail;
   int whole, pieces;  // attend_tile: units done by one workgroup; workgroups of a later one
+  int tile_rows;      // rows of a tile at most
 };
 
 template <int DT>
@@ -84,7 +85,8 @@ FVSR_DEV void split4(float a, float b, float c, float d, uint32_t (&w)[N]) {
     const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)t0, false);
     const v2f hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)t0, true);
     a -= lo[0], b -= lo[1], c -= hi[0], d -= hi[1];
-    v2s t = {};
+    // (Both halves of a destination are written; what it held does not matter.)
+    v2s t = __builtin_bit_cast(v2s, a);
     t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, a, b, 0x1p-5f, false);
     t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, c, d, 0x1p-5f, true);
     w[1] = __builtin_bit_cast(uint32_t, t);
@@ -92,10 +94,38 @@ FVSR_DEV void split4(float a, float b, float c, float d, uint32_t (&w)[N]) {
   if constexpr (N > 2) {
     const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], 0x1p-5f, false);
     const v2f hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[1], 0x1p-5f, true);
-    v2s t = {};
+    v2s t = __builtin_bit_cast(v2s, a);
     t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, a - lo[0], b - lo[1], 0x1p-10f, false);
     t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, c - hi[0], d - hi[1], 0x1p-10f, true);
     w[2] = __builtin_bit_cast(uint32_t, t);
+  }
+}
+
+// Four weights (0 to 256) as N e4m3 terms; `sum` grows by them.  Two terms (8
+// bits) come by way of fp16 (11 bits), whose pairs convert, subtract and sum two at a
+// time: 24 instructions for 8 weights against 32.  The sum is of the same fp16 values.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+template <int N>
+FVSR_DEV void weights4(float a, float b, float c, float d, uint32_t (&w)[N], float& sum) {
+  if constexpr (N == 2) {
+    v2h x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
+    const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
+    sum = __builtin_amdgcn_fdot2(x, one, sum, false);
+    sum = __builtin_amdgcn_fdot2(y, one, sum, false);
+    // (Both halves of a destination are written; what it held does not matter.)
+    v2s o = __builtin_bit_cast(v2s, x);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, x, 1.0f, false);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, y, 1.0f, true);
+    w[0] = __builtin_bit_cast(uint32_t, o);
+    x -= __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.0f, false));
+    y -= __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[0], 1.0f, true));
+    o = __builtin_bit_cast(v2s, x);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, x, 0x1p-5f, false);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, y, 0x1p-5f, true);
+    w[1] = __builtin_bit_cast(uint32_t, o);
+  } else {
+    sum += (a + b) + (c + d);
+    split4<N>(a, b, c, d, w);
   }
 }
 
@@ -135,12 +165,14 @@ FVSR_DEV v16f mfma(const v8i& a, const v8i& b, const v16f& c, int sa, int sb) {
 }
 
 FVSR_DEV v8i join(u32x4_t a, u32x4_t b) {
-  return v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+  return v8i{(int)a[0], (int)a[1], (int)a[2], (int)a[3],
+             (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }
 
 // The softmax of one row's N logits at hand (in s; -inf: hidden): s becomes
 // the weights, E - 8 - M goes to `shift`, and the reference M moves if need be
-// (`rescale` then multiplies O).  Every lane of a row calls it with the row's largest logit.
+// (`rescale` then multiplies O).  Every lane of a row calls it with the row's largest
+// logit; the sum of the weights, times 2^shift, is still to be added to l.
 template <class Acc, int N, class Rescale>
 FVSR_DEV void weigh(Acc (&s)[N], float top, float c, float& m, float& l, int& shift,
                     Rescale rescale) {
@@ -155,16 +187,12 @@ FVSR_DEV void weigh(Acc (&s)[N], float top, float c, float& m, float& l, int& sh
     rescale(f);
   }
   const float off = 8.0f - e;
-  float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
+    for (int j = 0; j < E; ++j)
       s[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], c, off));
-      sum += s[i][j];
-    }
   shift = (int)fmaxf(e - m, -300.0f) - 8;
-  l += __builtin_ldexpf(sum, shift);
 }
 
 // Keys that row i of a sequence sees.
@@ -312,13 +340,15 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
       for (int d = 0; d < DT16; ++d) acc[d] *= f;
     });
     v8i pf[N];
+    float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       uint32_t w[N];
-      split4<N>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], w);
+      weights4<N>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], w, sum);
 #pragma unroll
       for (int k = 0; k < N; ++k) pf[k][t] = (int)w[k];
     }
+    l += __builtin_ldexpf(sum, shift);
     if (masked) {
       // Hidden tokens weigh 0, which a NaN code would not survive: NaN codes
       // leave the product and are counted for the rows that see them.
@@ -620,7 +650,6 @@ struct RowTile {
     // Each product is followed by its share of the arithmetic, which it runs
     // beside; operands are read from LDS one product ahead.
     const float off = 8.0f - e;
-    float sum = 0.0f;
     v8i f{}, ahead{};
     constexpr int P1 = D / 32 * N;  // products of O
     if constexpr (PV) ahead = v_operand(v, pv_half, 0);
@@ -637,16 +666,13 @@ struct RowTile {
       }
       if constexpr (PV) acc[d] = mfma(f, pf[t], acc[d], vs, e8m0(shift - 5 * t));
 #pragma unroll
-      for (int x = 32 * i / P1; x < 32 * (i + 1) / P1; ++x) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x >> 4][x & 15], c, off));
-        s[x >> 4][x & 15] = p;
-        sum += p;
-      }
+      for (int x = 32 * i / P1; x < 32 * (i + 1) / P1; ++x)
+        s[x >> 4][x & 15] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x >> 4][x & 15], c, off));
     }
-    order<true, PV, (32 + P1 - 1) / P1, (64 + P1 - 1) / P1 + 1>(P1);
+    order<true, PV, (32 + P1 - 1) / P1, (32 + P1 - 1) / P1 + 1>(P1);
     __builtin_amdgcn_sched_barrier(0);
     shift = (int)fmaxf(e - m, -300.0f) - 8;
-    l += __builtin_ldexpf(sum, shift);
+    float sum = 0.0f;
     constexpr int P2 = D / 64 * 2 * N;  // products of the next S
     if constexpr (QK) next[0] = next[1] = v16f{};
 #pragma unroll
@@ -664,12 +690,13 @@ struct RowTile {
         uint32_t o[N];
         const v16f& sg = s[g >> 2];
         const int b = 4 * (g & 3);
-        split4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o);
+        weights4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o, sum);
 #pragma unroll
         for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
       }
     }
-    order<false, QK, 0, (10 * N * 4 + P2 - 1) / P2>(P2);
+    l += __builtin_ldexpf(sum, shift);
+    order<false, QK, 0, (8 * (N == 2 ? 12 : 22) + P2 - 1) / P2>(P2);
     __builtin_amdgcn_sched_barrier(0);
   }
   // A page at position `at`.
@@ -694,15 +721,17 @@ struct RowTile {
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= f;
       });
+      float sum = 0.0f;
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         uint32_t o[N];
         const v16f& sg = s[g >> 2];
         const int b = 4 * (g & 3);
-        split4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o);
+        weights4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o, sum);
 #pragma unroll
         for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
       }
+      l += __builtin_ldexpf(sum, shift);
       v8i seen{};  // 1.0 where this lane's row sees a token (masked halves)
       if (masked) {
         asm volatile("" :::);
@@ -738,7 +767,9 @@ struct TileUnit {
   SeqPart s;
   int head, h, pack, rows;  // h: key/value head; rows: of the sequence
   __device__ __forceinline__ int query(int r) const { return r / pack; }
-  __device__ __forceinline__ int q_head(const Args& a, int r) const { return a.keep ? head : h * a.group + r % pack; }
+  __device__ __forceinline__ int q_head(const Args& a, int r) const {
+    return a.keep ? head : h * a.group + r % pack;
+  }
 };
 FVSR_DEV bool unit_of(const Args& a, int u, TileUnit& t) {
   t.pack = a.keep ? 1 : a.group;
@@ -771,8 +802,8 @@ FVSR_DEV int xcd_order(int wg, int total) {
 
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void join_tile(Args a) {
-  const int cut = blockIdx.x / 128, r = blockIdx.x % 128;
-  const int64_t cuts = gridDim.x / 128;
+  const int cut = blockIdx.x / a.tile_rows, r = blockIdx.x % a.tile_rows;
+  const int64_t cuts = gridDim.x / a.tile_rows;
   TileUnit t;
   if (!unit_of(a, a.whole + cut, t)) return;
   const int row = t.s.part * 128 + r;
@@ -882,86 +913,86 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   if (threadIdx.x == 0) again = 0;
   // A wave without rows (`live` false) only streams and waits with the others.
   const auto all_pages = [&](auto live) {
-  for (bool piped = true;; piped = false) {
-    for (int from = p0; from < p1; from += kList) {
-      __syncthreads();
-      const Listed c = list_pages((v4i LDS_AS*)list, a, table, h, keep, kept, from, p1, tile_lo,
-                                  wave, bad);
-      const int n = c.n;
-      __syncthreads();
-      if (n == 0) continue;
-      v4i cur = entry(0), nxt = n > 1 ? entry(1) : cur;
-      stream<D>(k0, k_of(cur), wave, kp);
-      stream<D>(v0, v_of(cur), wave, vp);
-      int i = 0;
-      // The pipeline's pages: the first `e`, an odd number of them (a branch between
-      // two pages makes the compiler spill).
-      const int e = piped && c.whole > 2 ? (c.whole - 1) | 1 : 0;
-      if (e > 0) {
-        v16f sa[2], sb[2];
-        // Page i's second half and the first of page i + 1.
-        const auto pair = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
-                              uint8_t LDS_AS* v_next) {
+    for (bool piped = true;; piped = false) {
+      for (int from = p0; from < p1; from += kList) {
+        __syncthreads();
+        const Listed c = list_pages((v4i LDS_AS*)list, a, table, h, keep, kept, from, p1, tile_lo,
+                                    wave, bad);
+        const int n = c.n;
+        __syncthreads();
+        if (n == 0) continue;
+        v4i cur = entry(0), nxt = n > 1 ? entry(1) : cur;
+        stream<D>(k0, k_of(cur), wave, kp);
+        stream<D>(v0, v_of(cur), wave, vp);
+        int i = 0;
+        // The pipeline's pages: the first `e`, an odd number of them (a branch between
+        // two pages makes the compiler spill).
+        const int e = piped && c.whole > 2 ? (c.whole - 1) | 1 : 0;
+        if (e > 0) {
+          v16f sa[2], sb[2];
+          // Page i's second half and the first of page i + 1.
+          const auto pair = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
+                                uint8_t LDS_AS* v_next) {
+            wait_all();
+            const v4i behind = entry(min(i + 2, n - 1));  // (the last one again: no branch)
+            stream<D>(k, k_of(behind), wave, kp);
+            stream<D>(v_next, v_of(nxt), wave, vp);
+            if constexpr (live) {
+              const int vs = cur[2] >> 8, ks = nxt[2] & 255;
+              w.fresh();
+              w.template step<true, true>(sb, sa, v, 0, vs, k_next, 0, ks);
+              w.template step<true, true>(sa, sb, v, 1, vs, k_next, 1, ks);
+            }
+            cur = nxt;
+            nxt = behind;
+            ++i;
+          };
           wait_all();
-          const v4i behind = entry(min(i + 2, n - 1));  // (the last one again: no branch)
-          stream<D>(k, k_of(behind), wave, kp);
-          stream<D>(v_next, v_of(nxt), wave, vp);
+          stream<D>(k1, k_of(nxt), wave, kp);
           if constexpr (live) {
-            const int vs = cur[2] >> 8, ks = nxt[2] & 255;
-            w.fresh();
-            w.template step<true, true>(sb, sa, v, 0, vs, k_next, 0, ks);
-            w.template step<true, true>(sa, sb, v, 1, vs, k_next, 1, ks);
+            w.logits(sa, k0, 0, cur[2] & 255);
+            if (w.m == kNothing) w.m = w.exponent(sa);
+            w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
+          }
+          while (i + 1 < e) {
+            pair(k0, v0, k1, v1);
+            pair(k1, v1, k0, v0);
+          }
+          wait_all();
+          if (i + 1 < n) stream<D>(v1, v_of(nxt), wave, vp);
+          if constexpr (live) {
+            w.template step<true, false>(sb, sa, v0, 0, cur[2] >> 8, nullptr, 0, 0);
+            w.add_values(v0, 1, cur[2] >> 8);
           }
           cur = nxt;
-          nxt = behind;
+          ++i;
+        }
+        // Page i alone, its codes being on their way to k and v.
+        const auto single = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
+                                uint8_t LDS_AS* v_next) {
+          wait_all();
+          if (i + 1 < n) {
+            nxt = entry(i + 1);
+            stream<D>(k_next, k_of(nxt), wave, kp);
+            stream<D>(v_next, v_of(nxt), wave, vp);
+          }
+          if constexpr (live) w.one(k, v, cur[0], cur[2] & 255, cur[2] >> 8);
+          cur = nxt;
           ++i;
         };
-        wait_all();
-        stream<D>(k1, k_of(nxt), wave, kp);
-        if constexpr (live) {
-          w.logits(sa, k0, 0, cur[2] & 255);
-          if (w.m == kNothing) w.m = w.exponent(sa);
-          w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
+        while (i < n) {
+          if (!(i & 1)) single(k0, v0, k1, v1);
+          if (i < n) single(k1, v1, k0, v0);
         }
-        while (i + 1 < e) {
-          pair(k0, v0, k1, v1);
-          pair(k1, v1, k0, v0);
-        }
-        wait_all();
-        if (i + 1 < n) stream<D>(v1, v_of(nxt), wave, vp);
-        if constexpr (live) {
-          w.template step<true, false>(sb, sa, v0, 0, cur[2] >> 8, nullptr, 0, 0);
-          w.add_values(v0, 1, cur[2] >> 8);
-        }
-        cur = nxt;
-        ++i;
       }
-      // Page i alone, its codes being on their way to k and v.
-      const auto single = [&](uint8_t LDS_AS* k, uint8_t LDS_AS* v, uint8_t LDS_AS* k_next,
-                              uint8_t LDS_AS* v_next) {
-        wait_all();
-        if (i + 1 < n) {
-          nxt = entry(i + 1);
-          stream<D>(k_next, k_of(nxt), wave, kp);
-          stream<D>(v_next, v_of(nxt), wave, vp);
-        }
-        if constexpr (live) w.one(k, v, cur[0], cur[2] & 255, cur[2] >> 8);
-        cur = nxt;
-        ++i;
-      };
-      while (i < n) {
-        if (!(i & 1)) single(k0, v0, k1, v1);
-        if (i < n) single(k1, v1, k0, v0);
-      }
+      if (!piped || p0 >= p1) break;
+      if (__ballot(w.lost) != 0) again = 1;
+      __syncthreads();
+      if (!again) break;
+  #pragma unroll
+      for (int d = 0; d < D / 32; ++d) w.acc[d] = v16f{};
+      w.m = kNothing, w.l = 0.0f;
     }
-    if (!piped || p0 >= p1) break;
-    if (__ballot(w.lost) != 0) again = 1;
-    __syncthreads();
-    if (!again) break;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) w.acc[d] = v16f{};
-    w.m = kNothing, w.l = 0.0f;
-  }
   };
   if (first < rows)
     all_pages(std::true_type{});
@@ -1074,7 +1105,8 @@ void launch(const Args& a, const Plan& p, hipStream_t st) {
   hipLaunchKernelGGL((attend_tile<DT, D>), dim3((unsigned)(p.whole + cut * p.pieces)), block, 0, st,
                      a);
   if (cut > 0)
-    hipLaunchKernelGGL((join_tile<DT, D>), dim3((unsigned)(cut * 128)), block, 0, st, a);
+    hipLaunchKernelGGL((join_tile<DT, D>), dim3((unsigned)(cut * a.tile_rows)), block, 0, st,
+                       a);
 }
 
 }  // namespace
@@ -1107,7 +1139,10 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
     return FVSR_EUNSUPPORTED;
   if (T * q_heads > 0x7fffffff - 256) return FVSR_EUNSUPPORTED;
   const Plan p = plan_attn(cache, T, q_heads, keep != nullptr);
-  if (p.units > 0x3fffffff || (p.few && (cache->heads > 65535 || cache->sequences > 65535)))
+  if (p.units > kMaxBlocks / 2 || T * q_heads > kMaxBlocks * 64 ||
+      (p.few && (cache->heads > 65535 || cache->sequences > 65535 ||
+                 p.splits * cache->heads * cache->sequences > kMaxBlocks ||
+                 (p.splits > 1 && T * q_heads > kMaxBlocks))))
     return FVSR_EUNSUPPORTED;
   const int64_t need = p.floats(T, q_heads, cache->head_dim);
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;
@@ -1122,6 +1157,8 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
   a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / cache->heads);
   a.causal = causal != 0, a.splits = p.splits, a.tiles = (int)p.tiles, a.tail = fill_tail != 0;
   a.whole = (int)p.whole, a.pieces = p.pieces;
+  a.tile_rows = (int)std::min<int64_t>(
+      128, (cache->cu ? T : T / cache->sequences) * (keep ? 1 : a.group));
   const hipStream_t st = (hipStream_t)stream;
   const bool half = dtype == FVSR_DT_F16;
   if (cache->head_dim == 128)

@@ -356,8 +356,8 @@ def test_append_odd_layouts():
 
 
 def check_attention(out, q, pages, table, lengths, cu=None, causal=True, keep=None, sm_scale=None):
-    want, size, logit = O.attention(q, O.from_pages(*pages), table, lengths, cu, causal, keep,
-                                    sm_scale)
+    cache = pages if isinstance(pages, dict) else O.from_pages(*pages)
+    want, size, logit = O.attention(q, cache, table, lengths, cu, causal, keep, sm_scale)
     dt = q.dtype
     weight = 2.0 ** -8 if dt == torch.bfloat16 else 2.0 ** -12
     tol = torch.finfo(dt).eps / 2 * want.abs() + torch.finfo(dt).smallest_normal
@@ -513,6 +513,58 @@ def test_attention_far_logits():
             assert bool(torch.isfinite(out).all())
             if scale != 1.0:  # (there a logit's own error, 2^-12 of hundreds, is all)
                 check_attention(out, q, pages, table, lens, sm_scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pages", [3, 4, 9])
+def test_attention_later_page_far_above(dtype, D, pages):
+    """A later page's logits lie 2^100 above the first half page's for some rows and below
+    for others: the tiles' pipeline keeps the first one's reference and is done again."""
+    from flashvsr_sm89_ops import paged_attention
+    H, n, lens = 2, 70, [128 * pages + 90]
+    table, N = tables(lens)
+    pool_ = pool(N, H, D)
+    k = pool_.k.view(torch.uint8)
+    code = int(torch.tensor(64.0).to(torch.float8_e4m3fn).view(torch.uint8))
+    k[int(table[0, 0])] = 0
+    k[int(table[0, pages - 1]), :, 5, 0] = code
+    pool_.k_scale.view(torch.uint8).fill_(127)
+    q = torch.randn(n, H, D, generator=gen(3)) * 0.01
+    q[::2, :, 0], q[1::2, :, 0] = 1.5, -1.5
+    q = q.to(dtype)
+    for causal in (True, False):
+        out = paged_attention(q.to(DEV), pool_, table.to(DEV), i32(lens).to(DEV), causal=causal,
+                              sm_scale=1.0)
+        check_attention(out, q, pool_, table, lens, causal=causal, sm_scale=1.0)
+
+
+@pytest.mark.parametrize("D,Hq,H", [(128, 3, 3), (64, 4, 1), (128, 8, 2)])
+def test_attention_many_tiles(D, Hq, H):
+    """More units than the GPU has CUs, the last of them shared out over workgroups, packed and
+    equal; every row against the definition on a sample of rows."""
+    from flashvsr_sm89_ops import paged_attention
+    new, lens = [5000, 900, 64], [6000, 4900, 3000]
+    T = sum(new) * 3 if Hq == H else sum(new)
+    new = [n * T // sum(new) for n in new]
+    lens = [max(a, b) for a, b in zip(lens, new)]
+    T = sum(new)
+    table, N = tables(lens)
+    pages = pool(N, H, D)
+    q = torch.randn(T, Hq, D, generator=gen(2)).bfloat16()
+    cu = starts(new)
+    for causal in (True, False):
+        out = paged_attention(q.to(DEV), pages, table.to(DEV), i32(lens).to(DEV), cu.to(DEV),
+                              causal=causal).cpu()
+        cache = O.from_pages(*pages)
+        for b, (lo, n) in enumerate(O.rows_of(T, 3, cu)):
+            some = sorted({0, 1, n // 3, n // 2, n - 2, n - 1})
+            for i in some:
+                # one row alone, at its position: a sequence that ends there (causal) or not
+                L = lens[b] - n + i + 1 if causal else lens[b]
+                one = q[lo + i:lo + i + 1]
+                check_attention(out[lo + i:lo + i + 1], one, cache, table[b:b + 1], [L],
+                                causal=False)
 
 
 def test_attention_many_small_weights():
