@@ -204,6 +204,27 @@ FVSR_DEV int row_limit(const Args& a, const SeqPart& s, int i) {
 
 FVSR_DEV int range_at(int pages, int s, int splits) { return (int)((int64_t)pages * s / splits); }
 
+// The tile-th of all sequences' tiles of ROWS rows, n * pack rows to a sequence.
+template <int ROWS>
+FVSR_DEV bool tile_of(const Args& a, int tile, int pack, SeqPart& s) {
+  const auto tiles_of = [pack](int n, int) { return (n * pack + ROWS - 1) / ROWS; };
+  if (a.c.cu)
+    return find_part(a.c.cu, a.c.lengths, (int)a.c.sequences, a.T, tile, a.tail != 0, tiles_of, s);
+  const int each = a.tiles / (int)a.c.sequences;
+  s.b = tile / each;
+  s.part = tile % each;
+  s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
+  s.len = max(a.c.lengths[s.b], 0);
+  return true;
+}
+
+// Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous range of
+// `total` units, whose neighbours read the same pages.
+FVSR_DEV int xcd_order(int wg, int total) {
+  const int per = total / 8, rem = total % 8, xcd = wg % 8, loc = wg / 8;
+  return xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
+}
+
 // ---------------------------------------------------------------------------
 // attend_few.  Operand layout of v_mfma_scale_f32_16x16x128: lane (r, g) = (l %
 // 16, l / 16) holds positions 16 g .. and 64 + 16 g .. (16 each) of row r; the
@@ -221,17 +242,27 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   __shared__ float lds_ml[4][16][2];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x, H = (int)a.c.heads;
-  const int h = blockIdx.y;
+  const int H = (int)a.c.heads;
+  int split, h;
   SeqPart s;
-  s.b = blockIdx.z;
-  s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
-  s.len = max(a.c.lengths[s.b], 0);
-  const int rows = s.rows.n * a.group, r = min(col, rows - 1);
+  if (!a.c.cu) {  // one unit to a sequence and head
+    split = blockIdx.x, h = blockIdx.y;
+    s.b = blockIdx.z, s.part = 0;
+    s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
+    s.len = max(a.c.lengths[s.b], 0);
+  } else {
+    // Units are 16 rows of a sequence; those of one sequence, head and split are
+    // neighbours on one XCD, which read the same pages.
+    const int at = xcd_order(blockIdx.x, gridDim.x);
+    split = at / a.tiles % a.splits, h = at / a.tiles / a.splits;
+    if (!tile_of<16>(a, at % a.tiles, a.group, s)) return;
+  }
+  const int rows = s.rows.n * a.group, row0 = s.part * 16, row1 = min(row0 + 16, rows);
+  const int r = min(row0 + col, rows - 1);
   const int qi = r / a.group, hq = h * a.group + r % a.group;
   const int limit = row_limit(a, s, qi);
-  const int lim_lo = row_limit(a, s, 0);
-  const int lim_hi = row_limit(a, s, s.rows.n - 1);
+  const int lim_lo = row_limit(a, s, row0 / a.group);
+  const int lim_hi = row_limit(a, s, (row1 - 1) / a.group);
   const int pages = (lim_hi + kPage - 1) / kPage;
   const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
   const int32_t* const table = a.c.table + s.b * a.c.table_stride;
@@ -393,18 +424,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   if (g == 0) lds_ml[wave][col][0] = m, lds_ml[wave][col][1] = l;
   __syncthreads();
   constexpr int C = D / 8;  // threads of a row
-  const int row = threadIdx.x / C, d0 = threadIdx.x % C * 8;
-  if (row >= rows) return;
-  float top = lds_ml[0][row][0];
+  const int i = threadIdx.x / C, d0 = threadIdx.x % C * 8, row = row0 + i;
+  if (i >= 16 || row >= rows) return;
+  float top = lds_ml[0][i][0];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_ml[w][row][0]);
+  for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_ml[w][i][0]);
   float o[8] = {}, sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(lds_ml[w][row][0] - top);
-    sum += f * lds_ml[w][row][1];
-    const v4f x = *(const v4f*)&lds_o[(w * 16 + row) * P + d0];
-    const v4f y = *(const v4f*)&lds_o[(w * 16 + row) * P + d0 + 4];
+    const float f = __builtin_amdgcn_exp2f(lds_ml[w][i][0] - top);
+    sum += f * lds_ml[w][i][1];
+    const v4f x = *(const v4f*)&lds_o[(w * 16 + i) * P + d0];
+    const v4f y = *(const v4f*)&lds_o[(w * 16 + i) * P + d0 + 4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += f * x[e], o[4 + e] += f * y[e];
   }
@@ -463,6 +494,8 @@ FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void join_few(Args a) {
   const int64_t row = blockIdx.x, rows = (int64_t)a.T * a.q_heads;
+  // Rows behind the last sequence have pieces only where they are to be zeros.
+  if (a.c.cu && !a.tail && row / a.q_heads >= a.c.cu[a.c.sequences]) return;
   join_row<DT, D>(a.part + row * a.splits * D, D,
                   a.part + rows * a.splits * D + row * a.splits * 2, 2, a.splits,
                   a.out + row / a.q_heads * a.o_ts + row % a.q_heads * a.o_hs);
@@ -776,28 +809,10 @@ FVSR_DEV bool unit_of(const Args& a, int u, TileUnit& t) {
   t.head = u / a.tiles;
   t.h = a.keep ? t.head / a.group : t.head;
   // Under a causal mask later tiles see more: they go first.
-  const int tile = a.causal ? a.tiles - 1 - u % a.tiles : u % a.tiles;
-  const int pack = t.pack;
-  const auto tiles_of = [pack](int n, int) { return (n * pack + 127) / 128; };
-  if (a.c.cu) {
-    if (!find_part(a.c.cu, a.c.lengths, (int)a.c.sequences, a.T, tile, a.tail != 0, tiles_of, t.s))
-      return false;
-  } else {
-    const int each = a.tiles / (int)a.c.sequences;
-    t.s.b = tile / each;
-    t.s.part = tile % each;
-    t.s.rows = seq_rows(nullptr, t.s.b, (int)a.c.sequences, a.T);
-    t.s.len = max(a.c.lengths[t.s.b], 0);
-  }
-  t.rows = t.s.rows.n * pack;
+  if (!tile_of<128>(a, a.causal ? a.tiles - 1 - u % a.tiles : u % a.tiles, t.pack, t.s))
+    return false;
+  t.rows = t.s.rows.n * t.pack;
   return true;
-}
-
-// Workgroups go round robin over the 8 XCDs; each XCD takes a contiguous range of
-// `total` units, whose neighbours read the same pages.
-FVSR_DEV int xcd_order(int wg, int total) {
-  const int per = total / 8, rem = total % 8, xcd = wg % 8, loc = wg / 8;
-  return xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
 }
 
 template <int DT, int D>
@@ -989,7 +1004,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
       if (__ballot(w.lost) != 0) again = 1;
       __syncthreads();
       if (!again) break;
-  #pragma unroll
+#pragma unroll
       for (int d = 0; d < D / 32; ++d) w.acc[d] = v16f{};
       w.m = kNothing, w.l = 0.0f;
     }
@@ -1040,12 +1055,12 @@ int64_t cu_count() {
 
 // How a call is cut up: a function of its sizes (and the CUs) only.
 struct Plan {
-  bool few;
-  int64_t tiles;   // of 128 rows, per head, over all sequences
+  bool few;        // attend_few
+  int64_t tiles;   // of 16 or 128 rows, per head, over all sequences
   int64_t units;   // tiles of all heads
   int64_t whole;   // units done by one workgroup each; the others by `pieces` each
   int pieces;
-  int splits;      // attend_few: workgroups of a sequence and head
+  int splits;      // attend_few: workgroups of a unit
   int64_t floats(int64_t T, int64_t q_heads, int64_t D) const {
     if (few) return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
     return (units - whole) * pieces * 128 * (D + 2);
@@ -1055,37 +1070,53 @@ struct Plan {
 Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   Plan p{};
   const int64_t group = q_heads / c->heads, B = c->sequences, cus = cu_count();
-  p.few = !c->cu && !keep && T / B * group <= 16;
+  p.pieces = p.splits = 1;
+  // Packed rows: at most this many tiles over any counts that add up to T, the
+  // rows behind the last sequence included.
+  const auto tiles = [&](int64_t pack, int64_t rows) {
+    return c->cu ? T * pack / rows + B + 1 : B * ((T / B * pack + rows - 1) / rows);
+  };
+  // Rows of any number per sequence: where they are few on average, waiting for
+  // memory is what counts, and 16 rows to a workgroup with its waves on pages of their own
+  // wait less than 128 with one stream of pages, even if some units read the same pages (32
+  // sequences of 7.5 tokens x 32 / 8 heads 168 -> 134 us, 16 of 14 x 16 / 4 44 -> 24).
+  // The same number for each: only if one such unit holds them (20 rows 64 against 53).
+  p.few = !keep && T * group <= B * (c->cu ? 64 : 16);
   if (p.few) {
+    p.tiles = tiles(group, 16);
+    p.units = p.tiles * c->heads;
     // Sequences may be of any lengths: 16 workgroups per CU even them out (128
     // ragged sequences of up to 16000 tokens, us at 4 / 8 / 16 / 32: 390, 376, 364, 374).
     // Two pages to a wave, or one where that would leave CUs idle (20000 tokens x 12
     // heads 20.5 against 23.8 us; 4 sequences of 5000 x 2 heads 14.6 against 12.1).
-    const int64_t units = B * c->heads, pages = c->table_pages;
-    const int64_t each = units * (pages / 8) * 2 < cus ? 4 : 8;
-    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 16 * cus / units),
+    const int64_t pages = c->table_pages;
+    const int64_t each = p.units * (pages / 8) * 2 < cus ? 4 : 8;
+    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 16 * cus / p.units),
                                        std::max<int64_t>(1, pages / each), kMaxSplits});
     return p;
   }
   const int64_t pack = keep ? 1 : group;
-  // Packed rows: at most this many tiles over any counts that add up to T, the
-  // rows behind the last sequence included.
-  p.tiles = c->cu ? T * pack / 128 + B + 1 : B * ((T / B * pack + 127) / 128);
+  p.tiles = tiles(pack, 128);
   p.units = p.whole = p.tiles * (keep ? q_heads : c->heads);
-  p.pieces = 1;
-  // A CU is nearly as fast with one workgroup as with two, so it is whole units
-  // per CU that must come out even: the units past a multiple of the CUs are cut into
-  // pieces, as many as two per CU take at once.  A page costs a workgroup 1.8 us; a
-  // piece 132 KB written and read again (0.04 us of the GPU's time), and all of them
-  // the joining launch.
-  const int64_t rest = p.units % cus;
-  if (rest == 0) return p;
-  const int64_t pieces = std::min<int64_t>({2 * cus / rest, c->table_pages / 4, 16});
-  if (pieces < 2) return p;
-  const int64_t saved = c->table_pages - c->table_pages / pieces;
-  if (18 * saved < 80 + rest * pieces * 4 / 10) return p;
-  p.pieces = (int)pieces;
-  p.whole = p.units - rest;
+  // The units past a multiple of the slots (a CU is nearly as fast with one
+  // workgroup as with two, so it is whole units per CU that must come out even) are cut
+  // into the number of pieces that is done first, by prices from measured calls: 1.9 us
+  // a page; a workgroup's start like 3 pages; for pieces 5 us of joining launch, and 0.03
+  // us of the GPU's time for each piece of 128 rows written and read again.  Few rows
+  // leave the page loop waiting for memory: two workgroups then share a CU at full speed,
+  // and every unit may be cut.
+  const int64_t rows_of = std::min<int64_t>(128, (T * pack + B - 1) / B);
+  const int64_t slots = rows_of <= 64 ? 2 * cus : cus, pages = c->table_pages;
+  const int64_t rest = rows_of <= 64 ? p.units : p.units % cus;
+  double best = 0;
+  for (int64_t n = 1; n <= std::min<int64_t>(16, std::max<int64_t>(1, pages / 2)); ++n) {
+    const double us = (double)((rest * n + slots - 1) / slots) * (pages / (double)n + 3) * 1.9 +
+                      (n > 1 ? 5 + rest * n * rows_of * (0.03 / 128) : 0);
+    if (n > 1 && us >= best) continue;
+    best = us;
+    p.pieces = (int)n;
+  }
+  if (p.pieces > 1) p.whole = p.units - rest;
   return p;
 }
 
@@ -1093,9 +1124,10 @@ template <int DT, int D>
 void launch(const Args& a, const Plan& p, hipStream_t st) {
   const dim3 block(kThreads);
   if (p.few) {
-    hipLaunchKernelGGL((attend_few<DT, D>),
-                       dim3((unsigned)a.splits, (unsigned)a.c.heads, (unsigned)a.c.sequences),
-                       block, 0, st, a);
+    const dim3 grid = a.c.cu ? dim3((unsigned)(p.units * p.splits))
+                             : dim3((unsigned)p.splits, (unsigned)a.c.heads,
+                                    (unsigned)a.c.sequences);
+    hipLaunchKernelGGL((attend_few<DT, D>), grid, block, 0, st, a);
     if (p.splits > 1)
       hipLaunchKernelGGL((join_few<DT, D>), dim3((unsigned)((int64_t)a.T * a.q_heads)), block,
                          0, st, a);
@@ -1140,9 +1172,8 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
   if (T * q_heads > 0x7fffffff - 256) return FVSR_EUNSUPPORTED;
   const Plan p = plan_attn(cache, T, q_heads, keep != nullptr);
   if (p.units > kMaxBlocks / 2 || T * q_heads > kMaxBlocks * 64 ||
-      (p.few && (cache->heads > 65535 || cache->sequences > 65535 ||
-                 p.splits * cache->heads * cache->sequences > kMaxBlocks ||
-                 (p.splits > 1 && T * q_heads > kMaxBlocks))))
+      (p.few && (cache->heads > 65535 || (!cache->cu && cache->sequences > 65535) ||
+                 p.units * p.splits > kMaxBlocks || (p.splits > 1 && T * q_heads > kMaxBlocks))))
     return FVSR_EUNSUPPORTED;
   const int64_t need = p.floats(T, q_heads, cache->head_dim);
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;

@@ -603,6 +603,27 @@ def test_attention_split(D, Hq, H, n):
         assert torch.equal(out, paged_attention(*args))
 
 
+@pytest.mark.parametrize("new,Hq", [([2, 1, 0, 5], 4), ([20, 0, 33, 1], 2), ([90, 70, 1, 2], 4)])
+def test_attention_packed_split(new, Hq):
+    """Packed rows, few and many, whose pages are shared out over workgroups, with rows behind
+    the last sequence."""
+    from flashvsr_sm89_ops import paged_attention
+    H, D, lens = 2, 128, [128 * 40 + 3, 900, 50, 128 * 30]
+    T = sum(new) + 5
+    table, N = tables(lens)
+    pages = pool(N, H, D)
+    q = torch.randn(T, Hq, D, generator=gen(3)).bfloat16()
+    args = (q.to(DEV), pages, table.to(DEV), i32(lens).to(DEV), starts(new).to(DEV))
+    for causal in (True, False):
+        out = paged_attention(*args, causal=causal)
+        check_attention(out, q, pages, table, lens, starts(new), causal)
+        assert int(torch.count_nonzero(out[sum(new):])) == 0
+        given = torch.full_like(out, 7.0)
+        paged_attention(*args, causal=causal, out=given)
+        assert torch.equal(given[:sum(new)], out[:sum(new)])
+        assert bool((given[sum(new):] == 7).all())
+
+
 def test_attention_bad_pages():
     """A page id outside the pool makes the rows that read it NaN, and no others."""
     from flashvsr_sm89_ops import paged_attention
