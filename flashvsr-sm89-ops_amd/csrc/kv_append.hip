@@ -277,7 +277,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
   constexpr int C = kLanes<D>, R = kTokens<D>;
   const int tid = threadIdx.x, H = (int)a.c.heads;
   uint8_t* const sp = (uint8_t*)a.c.k_scale + j.ph;
-  const int old = *sp - 127;
+  const int held = *sp;  // (its use waits for it: after the rows' loads)
   // Row norms that no launch before has summed: a wave per token.
   if (a.k_norm == kRow && !a.row_stat) {
     for (int i = j.lo + (tid >> 6); i < j.hi; i += 4) {
@@ -296,7 +296,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
     // All positions and rows go out together, then all rotations: a load
     // behind a load eight times over took 22 of a 57 us call (16896 tokens x 12 heads).
     Raw8<DT> raw[R];
-    constexpr int Q = 4;  // rotations in flight
+    constexpr int Q = D == 64 ? 1 : 4;  // rotations in flight (registers)
     Raw8<FVSR_DT_F32> turn[Q];
     int pos[R];
 #pragma unroll
@@ -346,6 +346,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
         if (slot0 + i >= j.lo && slot0 + i < j.hi) t = fmaxf(t, finite_abs(x[i][k]));
     return t;
   }));
+  const int old = held - 127;
   if (j.lo > 0) e = max(e, old);
   if (tid == 0) *sp = (uint8_t)(e + 127);
   uint8_t* const page = (uint8_t*)a.c.k + j.ph * kPage * D;
@@ -369,7 +370,7 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
   constexpr int C = kLanes<D>, R = kTokens<D>;
   const int tid = threadIdx.x;
   uint8_t* const sp = (uint8_t*)a.c.v_scale + j.ph;
-  const int old = *sp - 127;
+  const int held = *sp;  // (its use waits for it: after the rows' loads)
   const int d0 = (tid % C) * 8, slot0 = tid / C * R;
   Raw8<DT> raw[R];
   float top = 0.0f;
@@ -399,6 +400,7 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
     }
     return t;
   }));
+  const int old = held - 127;
   if (j.lo > 0) e = max(e, old);
   if (tid == 0) *sp = (uint8_t)(e + 127);
   // [dim][token]: a thread's R tokens of a dim are one unit of R bytes; unit u
@@ -418,20 +420,33 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
   }
   __syncthreads();
   uint8_t* const page = (uint8_t*)a.c.v + j.ph * kPage * D;
-#pragma unroll
-  for (int it = 0; it < D * (kPage / 16) / kThreads; ++it) {
-    const int idx = it * kThreads + tid, d = idx / (kPage / 16), s0 = idx % (kPage / 16) * 16;
-    const bool grow = s0 < j.lo && e != old;  // held codes to round again
-    if ((s0 + 16 <= j.lo && !grow) || s0 >= j.hi) continue;
+  const auto piece = [&](int d, int s0) {  // 16 tokens' codes of a dim
     u32x4_t c;
 #pragma unroll
     for (int g = 0; g < 16 / R; ++g)
       __builtin_memcpy((uint8_t*)&c + g * R,
                        __builtin_assume_aligned(vt_at(d, s0 / R + g), R), R);
+    return c;
+  };
+  constexpr int P = kPage / 16;  // pieces of a dim
+  if (j.lo == 0 && j.hi == kPage) {
+#pragma unroll
+    for (int it = 0; it < D * P / kThreads; ++it) {
+      const int idx = it * kThreads + tid, d = idx / P, s0 = idx % P * 16;
+      *(u32x4_t*)(page + d * kPage + s0) = piece(d, s0);
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int idx = tid; idx < D * P; idx += kThreads) {
+    const int d = idx / P, s0 = idx % P * 16;
+    const bool grow = s0 < j.lo && e != old;  // held codes to round again
+    if ((s0 + 16 <= j.lo && !grow) || s0 >= j.hi) continue;
     uint8_t* const p = page + d * kPage + s0;
     if (s0 >= j.lo && s0 + 16 <= j.hi) {
-      *(u32x4_t*)p = c;
+      *(u32x4_t*)p = piece(d, s0);
     } else if (grow) {
+      const u32x4_t c = piece(d, s0);
       u32x4_t o = *(const u32x4_t*)p;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -447,9 +462,9 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
       }
       *(u32x4_t*)p = o;
     } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (s0 + k >= j.lo && s0 + k < j.hi) p[k] = (uint8_t)(c[k >> 2] >> (8 * (k & 3)));
+#pragma unroll 1
+      for (int k = max(j.lo - s0, 0); k < min(j.hi - s0, 16); ++k)
+        p[k] = vt_at(d, (s0 + k) / R)[(s0 + k) % R];
     }
   }
 }
@@ -547,82 +562,139 @@ FVSR_DEV void load2(const void* p, int64_t i, float (&x)[2]) {
   }
 }
 
-// The step of one token per sequence: a wave per (sequence, head), of k and v
-// or of q, two dims a lane (64 dims: the upper lanes repeat the lower ones).  It is
-// all latency: the row, lengths and positions load at once, then the page id and
-// the rotation, then the page's scales; a norm over the row is summed by
-// every wave for itself.  A page whose scale grows (rare: a power of two) has its held
-// codes rounded again by the wave.
-template <int DT, int D>
+// Norm and rotation of two dims d0, d0 + 1 of a head of N tokens t, a wave per head; `ts`,
+// `hs` and `heads` describe the rows of src (q or k).  Each kind of load goes out
+// for all tokens at once.
+template <int DT, int D, int N>
+FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int heads,
+                    const void* weight, int norm, const int (&t)[N], int h, int d0,
+                    float (&x)[N][2]) {
+  const int lane = threadIdx.x & 63;
+  int pos[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) pos[i] = a.positions ? a.positions[t[i]] : t[i];
+  float sq[N] = {}, cs[N][2];
+  if (norm == kRow) {
+    for (int c = lane; c < heads * (D / 8); c += 64) {
+      const int64_t at = (c / (D / 8)) * hs + (c % (D / 8)) * 8;
+      Raw8<DT> raw[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = load_raw<DT>(src, t[i] * ts + at);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float r[8];
+        widen(raw[i], r);
+        sq[i] += sum_sq(r);
+      }
+    }
+  } else if (norm == kHead) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      sq[i] = lane * 2 < D ? x[i][0] * x[i][0] + x[i][1] * x[i][1] : 0.0f;
+  }
+  if (a.cs) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = pos[i] >= 0 && pos[i] < a.cs_rows;
+      const float* p = a.cs + (int64_t)(in ? pos[i] : 0) * D + d0;
+      cs[i][0] = in ? p[0] : __builtin_nanf("");
+      cs[i][1] = p[1];
+    }
+  }
+  if (norm != kNone) {
+    float w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      w[e] = ld_elem(weight, a.w_dt, (norm == kRow ? h * D : 0) + d0 + e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float r = inv_rms(wave_sum(sq[i]), norm == kRow ? heads * D : D, a.eps);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[i][e] = x[i][e] * r * w[e];
+    }
+  }
+  if (a.cs) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float b = x[i][0];
+      x[i][0] = __builtin_fmaf(b, cs[i][0], -(x[i][1] * cs[i][1]));
+      x[i][1] = __builtin_fmaf(b, cs[i][1], x[i][1] * cs[i][0]);
+    }
+  }
+}
+
+// The step of at most N tokens per sequence, the same number for each: a wave per
+// (page of a sequence, head), of k and v, or per q head of a token; two dims a lane (64
+// dims: the upper lanes repeat the lower ones).  It is all latency: one token's row, lengths
+// and positions load at once, then the page id and the rotation, then the page's
+// scales; a norm over the row is summed by every wave for itself.  A page whose scale
+// grows (rare: a power of two) has its held codes rounded again by the wave.  64 x 5 tokens,
+// 32 / 8 heads: 17.7 us by pages as a prompt's, 11.1 so.
+template <int DT, int D, int N>
 __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
   const int lane = threadIdx.x & 63, d0 = lane * 2 % D;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int parts = N == 1 ? 1 : 2;  // pages that a sequence's tokens can touch
   const int H = (int)a.c.heads, unit = blockIdx.x * 4 + wave;
-  if (unit >= a.T * (H + a.q_heads)) return;
-  const bool is_q = unit >= a.T * H;
-  const int heads = is_q ? a.q_heads : H, u = is_q ? unit - a.T * H : unit;
-  const int t = u / heads, h = u % heads;
-  const int len = is_q ? 0 : max(a.c.lengths[t], 0);
-  const int64_t ts = is_q ? a.q_ts : a.k_ts, hs = is_q ? a.q_hs : a.k_hs;
-  const void* const src = is_q ? a.q : a.k;
-  const int norm = is_q ? a.q_norm : a.k_norm;
-  float x[2], y[2] = {}, cs[2] = {1.0f, 0.0f};
-  load2<DT>(src, t * ts + h * hs + d0, x);
-  if (!is_q) load2<DT>(a.v, t * a.v_ts + h * a.v_hs + d0, y);
-  if (a.cs) {
-    const int64_t p = a.positions ? (int64_t)a.positions[t] : t;
-    if (p >= 0 && p < a.cs_rows)
-      cs[0] = a.cs[p * D + d0], cs[1] = a.cs[p * D + d0 + 1];
-    else
-      cs[0] = cs[1] = __builtin_nanf("");
-  }
-  if (norm != kNone) {
-    const void* const wp = is_q ? a.q_weight : a.k_weight;
-    const int64_t w0 = (norm == kRow ? h * D : 0) + d0;
-    const float sq = norm == kRow ? row_sq<DT, D>(src, t * ts, hs, heads)
-                                  : wave_sum(lane * 2 < D ? x[0] * x[0] + x[1] * x[1] : 0.0f);
-    const float r = inv_rms(sq, norm == kRow ? heads * D : D, a.eps);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) x[e] = x[e] * r * ld_elem(wp, a.w_dt, w0 + e);
-  }
-  if (a.cs) {
-    const float b = x[0];
-    x[0] = __builtin_fmaf(b, cs[0], -(x[1] * cs[1]));
-    x[1] = __builtin_fmaf(b, cs[1], x[1] * cs[0]);
-  }
-  if (is_q) {
-    if (lane * 2 < D) {
-      const int64_t o = (int64_t)u * D + d0;
-      if constexpr (DT == FVSR_DT_F32) {
-        ((float*)a.q_out)[o] = x[0], ((float*)a.q_out)[o + 1] = x[1];
-      } else {
-        const uint32_t c =
-            DT == FVSR_DT_F16
-                ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[0]) |
-                      (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[1]) << 16
-                : pack_bf16x2(x[0], x[1]);
-        *(uint32_t*)((uint16_t*)a.q_out + o) = c;
-      }
+  const int B = (int)a.c.sequences, kv_units = B * parts * H;
+  if (unit >= kv_units + a.T * a.q_heads) return;
+  if (unit >= kv_units) {
+    const int u = unit - kv_units, t[1] = {u / a.q_heads}, h = u % a.q_heads;
+    float xs[1][2];
+    float(&x)[2] = xs[0];
+    load2<DT>(a.q, t[0] * a.q_ts + h * a.q_hs + d0, x);
+    turn2<DT, D, 1>(a, a.q, a.q_ts, a.q_hs, a.q_heads, a.q_weight, a.q_norm, t, h, d0, xs);
+    if (lane * 2 >= D) return;
+    const int64_t o = (int64_t)u * D + d0;
+    if constexpr (DT == FVSR_DT_F32) {
+      ((float*)a.q_out)[o] = x[0], ((float*)a.q_out)[o + 1] = x[1];
+    } else {
+      const uint32_t c = DT == FVSR_DT_F16
+                             ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[0]) |
+                                   (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x[1]) << 16
+                             : pack_bf16x2(x[0], x[1]);
+      *(uint32_t*)((uint16_t*)a.q_out + o) = c;
     }
     return;
   }
-  const int page = (len - 1) / kPage, slot = (len - 1) % kPage;
-  if (len == 0 || page >= a.c.table_pages) return;
-  const int64_t id = __builtin_amdgcn_readfirstlane(a.c.table[t * a.c.table_stride + page]);
+  const int b = unit / H / parts, part = unit / H % parts, h = unit % H;
+  const int n = N == 1 ? 1 : a.T / B, len = max(a.c.lengths[b], 0), at = len - n;
+  const int page = max(at, 0) / kPage + part;
+  const int lo = max(max(at, 0), page * kPage) - page * kPage, hi = min(len - page * kPage, kPage);
+  if (N > 1 && hi <= lo) return;
+  // Tokens of slots lo .. hi - 1, the last one repeated.
+  int t[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    t[i] = N == 1 ? b : b * n + page * kPage - at + lo + min(i, hi - lo - 1);
+  float x[N][2], y[N][2], kt = 0.0f, vt = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    load2<DT>(a.k, t[i] * a.k_ts + h * a.k_hs + d0, x[i]);
+    load2<DT>(a.v, t[i] * a.v_ts + h * a.v_hs + d0, y[i]);
+  }
+  turn2<DT, D, N>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, t, h, d0, x);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      kt = fmaxf(kt, finite_abs(x[i][e])), vt = fmaxf(vt, finite_abs(y[i][e]));
+  if (hi <= lo || page >= a.c.table_pages) return;
+  const int64_t id = __builtin_amdgcn_readfirstlane(a.c.table[b * a.c.table_stride + page]);
   if (id < 0 || id >= a.c.pages) return;
   const int64_t ph = id * H + h;
   uint8_t* const ksp = (uint8_t*)a.c.k_scale + ph;
   uint8_t* const vsp = (uint8_t*)a.c.v_scale + ph;
   const int k_old = *ksp - 127, v_old = *vsp - 127;
-  int ke = scale_exp(__float_as_uint(wave_max_abs(fmaxf(finite_abs(x[0]), finite_abs(x[1])))));
-  int ve = scale_exp(__float_as_uint(wave_max_abs(fmaxf(finite_abs(y[0]), finite_abs(y[1])))));
-  if (slot > 0) ke = max(ke, k_old), ve = max(ve, v_old);
+  int ke = scale_exp(__float_as_uint(wave_max_abs(kt)));
+  int ve = scale_exp(__float_as_uint(wave_max_abs(vt)));
+  if (lo > 0) ke = max(ke, k_old), ve = max(ve, v_old);
   uint8_t* const kp = (uint8_t*)a.c.k + ph * kPage * D;
   uint8_t* const vp = (uint8_t*)a.c.v + ph * kPage * D;
-  if (slot > 0 && (ke != k_old || ve != v_old)) {
+  if (lo > 0 && (ke != k_old || ve != v_old)) {
     if (ke != k_old) {
       const float f = pow2(k_old - ke);
-      for (int c = lane; c < slot * (D / 16); c += 64) {
+      for (int c = lane; c < lo * (D / 16); c += 64) {
         u32x4_t* const p = (u32x4_t*)(kp + c * 16);
         u32x4_t o = *p;
 #pragma unroll
@@ -632,40 +704,48 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     }
     if (ve != v_old) {
       const float f = pow2(v_old - ve);
-      const int per = (slot + 15) / 16;  // pieces of a dim with held tokens
+      const int per = (lo + 15) / 16;  // pieces of a dim with held tokens
       for (int c = lane; c < D * per; c += 64) {
         const int s0 = c % per * 16;
         u32x4_t* const p = (u32x4_t*)(vp + c / per * kPage + s0);
         u32x4_t o = *p;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int held = min(max(slot - s0 - 4 * g, 0), 4);  // of these four
+          const int held = min(max(lo - s0 - 4 * g, 0), 4);  // of these four
           const uint32_t m = held == 4 ? ~0u : (1u << (8 * held)) - 1;
           o[g] = (rescale4(o[g], f) & m) | (o[g] & ~m);
         }
         *p = o;
       }
     }
-    __builtin_amdgcn_s_waitcnt(0);  // before the new token goes into the same pieces
+    __builtin_amdgcn_s_waitcnt(0);  // before the new tokens go into the same pieces
   }
-  if (lane * 2 < D) {
-    *(uint16_t*)(kp + slot * D + d0) = (uint16_t)codes4(x[0], x[1], 0.0f, 0.0f, pow2(ke));
-    const uint32_t c = codes4(y[0], y[1], 0.0f, 0.0f, pow2(ve));
+  if (lane * 2 >= D) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (N > 1 && i >= hi - lo) continue;
+    const int slot = lo + i;
+    *(uint16_t*)(kp + slot * D + d0) =
+        (uint16_t)codes4(x[i][0], x[i][1], 0.0f, 0.0f, pow2(ke));
+    const uint32_t c = codes4(y[i][0], y[i][1], 0.0f, 0.0f, pow2(ve));
     vp[d0 * kPage + slot] = (uint8_t)c;
     vp[(d0 + 1) * kPage + slot] = (uint8_t)(c >> 8);
-    if (lane == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
   }
+  if (lane == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
 }
+
+constexpr int kFew = 8;  // tokens per sequence that a wave takes
 
 // Tokens up to which each workgroup sums its own rows for a row norm.
 constexpr int64_t kOwnStat = 64;
 
 template <int DT, int D>
 void launch(const Args& a, int64_t units, hipStream_t st) {
-  if (!a.c.cu && a.T == a.c.sequences) {
-    const int64_t waves = a.T * (a.c.heads + a.q_heads);
-    hipLaunchKernelGGL((kv_token_kernel<DT, D>), dim3((unsigned)((waves + 3) / 4)), dim3(kThreads),
-                       0, st, a);
+  if (!a.c.cu && a.T <= kFew * a.c.sequences) {
+    const bool one = a.T == a.c.sequences;
+    const int64_t waves = (one ? 1 : 2) * a.c.sequences * a.c.heads + (int64_t)a.T * a.q_heads;
+    const auto kernel = one ? kv_token_kernel<DT, D, 1> : kv_token_kernel<DT, D, kFew>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((waves + 3) / 4)), dim3(kThreads), 0, st, a);
     return;
   }
   Args b = a;

@@ -214,6 +214,37 @@ def test_append_token_with_q(D, Hq, H, dtype, norm, packed):
     check_append(pages, before, k, v, table, lengths, cu, fr, pos, kw)
 
 
+@pytest.mark.parametrize("D,Hq,H", [(64, 3, 3), (128, 6, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("norm", ["none", "head", "row"])
+@pytest.mark.parametrize("n", [2, 5, 8, 9])
+def test_append_few_tokens(D, Hq, H, dtype, norm, n):
+    """A few tokens for each sequence, within a page, over a border, from its start, behind
+    position 0; held codes of small pages are rounded again."""
+    from flashvsr_sm89_ops import append_kv
+    lengths, g = [n, 128, 130, 77, 1, 256, 128 + n], gen(D)
+    B = len(lengths)
+    table, N = tables(lengths, seed=1)
+    table[3, 0] = N
+    pages = pool(N, H, D, seed=2)
+    pages.k_scale.view(torch.uint8)[::2] -= 9
+    pages.v_scale.view(torch.uint8)[::2] -= 9
+    before = O.from_pages(*pages)
+    q, k, v = (torch.randn(B * n, h, D, generator=g).to(dtype) for h in (Hq, H, H))
+    kw = qw = None
+    if norm != "none":
+        kw = 1 + 0.2 * torch.randn(D * (H if norm == "row" else 1), generator=g)
+        qw = 1 + 0.2 * torch.randn(D * (Hq if norm == "row" else 1), generator=g)
+    fr = freqs_of(300, D)
+    pos = torch.cat([torch.arange(L - n, L) for L in lengths]).clamp(min=0).int()
+    out = append_kv(pages, k.to(DEV), v.to(DEV), table.to(DEV), i32(lengths).to(DEV),
+                    freqs_cis=fr.to(DEV), positions=pos.to(DEV),
+                    k_weight=None if kw is None else kw.to(DEV), q=q.to(DEV),
+                    q_weight=None if qw is None else qw.to(DEV))
+    check_q(out, q, fr, pos, qw)
+    check_append(pages, before, k, v, table, lengths, None, fr, pos, kw)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_append_token_special_values(D):
     """As test_append_special_values, a token at a time."""
