@@ -7,6 +7,9 @@ libfvsr.so through a C ABI (include/fvsr.h).  Importing the package installs
 the HIP-backed ``block_sparse_attn`` module (see compat_bsa), so import it
 before diffsynth, whose DiT imports block_sparse_attn at module load.
 
+Beside the reference's ops: an 8-bit paged K/V cache and its attention
+(``kv_pages``, ``append_kv``, ``paged_attention``).
+
 What differs from the reference package at its public surface:
 - the tiling helpers (``plan_tiles``, ``render_tiled``, ``auto_tile_limits``,
   ``tile_weight``) are not part of this build: they drive the pipeline over
