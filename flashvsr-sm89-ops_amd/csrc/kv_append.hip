@@ -15,7 +15,7 @@
 //
 // One workgroup per (page, head) and k or v: a page's scale needs all of its new
 // tokens at once, and 128 x 128 values fit a workgroup's registers, so they are
-// read once.  Thread t holds dims 8*(t % (D/8)).. of R consecutive tokens; v's codes
+// read once.  Thread t holds dims 8*(t % (D/8)).. of 4 consecutive tokens; v's codes
 // turn to [dim][token] through LDS.  The q rows are further workgroups of the
 // same launch.  An RMSNorm over whole rows needs other heads' values: the rows'
 // statistics come from a launch before (which also does q), or, for a few
@@ -27,7 +27,10 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // kv_token_kernel
+constexpr int kTokens = 4;     // tokens of a thread of a page's workgroup
+template <int D>
+constexpr int kWg = kPage / kTokens * (D / 8);  // its threads: 512 or 256
 enum { kNone = FVSR_NORM_NONE, kHead = FVSR_NORM_HEAD, kRow = FVSR_NORM_ROW };
 
 struct Args {
@@ -200,9 +203,9 @@ FVSR_DEV void q_row(const Args& a, int t) {
 template <int DT, int D>
 FVSR_DEV void q_rows(const Args& a, int64_t wg) {
   if (a.q_norm == kRow)
-    q_row<DT, D>(a, (int)(wg * 4 + (threadIdx.x >> 6)));
+    q_row<DT, D>(a, (int)(wg * (kWg<D> / 64) + (threadIdx.x >> 6)));
   else
-    q_chunk<DT, D>(a, wg * kThreads + threadIdx.x);
+    q_chunk<DT, D>(a, wg * kWg<D> + threadIdx.x);
 }
 
 // Scale exponent of a largest magnitude, given as its (finite) bits: 448 =
@@ -238,21 +241,18 @@ struct Job {
   int64_t ph;
 };
 
-// Threads of a token, and consecutive tokens of a thread: 16 and 8, or 8 and 4.
-template <int D>
-constexpr int kLanes = D / 8;
-template <int D>
-constexpr int kTokens = kPage / (kThreads / kLanes<D>);
-
 // The largest of all threads' magnitudes (not NaN), as bits.  An infinity among
 // them: once more over the finite ones, of which again() gives a thread's largest.
-template <class Again>
-FVSR_DEV uint32_t page_top(float top, float (&lds)[4], Again again) {
+template <int W, class Again>
+FVSR_DEV uint32_t page_top(float top, float (&lds)[W], Again again) {
   const auto reduce = [&](float t) {
     t = wave_max_abs(t);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = t;
     __syncthreads();
-    return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+    float m = lds[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) m = fmaxf(m, lds[w]);
+    return m;
   };
   top = reduce(top);
   if (__builtin_isinf(top)) {
@@ -273,14 +273,15 @@ FVSR_DEV void rows_of(const Job& j, Body body) {
 }
 
 template <int DT, int D>
-FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float (&tops)[4]) {
-  constexpr int C = kLanes<D>, R = kTokens<D>;
+FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
+                       float (&tops)[kWg<D> / 64]) {
+  constexpr int C = D / 8, R = kTokens;
   const int tid = threadIdx.x, H = (int)a.c.heads;
   uint8_t* const sp = (uint8_t*)a.c.k_scale + j.ph;
   const int held = *sp;  // (its use waits for it: after the rows' loads)
   // Row norms that no launch before has summed: a wave per token.
   if (a.k_norm == kRow && !a.row_stat) {
-    for (int i = j.lo + (tid >> 6); i < j.hi; i += 4) {
+    for (int i = j.lo + (tid >> 6); i < j.hi; i += kWg<D> / 64) {
       const float r = inv_rms(row_sq<DT, D>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
       if ((tid & 63) == 0) stat[i] = r;
     }
@@ -296,7 +297,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
     // All positions and rows go out together, then all rotations: a load
     // behind a load eight times over took 22 of a 57 us call (16896 tokens x 12 heads).
     Raw8<DT> raw[R];
-    constexpr int Q = D == 64 ? 1 : 4;  // rotations in flight (registers)
+    constexpr int Q = D == 64 ? 1 : 2;  // rotations in flight (registers)
     Raw8<FVSR_DT_F32> turn[Q];
     int pos[R];
 #pragma unroll
@@ -366,8 +367,8 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage], float 
 }
 
 template <int DT, int D>
-FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4]) {
-  constexpr int C = kLanes<D>, R = kTokens<D>;
+FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[kWg<D> / 64]) {
+  constexpr int C = D / 8, R = kTokens;
   const int tid = threadIdx.x;
   uint8_t* const sp = (uint8_t*)a.c.v_scale + j.ph;
   const int held = *sp;  // (its use waits for it: after the rows' loads)
@@ -431,14 +432,14 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[4
   constexpr int P = kPage / 16;  // pieces of a dim
   if (j.lo == 0 && j.hi == kPage) {
 #pragma unroll
-    for (int it = 0; it < D * P / kThreads; ++it) {
-      const int idx = it * kThreads + tid, d = idx / P, s0 = idx % P * 16;
+    for (int it = 0; it < D * P / kWg<D>; ++it) {
+      const int idx = it * kWg<D> + tid, d = idx / P, s0 = idx % P * 16;
       *(u32x4_t*)(page + d * kPage + s0) = piece(d, s0);
     }
     return;
   }
 #pragma unroll 1
-  for (int idx = tid; idx < D * P; idx += kThreads) {
+  for (int idx = tid; idx < D * P; idx += kWg<D>) {
     const int d = idx / P, s0 = idx % P * 16;
     const bool grow = s0 < j.lo && e != old;  // held codes to round again
     if ((s0 + 16 <= j.lo && !grow) || s0 >= j.hi) continue;
@@ -505,7 +506,7 @@ FVSR_DEV void page_part(const Args& a, int wg) {
   j.row0 = s.rows.lo + page * kPage - at;
   j.h = part / n;
   j.ph = id * H + j.h;
-  __shared__ float tops[4];
+  __shared__ float tops[kWg<D> / 64];
   if constexpr ((KINDS & kValues) != 0) {
     __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
     if (n == 1 || part % n) return append_v<DT, D>(a, j, vt, tops);
@@ -517,7 +518,7 @@ FVSR_DEV void page_part(const Args& a, int wg) {
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
+__global__ __launch_bounds__(kWg<D>) void kv_append_kernel(Args a) {
   if ((int)blockIdx.x < a.page_wgs)
     page_part<DT, D, kKeys | kValues>(a, blockIdx.x);
   else
@@ -527,13 +528,14 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(Args a) {
 // Row norms of many tokens take two launches: what needs no k statistics (v,
 // the q rows) beside the statistics, then k, read again.
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args a) {
-  const int stat_wgs = (a.T + 3) / 4;
+__global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
+  constexpr int W = kWg<D> / 64;
+  const int stat_wgs = (a.T + W - 1) / W;
   int wg = blockIdx.x;
   if (wg < a.page_wgs) return page_part<DT, D, kValues>(a, wg);
   wg -= a.page_wgs;
   if (wg >= stat_wgs) return q_rows<DT, D>(a, wg - stat_wgs);
-  const int t = wg * 4 + (threadIdx.x >> 6);
+  const int t = wg * W + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int H = (int)a.c.heads;
   const float r = inv_rms(row_sq<DT, D>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
@@ -541,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args a) {
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void kv_keys_kernel(Args a) {
+__global__ __launch_bounds__(kWg<D>) void kv_keys_kernel(Args a) {
   page_part<DT, D, kKeys>(a, blockIdx.x);
 }
 
@@ -751,14 +753,15 @@ void launch(const Args& a, int64_t units, hipStream_t st) {
   Args b = a;
   b.units = (int)units;
   b.page_wgs = (int)((units + 7) / 8 * 8 * a.c.heads) * (a.row_stat ? 1 : 2);
+  constexpr int W = kWg<D> / 64;
   const int64_t q_wgs =
       !a.q                ? 0
-      : a.q_norm == kRow ? (a.T + 3) / 4
-                         : ((int64_t)a.T * a.q_heads * (D / 8) + kThreads - 1) / kThreads;
-  const dim3 block(kThreads);
+      : a.q_norm == kRow ? (a.T + W - 1) / W
+                         : ((int64_t)a.T * a.q_heads * (D / 8) + kWg<D> - 1) / kWg<D>;
+  const dim3 block(kWg<D>);
   if (a.row_stat) {
     hipLaunchKernelGGL((kv_rows_kernel<DT, D>),
-                       dim3((unsigned)(b.page_wgs + (a.T + 3) / 4 + q_wgs)), block, 0, st, b);
+                       dim3((unsigned)(b.page_wgs + (a.T + W - 1) / W + q_wgs)), block, 0, st, b);
     hipLaunchKernelGGL((kv_keys_kernel<DT, D>), dim3((unsigned)b.page_wgs), block, 0, st, b);
   } else {
     hipLaunchKernelGGL((kv_append_kernel<DT, D>), dim3((unsigned)(b.page_wgs + q_wgs)), block, 0,
