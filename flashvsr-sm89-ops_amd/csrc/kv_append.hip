@@ -818,8 +818,9 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   a.units_max = (int)most(T / B);
   // Packed rows: the sum of those bounds over any B counts that add up to T.
   const int64_t units = cache->cu ? std::min(T, (T + 126 * B) / kPage + B) : B * a.units_max;
-  const int64_t q_wgs = q ? (T * q_heads * (D / 8)) / kThreads + T / 4 + 2 : 0;
-  if ((q && q_heads > kMaxBlocks) || (units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks ||
+  // Workgroups of either form of a launch, of 256 threads or twice that (kWg).
+  const int64_t q_wgs = q ? T * q_heads / 4 + T / 4 + 2 : 0;
+  if ((q && q_heads > kMaxBlocks) || (units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks / 2 ||
       T * (cache->heads + a.q_heads) > kMaxBlocks * 64)
     return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;

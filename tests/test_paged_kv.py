@@ -183,6 +183,25 @@ def test_c_entries_check_arguments():
     assert L.fvsr_paged_attn_workspace_floats(cache(head_dim=96), 4, 4, 0) == 0
 
 
+def test_launches_too_large_are_refused():
+    """A launch holds 2^32 threads; what needs more is refused before it."""
+    from flashvsr_sm89_ops import _lib
+    from flashvsr_sm89_ops.paged_kv import _Cache
+    L = _lib.lib()
+    fake = 1 << 20
+
+    def append(heads, T, B, packed=False, qh=0):
+        c = _Cache(fake, fake, fake, fake, 4, heads, 128, fake, 3, 3, fake,
+                   fake if packed else None, B)
+        return L.fvsr_kv_append(ctypes.byref(c), fake, 128 * heads, 128, fake, 128 * heads, 128,
+                                fake if qh else None, 128 * qh, 128, qh, fake if qh else None, 0,
+                                T, None, 0, None, 0, 0, 1e-6, None, 0, None, None, 0, None)
+    # 2^22 packed tokens x 2 heads: 2^24 workgroups of 512 threads
+    assert append(2, 0x3ffff0, 0x3ffff0, packed=True) == _lib.FVSR_EUNSUPPORTED
+    assert append(1, 1 << 21, 1 << 21, qh=128) == _lib.FVSR_EUNSUPPORTED  # 2^26 waves of q
+    assert append(1, 1 << 28, 1, qh=1) == _lib.FVSR_EUNSUPPORTED
+
+
 def test_definition_of_e4m3():
     """The oracle's rounding is torch's for every value between codes, and its exponent the
     least that holds a value."""
