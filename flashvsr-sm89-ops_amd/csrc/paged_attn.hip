@@ -328,7 +328,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
     const int64_t ph = id * H + h;
     const uint8_t* kp = (const uint8_t*)a.c.k + ph * kPage * D + k_off;
     const uint8_t* vp = (const uint8_t*)a.c.v + ph * kPage * D + v_off;
-    const int ks = ((const uint8_t*)a.c.k_scale)[ph], vs = ((const uint8_t*)a.c.v_scale)[ph];
+    const int ks = ((const uint8_t*)a.c.k_scale)[ph];
+    int vs = ((const uint8_t*)a.c.v_scale)[ph];
     v8i kf[8], vf[DT16];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
@@ -382,7 +383,16 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
     l += __builtin_ldexpf(sum, shift);
     if (masked) {
       // Hidden tokens weigh 0, which a NaN code would not survive: NaN codes
-      // leave the product and are counted for the rows that see them.
+      // leave the product and are counted for the rows that see them.  A NaN scale
+      // stands for a page of them.
+      if (vs == 255) {
+        asm volatile("" :::);  // a branch
+        vs = 127;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) vf[d][i] = 0x7f7f7f7f;
+      }
       bool any = false;
 #pragma unroll
       for (int d = 0; d < DT16; ++d) any |= has_nan(vf[d]);
@@ -777,7 +787,11 @@ struct RowTile {
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
         v8i f = v_operand(v, half, d);
-        if (masked && __ballot(has_nan(f)) != 0) {  // as in attend_few
+        if (masked && (vs == 255 || __ballot(has_nan(f)) != 0)) {  // as in attend_few
+          if (vs == 255) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0x7f7f7f7f;
+          }
           const v8i ones = take_nan(f);
           const v16f z = {};
           const v16f n = mfma(ones, seen, z, 127, 127);
@@ -786,7 +800,8 @@ struct RowTile {
             if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
         }
 #pragma unroll
-        for (int t = 0; t < N; ++t) acc[d] = mfma(f, pf[t], acc[d], vs, e8m0(shift - 5 * t));
+        for (int t = 0; t < N; ++t)
+          acc[d] = mfma(f, pf[t], acc[d], masked && vs == 255 ? 127 : vs, e8m0(shift - 5 * t));
       }
     }
   }

@@ -526,6 +526,26 @@ def test_attention_hidden_nan(n, Hq, D):
         assert bool(last[7]) and int(last.sum()) == 1
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,L", [(8, 130), (100, 200), (100, 460)])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_attention_hidden_nan_scale(D, n, L, which):
+    """A NaN scale makes the rows that see its page NaN and leaves the others' bits."""
+    from flashvsr_sm89_ops import paged_attention
+    H = 2
+    table, N = tables([L])
+    pages = pool(N, H, D)
+    q = torch.randn(n, H, D, generator=gen(3)).bfloat16().to(DEV)
+    args = (q, pages, table.to(DEV), i32([L]).to(DEV))
+    good = paged_attention(*args)
+    last = (L - 1) // 128
+    getattr(pages, which).view(torch.uint8)[int(table[0, last]), 1] = 255
+    out = paged_attention(*args)
+    sees = torch.arange(L - n, L) >= last * 128
+    assert bool(out[sees, 1].isnan().all()) and 0 < int(sees.sum()) < n
+    assert torch.equal(out[~sees], good[~sees]) and torch.equal(out[:, 0], good[:, 0])
+
+
 def test_attention_far_logits():
     """Large logits of either sign, one key far above all others in the last page, equal
     keys: the reference moves where it must."""
