@@ -117,17 +117,36 @@ FVSR_DEV float head_sum(float v) {
   return v;
 }
 
-// Sum of squares of a whole row of H heads by one wave.
-template <int DT, int D>
-FVSR_DEV float row_sq(const void* x, int64_t row, int64_t hs, int H) {
-  const int lane = threadIdx.x & 63;
+// A whole row of H heads by one wave: the first N pieces of eight per lane go out
+// together and stay in registers.  Returns the sum of squares.
+template <int DT, int D, int N>
+FVSR_DEV float load_row(const void* x, int64_t row, int64_t hs, int H, Raw8<DT> (&held)[N]) {
+  constexpr int C = D / 8;
+  const int lane = threadIdx.x & 63, n = H * C;
+  const auto at = [&](int c) { return row + (c / C) * hs + (c % C) * 8; };
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    held[i] = Raw8<DT>{};
+    if (lane + 64 * i < n) held[i] = load_raw<DT>(x, at(lane + 64 * i));
+  }
   float s = 0.0f;
-  for (int c = lane; c < H * (D / 8); c += 64) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
     float a[8];
-    load8(x, DT, row + (c / (D / 8)) * hs + (c % (D / 8)) * 8, a);
+    widen(held[i], a);
+    s += sum_sq(a);
+  }
+  for (int c = lane + 64 * N; c < n; c += 64) {
+    float a[8];
+    load8(x, DT, at(c), a);
     s += sum_sq(a);
   }
   return wave_sum(s);
+}
+template <int DT, int D, int N>
+FVSR_DEV float row_sq(const void* x, int64_t row, int64_t hs, int H) {
+  Raw8<DT> held[N];
+  return load_row<DT, D>(x, row, hs, H, held);
 }
 
 // A position outside the table gives NaN (every result has a cosine in it).
@@ -182,28 +201,41 @@ FVSR_DEV void q_chunk(const Args& a, int64_t chunk) {
   if (live) store8(a.q_out, DT, unit * D + d0, x);
 }
 
-// A q row with a norm over all of it: a wave per token.
-template <int DT, int D>
+// A q row with a norm over all of it: a wave per token.  (A lane's pieces are the
+// same dims of their heads, so one load of cos and sin serves them all.)
+template <int DT, int D, int N>
 FVSR_DEV void q_row(const Args& a, int t) {
   if (t >= a.T) return;
-  const int lane = threadIdx.x & 63;
-  const float r =
-      inv_rms(row_sq<DT, D>(a.q, t * a.q_ts, a.q_hs, a.q_heads), a.q_heads * D, a.eps);
-  for (int c = lane; c < a.q_heads * (D / 8); c += 64) {
-    const int h = c / (D / 8), d0 = (c % (D / 8)) * 8;
-    float x[8], w[8], cs[8] = {};
-    load8(a.q, DT, t * a.q_ts + h * a.q_hs + d0, x);
+  constexpr int C = D / 8;
+  const int lane = threadIdx.x & 63, n = a.q_heads * C, d0 = lane % C * 8;
+  float cs[8] = {};
+  if (a.cs) load_turn<D>(a, t, d0, cs);
+  Raw8<DT> held[N];
+  const float r = inv_rms(load_row<DT, D>(a.q, t * a.q_ts, a.q_hs, a.q_heads, held),
+                          a.q_heads * D, a.eps);
+  const auto put = [&](float(&x)[8], int c) {
+    float w[8];
     load8(a.q_weight, a.w_dt, c * 8, w);
-    if (a.cs) load_turn<D>(a, t, d0, cs);
     norm_turn(x, true, r, w, a.cs != nullptr, cs);
-    store8(a.q_out, DT, (int64_t)t * a.q_heads * D + c * 8, x);
+    store8(a.q_out, DT, (int64_t)t * n * 8 + c * 8, x);
+  };
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float x[8];
+    widen(held[i], x);
+    if (lane + 64 * i < n) put(x, lane + 64 * i);
+  }
+  for (int c = lane + 64 * N; c < n; c += 64) {
+    float x[8];
+    load8(a.q, DT, t * a.q_ts + (c / C) * a.q_hs + d0, x);
+    put(x, c);
   }
 }
 
-template <int DT, int D>
+template <int DT, int D, int N>
 FVSR_DEV void q_rows(const Args& a, int64_t wg) {
   if (a.q_norm == kRow)
-    q_row<DT, D>(a, (int)(wg * (kWg<D> / 64) + (threadIdx.x >> 6)));
+    q_row<DT, D, N>(a, (int)(wg * (kWg<D> / 64) + (threadIdx.x >> 6)));
   else
     q_chunk<DT, D>(a, wg * kWg<D> + threadIdx.x);
 }
@@ -235,10 +267,13 @@ FVSR_DEV uint32_t codes4(float a, float b, float c, float d, float f) {
   return __builtin_bit_cast(uint32_t, t);
 }
 
-// A page's new tokens: slots lo .. hi - 1, slot 0 being row row0 of the call; ph: (page id, head).
+// A page's new tokens: slots lo .. hi - 1, slot 0 being row row0 of the call.  The page id
+// is looked at only once the rows are on their way: it is one load more to wait for.
 struct Job {
   int lo, hi, row0, h;
-  int64_t ph;
+  int64_t id;
+  __device__ __forceinline__ bool there(const Args& a) const { return id >= 0 && id < a.c.pages; }
+  __device__ __forceinline__ int64_t ph(const Args& a) const { return id * a.c.heads + h; }
 };
 
 // The largest of all threads' magnitudes (not NaN), as bits.  An infinity among
@@ -277,12 +312,12 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
                        float (&tops)[kWg<D> / 64]) {
   constexpr int C = D / 8, R = kTokens;
   const int tid = threadIdx.x, H = (int)a.c.heads;
-  uint8_t* const sp = (uint8_t*)a.c.k_scale + j.ph;
-  const int held = *sp;  // (its use waits for it: after the rows' loads)
+  uint8_t* const scale = (uint8_t*)a.c.k_scale;
+  int held = 0;
   // Row norms that no launch before has summed: a wave per token.
   if (a.k_norm == kRow && !a.row_stat) {
     for (int i = j.lo + (tid >> 6); i < j.hi; i += kWg<D> / 64) {
-      const float r = inv_rms(row_sq<DT, D>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
+      const float r = inv_rms(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
       if ((tid & 63) == 0) stat[i] = r;
     }
     __syncthreads();
@@ -300,10 +335,12 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
     constexpr int Q = D == 64 ? 1 : 2;  // rotations in flight (registers)
     Raw8<FVSR_DT_F32> turn[Q];
     int pos[R];
+    float rs[R] = {};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
       pos[i] = a.positions ? a.positions[t] : t;
+      if (a.k_norm == kRow) rs[i] = a.row_stat ? a.row_stat[t] : stat[t - j.row0];
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -311,6 +348,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
       if (live(i))
         raw[i] = load_raw<DT>(a.k, (int64_t)(j.row0 + slot0 + i) * a.k_ts + j.h * a.k_hs + d0);
     }
+    if (j.there(a)) held = scale[j.ph(a)];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (a.cs && i % Q == 0) {
@@ -323,7 +361,6 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
       }
       widen(raw[i], x[i]);
       if (!full && __ballot(live(i)) == 0) continue;
-      const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
       float cs[8] = {};
       if (a.cs) {
         widen(turn[i % Q], cs);
@@ -331,13 +368,14 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
       }
       float r = 1.0f;
       if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
-      if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[t - j.row0];
+      if (a.k_norm == kRow) r = rs[i];
       norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
       if (!live(i)) continue;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) top = max3_abs(top, x[i][e], x[i][e + 1]);
     }
   });
+  if (!j.there(a)) return;  // no such page: dropped
   int e = scale_exp(page_top(top, tops, [&] {
     float t = 0.0f;
 #pragma unroll
@@ -349,8 +387,8 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
   }));
   const int old = held - 127;
   if (j.lo > 0) e = max(e, old);
-  if (tid == 0) *sp = (uint8_t)(e + 127);
-  uint8_t* const page = (uint8_t*)a.c.k + j.ph * kPage * D;
+  if (tid == 0) scale[j.ph(a)] = (uint8_t)(e + 127);
+  uint8_t* const page = (uint8_t*)a.c.k + j.ph(a) * kPage * D;
   const float f = pow2(e);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -370,8 +408,7 @@ template <int DT, int D>
 FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[kWg<D> / 64]) {
   constexpr int C = D / 8, R = kTokens;
   const int tid = threadIdx.x;
-  uint8_t* const sp = (uint8_t*)a.c.v_scale + j.ph;
-  const int held = *sp;  // (its use waits for it: after the rows' loads)
+  uint8_t* const scale = (uint8_t*)a.c.v_scale;
   const int d0 = (tid % C) * 8, slot0 = tid / C * R;
   Raw8<DT> raw[R];
   float top = 0.0f;
@@ -383,6 +420,8 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[k
         raw[i] = load_raw<DT>(a.v, (int64_t)(j.row0 + slot0 + i) * a.v_ts + j.h * a.v_hs + d0);
     }
   });
+  if (!j.there(a)) return;  // no such page: dropped
+  const int held = scale[j.ph(a)];  // (its use waits for it: after the rows)
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     float y[8];
@@ -403,7 +442,7 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[k
   }));
   const int old = held - 127;
   if (j.lo > 0) e = max(e, old);
-  if (tid == 0) *sp = (uint8_t)(e + 127);
+  if (tid == 0) scale[j.ph(a)] = (uint8_t)(e + 127);
   // [dim][token]: a thread's R tokens of a dim are one unit of R bytes; unit u
   // of row d sits at u ^ (d / 8 % 16), so that the D/8 threads of a token spread
   // over the banks.
@@ -420,7 +459,7 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[k
           codes4(y[0][k], y[1][k], y[2][k], y[3][k], f);
   }
   __syncthreads();
-  uint8_t* const page = (uint8_t*)a.c.v + j.ph * kPage * D;
+  uint8_t* const page = (uint8_t*)a.c.v + j.ph(a) * kPage * D;
   const auto piece = [&](int d, int s0) {  // 16 tokens' codes of a dim
     u32x4_t c;
 #pragma unroll
@@ -498,14 +537,12 @@ FVSR_DEV void page_part(const Args& a, int wg) {
   const int at = s.len - s.rows.n;          // position of the sequence's first new token
   const int page = max(at, 0) / kPage + s.part;
   if (page >= a.c.table_pages) return;      // past the table: dropped
-  const int64_t id = a.c.table[s.b * a.c.table_stride + page];
-  if (id < 0 || id >= a.c.pages) return;    // no such page: dropped
   Job j;
+  j.id = a.c.table[s.b * a.c.table_stride + page];
   j.lo = max(max(at, 0), page * kPage) - page * kPage;
   j.hi = min(s.len - page * kPage, kPage);
   j.row0 = s.rows.lo + page * kPage - at;
   j.h = part / n;
-  j.ph = id * H + j.h;
   __shared__ float tops[kWg<D> / 64];
   if constexpr ((KINDS & kValues) != 0) {
     __shared__ __attribute__((aligned(16))) uint8_t vt[D * kPage];  // v's codes, [dim][token]
@@ -522,11 +559,15 @@ __global__ __launch_bounds__(kWg<D>) void kv_append_kernel(Args a) {
   if ((int)blockIdx.x < a.page_wgs)
     page_part<DT, D, kKeys | kValues>(a, blockIdx.x);
   else
-    q_rows<DT, D>(a, blockIdx.x - a.page_wgs);
+    q_rows<DT, D, 1>(a, blockIdx.x - a.page_wgs);
 }
 
 // Row norms of many tokens take two launches: what needs no k statistics (v,
 // the q rows) beside the statistics, then k, read again.
+// Pieces of a row that its wave holds: rows of 2048 elements.  Eight cost the v pages of the
+// launch more (registers: 16896 tokens x 12 heads 82 us against 75) than they save
+// rows of twice the length (4 prompts of 2000 x 32/8 heads 20.1 against 21.1).
+constexpr int kHeld = 4;
 template <int DT, int D>
 __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
   constexpr int W = kWg<D> / 64;
@@ -534,11 +575,11 @@ __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
   int wg = blockIdx.x;
   if (wg < a.page_wgs) return page_part<DT, D, kValues>(a, wg);
   wg -= a.page_wgs;
-  if (wg >= stat_wgs) return q_rows<DT, D>(a, wg - stat_wgs);
+  if (wg >= stat_wgs) return q_rows<DT, D, kHeld>(a, wg - stat_wgs);
   const int t = wg * W + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int H = (int)a.c.heads;
-  const float r = inv_rms(row_sq<DT, D>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
+  const float r = inv_rms(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
   if ((threadIdx.x & 63) == 0) a.row_stat[t] = r;
 }
 
