@@ -18,8 +18,15 @@
 // read once.  Thread t holds dims 8*(t % (D/8)).. of 4 consecutive tokens; v's codes
 // turn to [dim][token] through LDS.  The q rows are further workgroups of the
 // same launch.  An RMSNorm over whole rows needs other heads' values: the rows'
-// statistics come from a launch before (which also does q), or, for a few
-// tokens, each workgroup sums its own rows.
+// statistics come from a launch before (which also does v), or, for a few
+// tokens, each workgroup sums its own rows.  Up to 8 tokens of each sequence go by
+// waves instead, without LDS or barriers.
+//
+// Measured, q with k and v: one token x 12 heads 5.3 us (latency: a chain of four loads),
+// 192 of 32/8 heads 5.8; 6 ragged prompts, 1200 tokens on average x 16/4 heads, fp16 10 us
+// (3.5 TB/s); 16896 tokens x 12 heads with row norms 69 us (3.9 TB/s; 5.1 is a copy's
+// rate, and k's second read is not counted).  Between them a page's chain of loads bounds
+// it: lengths, page id and positions, rows, rotations, codes.
 #include <algorithm>
 #include <type_traits>
 
@@ -562,21 +569,20 @@ __global__ __launch_bounds__(kWg<D>) void kv_append_kernel(Args a) {
     q_rows<DT, D, 1>(a, blockIdx.x - a.page_wgs);
 }
 
-// Row norms of many tokens take two launches: what needs no k statistics (v,
-// the q rows) beside the statistics, then k, read again.
-// Pieces of a row that its wave holds: rows of 2048 elements.  Eight cost the v pages of the
-// launch more (registers: 16896 tokens x 12 heads 82 us against 75) than they save
-// rows of twice the length (4 prompts of 2000 x 32/8 heads 20.1 against 21.1).
+// Row norms of many tokens take two launches: v beside the k statistics, then the q
+// rows and k, read again.  The q rows go first: they keep the memory busy while a
+// page's loads wait for each other (16896 tokens x 12 heads: 69 us, behind the pages 71, with
+// the statistics 73).
+
+// Pieces of a row that its wave holds: rows of 2048 elements.  Eight cost the pages of the
+// launch more (registers: 75 us; 8 prompts of 2000 x 32/8 heads 21.4 against 20.0)
+// than they save on rows of 4096 (4 of those prompts 16.8 against 17.3).
 constexpr int kHeld = 4;
 template <int DT, int D>
 __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
   constexpr int W = kWg<D> / 64;
-  const int stat_wgs = (a.T + W - 1) / W;
-  int wg = blockIdx.x;
-  if (wg < a.page_wgs) return page_part<DT, D, kValues>(a, wg);
-  wg -= a.page_wgs;
-  if (wg >= stat_wgs) return q_rows<DT, D, kHeld>(a, wg - stat_wgs);
-  const int t = wg * W + (threadIdx.x >> 6);
+  if ((int)blockIdx.x < a.page_wgs) return page_part<DT, D, kValues>(a, blockIdx.x);
+  const int t = ((int)blockIdx.x - a.page_wgs) * W + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int H = (int)a.c.heads;
   const float r = inv_rms(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
@@ -585,7 +591,11 @@ __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
 
 template <int DT, int D>
 __global__ __launch_bounds__(kWg<D>) void kv_keys_kernel(Args a) {
-  page_part<DT, D, kKeys>(a, blockIdx.x);
+  const int q_wgs = gridDim.x - a.page_wgs;
+  if ((int)blockIdx.x < q_wgs)
+    q_rows<DT, D, kHeld>(a, blockIdx.x);
+  else
+    page_part<DT, D, kKeys>(a, blockIdx.x - q_wgs);
 }
 
 // Two neighbouring elements as fp32.
@@ -802,8 +812,9 @@ void launch(const Args& a, int64_t units, hipStream_t st) {
   const dim3 block(kWg<D>);
   if (a.row_stat) {
     hipLaunchKernelGGL((kv_rows_kernel<DT, D>),
-                       dim3((unsigned)(b.page_wgs + (a.T + W - 1) / W + q_wgs)), block, 0, st, b);
-    hipLaunchKernelGGL((kv_keys_kernel<DT, D>), dim3((unsigned)b.page_wgs), block, 0, st, b);
+                       dim3((unsigned)(b.page_wgs + (a.T + W - 1) / W)), block, 0, st, b);
+    hipLaunchKernelGGL((kv_keys_kernel<DT, D>), dim3((unsigned)(b.page_wgs + q_wgs)), block, 0, st,
+                       b);
   } else {
     hipLaunchKernelGGL((kv_append_kernel<DT, D>), dim3((unsigned)(b.page_wgs + q_wgs)), block, 0,
                        st, b);
