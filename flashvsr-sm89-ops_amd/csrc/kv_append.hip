@@ -324,7 +324,8 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
   // Row norms that no launch before has summed: a wave per token.
   if (a.k_norm == kRow && !a.row_stat) {
     for (int i = j.lo + (tid >> 6); i < j.hi; i += kWg<D> / 64) {
-      const float r = inv_rms(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
+      const float r =
+          inv_rms(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
       if ((tid & 63) == 0) stat[i] = r;
     }
     __syncthreads();
