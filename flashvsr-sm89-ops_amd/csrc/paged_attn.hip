@@ -21,14 +21,24 @@
 // may therefore be any power of two near the maximum: it moves only when E exceeds
 // it by 64, which rescales O and the sum exactly and happens at a row's first keys
 // and hardly ever again.  Remainders keep w's error below 2^-8 (bf16) or
-// 2^-12 (fp16) of itself, or 2^-22 of the largest; sums are fp32 of the unrounded w.
+// 2^-12 (fp16) of itself, or 2^-22 of the largest; sums are fp32, of w (bf16: rounded to
+// fp16, which the terms come by too).  While M stays, O and the sum may grow by 2^64:
+// finite results take values below 2^63 over the number of keys.
 //
-// Two kernels.  attend_few: up to 16 (query, head) rows of one key/value head
+// Three kernels.  attend_few: up to 16 (query, head) rows of one key/value head
 // per workgroup, bound by the cache's bytes: 16x16x128 products, K and V loaded
 // straight into operand registers, pages shared out over waves and workgroups.
+// attend_some: the same for up to 32 rows, 32x32x64 products on half pages.
 // attend_tile: 128 rows, 32 a wave, bound by products and exponentials: 32x32x64
-// products from a double-buffered LDS stage.  Either splits a long axis over
+// products from a double-buffered LDS stage.  Each splits a long axis over
 // workgroups where rows alone leave CUs idle; join_few and join_tile add the pieces.
+//
+// Measured, 32 query and 8 key/value heads of 128: one token for each of 128 ragged
+// sequences of up to 16000 tokens 362 us (5.4 TB/s; 5.1 is a copy's rate), for one
+// sequence of 262000 97 us (5.5); 5 for each of 16 of 6000 47 us (4.2).  8448 rows over
+// 25344 tokens x 12 heads 1.15 ms: 1.15 PFLOP/s, where an 8192^3 bf16 product
+// reaches 1.21; the clock falls to 1.8 - 1.9 GHz, at which the vector units are busy for 71
+// % of the time and the matrix cores for 53.
 #include <algorithm>
 #include <type_traits>
 
@@ -225,6 +235,73 @@ FVSR_DEV int xcd_order(int wg, int total) {
   return xcd < rem ? xcd * (per + 1) + loc : rem * (per + 1) + (xcd - rem) * per + loc;
 }
 
+// A workgroup's unit of few rows: ROWS rows of a sequence, a head and a share of the
+// pages.
+struct FewUnit {
+  SeqPart s;
+  int split, h, rows, row0;  // rows: of the sequence; row0: the unit's first
+};
+template <int ROWS>
+FVSR_DEV bool few_unit(const Args& a, FewUnit& u) {
+  if (!a.c.cu) {  // one unit to a sequence and head
+    u.split = blockIdx.x, u.h = blockIdx.y;
+    u.s.b = blockIdx.z, u.s.part = 0;
+    u.s.rows = seq_rows(nullptr, u.s.b, (int)a.c.sequences, a.T);
+    u.s.len = max(a.c.lengths[u.s.b], 0);
+  } else {
+    // The units of one sequence, head and split are neighbours on one XCD, which
+    // read the same pages.
+    const int at = xcd_order(blockIdx.x, gridDim.x);
+    u.split = at / a.tiles % a.splits, u.h = at / a.tiles / a.splits;
+    if (!tile_of<ROWS>(a, at % a.tiles, a.group, u.s)) return false;
+  }
+  u.rows = u.s.rows.n * a.group, u.row0 = u.s.part * ROWS;
+  return true;
+}
+
+// Adds the waves' parts of each row (O at lds_o[wave][row], P floats apart; M and l in
+// lds_ml) and writes the output, or the piece of it that join_few adds.
+template <int DT, int D, int ROWS, int P>
+FVSR_DEV void finish_few(const Args& a, const FewUnit& u, const float* lds_o,
+                         const float (&lds_ml)[4][ROWS][2]) {
+  __syncthreads();
+  constexpr int C = D / 8;  // threads of a row
+  const int d0 = threadIdx.x % C * 8;
+  for (int i = threadIdx.x / C; i < ROWS && u.row0 + i < u.rows; i += kThreads / C) {
+    const int row = u.row0 + i;
+    float top = lds_ml[0][i][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_ml[w][i][0]);
+    float o[8] = {}, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds_ml[w][i][0] - top);
+      sum += f * lds_ml[w][i][1];
+      const v4f x = *(const v4f*)&lds_o[(w * ROWS + i) * P + d0];
+      const v4f y = *(const v4f*)&lds_o[(w * ROWS + i) * P + d0 + 4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * x[e], o[4 + e] += f * y[e];
+    }
+    const int64_t token = u.s.rows.lo + row / a.group;
+    const int oh = u.h * a.group + row % a.group;
+    if (a.splits == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      u32x2_t* op = (u32x2_t*)(a.out + token * a.o_ts + oh * a.o_hs + d0);
+      op[0] = u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+      op[1] = u32x2_t{pack2<DT>(o[4] * inv, o[5] * inv), pack2<DT>(o[6] * inv, o[7] * inv)};
+    } else {
+      const int64_t pr = (token * a.q_heads + oh) * a.splits + u.split;
+      v4f* po = (v4f*)(a.part + pr * D + d0);
+      po[0] = v4f{o[0], o[1], o[2], o[3]};
+      po[1] = v4f{o[4], o[5], o[6], o[7]};
+      if (d0 == 0) {
+        float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
+        ml[0] = top, ml[1] = sum;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // attend_few.  Operand layout of v_mfma_scale_f32_16x16x128: lane (r, g) = (l %
 // 16, l / 16) holds positions 16 g .. and 64 + 16 g .. (16 each) of row r; the
@@ -243,28 +320,17 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int H = (int)a.c.heads;
-  int split, h;
-  SeqPart s;
-  if (!a.c.cu) {  // one unit to a sequence and head
-    split = blockIdx.x, h = blockIdx.y;
-    s.b = blockIdx.z, s.part = 0;
-    s.rows = seq_rows(nullptr, s.b, (int)a.c.sequences, a.T);
-    s.len = max(a.c.lengths[s.b], 0);
-  } else {
-    // Units are 16 rows of a sequence; those of one sequence, head and split are
-    // neighbours on one XCD, which read the same pages.
-    const int at = xcd_order(blockIdx.x, gridDim.x);
-    split = at / a.tiles % a.splits, h = at / a.tiles / a.splits;
-    if (!tile_of<16>(a, at % a.tiles, a.group, s)) return;
-  }
-  const int rows = s.rows.n * a.group, row0 = s.part * 16, row1 = min(row0 + 16, rows);
+  FewUnit u;
+  if (!few_unit<16>(a, u)) return;
+  const SeqPart& s = u.s;
+  const int h = u.h, rows = u.rows, row0 = u.row0, row1 = min(row0 + 16, rows);
   const int r = min(row0 + col, rows - 1);
   const int qi = r / a.group, hq = h * a.group + r % a.group;
   const int limit = row_limit(a, s, qi);
   const int lim_lo = row_limit(a, s, row0 / a.group);
   const int lim_hi = row_limit(a, s, (row1 - 1) / a.group);
   const int pages = (lim_hi + kPage - 1) / kPage;
-  const int p0 = range_at(pages, split, a.splits), p1 = range_at(pages, split + 1, a.splits);
+  const int p0 = range_at(pages, u.split, a.splits), p1 = range_at(pages, u.split + 1, a.splits);
   const int32_t* const table = a.c.table + s.b * a.c.table_stride;
 
   // Q^T's terms.
@@ -427,45 +493,11 @@ __global__ __launch_bounds__(kThreads, 2) void attend_few(Args a) {
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 
-  // The waves' parts of each row.
 #pragma unroll
   for (int d = 0; d < DT16; ++d)
     *(v4f*)&lds_o[(wave * 16 + col) * P + d * 16 + 4 * g] = acc[d];
   if (g == 0) lds_ml[wave][col][0] = m, lds_ml[wave][col][1] = l;
-  __syncthreads();
-  constexpr int C = D / 8;  // threads of a row
-  const int i = threadIdx.x / C, d0 = threadIdx.x % C * 8, row = row0 + i;
-  if (i >= 16 || row >= rows) return;
-  float top = lds_ml[0][i][0];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_ml[w][i][0]);
-  float o[8] = {}, sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(lds_ml[w][i][0] - top);
-    sum += f * lds_ml[w][i][1];
-    const v4f x = *(const v4f*)&lds_o[(w * 16 + i) * P + d0];
-    const v4f y = *(const v4f*)&lds_o[(w * 16 + i) * P + d0 + 4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += f * x[e], o[4 + e] += f * y[e];
-  }
-  const int64_t token = s.rows.lo + row / a.group;
-  const int oh = h * a.group + row % a.group;
-  if (a.splits == 1) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    u32x2_t* op = (u32x2_t*)(a.out + token * a.o_ts + oh * a.o_hs + d0);
-    op[0] = u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
-    op[1] = u32x2_t{pack2<DT>(o[4] * inv, o[5] * inv), pack2<DT>(o[6] * inv, o[7] * inv)};
-  } else {
-    const int64_t pr = (token * a.q_heads + oh) * a.splits + split;
-    v4f* po = (v4f*)(a.part + pr * D + d0);
-    po[0] = v4f{o[0], o[1], o[2], o[3]};
-    po[1] = v4f{o[4], o[5], o[6], o[7]};
-    if (d0 == 0) {
-      float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
-      ml[0] = top, ml[1] = sum;
-    }
-  }
+  finish_few<DT, D, 16, P>(a, u, lds_o, lds_ml);
 }
 
 // A workgroup adds the n pieces of a row: O at o + k * o_step, (M, l) at ml + k *
@@ -609,10 +641,47 @@ struct RowTile {
   float c;
   int k_at[D / 32], v_at[2];  // this lane's pieces of an operand, half 0
 
+  // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
+  static __device__ __forceinline__ int k_row(int r) {
+    return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+  }
+  // The terms of this lane's row.
+  __device__ __forceinline__ void load_q(const uint16_t* row) {
+    const uint16_t* qp = row + 16 * ((threadIdx.x >> 5) & 1);
+    u32x4_t raw[D / 32][2];
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      raw[x][0] = *(const u32x4_t*)(qp + 32 * x);
+      raw[x][1] = *(const u32x4_t*)(qp + 32 * x + 8);
+    }
+    const auto el = [&](int x, int i) {
+      const uint32_t u = raw[x][i >> 3][(i >> 1) & 3];
+      return to_f<DT>((uint16_t)(i & 1 ? u >> 16 : u & 0xffff));
+    };
+    uint32_t top = 0;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max_mag(top, el(x, i));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int e = row_exp(top);
+    const float f = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+    for (int k = 0; k < N; ++k) qs[k] = e8m0(e - 5 * k);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t t[N];
+        split4<N>(el(x, 4 * i) * f, el(x, 4 * i + 1) * f, el(x, 4 * i + 2) * f,
+                  el(x, 4 * i + 3) * f, t);
+#pragma unroll
+        for (int k = 0; k < N; ++k) qf[x >> 1][k][(x & 1) * 4 + i] = (int)t[k];
+      }
+  }
   __device__ __forceinline__ void place() {
     const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
-    // Row r = 8 i + 4 g' + j of K subtile u is key 32 u + 16 g' + 4 i + j.
-    const int kr = 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3);
+    const int kr = k_row(r);
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) k_at[w] = kr * D + (((2 * w + g) ^ k_swap<D>(kr)) << 4);
 #pragma unroll
@@ -634,14 +703,16 @@ struct RowTile {
     return join(*(const u32x4_t LDS_AS*)(p + (v_at[0] ^ (half * 64))),
                 *(const u32x4_t LDS_AS*)(p + (v_at[1] ^ (half * 64))));
   }
-  __device__ __forceinline__ void logits(v16f (&s)[2], const uint8_t LDS_AS* k, int half, int ks) {
+  // (k_of(u, w): the K operand of 32 keys u and 64 dims w of the half.)
+  template <class K>
+  __device__ __forceinline__ void logits(v16f (&s)[2], K k_of, int ks) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) s[u] = v16f{};
 #pragma unroll
     for (int w = 0; w < D / 64; ++w)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const v8i kf = k_operand(k, half, u, w);
+        const v8i kf = k_of(u, w);
 #pragma unroll
         for (int t = 0; t < N; ++t) s[u] = mfma(kf, qf[w][t], s[u], ks, qs[t]);
       }
@@ -742,70 +813,163 @@ struct RowTile {
     order<false, QK, 0, (8 * (N == 2 ? 12 : 22) + P2 - 1) / P2>(P2);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // A page at position `at`.
+  // A half page at position `at`, v_of(d) being the V operand of 32 dims: any, with masks, a
+  // moving M and NaN codes.  after() runs once K is no longer needed.
+  template <class K, class V, class After>
+  __device__ __forceinline__ void half_page(K k_of, V v_of, int at, int ks, int vs, After after) {
+    v16f s[2];
+    logits(s, k_of, ks);
+    after();
+    const int room = limit - at - 16 * ((threadIdx.x >> 5) & 1);  // 32 u + e < it
+    const bool masked = at + 64 > lim_lo;
+    if (masked) {
+      asm volatile("" :::);  // a branch: most pages are seen whole
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * u + e >= room) s[u][e] = -__builtin_huge_valf();
+    }
+    weigh(s, top_of(s), c, m, l, shift, [&](float f) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] *= f;
+    });
+    float sum = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      uint32_t o[N];
+      const v16f& sg = s[g >> 2];
+      const int b = 4 * (g & 3);
+      weights4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o, sum);
+#pragma unroll
+      for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
+    }
+    l += __builtin_ldexpf(sum, shift);
+    v8i seen{};  // 1.0 where this lane's row sees a token (masked halves)
+    if (masked) {
+      asm volatile("" :::);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (32 * (i >> 2) + 4 * (i & 3) + j < room) seen[i] |= 0x38 << (8 * j);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      v8i f = v_of(d);
+      if (masked && (vs == 255 || __ballot(has_nan(f)) != 0)) {  // as in attend_few
+        if (vs == 255) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = 0x7f7f7f7f;
+        }
+        const v8i ones = take_nan(f);
+        const v16f z = {};
+        const v16f n = mfma(ones, seen, z, 127, 127);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
+      }
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+        acc[d] = mfma(f, pf[t], acc[d], masked && vs == 255 ? 127 : vs, e8m0(shift - 5 * t));
+    }
+  }
+  // A page at position `at` in a stage.
   __device__ __forceinline__ void one(const uint8_t LDS_AS* k, const uint8_t LDS_AS* v, int at,
                                       int ks, int vs) {
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       fresh();
-      v16f s[2];
-      logits(s, k, half, ks);
-      const int room = limit - at - half * 64 - 16 * ((threadIdx.x >> 5) & 1);  // 32 u + e < it
-      const bool masked = at + half * 64 + 64 > lim_lo;
-      if (masked) {
-        asm volatile("" :::);  // a branch: most pages are seen whole
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (32 * u + e >= room) s[u][e] = -__builtin_huge_valf();
-      }
-      weigh(s, top_of(s), c, m, l, shift, [&](float f) {
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) acc[d] *= f;
-      });
-      float sum = 0.0f;
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        uint32_t o[N];
-        const v16f& sg = s[g >> 2];
-        const int b = 4 * (g & 3);
-        weights4<N>(sg[b], sg[b + 1], sg[b + 2], sg[b + 3], o, sum);
-#pragma unroll
-        for (int n = 0; n < N; ++n) pf[n][g] = (int)o[n];
-      }
-      l += __builtin_ldexpf(sum, shift);
-      v8i seen{};  // 1.0 where this lane's row sees a token (masked halves)
-      if (masked) {
-        asm volatile("" :::);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (32 * (i >> 2) + 4 * (i & 3) + j < room) seen[i] |= 0x38 << (8 * j);
-      }
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        v8i f = v_operand(v, half, d);
-        if (masked && (vs == 255 || __ballot(has_nan(f)) != 0)) {  // as in attend_few
-          if (vs == 255) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0x7f7f7f7f;
-          }
-          const v8i ones = take_nan(f);
-          const v16f z = {};
-          const v16f n = mfma(ones, seen, z, 127, 127);
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (n[e] > 0.0f) acc[d][e] = __builtin_nanf("");
-        }
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-          acc[d] = mfma(f, pf[t], acc[d], masked && vs == 255 ? 127 : vs, e8m0(shift - 5 * t));
-      }
+      half_page([&](int u, int w) { return k_operand(k, half, u, w); },
+                [&](int d) { return v_operand(v, half, d); }, at + half * 64, ks, vs, [] {});
     }
   }
 };
+
+// attend_few for 17 to 32 rows: the same sharing out of pages, half a page at a time (a
+// whole one's operands beside 32 rows' O are more than 256 registers).  The K operand of the
+// half ahead loads as soon as the logits have used the one before it: 61 -> 47 us for 16 x 5
+// tokens x 32 / 8 heads over 6000 (4.2 TB/s), with the splits that follow from it.  Five tokens
+// over 262000: 104 us (5.2 TB/s); by tiles of 128 rows 262.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads, 2) void attend_some(Args a) {
+  constexpr int P = D + 4;
+  __shared__ __attribute__((aligned(16))) float lds_o[4 * 32 * P];
+  __shared__ float lds_ml[4][32][2];
+  const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int H = (int)a.c.heads;
+  FewUnit u;
+  if (!few_unit<32>(a, u)) return;
+  const SeqPart& s = u.s;
+  const int row1 = min(u.row0 + 32, u.rows), r = min(u.row0 + r32, u.rows - 1);
+  RowTile<DT, D> w;
+  w.limit = row_limit(a, s, r / a.group);
+  w.lim_lo = row_limit(a, s, u.row0 / a.group);
+  w.c = a.scale_log2;
+  const int last = row_limit(a, s, (row1 - 1) / a.group);
+  const int pages = (last + kPage - 1) / kPage;
+  const int p0 = range_at(pages, u.split, a.splits), p1 = range_at(pages, u.split + 1, a.splits);
+  const int32_t* const table = a.c.table + s.b * a.c.table_stride;
+  int look = p0 + wave, ahead = look < p1 ? table[look] : 0;
+  w.load_q(a.q + (int64_t)(s.rows.lo + r / a.group) * a.q_ts +
+           (int64_t)(u.h * a.group + r % a.group) * a.q_hs);
+  // The wave's next page that exists (none: false); rows that would read others are NaN.
+  int p = 0, ks = 0, vs = 0;
+  const uint8_t *kp = nullptr, *vp = nullptr;
+  const auto next = [&] {
+    for (; look < p1; look += 4) {
+      const int64_t id = __builtin_amdgcn_readfirstlane(ahead);
+      if (look + 4 < p1) ahead = table[look + 4];
+      if (id >= 0 && id < a.c.pages) {
+        const int64_t ph = id * H + u.h;
+        kp = (const uint8_t*)a.c.k + ph * kPage * D, vp = (const uint8_t*)a.c.v + ph * kPage * D;
+        ks = ((const uint8_t*)a.c.k_scale)[ph], vs = ((const uint8_t*)a.c.v_scale)[ph];
+        p = look;
+        look += 4;
+        return true;
+      }
+      if (look * kPage < w.limit) w.l = __builtin_nanf("");
+    }
+    return false;
+  };
+  const int k_off = RowTile<DT, D>::k_row(r32) * D + 16 * g, v_off = r32 * kPage + 16 * g;
+  v8i kf[2][D / 64], vf[D / 32];
+  const auto load_k = [&](const uint8_t* from) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < D / 64; ++y) {
+        const uint8_t* at = from + k_off + x * 32 * D + y * 64;
+        kf[x][y] = join(*(const u32x4_t*)at, *(const u32x4_t*)(at + 32));
+      }
+  };
+  bool more = next();
+  if (more) load_k(kp);
+#pragma unroll 1
+  for (int half = 0; more;) {
+    const int at = p * kPage + half * 64, k_scale = ks, v_scale = vs;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const uint8_t* from = vp + v_off + d * 32 * kPage + half * 64;
+      vf[d] = join(*(const u32x4_t*)from, *(const u32x4_t*)(from + 32));
+    }
+    if (half) more = next();
+    half ^= 1;
+    // (The last page's first half once more behind the last: no branch.)
+    w.half_page([&](int x, int y) { return kf[x][y]; }, [&](int d) { return vf[d]; }, at, k_scale,
+                v_scale, [&] { load_k(kp + half * 64 * D); });
+  }
+  const float l = w.l + __shfl_xor(w.l, 32);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *(v4f*)&lds_o[(wave * 32 + r32) * P + d * 32 + 8 * i + 4 * g] =
+          v4f{w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]};
+  if (g == 0) lds_ml[wave][r32][0] = w.m, lds_ml[wave][r32][1] = l;
+  finish_few<DT, D, 32, P>(a, u, lds_o, lds_ml);
+}
 
 // Unit u of a call: a head (of the queries with a block mask, else of the keys)
 // and 128 rows of one sequence.  Without a mask a tile's rows are (query, head of the
@@ -888,40 +1052,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   }
   const int p0 = range_at(pages, piece, pieces), p1 = range_at(pages, piece + 1, pieces);
 
-  {
-    const uint16_t* qp =
-        a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs + 16 * g;
-    u32x4_t raw[D / 32][2];
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
-      raw[w][0] = *(const u32x4_t*)(qp + 32 * w);
-      raw[w][1] = *(const u32x4_t*)(qp + 32 * w + 8);
-    }
-    const auto el = [&](int w, int i) {
-      const uint32_t u = raw[w][i >> 3][(i >> 1) & 3];
-      return to_f<DT>((uint16_t)(i & 1 ? u >> 16 : u & 0xffff));
-    };
-    uint32_t top = 0;
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = max_mag(top, el(w, i));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    const int e = row_exp(top);
-    const float f = __builtin_ldexpf(1.0f, -e);
-#pragma unroll
-    for (int k = 0; k < N; ++k) w.qs[k] = e8m0(e - 5 * k);
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t t[N];
-        split4<N>(el(x, 4 * i) * f, el(x, 4 * i + 1) * f, el(x, 4 * i + 2) * f,
-                  el(x, 4 * i + 3) * f, t);
-#pragma unroll
-        for (int k = 0; k < N; ++k) w.qf[x >> 1][k][(x & 1) * 4 + i] = (int)t[k];
-      }
-  }
+  w.load_q(a.q + (int64_t)(s.rows.lo + qi) * a.q_ts + (int64_t)hq * a.q_hs);
 
   const uint8_t* const kb = (const uint8_t*)a.c.k + (int64_t)h * kPage * D;
   const uint8_t* const vb = (const uint8_t*)a.c.v + (int64_t)h * kPage * D;
@@ -980,7 +1111,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
           wait_all();
           stream<D>(k1, k_of(nxt), wave, kp);
           if constexpr (live) {
-            w.logits(sa, k0, 0, cur[2] & 255);
+            w.logits(sa, [&](int u, int x) { return w.k_operand(k0, 0, u, x); }, cur[2] & 255);
             if (w.m == kNothing) w.m = w.exponent(sa);
             w.template step<false, true>(sa, sb, nullptr, 0, 0, k0, 1, cur[2] & 255);
           }
@@ -1070,7 +1201,7 @@ int64_t cu_count() {
 
 // How a call is cut up: a function of its sizes (and the CUs) only.
 struct Plan {
-  bool few;        // attend_few
+  int few;         // rows of a unit of attend_few (16) or attend_some (32); 0: attend_tile
   int64_t tiles;   // of 16 or 128 rows, per head, over all sequences
   int64_t units;   // tiles of all heads
   int64_t whole;   // units done by one workgroup each; the others by `pieces` each
@@ -1094,19 +1225,26 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   // Rows of any number per sequence: where they are few on average, waiting for
   // memory is what counts, and 16 rows to a workgroup with its waves on pages of their own
   // wait less than 128 with one stream of pages, even if some units read the same pages (32
-  // sequences of 7.5 tokens x 32 / 8 heads 168 -> 134 us, 16 of 14 x 16 / 4 44 -> 24).
-  // The same number for each: only if one such unit holds them (20 rows 64 against 53).
-  p.few = !keep && T * group <= B * (c->cu ? 64 : 16);
+  // sequences of 7.5 tokens x 32 / 8 heads 168 -> 134 us, 16 of 14 x 16 / 4 44 -> 24; 32 rows
+  // to a workgroup: no better, or 20 against 17).  The same number for each: if one unit
+  // of 16 or 32 holds them (20 rows over 6000 tokens: two units of 16 64 us, one of
+  // 32 47, a tile of 128 52).
+  if (!keep && T * group <= B * (c->cu ? 64 : 32))
+    p.few = c->cu || T * group <= B * 16 ? 16 : 32;
   if (p.few) {
-    p.tiles = tiles(group, 16);
+    p.tiles = tiles(group, p.few);
     p.units = p.tiles * c->heads;
     // Sequences may be of any lengths: 16 workgroups per CU even them out (128
     // ragged sequences of up to 16000 tokens, us at 4 / 8 / 16 / 32: 390, 376, 364, 374).
     // Two pages to a wave, or one where that would leave CUs idle (20000 tokens x 12
     // heads 20.5 against 23.8 us; 4 sequences of 5000 x 2 heads 14.6 against 12.1).
+    // 32 rows cost more to write and to add again, so there it is one workgroup per CU (16
+    // x 5 tokens x 32 / 8 heads over 6000, 1 to 8 splits: 60, 47, 55, 49, 54; over ragged ones of
+    // up to 12000: 107, 69, 80, 72, 66; 64 x 5 over 2000: 58, 72, 79, 79, 89).
     const int64_t pages = c->table_pages;
-    const int64_t each = p.units * (pages / 8) * 2 < cus ? 4 : 8;
-    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 16 * cus / p.units),
+    const int64_t each = p.few == 32 || p.units * (pages / 8) * 2 < cus ? 4 : 8;
+    const int64_t fill = p.few == 32 ? cus : 16 * cus;
+    p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, fill / p.units),
                                        std::max<int64_t>(1, pages / each), kMaxSplits});
     return p;
   }
@@ -1124,7 +1262,7 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   const int64_t slots = rows_of <= 64 ? 2 * cus : cus, pages = c->table_pages;
   const int64_t rest = rows_of <= 64 ? p.units : p.units % cus;
   double best = 0;
-  for (int64_t n = 1; n <= std::min<int64_t>(16, std::max<int64_t>(1, pages / 2)); ++n) {
+  for (int64_t n = 1; n <= std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, pages / 2)); ++n) {
     const double us = (double)((rest * n + slots - 1) / slots) * (pages / (double)n + 3) * 1.9 +
                       (n > 1 ? 5 + rest * n * rows_of * (0.03 / 128) : 0);
     if (n > 1 && us >= best) continue;
@@ -1142,7 +1280,10 @@ void launch(const Args& a, const Plan& p, hipStream_t st) {
     const dim3 grid = a.c.cu ? dim3((unsigned)(p.units * p.splits))
                              : dim3((unsigned)p.splits, (unsigned)a.c.heads,
                                     (unsigned)a.c.sequences);
-    hipLaunchKernelGGL((attend_few<DT, D>), grid, block, 0, st, a);
+    if (p.few == 16)
+      hipLaunchKernelGGL((attend_few<DT, D>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((attend_some<DT, D>), grid, block, 0, st, a);
     if (p.splits > 1)
       hipLaunchKernelGGL((join_few<DT, D>), dim3((unsigned)((int64_t)a.T * a.q_heads)), block,
                          0, st, a);

@@ -454,6 +454,50 @@ def test_attention_equal_rows(D, n):
     check_attention(out, q, pages, table, lens)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.bfloat16),
+                                     (64, torch.float16), (128, torch.float16)])
+@pytest.mark.parametrize("Hq,H,n", [(2, 2, 17), (8, 2, 5), (4, 1, 8), (20, 1, 1)])
+@pytest.mark.parametrize("lens", [(1, 30, 127, 129), (700, 0, 64, 257), (2900, 128, 18, 1100)])
+def test_attention_one_unit_of_32(D, dtype, Hq, H, n, lens):
+    """17 to 32 rows of a key/value head, the same number for every sequence."""
+    from flashvsr_sm89_ops import paged_attention
+    table, N = tables(lens, seed=5)
+    pages = pool(N, H, D, seed=6)
+    q = (2 * torch.randn(len(lens) * n, Hq, D, generator=gen(7))).to(dtype)
+    for causal in (True, False):
+        out = paged_attention(q.to(DEV), pages, table.to(DEV), i32(lens).to(DEV), causal=causal)
+        check_attention(out, q, pages, table, lens, causal=causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_one_unit_of_32_odd_pages(D):
+    """Missing pages between others, NaN behind the lengths, a last page far above all."""
+    from flashvsr_sm89_ops import paged_attention
+    H, n, lens = 2, 20, [1500, 400, 130]
+    table, N = tables(lens)
+    pages = pool(N, H, D, bad=True)
+    good = pool(N, H, D)
+    ku, vu = pages.k.view(torch.uint8), pages.v.view(torch.uint8)
+    for b, L in enumerate(lens):
+        for j in range(-(-L // 128)):
+            p, m = int(table[b, j]), min(128, L - 128 * j)
+            ku[p, :, :m] = good.k.view(torch.uint8)[p, :, :m]
+            vu[p, :, :, :m] = good.v.view(torch.uint8)[p, :, :, :m]
+    pages.k_scale.view(torch.uint8)[int(table[0, 11])] += 4
+    q = torch.randn(3 * n, H, D, generator=gen(3)).bfloat16()
+    args = (q.to(DEV), pages, table.to(DEV), i32(lens).to(DEV))
+    out = paged_attention(*args)
+    assert bool(torch.isfinite(out).all())
+    check_attention(out, q, pages, table, lens)
+    for at, page in (((1, 0), -1), ((1, 3), N), ((2, 1), 1 << 30)):
+        t = table.clone()
+        t[at] = page
+        out = paged_attention(args[0], pages, t.to(DEV), args[3])
+        check_attention(out, q, pages, t, lens)
+        sees = torch.arange(lens[at[0]] - n, lens[at[0]]) >= at[1] * 128
+        assert torch.equal(out[at[0] * n:(at[0] + 1) * n].isnan().all(-1).all(-1).cpu(), sees)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("Hq,H,causal,n", [(2, 2, False, 200), (4, 2, True, 140), (2, 1, False, 3)])
 def test_attention_keep(dtype, Hq, H, causal, n):
@@ -527,7 +571,7 @@ def test_attention_hidden_nan(n, Hq, D):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("n,L", [(8, 130), (100, 200), (100, 460)])
+@pytest.mark.parametrize("n,L", [(8, 130), (30, 150), (100, 200), (100, 460)])
 @pytest.mark.parametrize("which", ["k_scale", "v_scale"])
 def test_attention_hidden_nan_scale(D, n, L, which):
     """A NaN scale makes the rows that see its page NaN and leaves the others' bits."""
