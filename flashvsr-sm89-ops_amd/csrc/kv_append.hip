@@ -24,7 +24,7 @@
 //
 // Measured, q with k and v: one token x 12 heads 5.3 us (latency: a chain of four loads),
 // 192 of 32/8 heads 5.8; 6 ragged prompts, 1200 tokens on average x 16/4 heads, fp16 10 us
-// (3.5 TB/s); 16896 tokens x 12 heads with row norms 69 us (3.9 TB/s; 5.1 is a copy's
+// (3.4 TB/s); 16896 tokens x 12 heads with row norms 73 us (3.7 TB/s; 5.1 is a copy's
 // rate, and k's second read is not counted).  Between them a page's chain of loads bounds
 // it: lengths, page id and positions, rows, rotations, codes.
 #include <algorithm>
@@ -46,7 +46,7 @@ struct Args {
   void* q_out;
   const float* cs;           // [cs_rows][D/2][2] (cos, sin); null: no rotation
   const int32_t* positions;  // row of cs for each token; null: the token's own number
-  float* row_stat;           // 1/rms of each k row (row norm, from the launch before)
+  double* row_stat;          // 1/rms of each k row (row norm, from the launch before)
   int64_t k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, cs_rows;
   int T, q_heads, k_norm, q_norm, w_dt, units, units_max, page_wgs;
   float eps;
@@ -107,27 +107,81 @@ FVSR_DEV void store8(void* p, int dt, int64_t i, const float (&x)[8]) {
   }
 }
 
-FVSR_DEV float sum_sq(const float (&x)[8]) {
-  float s = 0.0f;
+// Sums and what follows from them in fp32, or (T double) in 64 bits.  q is rounded to its
+// own type in the end, where fp32's steps do not show, but k to a code of 4 bits: fp32's
+// steps put 1 or 2 in 10^6 on the other side of a border between codes, 1 / 16 off.  So
+// what lies near a border is computed again in 64 bits, from 64-bit sums.  (Errors of k
+// against 64 bits: 2e-5 of its norm without, 2e-7 so.  16896 tokens x 12 heads 69 us
+// without, 73 so, 84 with all of k in 64 bits.)
+template <class T>
+FVSR_DEV T sum_sq(const float (&x)[8]) {
+  T s = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s = __builtin_fmaf(x[e], x[e], s);
+  for (int e = 0; e < 8; ++e) s += (T)x[e] * (T)x[e];
   return s;
 }
 
 FVSR_DEV float inv_rms(float sq, int n, float eps) { return 1.0f / __builtin_sqrtf(sq / n + eps); }
+FVSR_DEV double inv_rms(double sq, int n, float eps) { return 1.0 / __builtin_sqrt(sq / n + eps); }
 
-// Sum over the D/8 lanes that hold one head.
-template <int C>
-FVSR_DEV float head_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < C; d *= 2) v += __shfl_xor(v, d);
+// Sum over the N = 8, 16 or 64 lanes around, from lane to lane (dpp).
+template <int CTRL, int ROWS = 0xf>
+FVSR_DEV float moved(float v) {
+  return dpp_f32<CTRL, ROWS>(v);
+}
+template <int CTRL, int ROWS = 0xf>
+FVSR_DEV double moved(double v) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f u = __builtin_bit_cast(v2f, v);
+  return __builtin_bit_cast(double, v2f{dpp_f32<CTRL, ROWS>(u[0]), dpp_f32<CTRL, ROWS>(u[1])});
+}
+FVSR_DEV double lane63(double v) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f u = __builtin_bit_cast(v2f, v);
+  return __builtin_bit_cast(double, v2f{::lane63(u[0]), ::lane63(u[1])});
+}
+template <int N, class T>
+FVSR_DEV T lanes_sum(T v) {
+  v += moved<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += moved<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += moved<0x141>(v);  // row_half_mirror
+  if constexpr (N > 8) v += moved<0x140>(v);  // row_mirror
+  if constexpr (N > 16) {
+    v += moved<0x142, 0xa>(v);  // row_bcast:15 into rows 1, 3
+    v += moved<0x143, 0xc>(v);  // row_bcast:31 into rows 2, 3
+    v = lane63(v);
+  }
   return v;
+}
+
+// Whether one of the values seen lies within kNear fp32 steps of a border between
+// codes of 4 bits (subnormal codes aside, whose steps are small): mantissas whose last 20
+// bits are near their half.  A value is four roundings off, more only where a rotation
+// leaves little of its terms.
+constexpr uint32_t kNear = 8;
+struct Border {
+  uint32_t least = ~0u;
+  __device__ __forceinline__ void see(float x) {
+    least = min(least, (__float_as_uint(x) << 12) + ((kNear << 12) - 0x80000000u));
+  }
+  __device__ __forceinline__ bool near() const { return least < 2 * kNear << 12; }
+};
+
+// d as fp32 with its last bit set if anything is cut off: the code that it rounds to is the
+// one that d itself would.
+FVSR_DEV float to_odd(double d) {
+  const float f = (float)d;
+  const double back = f;
+  uint32_t u = __float_as_uint(f);
+  u -= __builtin_fabs(back) > __builtin_fabs(d);
+  u |= back != d && back == back;
+  return __uint_as_float(u);
 }
 
 // A whole row of H heads by one wave: the first N pieces of eight per lane go out
 // together and stay in registers.  Returns the sum of squares.
-template <int DT, int D, int N>
-FVSR_DEV float load_row(const void* x, int64_t row, int64_t hs, int H, Raw8<DT> (&held)[N]) {
+template <class T, int DT, int D, int N>
+FVSR_DEV T load_row(const void* x, int64_t row, int64_t hs, int H, Raw8<DT> (&held)[N]) {
   constexpr int C = D / 8;
   const int lane = threadIdx.x & 63, n = H * C;
   const auto at = [&](int c) { return row + (c / C) * hs + (c % C) * 8; };
@@ -136,24 +190,24 @@ FVSR_DEV float load_row(const void* x, int64_t row, int64_t hs, int H, Raw8<DT> 
     held[i] = Raw8<DT>{};
     if (lane + 64 * i < n) held[i] = load_raw<DT>(x, at(lane + 64 * i));
   }
-  float s = 0.0f;
+  T s = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float a[8];
     widen(held[i], a);
-    s += sum_sq(a);
+    s += sum_sq<T>(a);
   }
   for (int c = lane + 64 * N; c < n; c += 64) {
     float a[8];
     load8(x, DT, at(c), a);
-    s += sum_sq(a);
+    s += sum_sq<T>(a);
   }
-  return wave_sum(s);
+  return lanes_sum<64>(s);
 }
 template <int DT, int D, int N>
-FVSR_DEV float row_sq(const void* x, int64_t row, int64_t hs, int H) {
+FVSR_DEV double row_sq(const void* x, int64_t row, int64_t hs, int H) {
   Raw8<DT> held[N];
-  return load_row<DT, D>(x, row, hs, H, held);
+  return load_row<double, DT, D>(x, row, hs, H, held);
 }
 
 // A position outside the table gives NaN (every result has a cosine in it).
@@ -188,6 +242,22 @@ FVSR_DEV void norm_turn(float (&x)[8], bool norm, float r, const float (&w)[8], 
   }
 }
 
+// The same in 64 bits (k): x * w is exact, its product with r rounded once.
+FVSR_DEV void norm_turn64(float (&x)[8], bool norm, double r, const float (&w)[8], bool turn,
+                          const float (&cs)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    double a = x[e], b = x[e + 1];
+    if (norm) a = a * w[e] * r, b = b * w[e + 1] * r;
+    if (turn) {
+      const double c = cs[e], s = cs[e + 1], t = __builtin_fma(a, c, -(b * s));
+      b = __builtin_fma(a, s, b * c);
+      a = t;
+    }
+    if (norm || turn) x[e] = to_odd(a), x[e + 1] = to_odd(b);
+  }
+}
+
 // q rows without a row norm: a thread per eight elements.
 template <int DT, int D>
 FVSR_DEV void q_chunk(const Args& a, int64_t chunk) {
@@ -202,7 +272,7 @@ FVSR_DEV void q_chunk(const Args& a, int64_t chunk) {
   float r = 1.0f;
   if (a.q_norm == kHead) {
     load8(a.q_weight, a.w_dt, d0, w);
-    r = inv_rms(head_sum<C>(sum_sq(x)), D, a.eps);
+    r = inv_rms(lanes_sum<C>(sum_sq<float>(x)), D, a.eps);
   }
   norm_turn(x, a.q_norm == kHead, r, w, a.cs != nullptr, cs);
   if (live) store8(a.q_out, DT, unit * D + d0, x);
@@ -218,7 +288,7 @@ FVSR_DEV void q_row(const Args& a, int t) {
   float cs[8] = {};
   if (a.cs) load_turn<D>(a, t, d0, cs);
   Raw8<DT> held[N];
-  const float r = inv_rms(load_row<DT, D>(a.q, t * a.q_ts, a.q_hs, a.q_heads, held),
+  const float r = inv_rms(load_row<float, DT, D>(a.q, t * a.q_ts, a.q_hs, a.q_heads, held),
                           a.q_heads * D, a.eps);
   const auto put = [&](float(&x)[8], int c) {
     float w[8];
@@ -315,7 +385,7 @@ FVSR_DEV void rows_of(const Job& j, Body body) {
 }
 
 template <int DT, int D>
-FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
+FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
                        float (&tops)[kWg<D> / 64]) {
   constexpr int C = D / 8, R = kTokens;
   const int tid = threadIdx.x, H = (int)a.c.heads;
@@ -324,7 +394,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
   // Row norms that no launch before has summed: a wave per token.
   if (a.k_norm == kRow && !a.row_stat) {
     for (int i = j.lo + (tid >> 6); i < j.hi; i += kWg<D> / 64) {
-      const float r =
+      const double r =
           inv_rms(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
       if ((tid & 63) == 0) stat[i] = r;
     }
@@ -335,6 +405,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
   if (a.k_norm != kNone) load8(a.k_weight, a.w_dt, (a.k_norm == kRow ? j.h * D : 0) + d0, w);
   float x[R][8];
   float top = 0.0f;
+  uint32_t near = 0;  // bit i: a value of token i is near a border
   rows_of(j, [&](auto full) {
     const auto live = [&](int i) { return full || (slot0 + i >= j.lo && slot0 + i < j.hi); };
     // All positions and rows go out together, then all rotations: a load
@@ -348,7 +419,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
     for (int i = 0; i < R; ++i) {
       const int t = j.row0 + (live(i) ? slot0 + i : j.lo);
       pos[i] = a.positions ? a.positions[t] : t;
-      if (a.k_norm == kRow) rs[i] = a.row_stat ? a.row_stat[t] : stat[t - j.row0];
+      if (a.k_norm == kRow) rs[i] = (float)(a.row_stat ? a.row_stat[t] : stat[t - j.row0]);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -375,10 +446,14 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
         outside(pos[i], a.cs_rows, cs);
       }
       float r = 1.0f;
-      if (a.k_norm == kHead) r = inv_rms(head_sum<C>(sum_sq(x[i])), D, a.eps);
+      if (a.k_norm == kHead) r = inv_rms(lanes_sum<C>(sum_sq<float>(x[i])), D, a.eps);
       if (a.k_norm == kRow) r = rs[i];
       norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
       if (!live(i)) continue;
+      Border b;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b.see(x[i][e]);
+      near |= (uint32_t)b.near() << i;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) top = max3_abs(top, x[i][e], x[i][e + 1]);
     }
@@ -409,6 +484,24 @@ FVSR_DEV void append_k(const Args& a, const Job& j, float (&stat)[kPage],
       const u32x2_t c = *p;
       *p = u32x2_t{rescale4(c[0], pow2(old - e)), rescale4(c[1], pow2(old - e))};
     }
+  }
+  if (__ballot(near) == 0 || (a.k_norm == kNone && !a.cs)) return;
+  // Tokens near a border, by now with the registers free.
+#pragma unroll 1
+  for (int i = 0; i < R; ++i) {
+    if (__ballot(near >> i & 1) == 0) continue;
+    const int slot = min(max(slot0 + i, j.lo), j.hi - 1), t = j.row0 + slot;
+    float y[8], cs[8] = {};
+    widen(load_raw<DT>(a.k, (int64_t)t * a.k_ts + j.h * a.k_hs + d0), y);
+    if (a.cs) load_turn<D>(a, t, d0, cs);
+    if (a.k_norm != kNone) load8(a.k_weight, a.w_dt, (a.k_norm == kRow ? j.h * D : 0) + d0, w);
+    double r = 1.0;
+    if (a.k_norm == kHead) r = inv_rms(lanes_sum<C>(sum_sq<double>(y)), D, a.eps);
+    if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[slot];
+    norm_turn64(y, a.k_norm != kNone, r, w, a.cs != nullptr, cs);
+    if (slot == slot0 + i)
+      *(u32x2_t*)(page + slot * D + d0) = u32x2_t{codes4(y[0], y[1], y[2], y[3], f),
+                                                  codes4(y[4], y[5], y[6], y[7], f)};
   }
 }
 
@@ -557,7 +650,7 @@ FVSR_DEV void page_part(const Args& a, int wg) {
     if (n == 1 || part % n) return append_v<DT, D>(a, j, vt, tops);
   }
   if constexpr ((KINDS & kKeys) != 0) {
-    __shared__ float stat[kPage];
+    __shared__ double stat[kPage];
     append_k<DT, D>(a, j, stat, tops);
   }
 }
@@ -586,7 +679,7 @@ __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
   const int t = ((int)blockIdx.x - a.page_wgs) * W + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int H = (int)a.c.heads;
-  const float r = inv_rms(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
+  const double r = inv_rms(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
   if ((threadIdx.x & 63) == 0) a.row_stat[t] = r;
 }
 
@@ -616,10 +709,13 @@ FVSR_DEV void load2(const void* p, int64_t i, float (&x)[2]) {
   }
 }
 
+FVSR_DEV float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+FVSR_DEV double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
 // Norm and rotation of two dims d0, d0 + 1 of a head of N tokens t, a wave per head; `ts`,
 // `hs` and `heads` describe the rows of src (q or k).  Each kind of load goes out
 // for all tokens at once.
-template <int DT, int D, int N>
+template <class F, int DT, int D, int N>
 FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int heads,
                     const void* weight, int norm, const int (&t)[N], int h, int d0,
                     float (&x)[N][2]) {
@@ -627,7 +723,8 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
   int pos[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) pos[i] = a.positions ? a.positions[t[i]] : t[i];
-  float sq[N] = {}, cs[N][2];
+  F sq[N] = {};
+  float cs[N][2];
   if (norm == kRow) {
     for (int c = lane; c < heads * (D / 8); c += 64) {
       const int64_t at = (c / (D / 8)) * hs + (c % (D / 8)) * 8;
@@ -638,13 +735,13 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
       for (int i = 0; i < N; ++i) {
         float r[8];
         widen(raw[i], r);
-        sq[i] += sum_sq(r);
+        sq[i] += sum_sq<F>(r);
       }
     }
   } else if (norm == kHead) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      sq[i] = lane * 2 < D ? x[i][0] * x[i][0] + x[i][1] * x[i][1] : 0.0f;
+      sq[i] = lane * 2 < D ? (F)x[i][0] * (F)x[i][0] + (F)x[i][1] * (F)x[i][1] : (F)0;
   }
   if (a.cs) {
 #pragma unroll
@@ -655,25 +752,29 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
       cs[i][1] = p[1];
     }
   }
+  if (norm == kNone && !a.cs) return;
+  float w[2] = {1.0f, 1.0f};
   if (norm != kNone) {
-    float w[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       w[e] = ld_elem(weight, a.w_dt, (norm == kRow ? h * D : 0) + d0 + e);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float r = inv_rms(wave_sum(sq[i]), norm == kRow ? heads * D : D, a.eps);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) x[i][e] = x[i][e] * r * w[e];
-    }
   }
-  if (a.cs) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float b = x[i][0];
-      x[i][0] = __builtin_fmaf(b, cs[i][0], -(x[i][1] * cs[i][1]));
-      x[i][1] = __builtin_fmaf(b, cs[i][1], x[i][1] * cs[i][0]);
+  for (int i = 0; i < N; ++i) {
+    F u = x[i][0], v = x[i][1];
+    if (norm != kNone) {
+      const F r = inv_rms(lanes_sum<64>(sq[i]), norm == kRow ? heads * D : D, a.eps);
+      u = u * w[0] * r, v = v * w[1] * r;
     }
+    if (a.cs) {
+      const F c = cs[i][0], s = cs[i][1], o = fused(u, c, -(v * s));
+      v = fused(u, s, v * c);
+      u = o;
+    }
+    if constexpr (std::is_same_v<F, double>)
+      x[i][0] = to_odd(u), x[i][1] = to_odd(v);
+    else
+      x[i][0] = u, x[i][1] = v;
   }
 }
 
@@ -697,7 +798,7 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     float xs[1][2];
     float(&x)[2] = xs[0];
     load2<DT>(a.q, t[0] * a.q_ts + h * a.q_hs + d0, x);
-    turn2<DT, D, 1>(a, a.q, a.q_ts, a.q_hs, a.q_heads, a.q_weight, a.q_norm, t, h, d0, xs);
+    turn2<float, DT, D, 1>(a, a.q, a.q_ts, a.q_hs, a.q_heads, a.q_weight, a.q_norm, t, h, d0, xs);
     if (lane * 2 >= D) return;
     const int64_t o = (int64_t)u * D + d0;
     if constexpr (DT == FVSR_DT_F32) {
@@ -727,7 +828,14 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     load2<DT>(a.k, t[i] * a.k_ts + h * a.k_hs + d0, x[i]);
     load2<DT>(a.v, t[i] * a.v_ts + h * a.v_hs + d0, y[i]);
   }
-  turn2<DT, D, N>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, t, h, d0, x);
+  turn2<float, DT, D, N>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, t, h, d0, x);
+  uint32_t near = 0;  // bit i: a value of token i is near a border
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    Border b;
+    b.see(x[i][0]), b.see(x[i][1]);
+    near |= (uint32_t)b.near() << i;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -774,18 +882,30 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     }
     __builtin_amdgcn_s_waitcnt(0);  // before the new tokens go into the same pieces
   }
-  if (lane * 2 >= D) return;
+  const auto put_k = [&](int slot, const float(&x)[2]) {
+    *(uint16_t*)(kp + slot * D + d0) = (uint16_t)codes4(x[0], x[1], 0.0f, 0.0f, pow2(ke));
+  };
+  const bool both = lane * 2 < D;  // (the upper lanes of 64 dims store nothing)
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (N > 1 && i >= hi - lo) continue;
+    if ((N > 1 && i >= hi - lo) || !both) continue;
     const int slot = lo + i;
-    *(uint16_t*)(kp + slot * D + d0) =
-        (uint16_t)codes4(x[i][0], x[i][1], 0.0f, 0.0f, pow2(ke));
+    put_k(slot, x[i]);
     const uint32_t c = codes4(y[i][0], y[i][1], 0.0f, 0.0f, pow2(ve));
     vp[d0 * kPage + slot] = (uint8_t)c;
     vp[(d0 + 1) * kPage + slot] = (uint8_t)(c >> 8);
   }
   if (lane == 0) *ksp = (uint8_t)(ke + 127), *vsp = (uint8_t)(ve + 127);
+  if (__ballot(near) == 0 || (a.k_norm == kNone && !a.cs)) return;
+#pragma unroll 1
+  for (int i = 0; i < min(N, hi - lo); ++i) {
+    if (__ballot(near >> i & 1) == 0) continue;
+    const int one[1] = {N == 1 ? b : b * n + page * kPage - at + lo + i};
+    float y[1][2];
+    load2<DT>(a.k, one[0] * a.k_ts + h * a.k_hs + d0, y[0]);
+    turn2<double, DT, D, 1>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, one, h, d0, y);
+    if (both) put_k(lo + i, y[0]);
+  }
 }
 
 constexpr int kFew = 8;  // tokens per sequence that a wave takes
@@ -829,7 +949,7 @@ bool rows_aligned(const void* p, int64_t ts, int64_t hs, int64_t size) {
 }  // namespace
 
 extern "C" int64_t fvsr_kv_append_workspace_floats(int64_t T, int k_norm) {
-  return k_norm == FVSR_NORM_ROW && T > kOwnStat ? T : 0;
+  return k_norm == FVSR_NORM_ROW && T > kOwnStat ? 2 * T : 0;
 }
 
 extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stride,
@@ -858,12 +978,13 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
     return FVSR_EUNSUPPORTED;
   const int64_t need = fvsr_kv_append_workspace_floats(T, k_norm);
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;
+  if (need && ((uintptr_t)workspace & 7)) return FVSR_EUNSUPPORTED;
   // Pages that n tokens touch: at most n, and at most (n + 126) / 128 + 1.
   const auto most = [](int64_t n) { return std::min(n, (n + 126) / kPage + 1); };
   Args a{};
   a.c = *cache;
   a.k = k, a.v = v, a.q = q, a.k_weight = k_weight, a.q_weight = q_weight, a.q_out = q_out;
-  a.cs = cs, a.positions = positions, a.row_stat = need ? workspace : nullptr;
+  a.cs = cs, a.positions = positions, a.row_stat = need ? (double*)workspace : nullptr;
   a.k_ts = k_tok_stride, a.k_hs = k_head_stride, a.v_ts = v_tok_stride, a.v_hs = v_head_stride;
   a.q_ts = q_tok_stride, a.q_hs = q_head_stride, a.cs_rows = cs_rows;
   a.T = (int)T, a.q_heads = q ? (int)q_heads : 0, a.k_norm = k_norm, a.q_norm = q_norm;

@@ -317,6 +317,38 @@ def test_append_long_row_norm():
         check_append(pages, before, k, v, table, lengths, None, fr, torch.arange(T), kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,n,norm", [(128, 1100, "none"), (128, 1100, "row"), (64, 1100, "row"),
+                                      (128, 1, "none"), (64, 5, "none")])
+def test_append_codes_of_64_bits(D, dtype, norm, n):
+    """Codes next to a border are those of the 64-bit value.  Four roundings of terms up to |a| +
+    |b| and one of the value: where it is at least 0.7 of those, 2^-24 * (4 / 0.7 + 1) < 8 steps
+    of it, which is the distance from a border within which it is computed in 64 bits.  (With
+    sums in 64 bits from the start, as the rows of many tokens have them.)"""
+    from flashvsr_sm89_ops import append_kv
+    H, B = 4, 1 if n > 8 else 300
+    lens, new = [n + 70] * B, [n] * B
+    table, N = tables(lens, seed=3)
+    pages, g = pool(N, H, D, seed=4), gen(D)
+    k = torch.randn(B * n, H, D, generator=g).to(dtype)
+    freqs = freqs_of(2000, D)
+    pos = torch.randint(0, 2000, (B * n,), generator=g).int()
+    kw = 1 + 0.1 * torch.randn(H * D, generator=g).to(dtype) if norm == "row" else None
+    append_kv(pages, k.to(DEV), k.to(DEV), table.to(DEV), i32(lens).to(DEV),
+              freqs_cis=freqs.to(DEV), positions=pos.to(DEV),
+              k_weight=None if kw is None else kw.to(DEV))
+    after = O.from_pages(*pages)
+    x, size = O.turned(k, kw, freqs, pos, 1e-6), pair_size(k, kw, 1e-6)
+    t = torch.arange(B * n)
+    b, p = t // n, 70 + t % n
+    page = table[b, p // 128].long()
+    got = after["k"][page, :, p % 128]
+    y = x / torch.exp2(after["ke"][page].double())[..., None]
+    plain = (x.abs() >= 0.7 * size) & (y.abs() >= 2.0 ** -6)
+    assert float(plain.double().mean()) > 0.2
+    assert torch.equal(got[plain], O.e4m3(y)[plain])
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_append_special_values(D):
     """Infinities and NaN are stored as NaN and leave the scale alone; zeros; values near

@@ -170,7 +170,7 @@ def test_c_entries_check_arguments():
     assert append(q=fake, qh=4) == _lib.FVSR_EINVAL
     assert append(cs=fake, rows=3) == _lib.FVSR_EINVAL
     assert append(T=4000, kw=fake, kn=2) == _lib.FVSR_EWORKSPACE
-    assert L.fvsr_kv_append_workspace_floats(4000, 2) == 4000
+    assert L.fvsr_kv_append_workspace_floats(4000, 2) == 8000
     assert L.fvsr_kv_append_workspace_floats(4000, 1) == 0
     assert attend(dt=2) == _lib.FVSR_EINVAL and attend(qh=3) == _lib.FVSR_EINVAL
     assert attend(scale=0.0) == _lib.FVSR_EINVAL and attend(scale=math.nan) == _lib.FVSR_EINVAL
