@@ -23,8 +23,8 @@
 // waves instead, without LDS or barriers.
 //
 // Measured, q with k and v: one token x 12 heads 5.3 us (latency: a chain of four loads),
-// 192 of 32/8 heads 5.8; 6 ragged prompts, 1200 tokens on average x 16/4 heads, fp16 10 us
-// (3.4 TB/s); 16896 tokens x 12 heads with row norms 73 us (3.7 TB/s; 5.1 is a copy's
+// 192 of 32/8 heads 5.9; 24 ragged prompts of 6119 tokens in all x 16/4 heads of 64, fp16
+// 10.4 us (3.5 TB/s); 16896 tokens x 12 heads with row norms 73 us (3.7 TB/s; 5.1 is a copy's
 // rate, and k's second read is not counted).  Between them a page's chain of loads bounds
 // it: lengths, page id and positions, rows, rotations, codes.
 #include <algorithm>

@@ -36,7 +36,7 @@
 // Measured, 32 query and 8 key/value heads of 128: one token for each of 128 ragged
 // sequences of up to 16000 tokens 362 us (5.4 TB/s; 5.1 is a copy's rate), for one
 // sequence of 262000 97 us (5.5); 5 for each of 16 of 6000 47 us (4.2).  8448 rows over
-// 25344 tokens x 12 heads 1.15 ms: 1.15 PFLOP/s, where an 8192^3 bf16 product
+// 25344 tokens x 12 heads 1.10 to 1.16 ms: 1.13 to 1.19 PFLOP/s, where an 8192^3 bf16 product
 // reaches 1.21; the clock falls to 1.8 - 1.9 GHz, at which the vector units are busy for 71
 // % of the time and the matrix cores for 53.
 #include <algorithm>
@@ -243,7 +243,7 @@ struct FewUnit {
 };
 template <int ROWS>
 FVSR_DEV bool few_unit(const Args& a, FewUnit& u) {
-  if (!a.c.cu) {  // one unit to a sequence and head
+  if (ROWS == 32 || !a.c.cu) {  // one unit to a sequence and head
     u.split = blockIdx.x, u.h = blockIdx.y;
     u.s.b = blockIdx.z, u.s.part = 0;
     u.s.rows = seq_rows(nullptr, u.s.b, (int)a.c.sequences, a.T);

@@ -163,8 +163,8 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     Values are rounded once, from fp32.  A page's scale is the least power of
     two that holds its new values within 448 (a non-finite one is stored as NaN and
     does not count); if the page already holds tokens, the scale never falls, and where it
-    grows their codes are rounded again.  Sequences that append must not share the
-    pages they append to."""
+    grows their codes are rounded again.  The pages that a call appends to must be
+    distinct."""
     r = (_lib._paged_host or _lib.paged_host()).append_kv(
         pages, k, v, page_table, lengths, cu_tokens, freqs_cis, positions, k_weight, q, q_weight,
         eps)

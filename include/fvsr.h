@@ -476,14 +476,14 @@ enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
  *          [cs_rows, head_dim / 2, 2] of (cos, sin) (NULL: not rotated); a position outside
  *          the table gives NaN
  *   q_out  [T, q_heads, head_dim] in dtype, every row of it written
- * fp32 from the loads to the one rounding.  A page's scale is the least 2^e, e
- * >= -126, with every finite new magnitude at most 448 * 2^e; where the page
- * holds tokens before the new ones, not below its old one, and their codes are
- * rounded again if it grows.  Infinities and NaN are stored as NaN.  Slots
- * behind the last new token keep their bytes.  Sequences that append must not
- * share the pages they append to.
- *   workspace  fvsr_kv_append_workspace_floats(T, k_norm) floats (0: NULL is
- *              fine), used until the call's kernels have run
+ * fp32 from the loads to the one rounding (64 bits where a code hangs on it).  A
+ * page's scale is the least 2^e, e >= -126, with every finite new magnitude at
+ * most 448 * 2^e; where the page holds tokens before the new ones, not below its
+ * old one, and their codes are rounded again if it grows.  Infinities and NaN are
+ * stored as NaN.  Slots behind the last new token keep their bytes.  The pages
+ * that a call appends to must be distinct.
+ *   workspace  fvsr_kv_append_workspace_floats(T, k_norm) floats, 8-byte
+ *              aligned (0: NULL is fine), used until the call's kernels have run
  */
 int64_t fvsr_kv_append_workspace_floats(int64_t T, int k_norm);
 int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stride,
