@@ -896,3 +896,70 @@ def test_graph_and_stream():
         assert torch.equal(out, want)
         for a, b in zip(pages, other):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("n", [5, 100])
+def test_graph_of_many_rows(n):
+    """A captured step of several rows per sequence (row norms: for many rows with their
+    workspaces) equals the eager one, replay after replay."""
+    from flashvsr_sm89_ops import append_kv, kv_pages, paged_attention
+    B, Hq, H, D = 2, 8, 2, 128
+    pages, other = kv_pages(60, H, D, DEV), kv_pages(60, H, D, DEV)
+    table = torch.randperm(60, generator=gen(0)).int().view(2, 30).to(DEV)
+    lengths = i32([n, 1500]).to(DEV)
+    q, k, v = (torch.randn(B * n, h, D, generator=gen(h)).bfloat16().to(DEV) for h in (Hq, H, H))
+    w, wq = torch.ones(H * D, device=DEV), torch.ones(Hq * D, device=DEV)
+    freqs = freqs_of(B * n, D).to(DEV)
+
+    def step(p):
+        r = append_kv(p, k, v, table, lengths, freqs_cis=freqs, k_weight=w, q=q, q_weight=wq)
+        return paged_attention(r, p, table, lengths)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = step(pages)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(warm, step(other))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(pages)
+    for i in range(4):
+        lengths += n
+        k.copy_(torch.randn(B * n, H, D, generator=gen(50 + i)).bfloat16())
+        q.copy_(torch.randn(B * n, Hq, D, generator=gen(60 + i)).bfloat16())
+        g.replay()
+        want = step(other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for a, b in zip(pages, other):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_two_streams_of_one_pool():
+    """Sequences of one pool stepping on two streams at once, their pages side by side."""
+    from flashvsr_sm89_ops import append_kv, kv_pages, paged_attention
+    Hq, H, D, steps = 8, 2, 128, 40
+    table = torch.arange(40).int().view(20, 2).t().contiguous().to(DEV)  # even pages, odd pages
+    q, k, v = (torch.randn(steps, 2, 60, h, D, generator=gen(h)).bfloat16().to(DEV)
+               for h in (Hq, H, H))
+    lens = [i32([60 * (i + 1)]).to(DEV) for i in range(steps)]
+
+    def step(p, i, b):
+        append_kv(p, k[i, b], v[i, b], table[b:b + 1], lens[i])
+        return paged_attention(q[i, b], p, table[b:b + 1], lens[i])
+    one, two = kv_pages(40, H, D, DEV), kv_pages(40, H, D, DEV)
+    want = [[step(one, i, b) for b in (0, 1)] for i in range(steps)]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(steps):
+        row = []
+        for b in (0, 1):
+            with torch.cuda.stream(side[b]):
+                row.append(step(two, i, b))
+        got.append(row)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for a, b in zip(one, two):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
