@@ -160,7 +160,7 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     (2i, 2i + 1) are rotated by row positions[t] (int32 [T]; default: row t); a
     position outside the table gives NaN.
 
-    Values are rounded once, from fp32.  A page's scale is the least power of
+    Values are rounded once, from fp32 or better.  A page's scale is the least power of
     two that holds its new values within 448 (a non-finite one is stored as NaN and
     does not count); if the page already holds tokens, the scale never falls, and where it
     grows their codes are rounded again.  The pages that a call appends to must be
