@@ -968,15 +968,16 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   if (q && (q_heads <= 0 || !q_out)) return FVSR_EINVAL;
   if ((k_norm && !k_weight) || (q && q_norm && !q_weight)) return FVSR_EINVAL;
   if (cs && (cs_rows <= 0 || (!positions && cs_rows < T))) return FVSR_EINVAL;
-  if (T == 0 || cache->sequences == 0) return FVSR_OK;
-  if (!k || !v) return FVSR_EINVAL;
   const int64_t size = dtype == FVSR_DT_F32 ? 4 : 2, D = cache->head_dim, B = cache->sequences;
-  if (!rows_aligned(k, k_tok_stride, k_head_stride, size) ||
-      !rows_aligned(v, v_tok_stride, v_head_stride, size) ||
+  // Without sequences no row of k and v has a place, but the q rows are turned.
+  if (T == 0 || (B == 0 && !q)) return FVSR_OK;
+  if (B > 0 && (!k || !v)) return FVSR_EINVAL;
+  if ((B > 0 && (!rows_aligned(k, k_tok_stride, k_head_stride, size) ||
+                 !rows_aligned(v, v_tok_stride, v_head_stride, size))) ||
       (q && !rows_aligned(q, q_tok_stride, q_head_stride, size)) ||
       (((uintptr_t)q_out | (uintptr_t)k_weight | (uintptr_t)q_weight | (uintptr_t)cs) & 15))
     return FVSR_EUNSUPPORTED;
-  const int64_t need = fvsr_kv_append_workspace_floats(T, k_norm);
+  const int64_t need = B > 0 ? fvsr_kv_append_workspace_floats(T, k_norm) : 0;
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;
   if (need && ((uintptr_t)workspace & 7)) return FVSR_EUNSUPPORTED;
   // Pages that n tokens touch: at most n, and at most (n + 126) / 128 + 1.
@@ -989,9 +990,10 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   a.q_ts = q_tok_stride, a.q_hs = q_head_stride, a.cs_rows = cs_rows;
   a.T = (int)T, a.q_heads = q ? (int)q_heads : 0, a.k_norm = k_norm, a.q_norm = q_norm;
   a.w_dt = weight_dtype, a.eps = eps;
-  a.units_max = (int)most(T / B);
+  a.units_max = B > 0 ? (int)most(T / B) : 0;
   // Packed rows: the sum of those bounds over any B counts that add up to T.
-  const int64_t units = cache->cu ? std::min(T, (T + 126 * B) / kPage + B) : B * a.units_max;
+  const int64_t units = B > 0 && cache->cu ? std::min(T, (T + 126 * B) / kPage + B)
+                                           : B * a.units_max;
   // Workgroups of either form of a launch, of 256 threads or twice that (kWg).
   const int64_t q_wgs = q ? T * q_heads / 4 + T / 4 + 2 : 0;
   if ((q && q_heads > kMaxBlocks) || (units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks / 2 ||

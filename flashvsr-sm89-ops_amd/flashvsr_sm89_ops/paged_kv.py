@@ -153,7 +153,8 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     positions lengths[b] - n .. lengths[b] - 1 (lengths [B] int32: with this
     step's tokens), position p to slot p % 128 of page page_table[b, p // 128]
     (int32 [B, P]).  Positions below 0 or past the table and pages outside the pool
-    are not stored; rows behind cu_tokens[B] belong to nobody.
+    are not stored; rows behind cu_tokens[B] belong to nobody (their q is turned all the
+    same).
 
     k_weight, q_weight: RMSNorm first, over each head ([head_dim]) or the whole
     row ([heads * head_dim]).  freqs_cis (complex [rows, head_dim / 2]): then the pairs

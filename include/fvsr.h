@@ -475,7 +475,8 @@ enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
  *          (2i, 2i + 1) rotated by row positions[t] (NULL: row t) of cs, fp32
  *          [cs_rows, head_dim / 2, 2] of (cos, sin) (NULL: not rotated); a position outside
  *          the table gives NaN
- *   q_out  [T, q_heads, head_dim] in dtype, every row of it written
+ *   q_out  [T, q_heads, head_dim] in dtype, every row of it written (rows of no
+ *          sequence too, and all of them where there are no sequences)
  * fp32 from the loads to the one rounding (64 bits where a code hangs on it).  A
  * page's scale is the least 2^e, e >= -126, with every finite new magnitude at
  * most 448 * 2^e; where the page holds tokens before the new ones, not below its
