@@ -209,8 +209,8 @@ FVSR_DEV uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 
 // max(m, |a|, |b|) in one v_max3_f32.  A NaN operand is passed over as
-// fmaxf does (the kernels' NaNs are quiet: bf16 data and conversions), and
-// the operands need no canonicalising maximum first.
+// fmaxf does if it is quiet, as results and conversions are; a signalling one
+// (bits from memory) loses m.  The operands get no canonicalising maximum first.
 FVSR_DEV float max3_abs(float m, float a, float b) {
   float r;
   asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));

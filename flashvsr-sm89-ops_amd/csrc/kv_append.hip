@@ -225,6 +225,12 @@ FVSR_DEV void load_turn(const Args& a, int t, int d0, float (&cs)[8]) {
   outside(p, a.cs_rows, cs);
 }
 
+// NaNs as they lie in memory may signal, of which v_max3_f32 would lose what it held.
+FVSR_DEV void quieten(float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __builtin_canonicalizef(x[e]);
+}
+
 // x * r * w, then the rotation of its four pairs.
 FVSR_DEV void norm_turn(float (&x)[8], bool norm, float r, const float (&w)[8], bool turn,
                         const float (&cs)[8]) {
@@ -449,6 +455,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
       if (a.k_norm == kHead) r = inv_rms(lanes_sum<C>(sum_sq<float>(x[i])), D, a.eps);
       if (a.k_norm == kRow) r = rs[i];
       norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
+      if (a.k_norm == kNone && !a.cs) quieten(x[i]);
       if (!live(i)) continue;
       Border b;
 #pragma unroll
@@ -527,6 +534,7 @@ FVSR_DEV void append_v(const Args& a, const Job& j, uint8_t* vt, float (&tops)[k
   for (int i = 0; i < R; ++i) {
     float y[8];
     widen(raw[i], y);
+    if constexpr (DT != FVSR_DT_F16) quieten(y);  // (fp16: its conversion did)
 #pragma unroll
     for (int k = 0; k < 8; k += 2) top = max3_abs(top, y[k], y[k + 1]);
   }
