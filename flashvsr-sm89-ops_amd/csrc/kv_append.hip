@@ -47,6 +47,7 @@ struct Args {
   const float* cs;           // [cs_rows][D/2][2] (cos, sin); null: no rotation
   const int32_t* positions;  // row of cs for each token; null: the token's own number
   double* row_stat;          // 1/rms of each k row (row norm, from the launch before)
+  double k_per;              // 1 / elements that a norm of k is over
   int64_t k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, cs_rows;
   int T, q_heads, k_norm, q_norm, w_dt, units, units_max, page_wgs;
   float eps;
@@ -110,7 +111,8 @@ FVSR_DEV void store8(void* p, int dt, int64_t i, const float (&x)[8]) {
 // Sums and what follows from them in fp32, or (T double) in 64 bits.  q is rounded to its
 // own type in the end, where fp32's steps do not show, but k to a code of 4 bits: fp32's
 // steps put 1 or 2 in 10^6 on the other side of a border between codes, 1 / 16 off.  So
-// what lies near a border is computed again in 64 bits, from 64-bit sums.  (Errors of k
+// k's sums are taken in 64 bits (beyond eight squares at least, which also keeps those that
+// fp32 does not hold), and what lies near a border is computed again in 64 bits.  (Errors of k
 // against 64 bits: 2e-5 of its norm without, 2e-7 so.  16896 tokens x 12 heads 69 us
 // without, 73 so, 84 with all of k in 64 bits.)
 template <class T>
@@ -122,7 +124,12 @@ FVSR_DEV T sum_sq(const float (&x)[8]) {
 }
 
 FVSR_DEV float inv_rms(float sq, int n, float eps) { return 1.0f / __builtin_sqrtf(sq / n + eps); }
-FVSR_DEV double inv_rms(double sq, int n, float eps) { return 1.0 / __builtin_sqrt(sq / n + eps); }
+// The same in 64 bits, with per = 1 / n: the instruction's 2^-23 and a Newton step, 2^-45.
+FVSR_DEV double inv_rms64(double sq, double per, float eps) {
+  const double m = __builtin_fma(sq, per, (double)eps), r = __builtin_amdgcn_rsq(m);
+  const double e = __builtin_fma(-0.5 * m * r, r, 0.5);
+  return e == e ? __builtin_fma(r, e, r) : r;  // (m 0 or infinite: r is it)
+}
 
 // Sum over the N = 8, 16 or 64 lanes around, from lane to lane (dpp).
 template <int CTRL, int ROWS = 0xf>
@@ -156,9 +163,11 @@ FVSR_DEV T lanes_sum(T v) {
 
 // Whether one of the values seen lies within kNear fp32 steps of a border between
 // codes of 4 bits (subnormal codes aside, whose steps are small): mantissas whose last 20
-// bits are near their half.  A value is four roundings off, more only where a rotation
-// leaves little of its terms.
-constexpr uint32_t kNear = 8;
+// bits are near their half.  In units of 2^-24 of itself a value is off by half of what
+// its sum of squares is (8, where eight at a time are summed in fp32) and 1 for 1 / rms as fp32,
+// alike in both terms of a rotation, 3 in each term (x r, w, cos or sin) and 1 in the result:
+// 5 + 3 / 0.7 + 1 < 11 steps where the rotation leaves 0.7 of its terms.
+constexpr uint32_t kNear = 12;
 struct Border {
   uint32_t least = ~0u;
   __device__ __forceinline__ void see(float x) {
@@ -401,7 +410,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
   if (a.k_norm == kRow && !a.row_stat) {
     for (int i = j.lo + (tid >> 6); i < j.hi; i += kWg<D> / 64) {
       const double r =
-          inv_rms(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), H * D, a.eps);
+          inv_rms64(row_sq<DT, D, 1>(a.k, (j.row0 + i) * a.k_ts, a.k_hs, H), a.k_per, a.eps);
       if ((tid & 63) == 0) stat[i] = r;
     }
     __syncthreads();
@@ -452,7 +461,8 @@ FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
         outside(pos[i], a.cs_rows, cs);
       }
       float r = 1.0f;
-      if (a.k_norm == kHead) r = inv_rms(lanes_sum<C>(sum_sq<float>(x[i])), D, a.eps);
+      if (a.k_norm == kHead)
+        r = (float)inv_rms64(lanes_sum<C>(sum_sq<double>(x[i])), a.k_per, a.eps);
       if (a.k_norm == kRow) r = rs[i];
       norm_turn(x[i], a.k_norm != kNone, r, w, a.cs != nullptr, cs);
       if (a.k_norm == kNone && !a.cs) quieten(x[i]);
@@ -503,7 +513,7 @@ FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
     if (a.cs) load_turn<D>(a, t, d0, cs);
     if (a.k_norm != kNone) load8(a.k_weight, a.w_dt, (a.k_norm == kRow ? j.h * D : 0) + d0, w);
     double r = 1.0;
-    if (a.k_norm == kHead) r = inv_rms(lanes_sum<C>(sum_sq<double>(y)), D, a.eps);
+    if (a.k_norm == kHead) r = inv_rms64(lanes_sum<C>(sum_sq<double>(y)), a.k_per, a.eps);
     if (a.k_norm == kRow) r = a.row_stat ? a.row_stat[t] : stat[slot];
     norm_turn64(y, a.k_norm != kNone, r, w, a.cs != nullptr, cs);
     if (slot == slot0 + i)
@@ -687,7 +697,7 @@ __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
   const int t = ((int)blockIdx.x - a.page_wgs) * W + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int H = (int)a.c.heads;
-  const double r = inv_rms(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), H * D, a.eps);
+  const double r = inv_rms64(row_sq<DT, D, kHeld>(a.k, t * a.k_ts, a.k_hs, H), a.k_per, a.eps);
   if ((threadIdx.x & 63) == 0) a.row_stat[t] = r;
 }
 
@@ -720,10 +730,11 @@ FVSR_DEV void load2(const void* p, int64_t i, float (&x)[2]) {
 FVSR_DEV float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 FVSR_DEV double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
-// Norm and rotation of two dims d0, d0 + 1 of a head of N tokens t, a wave per head; `ts`,
-// `hs` and `heads` describe the rows of src (q or k).  Each kind of load goes out
-// for all tokens at once.
-template <class F, int DT, int D, int N>
+// Norm and rotation of two dims d0, d0 + 1 of a head of N tokens t in F, a wave per head;
+// `ts`, `hs` and `heads` describe the rows of src (q or k).  Each kind of load goes out
+// for all tokens at once.  Sums are in S, but a row's of eight squares at a time in F: all
+// of it in 64 bits takes 64 x 5 tokens with row norms from 18.8 to 22.6 us.
+template <class F, class S, int DT, int D, int N>
 FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int heads,
                     const void* weight, int norm, const int (&t)[N], int h, int d0,
                     float (&x)[N][2]) {
@@ -731,7 +742,7 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
   int pos[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) pos[i] = a.positions ? a.positions[t[i]] : t[i];
-  F sq[N] = {};
+  S sq[N] = {};
   float cs[N][2];
   if (norm == kRow) {
     for (int c = lane; c < heads * (D / 8); c += 64) {
@@ -743,13 +754,13 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
       for (int i = 0; i < N; ++i) {
         float r[8];
         widen(raw[i], r);
-        sq[i] += sum_sq<F>(r);
+        sq[i] += (S)sum_sq<F>(r);
       }
     }
   } else if (norm == kHead) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      sq[i] = lane * 2 < D ? (F)x[i][0] * (F)x[i][0] + (F)x[i][1] * (F)x[i][1] : (F)0;
+      sq[i] = lane * 2 < D ? (S)x[i][0] * (S)x[i][0] + (S)x[i][1] * (S)x[i][1] : (S)0;
   }
   if (a.cs) {
 #pragma unroll
@@ -771,8 +782,20 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
   for (int i = 0; i < N; ++i) {
     F u = x[i][0], v = x[i][1];
     if (norm != kNone) {
-      const F r = inv_rms(lanes_sum<64>(sq[i]), norm == kRow ? heads * D : D, a.eps);
-      u = u * w[0] * r, v = v * w[1] * r;
+      F r;
+      S sum = lanes_sum<64>(sq[i]);
+      if constexpr (std::is_same_v<S, double>) {
+        // (Squares that fp32 does not hold: rare, and the same for the whole wave.)
+        if (std::is_same_v<F, float> && norm == kRow && !(sum > 0x1p-80 && sum < 0x1p127))
+          sum = row_sq<DT, D, 1>(src, t[i] * ts, hs, heads);
+        r = (F)inv_rms64(sum, a.k_per, a.eps);
+      } else {
+        r = inv_rms(sum, norm == kRow ? heads * D : D, a.eps);
+      }
+      if constexpr (std::is_same_v<F, double>)
+        u = u * w[0] * r, v = v * w[1] * r;  // (x * w is exact)
+      else
+        u = u * r * w[0], v = v * r * w[1];  // (x * w may be more than fp32 holds)
     }
     if (a.cs) {
       const F c = cs[i][0], s = cs[i][1], o = fused(u, c, -(v * s));
@@ -806,7 +829,8 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     float xs[1][2];
     float(&x)[2] = xs[0];
     load2<DT>(a.q, t[0] * a.q_ts + h * a.q_hs + d0, x);
-    turn2<float, DT, D, 1>(a, a.q, a.q_ts, a.q_hs, a.q_heads, a.q_weight, a.q_norm, t, h, d0, xs);
+    turn2<float, float, DT, D, 1>(a, a.q, a.q_ts, a.q_hs, a.q_heads, a.q_weight, a.q_norm, t, h,
+                                  d0, xs);
     if (lane * 2 >= D) return;
     const int64_t o = (int64_t)u * D + d0;
     if constexpr (DT == FVSR_DT_F32) {
@@ -836,7 +860,7 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     load2<DT>(a.k, t[i] * a.k_ts + h * a.k_hs + d0, x[i]);
     load2<DT>(a.v, t[i] * a.v_ts + h * a.v_hs + d0, y[i]);
   }
-  turn2<float, DT, D, N>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, t, h, d0, x);
+  turn2<float, double, DT, D, N>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, t, h, d0, x);
   uint32_t near = 0;  // bit i: a value of token i is near a border
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -911,7 +935,7 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
     const int one[1] = {N == 1 ? b : b * n + page * kPage - at + lo + i};
     float y[1][2];
     load2<DT>(a.k, one[0] * a.k_ts + h * a.k_hs + d0, y[0]);
-    turn2<double, DT, D, 1>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, one, h, d0, y);
+    turn2<double, double, DT, D, 1>(a, a.k, a.k_ts, a.k_hs, H, a.k_weight, a.k_norm, one, h, d0, y);
     if (both) put_k(lo + i, y[0]);
   }
 }
@@ -998,6 +1022,7 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
   a.q_ts = q_tok_stride, a.q_hs = q_head_stride, a.cs_rows = cs_rows;
   a.T = (int)T, a.q_heads = q ? (int)q_heads : 0, a.k_norm = k_norm, a.q_norm = q_norm;
   a.w_dt = weight_dtype, a.eps = eps;
+  a.k_per = 1.0 / (double)(k_norm == kRow ? cache->heads * D : D);
   a.units_max = B > 0 ? (int)most(T / B) : 0;
   // Packed rows: the sum of those bounds over any B counts that add up to T.
   const int64_t units = B > 0 && cache->cu ? std::min(T, (T + 126 * B) / kPage + B)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import paged_kv as O
-from test_gpu_paged_kv import DEV, check_append, check_q, freqs_of, gen, i32, pool, tables
+from test_gpu_paged_kv import DEV, check_append, check_q, freqs_of, gen, i32, pool, starts, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,88 @@ def test_append_signalling_nan(D, dtype, T, where):
         x.view(integer)[at] = bits
     append_kv(pages, k.to(DEV), v.to(DEV), table.to(DEV), i32([T]).to(DEV))
     check_append(pages, before, k, v, table, [T], None, None, None, None)
+
+
+def above_border(x, rms, low):
+    """Weights with which each x * w / rms (x nonzero) lies less than two fp32 steps above
+    the border `low` between two codes, in 64 bits."""
+    w = torch.where(x == 0, 1.0, low * rms / x.abs().double().clamp(min=1e-30)).float()
+    under = (x.abs().double() * w.double() / rms <= low) & (x != 0)
+    return torch.where(under, torch.nextafter(w, torch.full_like(w, math.inf)), w)
+
+
+@pytest.mark.parametrize("D,H", [(64, 256), (128, 128)])
+@pytest.mark.parametrize("n", [1, 5, 20])
+def test_append_row_norm_codes_next_to_a_border(D, H, n):
+    """A row whose squares add up badly in fp32: a lane's sum starts at 1, and each of the
+    31 squares behind it, a little over half a step, counts as a whole one.  That is 31 * 2^-24 of
+    the sum and half of it, 15 steps, in each value; their codes are those of the 64-bit value."""
+    from flashvsr_sm89_ops import append_kv
+    x = torch.zeros(H * D // 512, 64, 8)  # [turn of a wave, lane, element]
+    x[0, :, 0] = 1.0
+    x[1:, :, 0] = 2.0 ** -12 * (1 + 2.0 ** -10)
+    x = x.reshape(H * D)
+    rms = math.sqrt(float((x.double() ** 2).mean()) + 1e-6)
+    w = above_border(x, rms, 1.9375)
+    T = 2 * n
+    k = torch.where(torch.rand(T, H * D, generator=gen(n)) < 0.5, x, -x).view(T, H, D)
+    table, N = tables([n, n])
+    pages = pool(N, H, D)
+    append_kv(pages, k.to(DEV), k.to(DEV), table.to(DEV), i32([n, n]).to(DEV), k_weight=w.to(DEV))
+    got = O.from_pages(*pages)
+    for b in range(2):
+        page = int(table[b, 0])
+        s = torch.exp2(got["ke"][page].double())[:, None, None]
+        y = O.turned(k[b * n:(b + 1) * n], w, None, None, 1e-6).transpose(0, 1)
+        assert torch.equal(got["k"][page, :, :n], O.e4m3(y / s))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,norm", [(1100, "head"), (1, "head"), (5, "head"), (1, "row"),
+                                    (5, "row"), (30, "row")])
+def test_append_codes_of_64_bits_with_norms(D, dtype, norm, n):
+    """Codes are those of the 64-bit value where the rotation leaves 0.7 of its terms, for the
+    norms and counts of tokens whose sums are taken beside the values."""
+    from flashvsr_sm89_ops import append_kv
+    H, B = 4, 1 if n > 8 else 300
+    lens = [n + 70] * B
+    table, N = tables(lens, seed=3)
+    pages, g = pool(N, H, D, seed=4), gen(D + n)
+    k = torch.randn(B * n, H, D, generator=g).to(dtype)
+    freqs = freqs_of(2000, D)
+    pos = torch.randint(0, 2000, (B * n,), generator=g).int()
+    kw = 1 + 0.1 * torch.randn(D * (H if norm == "row" else 1), generator=g)
+    append_kv(pages, k.to(DEV), k.to(DEV), table.to(DEV), i32(lens).to(DEV),
+              freqs_cis=freqs.to(DEV), positions=pos.to(DEV), k_weight=kw.to(DEV))
+    after = O.from_pages(*pages)
+    x = O.turned(k, kw, freqs, pos, 1e-6)
+    a = O.turned(k, kw, None, None, 1e-6).abs()
+    size = (a[..., 0::2] + a[..., 1::2]).repeat_interleave(2, -1)
+    t = torch.arange(B * n)
+    b, p = t // n, 70 + t % n
+    page = table[b, p // 128].long()
+    y = x / torch.exp2(after["ke"][page].double())[..., None]
+    plain = (x.abs() >= 0.7 * size) & (y.abs() >= 2.0 ** -6)
+    assert float(plain.double().mean()) > 0.2
+    assert torch.equal(after["k"][page, :, p % 128][plain], O.e4m3(y)[plain])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("norm", ["head", "row"])
+@pytest.mark.parametrize("n", [1, 5, 30, 100])
+@pytest.mark.parametrize("size", [1e-30, 1e25, 1e38])
+def test_append_norm_of_far_values(D, norm, n, size):
+    """Keys whose squares fp32 does not hold are normed as any others."""
+    from flashvsr_sm89_ops import append_kv
+    H, g = 4, gen(n)
+    table, N = tables([n])
+    pages = pool(N, H, D)
+    before = O.from_pages(*pages)
+    k = (torch.randn(n, H, D, generator=g) * size).clamp(-3e38, 3e38).bfloat16()
+    v = torch.randn(n, H, D, generator=g).bfloat16()
+    kw = 1 + 0.2 * torch.randn(D * (H if norm == "row" else 1), generator=g)
+    eps = 1e-70 if size < 1 else 1e-6  # (fp32: 0)
+    append_kv(pages, k.to(DEV), v.to(DEV), table.to(DEV), i32([n]).to(DEV), k_weight=kw.to(DEV),
+              eps=eps)
+    check_append(pages, before, k, v, table, [n], None, None, None, kw, 0.0 if size < 1 else eps)
