@@ -26,7 +26,6 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .fused_rms_rope import _freqs_table
 
 PAGE = 128
 _HEAD_DIMS = (64, 128)
@@ -140,6 +139,13 @@ def _norm(name: str, weight, heads: int, D: int, what: str) -> int:
     return _lib.NORM_ROW
 
 
+def _rotations(freqs: torch.Tensor) -> torch.Tensor:
+    """complex [.., rows, D / 2] -> fp32 [rows, D / 2, 2] (cos, sin): a contiguous complex64 table
+    itself, any other converted by this call (and so by every replay of a captured one)."""
+    f = freqs.reshape(-1, freqs.shape[-1]).resolve_conj()
+    return torch.view_as_real(f.to(torch.complex64).contiguous())
+
+
 def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
               lengths: torch.Tensor, cu_tokens: torch.Tensor | None = None, *, freqs_cis=None,
               positions: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
@@ -157,9 +163,9 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     same).
 
     k_weight, q_weight: RMSNorm first, over each head ([head_dim]) or the whole
-    row ([heads * head_dim]).  freqs_cis (complex [rows, head_dim / 2]): then the pairs
-    (2i, 2i + 1) are rotated by row positions[t] (int32 [T]; default: row t); a
-    position outside the table gives NaN.
+    row ([heads * head_dim]).  freqs_cis (complex [rows, head_dim / 2]; complex64 is read as it
+    lies, complex128 converted by each call): then the pairs (2i, 2i + 1) are rotated by row
+    positions[t] (int32 [T]; default: row t); a position outside the table gives NaN.
 
     Values are rounded once, from fp32 or better.  A page's scale is the least power of
     two that holds its new values within 448 (a non-finite one is stored as NaN and
@@ -197,7 +203,7 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     if freqs_cis is not None:
         _check(torch.is_complex(freqs_cis) and freqs_cis.shape[-1] == D // 2,
                f"{name}: freqs_cis must be complex [rows, {D // 2}]")
-        cs = _freqs_table(freqs_cis)
+        cs = _rotations(freqs_cis)
         if positions is None:
             _check(cs.shape[0] >= T, f"{name}: freqs_cis has {cs.shape[0]} rows for {T} tokens")
         else:

@@ -148,3 +148,40 @@ def test_append_norm_of_far_values(D, norm, n, size):
     append_kv(pages, k.to(DEV), v.to(DEV), table.to(DEV), i32([n]).to(DEV), k_weight=kw.to(DEV),
               eps=eps)
     check_append(pages, before, k, v, table, [n], None, None, None, kw, 0.0 if size < 1 else eps)
+
+
+def test_append_double_rotations_are_not_kept():
+    """A complex128 table is read as it is at the call: changed behind autograd's back, first
+    used by a captured call, made in inference mode."""
+    from flashvsr_sm89_ops import append_kv
+    H, D, T, g = 2, 64, 20, gen(1)
+    table, N = tables([T])
+    pages = pool(N, H, D)
+    q, k = (torch.randn(T, H, D, generator=g).bfloat16() for _ in range(2))
+    dq, dk, t, n = q.to(DEV), k.to(DEV), table.to(DEV), i32([T]).to(DEV)
+    host = freqs_of(2 * T, D).to(torch.complex128)
+    fr = host[:T].to(DEV)
+
+    def step():
+        return append_kv(pages, dk, dk, t, n, freqs_cis=fr, q=dq)
+    pos = torch.arange(T)
+    check_q(step(), q, host[:T], pos, None)
+    fr.data.copy_(host[T:])
+    check_q(step(), q, host[T:], pos, None)
+    # A call that is captured first, and an eager one before any replay.
+    fr = host[:T].to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    check_q(step(), q, host[:T], pos, None)
+    for rows in (host[T:], host[:T], host[T:]):
+        fr.copy_(rows)
+        graph.replay()
+        check_q(out, q, rows, pos, None)
+        check_q(step(), q, rows, pos, None)
+    with torch.inference_mode():
+        fr = host[:T].to(DEV) * 1
+        check_q(step(), q, host[:T], pos, None)
+    for dtype in (torch.complex64, torch.complex128):
+        fr = host[:T].to(dtype).to(DEV).conj()
+        check_q(step(), q, host[:T].conj(), pos, None)
