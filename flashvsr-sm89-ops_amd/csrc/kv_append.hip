@@ -847,6 +847,7 @@ __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
   const int b = unit / H / parts, part = unit / H % parts, h = unit % H;
   const int n = N == 1 ? 1 : a.T / B, len = max(a.c.lengths[b], 0), at = len - n;
   const int page = max(at, 0) / kPage + part;
+  if (N > 1 && page > max(len - 1, 0) / kPage) return;  // (its positions may pass 32 bits)
   const int lo = max(max(at, 0), page * kPage) - page * kPage, hi = min(len - page * kPage, kPage);
   if (N > 1 && hi <= lo) return;
   // Tokens of slots lo .. hi - 1, the last one repeated.

@@ -185,3 +185,19 @@ def test_append_double_rotations_are_not_kept():
     for dtype in (torch.complex64, torch.complex128):
         fr = host[:T].to(dtype).to(DEV).conj()
         check_q(step(), q, host[:T].conj(), pos, None)
+
+
+@pytest.mark.parametrize("n", [1, 5, 9])
+def test_append_lengths_near_two_billion(n):
+    """Positions up to 2^31 - 1 lie past every table: nothing is stored, and q comes back."""
+    from flashvsr_sm89_ops import append_kv
+    H, D = 2, 64
+    pages = pool(4, H, D)
+    before = [p.view(torch.uint8).clone() for p in pages]
+    q = torch.randn(3 * n, H, D, generator=gen(n)).bfloat16()
+    d = q.to(DEV)
+    table = i32([[0, 1], [2, 3], [0, 1]]).to(DEV)
+    lengths = i32([2 ** 31 - 1, 2 ** 31 - 3, 2 ** 31 - 128]).to(DEV)
+    for cu in (None, starts([n, n, n]).to(DEV)):
+        assert torch.equal(append_kv(pages, d, d, table, lengths, cu, q=d), d)
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, pages))
