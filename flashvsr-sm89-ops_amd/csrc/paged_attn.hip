@@ -56,6 +56,7 @@ typedef short v2s __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 constexpr float kNothing = -1e30f;  // reference of a row that has seen no key (finite)
 constexpr int kMaxSplits = 64;
+constexpr int64_t kMaxGridYZ = 65535;
 
 struct Args {
   fvsr_kv_cache c;
@@ -1228,8 +1229,9 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   // sequences of 7.5 tokens x 32 / 8 heads 168 -> 134 us, 16 of 14 x 16 / 4 44 -> 24; 32 rows
   // to a workgroup: no better, or 20 against 17).  The same number for each: if one unit
   // of 16 or 32 holds them (20 rows over 6000 tokens: two units of 16 64 us, one of
-  // 32 47, a tile of 128 52).
-  if (!keep && T * group <= B * (c->cu ? 64 : 32))
+  // 32 47, a tile of 128 52) and a grid holds their heads and sequences.
+  if (!keep && T * group <= B * (c->cu ? 64 : 32) &&
+      (c->cu || (c->heads <= kMaxGridYZ && B <= kMaxGridYZ)))
     p.few = c->cu || T * group <= B * 16 ? 16 : 32;
   if (p.few) {
     p.tiles = tiles(group, p.few);
@@ -1328,8 +1330,7 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
   if (T * q_heads > 0x7fffffff - 256) return FVSR_EUNSUPPORTED;
   const Plan p = plan_attn(cache, T, q_heads, keep != nullptr);
   if (p.units > kMaxBlocks / 2 || T * q_heads > kMaxBlocks * 64 ||
-      (p.few && (cache->heads > 65535 || (!cache->cu && cache->sequences > 65535) ||
-                 p.units * p.splits > kMaxBlocks || (p.splits > 1 && T * q_heads > kMaxBlocks))))
+      (p.few && (p.units * p.splits > kMaxBlocks || (p.splits > 1 && T * q_heads > kMaxBlocks))))
     return FVSR_EUNSUPPORTED;
   const int64_t need = p.floats(T, q_heads, cache->head_dim);
   if (need && (!workspace || workspace_floats < need)) return FVSR_EWORKSPACE;

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from oracle import paged_kv as O
-from test_gpu_paged_kv import DEV, check_append, check_q, freqs_of, gen, i32, pool, starts, tables
+from test_gpu_paged_kv import (DEV, check_append, check_attention, check_q, freqs_of, gen, i32,
+                               pool, starts, tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -201,3 +202,19 @@ def test_append_lengths_near_two_billion(n):
     for cu in (None, starts([n, n, n]).to(DEV)):
         assert torch.equal(append_kv(pages, d, d, table, lengths, cu, q=d), d)
     assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, pages))
+
+
+@pytest.mark.parametrize("n,Hq", [(1, 1), (2, 2), (20, 1)])
+def test_attention_of_many_sequences(n, Hq):
+    """More sequences of few rows than a grid's third dimension holds."""
+    from flashvsr_sm89_ops import paged_attention
+    B, D, some = 66000, 64, 6
+    lens = [200, n, 0, 129, 128, 1]
+    table, N = tables(lens)
+    pages = pool(N, 1, D)
+    q = torch.randn(some * n, Hq, D, generator=gen(n)).bfloat16()
+    t, L = table.repeat(B // some, 1).to(DEV), i32(lens).repeat(B // some).to(DEV)
+    out = paged_attention(q.to(DEV).repeat(B // some, 1, 1), pages, t, L)
+    check_attention(out[:some * n], q, pages, table, lens)
+    assert torch.equal(out.view(B // some, some * n, Hq, D),
+                       out[:some * n].expand(B // some, -1, -1, -1))
