@@ -999,6 +999,7 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
       k_norm < 0 || k_norm > FVSR_NORM_ROW || q_norm < 0 || q_norm > FVSR_NORM_ROW)
     return FVSR_EINVAL;
   if (q && (q_heads <= 0 || !q_out)) return FVSR_EINVAL;
+  if (q && q_heads > kMaxBlocks) return FVSR_EUNSUPPORTED;
   if ((k_norm && !k_weight) || (q && q_norm && !q_weight)) return FVSR_EINVAL;
   if (cs && (cs_rows <= 0 || (!positions && cs_rows < T))) return FVSR_EINVAL;
   const int64_t size = dtype == FVSR_DT_F32 ? 4 : 2, D = cache->head_dim, B = cache->sequences;
@@ -1030,7 +1031,7 @@ extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t
                                            : B * a.units_max;
   // Workgroups of either form of a launch, of 256 threads or twice that (kWg).
   const int64_t q_wgs = q ? T * q_heads / 4 + T / 4 + 2 : 0;
-  if ((q && q_heads > kMaxBlocks) || (units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks / 2 ||
+  if ((units + 7) * 2 * cache->heads + q_wgs > kMaxBlocks / 2 ||
       T * (cache->heads + a.q_heads) > kMaxBlocks * 64)
     return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;

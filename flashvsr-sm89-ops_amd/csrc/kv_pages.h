@@ -80,8 +80,8 @@ static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T) {
       c->table_stride < c->table_pages)
     return FVSR_EINVAL;
   if (c->head_dim != 64 && c->head_dim != 128) return FVSR_EUNSUPPORTED;
-  if (T > 0x3fffffff || T * c->heads > kMaxBlocks * 64 || c->sequences > 0x3fffff ||
-      c->pages > 0x7fffffff || c->table_pages > 0xffffff)
+  if (T > 0x3fffffff || c->heads > kMaxBlocks || T * c->heads > kMaxBlocks * 64 ||
+      c->sequences > 0x3fffff || c->pages > 0x7fffffff || c->table_pages > 0xffffff)
     return FVSR_EUNSUPPORTED;
   if (T == 0 || c->sequences == 0) return FVSR_OK;
   if ((c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) || !c->lengths ||

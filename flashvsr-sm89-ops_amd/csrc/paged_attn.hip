@@ -1304,7 +1304,7 @@ void launch(const Args& a, const Plan& p, hipStream_t st) {
 extern "C" int64_t fvsr_paged_attn_workspace_floats(const fvsr_kv_cache* cache, int64_t T,
                                                     int64_t q_heads, int has_keep) {
   if (kv_cache_ok(cache, T) != FVSR_OK || T == 0 || cache->sequences == 0 || q_heads <= 0 ||
-      q_heads % cache->heads)
+      q_heads > kMaxBlocks || q_heads % cache->heads)
     return 0;
   return plan_attn(cache, T, q_heads, has_keep != 0).floats(T, q_heads, cache->head_dim);
 }
@@ -1321,6 +1321,7 @@ extern "C" int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_
   if (q_heads <= 0 || q_heads % cache->heads || !(sm_scale > 0.0f) || sm_scale > 3e38f)
     return FVSR_EINVAL;
   if (keep && (keep_q < 0 || keep_k < 0)) return FVSR_EINVAL;
+  if (q_heads > kMaxBlocks) return FVSR_EUNSUPPORTED;
   if (T == 0 || cache->sequences == 0) return FVSR_OK;
   if (!q || !out) return FVSR_EINVAL;
   if ((((uintptr_t)q) | (uint64_t)(q_tok_stride * 2) | (uint64_t)(q_head_stride * 2)) & 15)

@@ -1,0 +1,42 @@
+"""The paged cache's C entries at sizes beyond any memory; nothing here launches a kernel."""
+import ctypes
+
+import pytest
+
+FAKE = 1 << 20
+
+
+def cache(heads=1, sequences=1, columns=3):
+    from flashvsr_sm89_ops.paged_kv import _Cache
+    return ctypes.byref(_Cache(FAKE, FAKE, FAKE, FAKE, 4, heads, 128, FAKE, columns, columns, FAKE,
+                               None, sequences))
+
+
+def append(c, T, q_heads=0):
+    from flashvsr_sm89_ops import _lib
+    q = FAKE if q_heads else None
+    return _lib.lib().fvsr_kv_append(c, FAKE, 128, 128, FAKE, 128, 128, q, 128, 128, q_heads, q, 0,
+                                     T, None, 0, None, 0, 0, 1e-6, None, 0, None, None, 0, None)
+
+
+def attend(c, T, q_heads):
+    from flashvsr_sm89_ops import _lib
+    return _lib.lib().fvsr_paged_attn(c, FAKE, 128, 128, q_heads, FAKE, 128, 128, 0, T, 1, None, 0,
+                                      0, 1.0, 1, None, 0, None)
+
+
+def floats(c, T, q_heads):
+    from flashvsr_sm89_ops import _lib
+    return _lib.lib().fvsr_paged_attn_workspace_floats(c, T, q_heads, 0)
+
+
+@pytest.mark.parametrize("T", [1, 1 << 24, (1 << 30) - 1])
+@pytest.mark.parametrize("heads", [1 << 40, 1 << 62, (1 << 63) - 1])
+def test_heads_past_any_launch_are_refused(heads, T):
+    """Their products with T pass 64 bits: a status, not a plan from what is left of them (which
+    divided by zero)."""
+    from flashvsr_sm89_ops import _lib
+    for c, q_heads in ((cache(), heads), (cache(heads=heads), heads)):
+        assert append(c, T, q_heads) == _lib.FVSR_EUNSUPPORTED
+        assert attend(c, T, q_heads) == _lib.FVSR_EUNSUPPORTED
+        assert floats(c, T, q_heads) == 0
