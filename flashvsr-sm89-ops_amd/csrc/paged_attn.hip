@@ -1263,8 +1263,12 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   const int64_t rows_of = std::min<int64_t>(128, (T * pack + B - 1) / B);
   const int64_t slots = rows_of <= 64 ? 2 * cus : cus, pages = c->table_pages;
   const int64_t rest = rows_of <= 64 ? p.units : p.units % cus;
+  // (join_tile takes up to 128 workgroups for each unit that is cut.)
+  const int64_t most = rest * 128 > kMaxBlocks
+                           ? 1
+                           : std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, pages / 2));
   double best = 0;
-  for (int64_t n = 1; n <= std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, pages / 2)); ++n) {
+  for (int64_t n = 1; n <= most; ++n) {
     const double us = (double)((rest * n + slots - 1) / slots) * (pages / (double)n + 3) * 1.9 +
                       (n > 1 ? 5 + rest * n * rows_of * (0.03 / 128) : 0);
     if (n > 1 && us >= best) continue;

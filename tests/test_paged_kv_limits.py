@@ -40,3 +40,11 @@ def test_heads_past_any_launch_are_refused(heads, T):
         assert append(c, T, q_heads) == _lib.FVSR_EUNSUPPORTED
         assert attend(c, T, q_heads) == _lib.FVSR_EUNSUPPORTED
         assert floats(c, T, q_heads) == 0
+
+
+def test_units_past_a_joining_launch_are_not_cut():
+    """Pieces of a unit are added by a workgroup for each of its rows, up to 128: what a launch
+    does not hold goes uncut, without a workspace, and fewer units are still cut."""
+    for B in (200000, 1 << 21):
+        assert floats(cache(sequences=B, columns=100000), B * 40, 1) == 0
+    assert floats(cache(sequences=20, columns=100000), 20 * 40, 1) > 0
