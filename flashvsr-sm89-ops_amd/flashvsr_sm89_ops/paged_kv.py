@@ -284,8 +284,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor,
     if not fresh:
         _lib.require_dtype(out, q.dtype, "out")
         _check(out.shape == q.shape and out.stride(2) == 1 and out.stride(0) % 4 == 0 and
-               out.stride(1) % 4 == 0 and out.data_ptr() % 8 == 0,
-               f"{name}: out must be {tuple(q.shape)} with 8-byte aligned rows")
+               out.stride(1) % 4 == 0 and out.data_ptr() % 8 == 0 and
+               all(n == 1 or s > 0 for n, s in zip(out.shape, out.stride())),
+               f"{name}: out must be {tuple(q.shape)} with 8-byte aligned rows of their own")
     _one_device(name, q, *pages, page_table, lengths, cu_tokens, keep, out)
     with torch.cuda.device(q.device):
         q = _aligned(q)
