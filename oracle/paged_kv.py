@@ -135,3 +135,50 @@ def attention(q, cache, table, lengths, cu=None, causal=True, keep=None, sm_scal
                 size[lo + i, c] = p @ v[sees].abs()
                 logit[lo + i, c] = (k[sees].abs() @ q[lo + i, c].abs()).max() * scale
     return out, size, logit
+
+
+def counting_pool(N, H, D, table, seed=0):
+    """A pool in which attention counts tokens: every key is 0, so that what a row sees weighs the
+    same, and every value of a sequence's page j is 1 in dim (j + 5 h) % D of head h and 0 in
+    the others, as a power of two and a scale that differ from page to page.  An output is then a
+    dim's share of the tokens seen, in which one page, or a token, more or less shows.  Codes
+    and scales as bytes: (k, v, k_scale, v_scale)."""
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.zeros(s, dtype=torch.uint8) for s in ((N, H, PAGE, D), (N, H, D, PAGE)))
+    ke, ve = torch.randint(120, 130, (2, N, H), generator=g, dtype=torch.uint8)
+    ve = 127 + (ve.int() - 125).clamp(-4, 4)
+    for row in table.tolist():
+        for j, page in enumerate(row):
+            if 0 <= page < N:
+                for h in range(H):
+                    v[page, h, (j + 5 * h) % D] = (7 - (int(ve[page, h]) - 127)) << 3
+    return k, v, ke, ve.to(torch.uint8)
+
+
+def counted(T, Hq, H, D, columns, lengths, cu=None, causal=True, keep=None):
+    """[T, Hq, D]: what attention over a counting_pool gives."""
+    want = torch.zeros(T, Hq, D).double()
+    j = torch.arange(columns)
+    for b, (lo, n) in enumerate(rows_of(T, len(lengths), cu)):
+        i = torch.arange(n)
+        last = int(lengths[b]) - n + i + 1 if causal else torch.full((n,), int(lengths[b]))
+        sees = (last[:, None] - PAGE * j).clamp(0, PAGE).double()  # [n, columns]
+        for c in range(Hq):
+            s = sees
+            if keep is not None:
+                m = torch.zeros(-(-n // PAGE) + 1, columns).double()
+                a = keep[b, c][:m.shape[0], :columns].double()
+                m[:a.shape[0], :a.shape[1]] = a
+                s = sees * m[i // PAGE]
+            total = s.sum(1, keepdim=True)
+            dims = torch.zeros(columns, D).double()
+            dims[j, (j + 5 * (c // (Hq // H))) % D] = 1
+            want[lo:lo + n, c] = torch.where(total > 0, s @ dims / total.clamp(min=1), 0.0)
+    return want
+
+
+def counts_agree(got, want):
+    """Whether outputs in a type of 16 bits are `want` from a counting_pool: one rounding to the
+    type, 2^-12 for the matrix cores' sums and 2^-17 for those of up to 64 pieces."""
+    step = torch.finfo(got.dtype).eps / 2
+    return bool(((got.double() - want).abs() <= (step + 2.0 ** -12 + 2.0 ** -17) * want).all())
