@@ -137,25 +137,35 @@ def attention(q, cache, table, lengths, cu=None, causal=True, keep=None, sm_scal
     return out, size, logit
 
 
-def counting_pool(N, H, D, table, seed=0):
+def lift(j, h, most):
+    """Log2 of the weight of page j's tokens for head h in a lifted counting_pool: a whole number
+    of e4m3, at most `most` either way."""
+    steps = [x for x in (0, 1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20) if x <= most]
+    x = steps[(5 * j + 3 * h) % len(steps)]
+    return x if (j + h) % 3 else -x
+
+
+def counting_pool(N, H, D, table, seed=0, most=0):
     """A pool in which attention counts tokens: every key is 0, so that what a row sees weighs the
-    same, and every value of a sequence's page j is 1 in dim (j + 5 h) % D of head h and 0 in
+    same (most > 0: lift() in dim 0, for queries of 1 there and sm_scale = ln 2), and every value of a sequence's page j is 1 in dim (j + 5 h) % D of head h and 0 in
     the others, as a power of two and a scale that differ from page to page.  An output is then a
     dim's share of the tokens seen, in which one page, or a token, more or less shows.  Codes
     and scales as bytes: (k, v, k_scale, v_scale)."""
     g = torch.Generator().manual_seed(seed)
     k, v = (torch.zeros(s, dtype=torch.uint8) for s in ((N, H, PAGE, D), (N, H, D, PAGE)))
-    ke, ve = torch.randint(120, 130, (2, N, H), generator=g, dtype=torch.uint8)
-    ve = 127 + (ve.int() - 125).clamp(-4, 4)
+    # (The largest lift at the least scale, 20 * 2^4, is below 448.)
+    ke, ve = torch.randint(123, 130, (2, N, H), generator=g, dtype=torch.uint8)
     for row in table.tolist():
         for j, page in enumerate(row):
             if 0 <= page < N:
                 for h in range(H):
                     v[page, h, (j + 5 * h) % D] = (7 - (int(ve[page, h]) - 127)) << 3
-    return k, v, ke, ve.to(torch.uint8)
+                    x = torch.tensor(lift(j, h, most) * 2.0 ** (127 - int(ke[page, h])))
+                    k[page, h, :, 0] = x.to(torch.float8_e4m3fn).view(torch.uint8)
+    return k, v, ke, ve
 
 
-def counted(T, Hq, H, D, columns, lengths, cu=None, causal=True, keep=None):
+def counted(T, Hq, H, D, columns, lengths, cu=None, causal=True, keep=None, most=0):
     """[T, Hq, D]: what attention over a counting_pool gives."""
     want = torch.zeros(T, Hq, D).double()
     j = torch.arange(columns)
@@ -170,15 +180,19 @@ def counted(T, Hq, H, D, columns, lengths, cu=None, causal=True, keep=None):
                 a = keep[b, c][:m.shape[0], :columns].double()
                 m[:a.shape[0], :a.shape[1]] = a
                 s = sees * m[i // PAGE]
+            h = c // (Hq // H)
+            s = s * torch.tensor([2.0 ** lift(x, h, most) for x in range(columns)]).double()
             total = s.sum(1, keepdim=True)
             dims = torch.zeros(columns, D).double()
-            dims[j, (j + 5 * (c // (Hq // H))) % D] = 1
-            want[lo:lo + n, c] = torch.where(total > 0, s @ dims / total.clamp(min=1), 0.0)
+            dims[j, (j + 5 * h) % D] = 1
+            want[lo:lo + n, c] = torch.where(total > 0, s @ dims / total, 0.0)
     return want
 
 
 def counts_agree(got, want):
     """Whether outputs in a type of 16 bits are `want` from a counting_pool: one rounding to the
-    type, 2^-12 for the matrix cores' sums and 2^-17 for those of up to 64 pieces."""
-    step = torch.finfo(got.dtype).eps / 2
-    return bool(((got.double() - want).abs() <= (step + 2.0 ** -12 + 2.0 ** -17) * want).all())
+    type (or half of its least step), 2^-12 for the matrix cores' sums and 2^-17 for those of up
+    to 64 pieces and the fp32 steps of a weight."""
+    t = torch.finfo(got.dtype)
+    tol = (t.eps / 2 + 2.0 ** -12 + 2.0 ** -17) * want + t.smallest_normal * t.eps / 2
+    return bool(((got.double() - want).abs() <= torch.where(want > 0, tol, 0.0)).all())

@@ -1,6 +1,8 @@
 """paged_attention counting tokens (oracle.counting_pool): every page, piece and token of every kernel
-form counts once, over tables of up to 1100 pages and up to 150 packed sequences; and append_kv
-of as many."""
+form counts once, with its weight, over tables of up to 1100 pages and up to 150 packed sequences;
+and append_kv of as many."""
+import math
+
 import pytest
 import torch
 
@@ -11,18 +13,21 @@ pytestmark = pytest.mark.gpu
 TYPES = [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float16), (128, torch.float16)]
 
 
-def check_counts(D, dtype, Hq, H, lens, new, packed, causal=True, keep=None, width=None, tail=0):
+def check_counts(D, dtype, Hq, H, lens, new, packed, causal=True, keep=None, width=None, tail=0,
+                 most=0):
     from flashvsr_sm89_ops import KVPages, paged_attention
     table, N = tables(lens, seed=5, width=width)
-    k, v, ks, vs = (t.to(DEV) for t in O.counting_pool(N, H, D, table))
+    k, v, ks, vs = (t.to(DEV) for t in O.counting_pool(N, H, D, table, most=most))
     e4, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
     pages = KVPages(k.view(e4), v.view(e4), ks.view(e8), vs.view(e8))
     T, cu = sum(new) + tail, starts(new) if packed else None
-    q = (2 * torch.randn(T, Hq, D, generator=gen(7))).to(dtype).to(DEV)
-    out = paged_attention(q, pages, table.to(DEV), i32(lens).to(DEV),
+    q = 2 * torch.randn(T, Hq, D, generator=gen(7))
+    q[..., 0] = 1.0
+    out = paged_attention(q.to(dtype).to(DEV), pages, table.to(DEV), i32(lens).to(DEV),
                           None if cu is None else cu.to(DEV), causal=causal,
-                          keep=None if keep is None else keep.to(DEV)).cpu()
-    want = O.counted(T, Hq, H, D, table.shape[1], lens, cu, causal, keep)
+                          keep=None if keep is None else keep.to(DEV),
+                          sm_scale=math.log(2) if most else None).cpu()
+    want = O.counted(T, Hq, H, D, table.shape[1], lens, cu, causal, keep, most)
     assert O.counts_agree(out, want)
 
 
@@ -76,6 +81,18 @@ def test_kept_pages(D, dtype, n, share):
     keep[0, 1, 0] = False
     for causal in (True, False):
         check_counts(D, dtype, 4, 2, lens, [n, n], False, causal, keep)
+
+
+@pytest.mark.parametrize("D,dtype", TYPES)
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("Hq,H,n", [(2, 2, 1), (4, 1, 5), (2, 2, 40), (4, 1, 150)])
+def test_weights_of_pages(D, dtype, packed, Hq, H, n):
+    """Pages whose tokens weigh 2^x, x from page to page and head to head: waves, pieces and
+    list after list are added at their references.  (fp16: shares within its range.)"""
+    most = 20 if dtype == torch.bfloat16 else 3
+    check_counts(D, dtype, Hq, H, [128 * 59 + 31, 700], [n, n], packed, most=most)
+    check_counts(D, dtype, Hq, H, [128 * 59 + 31, 700], [n, n], packed, False, width=700, most=most)
+    check_counts(D, dtype, Hq, H, [128 * 1099 + 31], [n], packed, most=most)
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -1,13 +1,15 @@
 """The check by counted tokens: it takes the definition's own outputs and sees every page, piece and
 token left out or taken twice, at the lengths at which the kernels are checked."""
+import math
+
 import pytest
 import torch
 
 from oracle import paged_kv as O
 
 
-def cache_of(N, H, D, table):
-    k, v, ks, vs = O.counting_pool(N, H, D, table)
+def cache_of(N, H, D, table, most=0):
+    k, v, ks, vs = O.counting_pool(N, H, D, table, most=most)
     e4, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
     return O.from_pages(k.view(e4), v.view(e4), ks.view(e8), vs.view(e8))
 
@@ -25,6 +27,24 @@ def test_definition_is_taken(D, H, Hq, dtype, causal):
         want = O.counted(T, Hq, H, D, 3, lens, cu, causal, k)
         assert float((out - want).abs().max()) < 1e-12
         assert O.counts_agree(out.to(dtype), want)
+    q[..., 0] = 1.0
+    for most in (3, 20):
+        cache = cache_of(12, H, D, table, most)
+        out = O.attention(q, cache, table, lens, cu, causal, keep, math.log(2))[0]
+        want = O.counted(T, Hq, H, D, 3, lens, cu, causal, keep, most)
+        assert float((out - want).abs().max()) < 1e-12 and O.counts_agree(out.to(dtype), want)
+
+
+def test_pool_holds_its_numbers():
+    """Every lift and value is a code times its scale, whatever the scale."""
+    table = torch.arange(600).int().view(1, 600)
+    c = cache_of(600, 3, 64, table, 20)
+    for h in range(3):
+        k, v = (c[a][:, h] * torch.exp2(c[e][:, h].double())[:, None, None]
+                for a, e in (("k", "ke"), ("v", "ve")))
+        assert torch.equal(k[..., 0], torch.tensor([[float(O.lift(j, h, 20))] * 128
+                                                    for j in range(600)]).double())
+        assert int((k[..., 1:] != 0).sum()) == 0 and set(v.unique().tolist()) == {0.0, 1.0}
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
