@@ -22,11 +22,11 @@
 // tokens, each workgroup sums its own rows.  Up to 8 tokens of each sequence go by
 // waves instead, without LDS or barriers.
 //
-// Measured, q with k and v: one token x 12 heads 5.3 us (latency: a chain of four loads),
-// 192 of 32/8 heads 5.9; 24 ragged prompts of 6119 tokens in all x 16/4 heads of 64, fp16
-// 10.4 us (3.5 TB/s); 16896 tokens x 12 heads with row norms 73 us (3.7 TB/s; 5.1 is a copy's
-// rate, and k's second read is not counted).  Between them a page's chain of loads bounds
-// it: lengths, page id and positions, rows, rotations, codes.
+// Measured, q with k and v: one token x 12 heads 5.5 us (latency: a chain of four loads),
+// 192 of 32/8 heads 6.0; 24 ragged prompts of 6119 tokens in all x 16/4 heads of 64, fp16
+// 10.5 us (3.5 TB/s); 16896 tokens x 12 heads with row norms 73 us (3.7 TB/s; 5.1 is a copy's
+// rate, and k's second read is not counted), in fp32 128 (3.7).  Between them a page's chain of
+// loads bounds it: lengths, page id and positions, rows, rotations, codes.
 #include <algorithm>
 #include <type_traits>
 
@@ -112,9 +112,9 @@ FVSR_DEV void store8(void* p, int dt, int64_t i, const float (&x)[8]) {
 // own type in the end, where fp32's steps do not show, but k to a code of 4 bits: fp32's
 // steps put 1 or 2 in 10^6 on the other side of a border between codes, 1 / 16 off.  So
 // k's sums are taken in 64 bits (beyond eight squares at least, which also keeps those that
-// fp32 does not hold), and what lies near a border is computed again in 64 bits.  (Errors of k
-// against 64 bits: 2e-5 of its norm without, 2e-7 so.  16896 tokens x 12 heads 69 us
-// without, 73 so, 84 with all of k in 64 bits.)
+// fp32 does not hold), and what lies near a border is computed again in 64 bits.  (16896
+// tokens x 12 heads: errors of k against 64 bits 2e-5 of its norm without that, 1e-7 so; 70.7 us
+// without, 73.3 so.  6119 tokens in ragged prompts 10.0 us, 10.6.)
 template <class T>
 FVSR_DEV T sum_sq(const float (&x)[8]) {
   T s = 0;
@@ -423,8 +423,8 @@ FVSR_DEV void append_k(const Args& a, const Job& j, double (&stat)[kPage],
   uint32_t near = 0;  // bit i: a value of token i is near a border
   rows_of(j, [&](auto full) {
     const auto live = [&](int i) { return full || (slot0 + i >= j.lo && slot0 + i < j.hi); };
-    // All positions and rows go out together, then all rotations: a load
-    // behind a load eight times over took 22 of a 57 us call (16896 tokens x 12 heads).
+    // All positions and rows go out together, then the rotations: not one load behind
+    // another for each of the four tokens.
     Raw8<DT> raw[R];
     constexpr int Q = D == 64 ? 1 : 2;  // rotations in flight (registers)
     Raw8<FVSR_DT_F32> turn[Q];
@@ -682,13 +682,12 @@ __global__ __launch_bounds__(kWg<D>) void kv_append_kernel(Args a) {
 }
 
 // Row norms of many tokens take two launches: v beside the k statistics, then the q
-// rows and k, read again.  The q rows go first: they keep the memory busy while a
-// page's loads wait for each other (16896 tokens x 12 heads: 69 us, behind the pages 71, with
-// the statistics 73).
+// rows and k, read again.  (The q rows first or last: 16896 tokens x 12 heads 73.2 us, 72.2.)
 
-// Pieces of a row that its wave holds: rows of 2048 elements.  Eight cost the pages of the
-// launch more (registers: 75 us; 8 prompts of 2000 x 32/8 heads 21.4 against 20.0)
-// than they save on rows of 4096 (4 of those prompts 16.8 against 17.3).
+// Pieces of a row that its wave holds: rows of 2048 elements.  Eight take registers from the
+// pages of the launch (16896 tokens x 12 heads 73.4 us, 80.2 with eight; one prompt of 2000 x 32
+// heads 25.6, 27.7) and save a second read of longer q rows (8 prompts of 2000 x 32/8 heads 107
+// us, 102 with eight).
 constexpr int kHeld = 4;
 template <int DT, int D>
 __global__ __launch_bounds__(kWg<D>) void kv_rows_kernel(Args a) {
@@ -815,7 +814,7 @@ FVSR_DEV void turn2(const Args& a, const void* src, int64_t ts, int64_t hs, int 
 // and positions load at once, then the page id and the rotation, then the page's
 // scales; a norm over the row is summed by every wave for itself.  A page whose scale
 // grows (rare: a power of two) has its held codes rounded again by the wave.  64 x 5 tokens,
-// 32 / 8 heads: 17.7 us by pages as a prompt's, 11.1 so.
+// 32 / 8 heads: 16.6 us by pages as a prompt's, 9.6 so (row norms: 21.7, 18.8); 64 x 8 17.7, 12.9.
 template <int DT, int D, int N>
 __global__ __launch_bounds__(kThreads) void kv_token_kernel(Args a) {
   const int lane = threadIdx.x & 63, d0 = lane * 2 % D;

@@ -20,10 +20,16 @@
 // maximum is; their operand's scale is 2^(E - 8 - M).  M, the row's reference,
 // may therefore be any power of two near the maximum: it moves only when E exceeds
 // it by 64, which rescales O and the sum exactly and happens at a row's first keys
-// and hardly ever again.  Remainders keep w's error below 2^-8 (bf16) or
-// 2^-12 (fp16) of itself, or 2^-22 of the largest; sums are fp32, of w (bf16: rounded to
-// fp16, which the terms come by too).  While M stays, O and the sum may grow by 2^64:
+// and hardly ever again.  While M stays, O and the sum may grow by 2^64:
 // finite results take values below 2^63 over the number of keys.
+//
+// Precision.  Remainders keep w's error below 2^-8 (bf16) or 2^-12 (fp16) of itself, or
+// 2^-22 of the largest; its sum is fp32, of w (bf16: rounded to fp16, 11 bits, which the
+// terms come by too).  Accumulators are fp32, but the instructions align a sum's products
+// before they add them: it is off by up to 2^-12 of the sum of their magnitudes (measured on
+// codes of any exponents 2.0e-4 at worst and 2.9e-5 in the mean square, on Gaussian q and K
+// 2.9e-5 and 2.8e-6).  A logit is off by as much of sm_scale * sum |q k|, and its weight by
+// that part of itself.
 //
 // Three kernels.  attend_few: up to 16 (query, head) rows of one key/value head
 // per workgroup, bound by the cache's bytes: 16x16x128 products, K and V loaded
@@ -34,11 +40,13 @@
 // workgroups where rows alone leave CUs idle; join_few and join_tile add the pieces.
 //
 // Measured, 32 query and 8 key/value heads of 128: one token for each of 128 ragged
-// sequences of up to 16000 tokens 362 us (5.4 TB/s; 5.1 is a copy's rate), for one
+// sequences of up to 16000 tokens 365 us (5.4 TB/s; 5.1 is a copy's rate), for one
 // sequence of 262000 97 us (5.5); 5 for each of 16 of 6000 47 us (4.2).  8448 rows over
-// 25344 tokens x 12 heads 1.10 to 1.16 ms: 1.13 to 1.19 PFLOP/s, where an 8192^3 bf16 product
-// reaches 1.21; the clock falls to 1.8 - 1.9 GHz, at which the vector units are busy for 71
-// % of the time and the matrix cores for 53.
+// 25344 tokens x 12 heads 1.10 to 1.17 ms: 1.12 to 1.19 PFLOP/s, where an 8192^3 bf16 product
+// reaches 1.21; the clock falls to 1.9 GHz, at which the vector units are busy for 70
+// % of the time and the matrix cores for 53.  The same in fp16 1.60 ms (three terms are one and a
+// half fp16 products, and more vector work), with 24 heads of 64 1.55 ms (the softmax's work for
+// half the products).
 #include <algorithm>
 #include <type_traits>
 
@@ -889,9 +897,9 @@ struct RowTile {
 
 // attend_few for 17 to 32 rows: the same sharing out of pages, half a page at a time (a
 // whole one's operands beside 32 rows' O are more than 256 registers).  The K operand of the
-// half ahead loads as soon as the logits have used the one before it: 61 -> 47 us for 16 x 5
-// tokens x 32 / 8 heads over 6000 (4.2 TB/s), with the splits that follow from it.  Five tokens
-// over 262000: 104 us (5.2 TB/s); by tiles of 128 rows 262.
+// half ahead loads as soon as the logits have used the one before it.  16 x 5 tokens x 32 / 8
+// heads over 6000: 47 us (4.2 TB/s), by tiles of 128 rows 52.  Five tokens over 262000: 101 us (5.3
+// TB/s), by tiles 108.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads, 2) void attend_some(Args a) {
   constexpr int P = D + 4;
@@ -1225,11 +1233,13 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   };
   // Rows of any number per sequence: where they are few on average, waiting for
   // memory is what counts, and 16 rows to a workgroup with its waves on pages of their own
-  // wait less than 128 with one stream of pages, even if some units read the same pages (32
-  // sequences of 7.5 tokens x 32 / 8 heads 168 -> 134 us, 16 of 14 x 16 / 4 44 -> 24; 32 rows
-  // to a workgroup: no better, or 20 against 17).  The same number for each: if one unit
-  // of 16 or 32 holds them (20 rows over 6000 tokens: two units of 16 64 us, one of
-  // 32 47, a tile of 128 52) and a grid holds their heads and sequences.
+  // wait less than 128 with one stream of pages, even if some units read the same pages.
+  // (us in units of 16 / in tiles.  32 sequences of 1 to 16 tokens over up to 9000 x 32 / 8
+  // heads 120 / 159, 16 of 1 to 32 over up to 9000 x 16 / 4 54 / 72, over up to 3000 25 / 42.  It
+  // loses where lengths are short or one prompt holds most rows: 32 of 1 to 32 over up to 2000 x
+  // 32 / 8 58 / 43, 128 single tokens over 3000 and a prompt of 1500 230 / 185.)  The same number
+  // for each: if one unit of 16 or 32 holds them (20 rows over 6000 tokens: one of 32 47 us,
+  // tiles 52) and a grid holds their heads and sequences.
   if (!keep && T * group <= B * (c->cu ? 64 : 32) &&
       (c->cu || (c->heads <= kMaxGridYZ && B <= kMaxGridYZ)))
     p.few = c->cu || T * group <= B * 16 ? 16 : 32;
@@ -1237,12 +1247,15 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
     p.tiles = tiles(group, p.few);
     p.units = p.tiles * c->heads;
     // Sequences may be of any lengths: 16 workgroups per CU even them out (128
-    // ragged sequences of up to 16000 tokens, us at 4 / 8 / 16 / 32: 390, 376, 364, 374).
+    // ragged sequences of up to 16000 tokens, us at 4 / 8 / 16 / 32: 426, 376, 366, 373).
     // Two pages to a wave, or one where that would leave CUs idle (20000 tokens x 12
-    // heads 20.5 against 23.8 us; 4 sequences of 5000 x 2 heads 14.6 against 12.1).
+    // heads 17.9 us, 19.0 with one; 4 sequences of 5000 x 2 heads 14.3, 11.2 with one).
     // 32 rows cost more to write and to add again, so there it is one workgroup per CU (16
-    // x 5 tokens x 32 / 8 heads over 6000, 1 to 8 splits: 60, 47, 55, 49, 54; over ragged ones of
-    // up to 12000: 107, 69, 80, 72, 66; 64 x 5 over 2000: 58, 72, 79, 79, 89).
+    // x 5 tokens x 32 / 8 heads over 6000, us in 1, 2, 3, 4, 5 splits: 59, 47, 55, 49, 55; over ragged
+    // ones of up to 12000: 106, 69, 80, 72, 69; 64 x 5 over ragged ones of up to 2000: 47, 57, 59,
+    // 61, 63).  The table's width stands for the lengths, which only the device knows: over short
+    // ones in a wide table pieces are empty (one token over 500 x 12 heads 7.8 us, 15.2 in a table
+    // of 2048 pages).
     const int64_t pages = c->table_pages;
     const int64_t each = p.few == 32 || p.units * (pages / 8) * 2 < cus ? 4 : 8;
     const int64_t fill = p.few == 32 ? cus : 16 * cus;
@@ -1257,9 +1270,11 @@ Plan plan_attn(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, bool keep) {
   // workgroup as with two, so it is whole units per CU that must come out even) are cut
   // into the number of pieces that is done first, by prices from measured calls: 1.9 us
   // a page; a workgroup's start like 3 pages; for pieces 5 us of joining launch, and 0.03
-  // us of the GPU's time for each piece of 128 rows written and read again.  Few rows
-  // leave the page loop waiting for memory: two workgroups then share a CU at full speed,
-  // and every unit may be cut.
+  // us of the GPU's time for each piece of 128 rows written and read again.  (Of bf16 and 128
+  // dims, with a full table.)  Few rows leave the page loop waiting for memory: two workgroups
+  // then share a CU at full speed, and every unit may be cut.  (us with cut units / without: 8448
+  // rows over 25344 x 12 heads 1170 / 1403, 40 over 20000 30.7 / 320; 5 ragged prompts, whose tiles
+  // are of any lengths, 488 / 476.)
   const int64_t rows_of = std::min<int64_t>(128, (T * pack + B - 1) / B);
   const int64_t slots = rows_of <= 64 ? 2 * cus : cus, pages = c->table_pages;
   const int64_t rest = rows_of <= 64 ? p.units : p.units % cus;

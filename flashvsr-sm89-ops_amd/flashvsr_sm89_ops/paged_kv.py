@@ -12,10 +12,11 @@ sequences of any lengths share one pool:
     out = paged_attention(q, pages, table, lengths)
 
 Both take a step of any mix: ``[T, heads, head_dim]`` rows packed by
-``cu_tokens`` (as a prompt each), or, without it, the same number for every sequence
+``cu_tokens`` (int32 [B + 1], from 0 and never falling), or, without it, the same number for every sequence
 (one each: the next token).  Lengths, table and cu_tokens stay on the device and are
 never read back, so a step can be captured into a graph and replayed as they
-change.  Inference only: no gradients.
+change.  How a call's work is cut up follows from its sizes alone, the table's width among
+them; a table far wider than the lengths costs some time.  Inference only: no gradients.
 """
 from __future__ import annotations
 
@@ -167,7 +168,9 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     lies, complex128 converted by each call): then the pairs (2i, 2i + 1) are rotated by row
     positions[t] (int32 [T]; default: row t); a position outside the table gives NaN.
 
-    Values are rounded once, from fp32 or better.  A page's scale is the least power of
+    Values are rounded once, from fp32 or better; k's codes are those of the 64-bit value
+    but where a rotation leaves little of its terms.  q comes back in its own type (fp32 too,
+    which paged_attention does not take).  A page's scale is the least power of
     two that holds its new values within 448 (a non-finite one is stored as NaN and
     does not count); if the page already holds tokens, the scale never falls, and where it
     grows their codes are rounded again.  The pages that a call appends to must be
@@ -251,8 +254,10 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor,
     Returns out, or a new tensor like q.  A row that sees nothing is zero; rows
     behind cu_tokens[B] are zero in a new tensor and left alone in a given one.  A page
     id outside the pool makes the rows that read it NaN; what a mask hides, or lies
-    behind a length, does not count even if it is NaN.  Logits and sums are fp32;
-    the weights count with q's precision."""
+    behind a length, does not count even if it is NaN.  Logits and sums are fp32
+    accumulators of the matrix cores, which keep a sum to 2^-12 of its terms' magnitudes (2^-15
+    on Gaussian values): a logit is off by as much of sm_scale * sum |q k|.  The weights
+    count with q's precision (2^-8 or 2^-12) or 2^-22 of the largest."""
     if out is None:
         r = (_lib._paged_host or _lib.paged_host()).paged_attention(
             q, pages, page_table, lengths, cu_tokens, causal, keep, sm_scale)

@@ -451,7 +451,9 @@ int fvsr_attn_dense(const void* q, const void* k, const void* v, void* o, int64_
  * whatever they hold, no kernel reaches outside the tensors: positions below 0
  * or past the table are not stored, a page id outside 0 .. pages - 1 is not written
  * and turns the rows that read it NaN.  Rows behind cu[sequences] belong to
- * nobody.  head_dim 64 or 128.  k and v are 16-byte aligned.
+ * nobody.  head_dim 64 or 128.  k and v are 16-byte aligned.  FVSR_EUNSUPPORTED also
+ * where a launch would need more than 2^32 threads, for more than 2^30 rows, 2^22
+ * sequences or 2^24 table columns or heads.
  */
 enum { FVSR_PAGE = 128 };
 typedef struct {
@@ -508,8 +510,10 @@ int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stri
  *           nonzero; blocks outside keep_q x keep_k are not kept
  *   out     rows that see nothing are zeros; rows behind cu[sequences] are zeros
  *           if fill_tail, else left as they are
- * Logits and sums in fp32.  What a mask hides does not count, whatever it holds
- * (NaN included).  sm_scale positive.
+ * Logits and sums in fp32 accumulators (the matrix cores keep a sum to 2^-12 of
+ * its terms' magnitudes), weights to 2^-8 (bf16) or 2^-12 (fp16) of themselves or
+ * 2^-22 of the largest.  What a mask hides does not count, whatever it holds (NaN
+ * included).  sm_scale positive.
  *   workspace  fvsr_paged_attn_workspace_floats(...) floats, 16-byte aligned
  *              (0: NULL is fine), used until the call's kernels have run
  */
