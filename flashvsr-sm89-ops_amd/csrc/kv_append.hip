@@ -981,7 +981,7 @@ bool rows_aligned(const void* p, int64_t ts, int64_t hs, int64_t size) {
 }  // namespace
 
 extern "C" int64_t fvsr_kv_append_workspace_floats(int64_t T, int k_norm) {
-  return k_norm == FVSR_NORM_ROW && T > kOwnStat ? 2 * T : 0;
+  return k_norm == FVSR_NORM_ROW && T > kOwnStat && T <= kMaxRows ? 2 * T : 0;
 }
 
 extern "C" int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stride,

@@ -6,6 +6,7 @@
 
 constexpr int kPage = FVSR_PAGE;  // tokens of a page
 constexpr int64_t kMaxBlocks = 0xffffff;  // workgroups of a launch: 2^32 threads, 256 each
+constexpr int64_t kMaxRows = 0x3fffffff;
 
 // Rows of a call that belong to sequence b: T rows packed at cu[0..B], or
 // the same number each.  Clamped, so that no offsets reach outside the T rows.
@@ -80,7 +81,7 @@ static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T) {
       c->table_stride < c->table_pages)
     return FVSR_EINVAL;
   if (c->head_dim != 64 && c->head_dim != 128) return FVSR_EUNSUPPORTED;
-  if (T > 0x3fffffff || c->heads > kMaxBlocks || T * c->heads > kMaxBlocks * 64 ||
+  if (T > kMaxRows || c->heads > kMaxBlocks || T * c->heads > kMaxBlocks * 64 ||
       c->sequences > 0x3fffff || c->pages > 0x7fffffff || c->table_pages > 0xffffff)
     return FVSR_EUNSUPPORTED;
   if (T == 0 || c->sequences == 0) return FVSR_OK;

@@ -487,6 +487,7 @@ enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
  * that a call appends to must be distinct.
  *   workspace  fvsr_kv_append_workspace_floats(T, k_norm) floats, 8-byte
  *              aligned (0: NULL is fine), used until the call's kernels have run
+ *              (0 too for what the call refuses)
  */
 int64_t fvsr_kv_append_workspace_floats(int64_t T, int k_norm);
 int fvsr_kv_append(const fvsr_kv_cache* cache, const void* k, int64_t k_tok_stride,

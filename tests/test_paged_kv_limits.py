@@ -48,3 +48,11 @@ def test_units_past_a_joining_launch_are_not_cut():
     for B in (200000, 1 << 21):
         assert floats(cache(sequences=B, columns=100000), B * 40, 1) == 0
     assert floats(cache(sequences=20, columns=100000), 20 * 40, 1) > 0
+
+
+def test_workspace_of_rows_past_any_call():
+    from flashvsr_sm89_ops import _lib
+    f = _lib.lib().fvsr_kv_append_workspace_floats
+    assert f((1 << 30) - 1, _lib.NORM_ROW) == (1 << 31) - 2
+    for T in (1 << 30, 1 << 62, (1 << 63) - 1, -1):
+        assert f(T, _lib.NORM_ROW) == 0
