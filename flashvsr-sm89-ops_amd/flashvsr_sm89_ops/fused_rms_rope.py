@@ -42,6 +42,8 @@ def _freqs_table(freqs: torch.Tensor) -> torch.Tensor:
     if entry is not None and entry[0]() is freqs and entry[1] == freqs._version:
         return entry[2]
     t = torch.view_as_real(f.to(torch.complex64)).contiguous()
+    if f.is_cuda and torch.cuda.is_current_stream_capturing():
+        return t                              # written by the graph's replays only
     for k in [k for k, e in _CS_CACHE.items() if e[0]() is None]:
         del _CS_CACHE[k]                      # sources already freed
     while len(_CS_CACHE) >= _CS_CACHE_MAX:
