@@ -480,8 +480,8 @@ enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
  *   q_out  [T, q_heads, head_dim] in dtype, every row of it written (rows of no
  *          sequence too, and all of them where there are no sequences)
  * fp32 from the loads to the one rounding (64 bits where a code hangs on it).  A
- * page's scale is the least 2^e, e >= -126, with every finite new magnitude at
- * most 448 * 2^e; where the page holds tokens before the new ones, not below its
+ * page's scale is the least 2^e, e >= -126, with every finite new magnitude (as
+ * fp32 has it) at most 448 * 2^e; where the page holds tokens before the new ones, not below its
  * old one, and their codes are rounded again if it grows.  Infinities and NaN are
  * stored as NaN.  Slots behind the last new token keep their bytes.  The pages
  * that a call appends to must be distinct.
