@@ -13,9 +13,9 @@ sequences of any lengths share one pool:
 
 Both take a step of any mix: ``[T, heads, head_dim]`` rows packed by
 ``cu_tokens`` (int32 [B + 1], from 0 and never falling), or, without it, the same number
-for every sequence (one each: the next token).  Lengths, table and cu_tokens stay on the device and are
-never read back, so a step can be captured into a graph and replayed as they
-change.  How a call's work is cut up follows from its sizes alone, the table's width among
+for every sequence (one each: the next token).  Lengths, table and cu_tokens stay on the
+device and are never read back, so a step can be captured into a graph and replayed as
+they change.  How a call's work is cut up follows from its sizes alone, the table's width among
 them; a table far wider than the lengths costs some time.  Inference only: no gradients.
 """
 from __future__ import annotations
@@ -169,8 +169,8 @@ def append_kv(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torc
     positions[t] (int32 [T]; default: row t); a position outside the table gives NaN.
 
     Values are rounded once, from fp32 or better; k's codes are those of the 64-bit value
-    but where a rotation leaves little of its terms or a code is subnormal.  q comes back in its own type (fp32 too,
-    which paged_attention does not take).  A page's scale is the least power of
+    but where a rotation leaves little of its terms or a code is subnormal.  q comes
+    back in its own type (fp32 too, which paged_attention does not take).  A page's scale is the least power of
     two that holds its new values within 448 (a non-finite one is stored as NaN and
     does not count); if the page already holds tokens, the scale never falls, and where it
     grows their codes are rounded again.  The pages that a call appends to must be

@@ -481,10 +481,10 @@ enum { FVSR_NORM_NONE = 0, FVSR_NORM_HEAD = 1, FVSR_NORM_ROW = 2 };
  *          sequence too, and all of them where there are no sequences)
  * fp32 from the loads to the one rounding (64 bits where a code hangs on it).  A
  * page's scale is the least 2^e, e >= -126, with every finite new magnitude (as
- * fp32 has it) at most 448 * 2^e; where the page holds tokens before the new ones, not below its
- * old one, and their codes are rounded again if it grows.  Infinities and NaN are
- * stored as NaN.  Slots behind the last new token keep their bytes.  The pages
- * that a call appends to must be distinct.
+ * fp32 has it) at most 448 * 2^e; where the page holds tokens before the new ones,
+ * not below its old one, and their codes are rounded again if it grows.  Infinities
+ * and NaN are stored as NaN.  Slots behind the last new token keep their bytes.  The
+ * pages that a call appends to must be distinct.
  *   workspace  fvsr_kv_append_workspace_floats(T, k_norm) floats, 8-byte
  *              aligned (0: NULL is fine), used until the call's kernels have run
  *              (0 too for what the call refuses)

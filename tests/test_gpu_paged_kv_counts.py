@@ -1,5 +1,5 @@
-"""paged_attention counting tokens (oracle.counting_pool): every page, piece and token of every kernel
-form counts once, with its weight, over tables of up to 1100 pages and up to 150 packed sequences;
+"""paged_attention counting tokens (oracle.counting_pool): every page, piece and token of every
+kernel form counts once, with its weight, over tables of up to 1100 pages and up to 150 packed sequences;
 and append_kv of as many."""
 import math
 
@@ -32,8 +32,8 @@ def check_counts(D, dtype, Hq, H, lens, new, packed, causal=True, keep=None, wid
 
 
 @pytest.mark.parametrize("D,dtype", TYPES)
-@pytest.mark.parametrize("Hq,H,n", [(3, 3, 1), (8, 2, 1), (2, 1, 8), (2, 2, 17), (8, 2, 5), (20, 1, 1),
-                                    (2, 2, 40), (4, 1, 60), (2, 1, 200)])
+@pytest.mark.parametrize("Hq,H,n", [(3, 3, 1), (8, 2, 1), (2, 1, 8), (2, 2, 17), (8, 2, 5),
+                                    (20, 1, 1), (2, 2, 40), (4, 1, 60), (2, 1, 200)])
 def test_equal_rows(D, dtype, Hq, H, n):
     """Units of 16 and 32 rows and tiles; a table as wide as the lengths and one far wider."""
     for lens in ([128 * 70 + 31, 300, 0, 128 * 9], [128 * 20 + 1]):
