@@ -148,9 +148,10 @@ def lift(j, h, most):
 def counting_pool(N, H, D, table, seed=0, most=0):
     """A pool in which attention counts tokens: every key is 0, so that what a row sees weighs the
     same (most > 0: lift() in dim 0, for queries of 1 there and sm_scale = ln 2), and every
-    value of a sequence's page j is 1 in dim (j + 5 h) % D of head h and 0 in the others, as a power of two and a scale that differ from page to page.  An output is then a
-    dim's share of the tokens seen, in which one page, or a token, more or less shows.  Codes
-    and scales as bytes: (k, v, k_scale, v_scale)."""
+    value of a sequence's page j is 1 in dim (j + 5 h) % D of head h and 0 in the others, as a
+    power of two and a scale that differ from page to page.  An output is then a dim's share
+    of the tokens seen, in which one page, or a token, more or less shows.  Codes and scales
+    as bytes: (k, v, k_scale, v_scale)."""
     g = torch.Generator().manual_seed(seed)
     k, v = (torch.zeros(s, dtype=torch.uint8) for s in ((N, H, PAGE, D), (N, H, D, PAGE)))
     # (The largest lift at the least scale, 20 * 2^4, is below 448.)
