@@ -73,9 +73,9 @@ FVSR_DEV bool find_part(const int32_t* cu, const int32_t* lengths, int B, int T,
   return false;
 }
 
-// What both entry points check of the cache and the call's rows (rows and units
-// are counted in 32 bits).
-static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T) {
+// What the entry points check of the cache and the call's rows (rows and units
+// are counted in 32 bits); codes: whether the call reads or writes them.
+static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T, bool codes = true) {
   if (!c) return FVSR_EINVAL;
   if (c->pages < 0 || c->heads <= 0 || c->sequences < 0 || c->table_pages < 0 || T < 0 ||
       c->table_stride < c->table_pages)
@@ -85,10 +85,10 @@ static inline int kv_cache_ok(const fvsr_kv_cache* c, int64_t T) {
       c->sequences > 0x3fffff || c->pages > 0x7fffffff || c->table_pages > 0xffffff)
     return FVSR_EUNSUPPORTED;
   if (T == 0 || c->sequences == 0) return FVSR_OK;
-  if ((c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) || !c->lengths ||
+  if ((codes && c->pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale)) || !c->lengths ||
       (!c->table && c->sequences * c->table_pages > 0))
     return FVSR_EINVAL;
   if (!c->cu && T % c->sequences) return FVSR_EINVAL;
-  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return FVSR_EUNSUPPORTED;
+  if (codes && (((uintptr_t)c->k | (uintptr_t)c->v) & 15)) return FVSR_EUNSUPPORTED;
   return FVSR_OK;
 }

@@ -8,7 +8,9 @@ the HIP-backed ``block_sparse_attn`` module (see compat_bsa), so import it
 before diffsynth, whose DiT imports block_sparse_attn at module load.
 
 Beside the reference's ops: an 8-bit paged K/V cache and its attention
-(``kv_pages``, ``append_kv``, ``paged_attention``).
+(``kv_pages``, ``append_kv``, ``paged_attention``), attention over pages that each row
+chooses (``page_means``, ``pool_pages``, ``select_pages``, ``selected_attention``), and
+rotary positions with their gradient (``rotary_frequencies``, ``rotary``).
 
 What differs from the reference package at its public surface:
 - the tiling helpers (``plan_tiles``, ``render_tiled``, ``auto_tile_limits``,
@@ -38,6 +40,9 @@ from .integrate import enable  # noqa: E402
 from .lcsa import block_sparse_attention, build_csr, draft_block_mask  # noqa: E402
 from .cross_attn import cross_attention, cross_attention_residual  # noqa: E402
 from .paged_kv import KVPages, append_kv, kv_pages, paged_attention  # noqa: E402
+from .page_select import (PageMeans, page_means, pool_pages, select_pages,  # noqa: E402
+                          selected_attention)
+from .rotary import RotaryFrequencies, rotary, rotary_frequencies  # noqa: E402
 
 __version__ = "0.1.0"
 
@@ -70,6 +75,14 @@ __all__ = [
     "kv_pages",
     "append_kv",
     "paged_attention",
+    "PageMeans",
+    "page_means",
+    "pool_pages",
+    "select_pages",
+    "selected_attention",
+    "RotaryFrequencies",
+    "rotary_frequencies",
+    "rotary",
     "active_backend",
     "ensure_bsa_available",
 ]

@@ -23,6 +23,7 @@ SCALE_TENSOR, SCALE_ROW = 0, 1
 EPI_BIAS, EPI_ROWMAX, EPI_GATE_ADD = 0, 1, 2
 DT_BF16, DT_F16, DT_F32 = 0, 1, 2
 NORM_NONE, NORM_HEAD, NORM_ROW = 0, 1, 2
+PAIRS_HALF, PAIRS_INTERLEAVED = 0, 1
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 
 _ERR = {
@@ -89,6 +90,13 @@ _SIGS = {
     "fvsr_paged_attn_workspace_floats": ([_P, _I64, _I64, _I], _I64),
     "fvsr_paged_attn": ([_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I, _I64, _I, _P, _I64, _I64, _F,
                          _I, _P, _I64, _P], _I),
+    "fvsr_pool_pages": ([_P, _P, _P, _I64, _P], _I),
+    "fvsr_select_pages": ([_P, _P, _P, _P, _I64, _I64, _I64, _I, _I64, _I64, _I64, _I64, _P, _P],
+                          _I),
+    "fvsr_selected_attn_workspace_floats": ([_P, _I64, _I64, _I64], _I64),
+    "fvsr_selected_attn": ([_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I, _I64, _P, _I64, _F, _I,
+                            _P, _I64, _P], _I),
+    "fvsr_rotary": ([_P, _P, _I, _I64, _I64, _I64, _I64, _P, _P, _I64, _F, _I, _I, _P], _I),
 }
 
 _lib = None

@@ -59,22 +59,11 @@ def _check(ok: bool, what: str):
         raise ValueError(what)
 
 
-def _check_cache(name: str, pages: KVPages, table, lengths, cu, T: int):
-    k, v, ks, vs = pages
-    _check(k.dim() == 4 and k.shape[2] == PAGE and k.shape[3] in _HEAD_DIMS and k.shape[1] > 0,
-           f"{name}: pages.k must be [pages, heads, {PAGE}, 64 or 128], got {tuple(k.shape)}")
-    N, H, _, D = k.shape
-    _check(tuple(v.shape) == (N, H, D, PAGE) and tuple(ks.shape) == (N, H) == tuple(vs.shape),
-           f"{name}: pages.v must be {(N, H, D, PAGE)} and the scales {(N, H)}, got "
-           f"{tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
-    for t, n in ((k, "pages.k"), (v, "pages.v")):
-        _lib.require_dtype(t, torch.float8_e4m3fn, n)
-    for t, n in ((ks, "pages.k_scale"), (vs, "pages.v_scale")):
-        _lib.require_dtype(t, torch.float8_e8m0fnu, n)
+def _check_steps(name: str, table, lengths, cu, T: int):
+    """Page table, lengths and cu_tokens of a call with T rows."""
     for t, n in ((table, "page_table"), (lengths, "lengths"), (cu, "cu_tokens")):
         if t is not None:
             _lib.require_dtype(t, torch.int32, n)
-    _check(all(t.is_contiguous() for t in pages), f"{name}: the pages must be contiguous")
     _check(table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1) and
            (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]),
            f"{name}: page_table must be [sequences, pages] with unit-stride rows")
@@ -88,6 +77,22 @@ def _check_cache(name: str, pages: KVPages, table, lengths, cu, T: int):
         _check(T % B == 0 if B else T == 0,
                f"{name}: {T} rows are not the same number for each of {B} sequences (give "
                "cu_tokens)")
+
+
+def _check_cache(name: str, pages: KVPages, table, lengths, cu, T: int):
+    k, v, ks, vs = pages
+    _check(k.dim() == 4 and k.shape[2] == PAGE and k.shape[3] in _HEAD_DIMS and k.shape[1] > 0,
+           f"{name}: pages.k must be [pages, heads, {PAGE}, 64 or 128], got {tuple(k.shape)}")
+    N, H, _, D = k.shape
+    _check(tuple(v.shape) == (N, H, D, PAGE) and tuple(ks.shape) == (N, H) == tuple(vs.shape),
+           f"{name}: pages.v must be {(N, H, D, PAGE)} and the scales {(N, H)}, got "
+           f"{tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
+    for t, n in ((k, "pages.k"), (v, "pages.v")):
+        _lib.require_dtype(t, torch.float8_e4m3fn, n)
+    for t, n in ((ks, "pages.k_scale"), (vs, "pages.v_scale")):
+        _lib.require_dtype(t, torch.float8_e8m0fnu, n)
+    _check(all(t.is_contiguous() for t in pages), f"{name}: the pages must be contiguous")
+    _check_steps(name, table, lengths, cu, T)
     return H, D
 
 

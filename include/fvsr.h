@@ -526,6 +526,74 @@ int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_str
                     int64_t keep_q, int64_t keep_k, float sm_scale, int fill_tail,
                     float* workspace, int64_t workspace_floats, void* stream);
 
+/*
+ * Mean keys of the pages that fill up.  mean [pages, heads, head_dim] int8 (16-byte
+ * aligned) and mean_scale [pages, heads] e8m0 get, for each page of a sequence's table that holds
+ * 128 of its tokens now and held fewer before the call's T rows (T -1: each that holds
+ * 128, whatever cu says), the mean of its 128 keys:
+ *   scale  the least 2^e, e >= -127, with every |mean| at most 127 * 2^e
+ *   mean   the nearest integers to mean / scale, ties to even
+ * A NaN among a head's codes, or as its scale, gives scale NaN (byte 255) and zeros.  Of the cache
+ * v and its scales are not read.  Page ids outside the pool are passed over.
+ */
+int fvsr_pool_pages(const fvsr_kv_cache* cache, void* mean, void* mean_scale, int64_t T,
+                    void* stream);
+
+/*
+ * Columns of the page table that each row's queries are to read: columns [T, heads, top] int32,
+ * rising, -1 behind the last.  A row at position p sees the columns 0 .. p / 128 (of the table).
+ * At most `top` of them: all; otherwise the first `first`, the last `recent` (at least 1) and the
+ * best top - first - recent of the others by
+ *   max over the head's group of  q' . mean * mean_scale
+ * q' the group's queries at position p as integers, rounded (ties to even) from multiples of the
+ * least power of two with all of them at most 127 of it; exact, ties to the lower
+ * column.  A page whose scale is NaN, or whose id is outside the pool, comes behind all
+ * others; a group with an infinity or NaN counts as zeros.  Rows behind cu[sequences]
+ * get -1.  q as in fvsr_paged_attn; of the cache k, v and their scales are not read (NULL is
+ * fine).  FVSR_EUNSUPPORTED for more than 32768 table columns.
+ */
+int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean, const void* mean_scale,
+                      const void* q, int64_t q_tok_stride, int64_t q_head_stride, int64_t q_heads,
+                      int dtype, int64_t T, int64_t top, int64_t first, int64_t recent,
+                      int32_t* columns, void* stream);
+
+/*
+ * fvsr_paged_attn (causal) over the pages in columns [T, heads, top] alone: row t's queries
+ * of key/value head h see the tokens up to their own position in the table columns columns[t][h].
+ * Entries outside 0 .. the row's last column are passed over; a column that stands twice counts
+ * twice.  Everything else as there.
+ *   workspace  fvsr_selected_attn_workspace_floats(...) floats, 16-byte aligned
+ *              (0: NULL is fine), used until the call's kernels have run
+ */
+int64_t fvsr_selected_attn_workspace_floats(const fvsr_kv_cache* cache, int64_t T, int64_t q_heads,
+                                            int64_t top);
+int fvsr_selected_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_stride,
+                       int64_t q_head_stride, int64_t q_heads, void* out, int64_t o_tok_stride,
+                       int64_t o_head_stride, int dtype, int64_t T, const int32_t* columns,
+                       int64_t top, float sm_scale, int fill_tail, float* workspace,
+                       int64_t workspace_floats, void* stream);
+
+/*
+ * Rotary positions of q and k (k: NULL for none): x [batch, tokens, heads, head_dim], heads'
+ * channels contiguous, strides in elements; y the same, contiguous, other memory.  In the first
+ * `turned` channels of each head the pairs (FVSR_PAIRS_HALF: (i, i + turned / 2),
+ * FVSR_PAIRS_INTERLEAVED: (2i, 2i + 1)) become
+ *   gain * (a cos t - b sin t, a sin t + b cos t),  t = 2 pi * position * turns[i]
+ * (back: -t); the other channels are copied.  turns [turned / 2] fp64; positions int32, entry
+ * [b * pos_batch_stride + s] of token s, NULL: s.  Whole turns are taken off in 64 bits,
+ * everything behind is fp32 with one rounding.
+ */
+enum { FVSR_PAIRS_HALF = 0, FVSR_PAIRS_INTERLEAVED = 1 };
+typedef struct {
+  const void* x;
+  void* y;
+  int64_t heads, x_batch, x_tok, x_head;
+} fvsr_rotary_rows;
+int fvsr_rotary(const fvsr_rotary_rows* q, const fvsr_rotary_rows* k, int dtype, int64_t batch,
+                int64_t tokens, int64_t head_dim, int64_t turned, const double* turns,
+                const int32_t* positions, int64_t pos_batch_stride, float gain, int pairs,
+                int back, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

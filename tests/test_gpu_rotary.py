@@ -1,0 +1,251 @@
+"""rotary against its definition in 64 bits, and its gradient against the formula's and
+differences.
+
+Bounds.  The angle's fraction of a turn is rounded to fp32 from 64 bits (|t| <= 1 half turns: 2^-25
+of one, pi * 2^-25 < 2^-23 rad), sine and cosine are off by 2 steps of 2^-24 and their product with the
+gain by one: (2^-23 + 3 * 2^-24) * gain * (|a| + |b|), with three roundings of the products
+and sum 2^-24 of that each: below 8 * 2^-24 = 2^-21 of gain * (|a| + |b|); then half a step of the
+type.  64 bits themselves leave |position * turns| * 2^-53 turns twice: 2^-20 rad at 2^31 for
+turns of 1, added where it counts."""
+import math
+
+import pytest
+import torch
+
+from oracle import page_select as S
+
+DEV = "cuda"
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def freqs_of(R, base=10000.0, gain=1.0):
+    from flashvsr_sm89_ops import RotaryFrequencies
+    return RotaryFrequencies(base ** (-torch.arange(0, R, 2).double() / max(R, 1)) / (2 * math.pi), gain)
+
+
+def on_gpu(f):
+    return type(f)(f.turns.to(DEV), f.gain)
+
+
+def check(got, x, f, pos, pairs, back=False):
+    """got of x [B, S, H, D] (CPU)."""
+    R = 2 * f.turns.numel()
+    want = S.rotated(x, f.turns, f.gain, pos, pairs, back)
+    size = x.double().abs().clone()
+    half = R // 2
+    a, b = (size[..., :half], size[..., half:R]) if pairs == "half" else \
+        (size[..., 0:R:2], size[..., 1:R:2])
+    both = a + b
+    size[..., :R] = torch.cat([both, both], -1) if pairs == "half" else both.repeat_interleave(2, -1)
+    far = 0 if pos is None else float(pos.abs().max())
+    angle = 2 * math.pi * far * 2.0 ** -52 * float(f.turns.max() if R else 0)
+    t = torch.finfo(x.dtype)
+    tol = t.eps / 2 * want.abs() + (2.0 ** -21 + angle) * abs(f.gain) * size + t.smallest_normal * t.eps
+    got = got.cpu()
+    assert got.dtype == x.dtype and got.shape == x.shape
+    ok = ((got.double() - want).abs() <= tol) | (torch.isnan(got) & torch.isnan(want)) | \
+        (got.double() == want)
+    assert bool(ok.all()), float((got.double() - want).abs().nan_to_num().max())
+    assert torch.equal(got[..., R:].nan_to_num(nan=7.0), x[..., R:].nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("D,R", [(128, 128), (128, 64), (64, 64), (64, 16), (80, 32), (96, 96),
+                                 (40, 36), (24, 8), (2, 2), (7, 4), (5, 0), (256, 240)])
+def test_heads(dtype, pairs, D, R):
+    """Whole and part heads, widths that vectors hold and that they do not."""
+    from flashvsr_sm89_ops import rotary
+    B, T, Hq, Hk = 2, 5, 3, 2
+    q, k = (torch.randn(B, T, h, D, generator=gen(h)).to(dtype) for h in (Hq, Hk))
+    f, pos = freqs_of(R, gain=1.25), torch.tensor([0, 1, 77, 100000, -3], dtype=torch.int32)
+    oq, ok = rotary(q.to(DEV), k.to(DEV), on_gpu(f), pos.to(DEV), pairs=pairs)
+    check(oq, q, f, pos, pairs)
+    check(ok, k, f, pos, pairs)
+    alone = rotary(q.to(DEV), None, on_gpu(f), pos.to(DEV), pairs=pairs)
+    assert torch.equal(alone, oq)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,pshape", [((1, 1, 4, 128), (1,)), ((3, 7, 2, 64), (3, 7)),
+                                          ((2, 300, 5, 64), (300,)), ((9, 2, 64), (9,)),
+                                          ((2, 33, 3, 64), None), ((700, 12, 128), None)])
+def test_positions(dtype, shape, pshape):
+    from flashvsr_sm89_ops import rotary
+    x = torch.randn(shape, generator=gen(1)).to(dtype)
+    f = freqs_of(shape[-1])
+    pos = None if pshape is None else torch.randint(-50000, 1000000, pshape, generator=gen(2)).int()
+    out = rotary(x.to(DEV), None, on_gpu(f), None if pos is None else pos.to(DEV))
+    four = x if x.dim() == 4 else x[None]
+    check(out if out.dim() == 4 else out[None], four, f, pos, "half")
+
+
+def test_far_positions():
+    """Up to the ends of int32, where 32-bit angles would be off by whole turns."""
+    from flashvsr_sm89_ops import rotary
+    pos = torch.tensor([2 ** 31 - 1, -2 ** 31, 2 ** 30 + 1, 16777217, 1], dtype=torch.int32)
+    x = torch.randn(1, 5, 2, 64, generator=gen(0))
+    for base in (10000.0, 1.5):
+        f = freqs_of(64, base)
+        check(rotary(x.to(DEV), None, on_gpu(f), pos.to(DEV)), x, f, pos, "half")
+
+
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(pairs, dtype):
+    """Columns of one projection, heads before tokens, odd offsets, rows that share their place."""
+    from flashvsr_sm89_ops import rotary
+    D, f = 64, freqs_of(32)
+    base = torch.randn(2, 9, 8 * D + 6, generator=gen(0)).to(dtype)
+    views = [base[..., :6 * D].unflatten(-1, (6, D)), base[..., 3:3 + 4 * D].unflatten(-1, (4, D)),
+             base[..., 8:8 + 4 * D].unflatten(-1, (4, D)).transpose(1, 2),
+             base[:1, :, :4 * D].unflatten(-1, (4, D)).expand(2, 9, 4, D),
+             base[..., :2 * D:2].unflatten(-1, (1, D)),
+             base[0, 0, :D].expand(2, 9, 3, D)]
+    dev = base.to(DEV)
+    for v in views:
+        d = torch.as_strided(dev, v.shape, v.stride(), v.storage_offset())
+        out = rotary(d, d, on_gpu(f), pairs=pairs)
+        for o in out:
+            check(o, v, f, None, pairs)
+            assert o.is_contiguous()
+
+
+def test_special_values():
+    """Infinities and NaN stay in their pair; subnormals; copied channels keep their bits."""
+    from flashvsr_sm89_ops import rotary
+    for dtype in TYPES:
+        x = torch.randn(1, 4, 2, 64, generator=gen(0)).to(dtype)
+        x[0, 1, 0, 3], x[0, 2, 1, 40], x[0, 3, 0, 63] = math.nan, math.nan, math.nan
+        x[0, 0, 0] = torch.finfo(dtype).smallest_normal / 4
+        f = freqs_of(32)
+        check(rotary(x.to(DEV), None, on_gpu(f)), x, f, None, "half")
+        x[0, 1, 1, 0] = math.inf
+        out = rotary(x.to(DEV), None, on_gpu(f))
+        assert not bool(torch.isfinite(out[0, 1, 1, 0])) and bool(torch.isfinite(out[0, 1, 1, 1:16]).all())
+
+
+def test_nothing():
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    for shape in ((0, 4, 64), (2, 0, 3, 64), (5, 0, 64), (0, 3, 2, 64)):
+        assert rotary(torch.empty(shape, device=DEV), None, f).shape == shape
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("D,R", [(128, 128), (64, 32), (24, 20)])
+def test_gradient(dtype, pairs, D, R):
+    """dq and dk are the rotation back of the gradients, whatever their layout, and q's or k's
+    alone where only one is asked for."""
+    from flashvsr_sm89_ops import rotary
+    B, T, Hq, Hk = 2, 6, 4, 2
+    f = freqs_of(R, gain=1.5)
+    pos = torch.randint(0, 5000, (B, T), generator=gen(4)).int()
+    x = torch.randn(B, T, Hq + Hk, D, generator=gen(0)).to(dtype).to(DEV)
+    q, k = x[:, :, :Hq].detach().requires_grad_(), x[:, :, Hq:].detach().requires_grad_()
+    oq, ok = rotary(q, k, on_gpu(f), pos.to(DEV), pairs=pairs)
+    gq, gk = (torch.randn(B, T, h, D, generator=gen(h)).to(dtype) for h in (Hq, Hk))
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (gq.to(DEV), gk.to(DEV)), retain_graph=True)
+    check(dq, gq, f, pos, pairs, back=True)
+    check(dk, gk, f, pos, pairs, back=True)
+    strided = gq.transpose(1, 2).contiguous().transpose(1, 2)
+    d2, = torch.autograd.grad(oq, q, strided.to(DEV), retain_graph=True)
+    assert torch.equal(d2, dq)
+    d3, = torch.autograd.grad(ok.sum(), k, retain_graph=True)  # one value for every element
+    check(d3, torch.ones_like(gk), f, pos, pairs, back=True)
+    d4, = torch.autograd.grad((oq, ok), k, (gq.to(DEV), gk.to(DEV)))
+    assert torch.equal(d4, dk)
+
+
+def test_gradient_of_one_input_and_shared_heads():
+    """k without a gradient; one k spread over heads (a broadcast) gets the sum."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    q = torch.randn(3, 2, 64, device=DEV, requires_grad=True)
+    k = torch.randn(3, 2, 64, device=DEV)
+    oq, ok = rotary(q, k, f)
+    assert ok.requires_grad and oq.requires_grad  # (outputs of one node)
+    oq.backward(torch.ones_like(oq))
+    assert q.grad is not None and k.grad is None
+    one = torch.randn(3, 1, 64, device=DEV, requires_grad=True)
+    g = torch.randn(3, 4, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(0))
+    out = rotary(one.expand(3, 4, 64), None, f)
+    d, = torch.autograd.grad(out, one, g)
+    want = S.rotated(g.cpu()[None], freqs_of(64).turns, 1.0, None, "half", True)[0].sum(1, keepdim=True)
+    assert bool(((d.cpu().double() - want).abs() <= 2.0 ** -20 * g.cpu().abs().sum(1).max()).all())
+
+
+def test_gradient_by_differences():
+    """fp32, the derivative of a random product along a random direction.  The map is linear, so a
+    difference over a step of 1 has no error of its own: both sides are sums of 768 products
+    that fp32 rounds, 2^-21 of their magnitudes each (the bound above)."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(48, gain=1.3))
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, d, w = (torch.randn(4, 3, 64, device=DEV, generator=g) for _ in range(3))
+    q.requires_grad_()
+    out = rotary(q, None, f, pairs="interleaved")
+    dq, = torch.autograd.grad(out, q, w)
+    slope = ((rotary(q.detach() + d, None, f, pairs="interleaved") - out.detach()).double() * w).sum()
+    size = (w.abs().double() * (q.abs() + d.abs()).double()).sum() + (dq * d).abs().double().sum()
+    assert float((slope - (dq.double() * d).sum()).abs()) <= 3 * 2.0 ** -21 * 2 * 1.3 * float(size)
+
+
+def test_second_gradient():
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    q = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
+    g = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
+    dq, = torch.autograd.grad(rotary(q, None, f), q, g, create_graph=True)
+    w = torch.randn(4, 2, 64, device=DEV)
+    dg, = torch.autograd.grad(dq, g, w)  # the rotation of w
+    check(dg[None], w.cpu()[None], freqs_of(64), None, "half")
+
+
+def test_graph_of_forward_and_backward():
+    """Captured with leaves of its own, replayed with other inputs between eager steps."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(128))
+    x, g = (torch.randn(2, 40, 4, 128, device=DEV).bfloat16() for _ in range(2))
+    pos = torch.arange(40, dtype=torch.int32, device=DEV)
+
+    def step(x):
+        leaf = x.detach().requires_grad_()
+        out = rotary(leaf, None, f, pos)
+        return out.detach(), torch.autograd.grad(out, leaf, g)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        x.normal_()
+        g.normal_()
+        pos += 1000
+        want = step(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_on_another_stream():
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(128))
+    x = torch.randn(500, 8, 128, device=DEV)
+    want = rotary(x, None, f)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = x * 1.0
+        out = rotary(y, None, f)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want)
