@@ -1,6 +1,6 @@
 // Host side of the calls whose kernels are shorter than their Python path:
 // those an FP8 linear makes (quantisation and GEMM) and those of a paged cache's
-// step (append and attention), as a CPython extension: argument checks, output
+// step (append, attention, the choice of pages, rotary positions), as a CPython extension: argument checks, output
 // allocation and the C ABI call in one crossing.  Through Python checks, torch.empty
 // and ctypes a call costs the host 10-13 us (a paged cache's 20-40), more than a
 // kernel on a few hundred rows takes; here 5.3
@@ -22,6 +22,7 @@
 #include <cmath>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -184,6 +185,27 @@ bool rows_ok(const at::Tensor& x, int64_t T, int64_t D) {
   return aligned16(x) && x.stride(0) * b % 16 == 0 && x.stride(1) * b % 16 == 0;
 }
 
+// Page table, lengths and cu_tokens of a call with T rows.
+bool steps_of(PyObject* table, PyObject* lengths, PyObject* cu, int64_t T, const at::Device& dev,
+              fvsr_kv_cache& c) {
+  const at::Tensor *t = plain_gpu(table), *l = plain_gpu(lengths), *u = nullptr;
+  if (!t || !l || t->device() != dev || l->device() != dev || !optional_on(cu, dev, u))
+    return false;
+  if (t->scalar_type() != at::kInt || l->scalar_type() != at::kInt ||
+      (u && u->scalar_type() != at::kInt))
+    return false;
+  if (t->dim() != 2 || l->dim() != 1) return false;
+  const int64_t B = t->size(0), P = t->size(1);
+  if (B <= 0 || P <= 0 || t->stride(1) != 1 || (B > 1 && t->stride(0) < P)) return false;
+  if (l->size(0) != B || !l->is_contiguous()) return false;
+  if (u ? u->dim() != 1 || u->size(0) != B + 1 || !u->is_contiguous() : T % B != 0) return false;
+  c = fvsr_kv_cache{};
+  c.table = (const int32_t*)t->data_ptr(), c.table_stride = B > 1 ? t->stride(0) : P;
+  c.table_pages = P, c.lengths = (const int32_t*)l->data_ptr();
+  c.cu = u ? (const int32_t*)u->data_ptr() : nullptr, c.sequences = B;
+  return true;
+}
+
 // The cache of a call with T rows from (pages, page_table, lengths, cu_tokens).
 bool cache_of(PyObject* pages, PyObject* table, PyObject* lengths, PyObject* cu, int64_t T,
               const at::Device& dev, fvsr_kv_cache& c) {
@@ -202,20 +224,9 @@ bool cache_of(PyObject* pages, PyObject* table, PyObject* lengths, PyObject* cu,
     return false;
   for (int i = 2; i < 4; ++i)
     if (p[i]->dim() != 2 || p[i]->size(0) != N || p[i]->size(1) != H) return false;
-  const at::Tensor *t = plain_gpu(table), *l = plain_gpu(lengths), *u = nullptr;
-  if (!t || !l || t->device() != dev || l->device() != dev || !optional_on(cu, dev, u))
-    return false;
-  if (t->scalar_type() != at::kInt || l->scalar_type() != at::kInt ||
-      (u && u->scalar_type() != at::kInt))
-    return false;
-  if (t->dim() != 2 || l->dim() != 1) return false;
-  const int64_t B = t->size(0), P = t->size(1);
-  if (B <= 0 || P <= 0 || t->stride(1) != 1 || (B > 1 && t->stride(0) < P)) return false;
-  if (l->size(0) != B || !l->is_contiguous()) return false;
-  if (u ? u->dim() != 1 || u->size(0) != B + 1 || !u->is_contiguous() : T % B != 0) return false;
-  c = fvsr_kv_cache{k.data_ptr(), v.data_ptr(), p[2]->data_ptr(), p[3]->data_ptr(), N, H, D,
-                    (const int32_t*)t->data_ptr(), B > 1 ? t->stride(0) : P, P,
-                    (const int32_t*)l->data_ptr(), u ? (const int32_t*)u->data_ptr() : nullptr, B};
+  if (!steps_of(table, lengths, cu, T, dev, c)) return false;
+  c.k = k.data_ptr(), c.v = v.data_ptr(), c.k_scale = p[2]->data_ptr(), c.v_scale = p[3]->data_ptr();
+  c.pages = N, c.heads = H, c.head_dim = D;
   return true;
 }
 
@@ -354,6 +365,206 @@ PyObject* bind_paged(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------------------
+// Chosen pages, and rotary positions.
+// ---------------------------------------------------------------------------
+struct SelectedAbi {
+  decltype(&fvsr_pool_pages) pool;
+  decltype(&fvsr_select_pages) select;
+  decltype(&fvsr_selected_attn_workspace_floats) attn_floats;
+  decltype(&fvsr_selected_attn) attn;
+  decltype(&fvsr_rotary) rotary;
+} selected{};
+
+// (mean, scale) of a pool on `dev`.
+bool means_of(PyObject* means, const at::Device& dev, const at::Tensor*& m, const at::Tensor*& s) {
+  if (!PyTuple_Check(means) || PyTuple_GET_SIZE(means) != 2) return false;
+  m = plain_gpu(PyTuple_GET_ITEM(means, 0)), s = plain_gpu(PyTuple_GET_ITEM(means, 1));
+  return m && s && m->device() == dev && s->device() == dev && m->scalar_type() == at::kChar &&
+         s->scalar_type() == at::kFloat8_e8m0fnu && m->dim() == 3 && s->dim() == 2 &&
+         m->size(1) > 0 && (m->size(2) == 64 || m->size(2) == 128) && s->size(0) == m->size(0) &&
+         s->size(1) == m->size(1) && m->is_contiguous() && s->is_contiguous() && aligned16(*m);
+}
+
+// A Python int of int64_t's range.
+bool whole(PyObject* o, int64_t& v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  v = PyLong_AsLongLongAndOverflow(o, &over);
+  return over == 0;
+}
+
+// pool_pages(means, pages, page_table, lengths, cu_tokens, tokens | None) -> means or None
+PyObject* pool_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !selected.pool) Py_RETURN_NONE;
+  const at::Tensor *t = plain_gpu(args[2]), *mean, *scale;
+  int64_t T = -1;
+  if (!t || (args[5] != Py_None && (!whole(args[5], T) || T < 0))) Py_RETURN_NONE;
+  const at::Device dev = t->device();
+  fvsr_kv_cache c;
+  if (!is_current(dev) || !cache_of(args[1], args[2], args[3], args[4], T < 0 ? 0 : T, dev, c) ||
+      !means_of(args[0], dev, mean, scale) || mean->size(0) != c.pages ||
+      mean->size(1) != c.heads || mean->size(2) != c.head_dim || modes_active())
+    Py_RETURN_NONE;
+  void* st = stream_of(*t);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = selected.pool(&c, mean->data_ptr(), scale->data_ptr(), T, st);
+  Py_END_ALLOW_THREADS
+  if (rc != FVSR_OK) return not_done(rc, "pool_pages");
+  Py_INCREF(args[0]);
+  return args[0];
+  END_HANDLE_TH_ERRORS
+}
+
+// select_pages(q, means, page_table, lengths, cu_tokens, top, first, recent) -> columns or None
+PyObject* select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !selected.select) Py_RETURN_NONE;
+  const at::Tensor *q = plain_gpu(args[0]), *mean, *scale;
+  if (!q || q->dim() != 3 || q->numel() == 0) Py_RETURN_NONE;
+  const at::Device dev = q->device();
+  const int64_t T = q->size(0), Hq = q->size(1);
+  const int dt = dtype_code(*q);
+  int64_t top, first, recent;
+  fvsr_kv_cache c;
+  if ((dt != FVSR_DT_BF16 && dt != FVSR_DT_F16) || !is_current(dev) ||
+      !means_of(args[1], dev, mean, scale) || !rows_ok(*q, T, mean->size(2)) ||
+      !steps_of(args[2], args[3], args[4], T, dev, c) || !whole(args[5], top) ||
+      !whole(args[6], first) || !whole(args[7], recent))
+    Py_RETURN_NONE;
+  // (Lists past 2^24 entries are refused before they are allocated.)
+  if (top < 1 || top > 0xffffff || modes_active()) Py_RETURN_NONE;
+  c.pages = mean->size(0), c.heads = mean->size(1), c.head_dim = mean->size(2);
+  at::Tensor out = at::empty({T, c.heads, top}, q->options().dtype(at::kInt));
+  void* st = stream_of(*q);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = selected.select(&c, mean->data_ptr(), scale->data_ptr(), q->data_ptr(), q->stride(0),
+                       q->stride(1), Hq, dt, T, top, first, recent, (int32_t*)out.data_ptr(), st);
+  Py_END_ALLOW_THREADS
+  if (rc != FVSR_OK) return not_done(rc, "select_pages");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// selected_attention(q, pages, page_table, lengths, columns, cu_tokens, sm_scale | None) -> out or
+// None
+PyObject* selected_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !selected.attn) Py_RETURN_NONE;
+  const at::Tensor *q = plain_gpu(args[0]), *cols = plain_gpu(args[4]);
+  if (!q || !cols || q->dim() != 3 || q->numel() == 0) Py_RETURN_NONE;
+  const at::Device dev = q->device();
+  const int64_t T = q->size(0), Hq = q->size(1);
+  const int dt = dtype_code(*q);
+  fvsr_kv_cache c;
+  if ((dt != FVSR_DT_BF16 && dt != FVSR_DT_F16) || !is_current(dev) ||
+      !cache_of(args[1], args[2], args[3], args[5], T, dev, c) || !rows_ok(*q, T, c.head_dim))
+    Py_RETURN_NONE;
+  if (cols->device() != dev || cols->scalar_type() != at::kInt || cols->dim() != 3 ||
+      cols->size(0) != T || cols->size(1) != c.heads || !cols->is_contiguous())
+    Py_RETURN_NONE;
+  const int64_t top = cols->size(2);
+  double scale = 1.0 / std::sqrt((double)c.head_dim);
+  if (args[6] != Py_None) {
+    scale = PyFloat_AsDouble(args[6]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  }
+  if (modes_active()) Py_RETURN_NONE;
+  at::Tensor out = at::empty({T, Hq, c.head_dim}, q->options()), ws;
+  const int64_t wn = selected.attn_floats(&c, T, Hq, top);
+  if (wn > 0) ws = at::empty({wn}, q->options().dtype(at::kFloat));
+  void* st = stream_of(*q);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = selected.attn(&c, q->data_ptr(), q->stride(0), q->stride(1), Hq, out.data_ptr(),
+                     out.stride(0), out.stride(1), dt, T, (const int32_t*)cols->data_ptr(), top,
+                     (float)scale, 1, wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
+  Py_END_ALLOW_THREADS
+  if (rc != FVSR_OK) return not_done(rc, "selected_attention");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary(q, k | None, freqs, positions | None, pairs): q or (q, k) turned, or None; a call
+// that is recorded for a gradient goes by the general path.
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !selected.rotary) Py_RETURN_NONE;
+  const at::Tensor *q = plain_gpu(args[0]), *k = nullptr, *pos = nullptr;
+  if (!q || (q->dim() != 3 && q->dim() != 4) || q->numel() == 0) Py_RETURN_NONE;
+  const at::Device dev = q->device();
+  const int64_t d = q->dim(), D = q->size(d - 1), S = q->size(d - 3);
+  const int64_t B = d == 4 ? q->size(0) : 1;
+  const int dt = dtype_code(*q);
+  if (dt < 0 || !is_current(dev) || !optional_on(args[1], dev, k) ||
+      !optional_on(args[3], dev, pos) || !PyTuple_Check(args[2]) ||
+      PyTuple_GET_SIZE(args[2]) != 2 || !PyUnicode_Check(args[4]))
+    Py_RETURN_NONE;
+  if (q->stride(d - 1) != 1) Py_RETURN_NONE;
+  if (k && (k->dim() != d || k->scalar_type() != q->scalar_type() || k->size(d - 3) != S ||
+            (d == 4 && k->size(0) != B) || k->size(d - 1) != D || k->numel() == 0 ||
+            k->stride(d - 1) != 1))
+    Py_RETURN_NONE;
+  const at::Tensor* turns = plain_gpu(PyTuple_GET_ITEM(args[2], 0));
+  if (!turns || turns->device() != dev || turns->scalar_type() != at::kDouble ||
+      turns->dim() != 1 || !turns->is_contiguous() || 2 * turns->size(0) > D ||
+      turns->requires_grad())
+    Py_RETURN_NONE;
+  if (pos) {
+    const int64_t e = pos->dim();
+    if (pos->scalar_type() != at::kInt || (e != 1 && (e != 2 || d != 4 || pos->size(0) != B)) ||
+        pos->size(e - 1) != S || pos->stride(e - 1) != 1)
+      Py_RETURN_NONE;
+  }
+  if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad())))
+    Py_RETURN_NONE;
+  const bool half = PyUnicode_CompareWithASCIIString(args[4], "half") == 0;
+  if (!half && PyUnicode_CompareWithASCIIString(args[4], "interleaved") != 0) Py_RETURN_NONE;
+  const double gain = PyFloat_AsDouble(PyTuple_GET_ITEM(args[2], 1));
+  if (gain == -1.0 && PyErr_Occurred()) return nullptr;
+  if (modes_active()) Py_RETURN_NONE;
+  const auto rows = [d](const at::Tensor& x, const at::Tensor& y) {
+    return fvsr_rotary_rows{x.data_ptr(), y.data_ptr(),    x.size(d - 2), d == 4 ? x.stride(0) : 0,
+                            x.stride(d - 3), x.stride(d - 2)};
+  };
+  at::Tensor yq = at::empty(q->sizes(), q->options()), yk;
+  if (k) yk = at::empty(k->sizes(), k->options());
+  const fvsr_rotary_rows rq = rows(*q, yq), rk = k ? rows(*k, yk) : fvsr_rotary_rows{};
+  void* st = stream_of(*q);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = selected.rotary(&rq, k ? &rk : nullptr, dt, B, S, D, 2 * turns->size(0),
+                       (const double*)turns->data_ptr(),
+                       pos ? (const int32_t*)pos->data_ptr() : nullptr,
+                       pos && pos->dim() == 2 ? pos->stride(0) : 0, (float)gain,
+                       half ? FVSR_PAIRS_HALF : FVSR_PAIRS_INTERLEAVED, 0, st);
+  Py_END_ALLOW_THREADS
+  if (rc != FVSR_OK) return not_done(rc, "rotary");
+  PyObject* qo = THPVariable_Wrap(std::move(yq));
+  if (!k || !qo) return qo;
+  PyObject* ko = THPVariable_Wrap(std::move(yk));
+  PyObject* r = ko ? PyTuple_Pack(2, qo, ko) : nullptr;
+  Py_DECREF(qo);
+  Py_XDECREF(ko);
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_selected(pool_pages, select_pages, selected_attn_workspace_floats, selected_attn, rotary).
+PyObject* bind_selected(PyObject*, PyObject* args) {
+  unsigned long long p[5];
+  if (!PyArg_ParseTuple(args, "KKKKK", &p[0], &p[1], &p[2], &p[3], &p[4])) return nullptr;
+  selected.pool = (decltype(selected.pool))(uintptr_t)p[0];
+  selected.select = (decltype(selected.select))(uintptr_t)p[1];
+  selected.attn_floats = (decltype(selected.attn_floats))(uintptr_t)p[2];
+  selected.attn = (decltype(selected.attn))(uintptr_t)p[3];
+  selected.rotary = (decltype(selected.rotary))(uintptr_t)p[4];
+  Py_RETURN_NONE;
+}
+
 // bind(quant_workspace_floats, quant_fp8_dt, fp8_gemm, gemm_amax_parts): the
 // addresses of the C ABI functions.
 PyObject* bind(PyObject*, PyObject* args) {
@@ -376,6 +587,16 @@ PyMethodDef kMethods[] = {
      "q_weight, eps)"},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL,
      "paged_attention(q, pages, page_table, lengths, cu_tokens, causal, keep, sm_scale)"},
+    {"bind_selected", bind_selected, METH_VARARGS,
+     "addresses of the C ABI functions of chosen pages and rotary positions"},
+    {"pool_pages", (PyCFunction)(void*)pool_pages, METH_FASTCALL,
+     "pool_pages(means, pages, page_table, lengths, cu_tokens, tokens)"},
+    {"select_pages", (PyCFunction)(void*)select_pages, METH_FASTCALL,
+     "select_pages(q, means, page_table, lengths, cu_tokens, top, first, recent)"},
+    {"selected_attention", (PyCFunction)(void*)selected_attention, METH_FASTCALL,
+     "selected_attention(q, pages, page_table, lengths, columns, cu_tokens, sm_scale)"},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL,
+     "rotary(q, k, freqs, positions, pairs)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fvsr_host", nullptr, -1, kMethods};
 

@@ -131,6 +131,7 @@ class _GeneralPath:
     """Stands in for the extension where it cannot be used: every call is left
     to the Python path, which reaches the same kernels through ctypes."""
     quantize = gemm = append_kv = paged_attention = staticmethod(lambda *args: None)
+    pool_pages = select_pages = selected_attention = rotary = staticmethod(lambda *args: None)
 
 
 _host = None
@@ -181,6 +182,22 @@ def paged_host():
                 "fvsr_paged_attn_workspace_floats", "fvsr_paged_attn")))
         _paged_host = h
     return _paged_host
+
+
+_selected_host = None
+
+
+def selected_host():
+    """host(), with the functions of chosen pages and rotary positions bound too."""
+    global _selected_host
+    if _selected_host is None:
+        h, L = host(), lib()
+        if h is not _GeneralPath:
+            h.bind_selected(*(ctypes.cast(getattr(L, n), _P).value for n in (
+                "fvsr_pool_pages", "fvsr_select_pages", "fvsr_selected_attn_workspace_floats",
+                "fvsr_selected_attn", "fvsr_rotary")))
+        _selected_host = h
+    return _selected_host
 
 
 def check(rc: int, what: str):

@@ -65,6 +65,10 @@ def pool_pages(means: PageMeans, pages: KVPages, page_table: torch.Tensor, lengt
     is at most 127 times, and mean the nearest integers, ties to even: exactly.  A NaN among a
     head's codes, or as its scale, gives scale NaN.  Page ids outside the pool are passed
     over."""
+    r = (_lib._selected_host or _lib.selected_host()).pool_pages(
+        means, pages, page_table, lengths, cu_tokens, tokens)
+    if r is not None:
+        return r
     name = "pool_pages"
     _check(tokens is None or int(tokens) >= 0, f"{name}: tokens {tokens}")
     T = -1 if tokens is None else int(tokens)
@@ -97,6 +101,10 @@ def select_pages(q: torch.Tensor, means: PageMeans, page_table: torch.Tensor,
     go to the lower column.  A page whose mean is NaN, or whose id is outside the pool, comes
     behind all others; for a group of queries with an infinity or NaN all other pages tie.  Rows
     of no sequence get -1.  Tables of up to 32768 columns."""
+    r = (_lib._selected_host or _lib.selected_host()).select_pages(
+        q, means, page_table, lengths, cu_tokens, top, first, recent)
+    if r is not None:
+        return r
     name = "select_pages"
     _check(q.dim() == 3, f"{name}: q must be [T, heads, head_dim], got {tuple(q.shape)}")
     T, Hq = q.shape[:2]
@@ -142,6 +150,11 @@ def selected_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor
     passed over; a column that stands twice counts twice.  Everything else, precision
     included, as in paged_attention with causal=True: a row that sees nothing is zero, a page id outside
     the pool makes the rows that read it NaN."""
+    if out is None:
+        r = (_lib._selected_host or _lib.selected_host()).selected_attention(
+            q, pages, page_table, lengths, columns, cu_tokens, sm_scale)
+        if r is not None:
+            return r
     name = "selected_attention"
     _check(q.dim() == 3, f"{name}: q must be [T, heads, head_dim], got {tuple(q.shape)}")
     T, Hq = q.shape[:2]

@@ -121,6 +121,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
     are taken off position * turns in 64 bits; sines, products and sums are fp32, rounded once.
 
     Differentiable in q and k (any number of times); freqs and positions have no gradient."""
+    r = (_lib._selected_host or _lib.selected_host()).rotary(q, k, freqs, positions, pairs)
+    if r is not None:
+        return r
     name = "rotary"
 
     def check(ok, what):

@@ -552,3 +552,73 @@ def test_graph_and_stream():
         torch.cuda.synchronize()
         for u, v in zip((*want, *a[0], *a[1]), (*got, *b[0], *b[1])):
             assert torch.equal(u.view(torch.uint8), v.view(torch.uint8)), i
+
+
+def test_native_and_general_path(monkeypatch):
+    """The native host path serves these calls and gives what the general one does."""
+    from flashvsr_sm89_ops import (RotaryFrequencies, _lib, page_means, pool_pages, rotary,
+                                   select_pages, selected_attention)
+    H, D, B = 2, 128, 3
+    lengths = [1400, 1300, 20]
+    table, N = tables(lengths)
+    q = torch.randn(B * 7, 4, D, generator=gen(1)).bfloat16().to(DEV)
+    k = torch.randn(B * 7, 2, D, generator=gen(2)).bfloat16().to(DEV)
+    f = RotaryFrequencies(torch.rand(32, generator=gen(3)).double().to(DEV), 1.5)
+    pos = torch.randint(0, 99, (B, 7), generator=gen(4)).int().to(DEV)
+    pages, t, n = pool(N, H, D), table.to(DEV), i32(lengths).to(DEV)
+    cu = starts([7] * B).to(DEV)
+    host, got = _lib.selected_host(), []
+    assert host is not _lib._GeneralPath
+    for general in (False, True):
+        monkeypatch.setattr(_lib, "_selected_host", _lib._GeneralPath if general else host)
+        means = pool_pages(page_means(pages), pages, t, n)
+        pool_pages(means, pages, t, n, cu, tokens=B * 7)
+        cols = select_pages(q, means, t, n, top=5, first=0, recent=2)
+        r = [*means, cols, select_pages(q, means, t, n, cu, top=5)]
+        r += [selected_attention(q, pages, t, n, cols),
+              selected_attention(q, pages, t, n, cols, cu, sm_scale=0.3)]
+        r += [*rotary(q, k, f), rotary(q, None, f, pairs="interleaved"),
+              rotary(q.view(B, 7, 4, D), None, f, pos)]
+        got.append([x.view(torch.uint8) for x in r])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    c = (means, pages, t, n, None, 21)
+    assert host.pool_pages(*c) is means and host.pool_pages(*c[:5], None) is means
+    for i, bad in ((0, means[:1]), (0, (means.mean[:2], means.scale[:2])), (1, pages[:3]),
+                   (2, t.long()), (3, n[:2]), (4, n), (5, 20), (5, -1), (5, 2.0), (5, 1 << 70)):
+        assert host.pool_pages(*c[:i], bad, *c[i + 1:]) is None, i
+    c = (q, means, t, n, None, 5, 1, 1)
+    assert host.select_pages(*c).shape == (B * 7, H, 5)
+    for i, bad in ((0, q.float()), (0, q[:, :3]), (0, q[..., :64]), (0, q.cpu()), (1, means[:1]),
+                   (2, t[:2]), (5, 1), (5, 5.0), (5, 1 << 30), (6, -1), (7, 0)):
+        assert host.select_pages(*c[:i], bad, *c[i + 1:]) is None, i
+    c = (q, pages, t, n, cols, None, None)
+    assert host.selected_attention(*c).shape == q.shape
+    for i, bad in ((0, q.float()), (1, pages[:3]), (4, cols.long()), (4, cols[:, :1]),
+                   (4, cols[..., ::2]), (5, n), (6, 0.0)):
+        assert host.selected_attention(*c[:i], bad, *c[i + 1:]) is None, i
+    c = (q, k, f, None, "half")
+    assert len(host.rotary(*c)) == 2
+    for i, bad in ((0, q.double()), (0, q[:5]), (0, q.transpose(1, 2)), (1, k.float()),
+                   (1, k[..., :64]), (2, f[:1]), (2, (f.turns.float(), 1.0)), (3, pos),
+                   (3, pos[0].long()), (4, "other"), (4, 3), (0, q.detach().requires_grad_())):
+        assert host.rotary(*c[:i], bad, *c[i + 1:]) is None, i
+
+
+def test_dispatch_modes():
+    """A call inside a dispatch mode goes by the general path and is seen by it."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from flashvsr_sm89_ops import rotary, rotary_frequencies
+
+    class Seen(TorchDispatchMode):
+        names = []
+
+        def __torch_dispatch__(self, f, types, args=(), kwargs=None):
+            self.names.append(str(f))
+            return f(*args, **(kwargs or {}))
+    x = torch.randn(3, 2, 64, device=DEV)
+    f = rotary_frequencies(64)
+    want = rotary(x, None, f)
+    with Seen():
+        got = rotary(x, None, f)
+    assert torch.equal(got, want) and any("empty" in n for n in Seen.names)
