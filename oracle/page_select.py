@@ -94,6 +94,11 @@ def selected(q, mean, scale, table, lengths, top, first, recent, cu=None):
     return out
 
 
+def power(e) -> float:
+    """A scale of exponent e; 128 is the byte 255, NaN."""
+    return math.nan if int(e) == 128 else 2.0 ** int(e)
+
+
 def attended(q, cache, table, lengths, columns, cu=None, sm_scale=None):
     """(o, size, logit) as paged_kv.attention gives them, over the listed columns alone."""
     T, Hq, D = q.shape
@@ -117,8 +122,8 @@ def attended(q, cache, table, lengths, columns, cu=None, sm_scale=None):
                         ks.append(torch.full((m, D), math.nan).double())
                         vs.append(torch.zeros(m, D).double())
                         continue
-                    ks.append(cache["k"][page, h, :m] * 2.0 ** int(cache["ke"][page, h]))
-                    vs.append(cache["v"][page, h, :, :m].T * 2.0 ** int(cache["ve"][page, h]))
+                    ks.append(cache["k"][page, h, :m] * power(cache["ke"][page, h]))
+                    vs.append(cache["v"][page, h, :, :m].T * power(cache["ve"][page, h]))
                 k, v = torch.cat(ks), torch.cat(vs)
                 p = torch.softmax(k @ q[lo + i, c] * scale, 0)
                 o[lo + i, c] = p @ v

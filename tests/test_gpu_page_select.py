@@ -407,6 +407,31 @@ def test_attention_bad_pages_and_hidden_nan(T):
     check_attention(out, q, pages, table, lengths, cols)
 
 
+@pytest.mark.parametrize("Hq,H,D,dtype", [(1, 1, 128, BF), (4, 1, 64, FP), (10, 2, 128, BF), (3, 1, 64, BF)])
+@pytest.mark.parametrize("where", ["k", "v", "k_scale", "v_scale"])
+def test_attention_neighbours_of_nan(Hq, H, D, dtype, where):
+    """A NaN in a page is for the rows that list it and see it, and for none of the rows beside them."""
+    from flashvsr_sm89_ops import selected_attention
+    T, lengths = 50, [900]
+    table, N = tables(lengths, seed=1)
+    pages = pool(N, H, D, seed=2)
+    for col in (1, 4, 7):
+        page = int(table[0, col])
+        if where == "k":
+            pages.k[page, :, 5, 3] = math.nan
+        elif where == "v":
+            pages.v[page, :, 3, 3] = math.nan
+        else:
+            getattr(pages, where).view(torch.uint8)[page] = 255
+    pages.v[int(table[0, 6]), :, 9, 100] = math.nan          # position 868: behind the first rows
+    cols = random_columns(T, H, 3, lengths, [T], seed=4)
+    q = torch.randn(T, Hq, D, generator=gen(3)).to(dtype)
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV))
+    clean = ~torch.isnan(out.cpu()).any(-1).all(-1)
+    assert 0 < int(clean.sum()) < T
+    check_attention(out, q, pages, table, lengths, cols)
+
+
 def test_attention_nothing():
     from flashvsr_sm89_ops import selected_attention
     lengths = [300, 128]
