@@ -130,10 +130,11 @@ FVSR_DEV v8i join(u32x4_t a, u32x4_t b) {
 // The softmax of one row's N logits at hand (in s; -inf: hidden): s becomes
 // the weights, E - 8 - M goes to `shift`, and the reference M moves if need be
 // (`rescale` then multiplies O).  Every lane of a row calls it with the row's largest
-// logit; the sum of the weights, times 2^shift, is still to be added to l.
-template <class Acc, int N, class Rescale>
+// logit; the sum of the weights, times 2^shift, is still to be added to l.  `hide`, if given, is
+// added to every exponent: -inf where a row sees none of finite logits (top then -inf), else 0.
+template <class Acc, int N, class Rescale, class... Hide>
 FVSR_DEV void weigh(Acc (&s)[N], float top, float c, float& m, float& l, int& shift,
-                    Rescale rescale) {
+                    Rescale rescale, Hide... hide) {
   constexpr int E = sizeof(Acc) / 4;
   const float e = fmaxf(__builtin_ceilf(top * c), kNothing);
   if (__ballot(e > m + 64.0f) != 0) {
@@ -144,7 +145,7 @@ FVSR_DEV void weigh(Acc (&s)[N], float top, float c, float& m, float& l, int& sh
     l *= f;
     rescale(f);
   }
-  const float off = 8.0f - e;
+  const float off = ((8.0f - e) + ... + hide);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -193,6 +194,16 @@ FVSR_DEV void join_row(const float* po, int64_t o_step, const float* ml, int64_t
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   *(u32x2_t*)(out + lane * 4) =
       u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+}
+
+// Compute units of the current device, a multiple of the 8 XCDs.
+int64_t cu_count() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus < 8)
+    cus = 256;
+  return cus & ~7;
 }
 
 }  // namespace

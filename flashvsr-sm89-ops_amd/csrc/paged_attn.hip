@@ -1011,15 +1011,6 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
   }
 }
 
-int64_t cu_count() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-      cus < 8)
-    cus = 256;
-  return cus & ~7;
-}
-
 // How a call is cut up: a function of its sizes (and the CUs) only.
 struct Plan {
   int few;         // rows of a unit of attend_few (16) or attend_some (32); 0: attend_tile

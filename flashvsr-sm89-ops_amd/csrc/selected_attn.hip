@@ -3,10 +3,20 @@
 //   o[q] = sum_k w[k] v[k] / sum_k w[k],  w[k] = exp(sm_scale * q.k) over the tokens up to
 //          q's own position in the pages of its list
 //
-// A list belongs to a row and a key/value head, so a unit of work is the queries of one head's
-// group (up to 16, one operand) over up to `top` pages.  Operands, weights and their precision
-// are those of paged_attn.hip: K and V are operand A as stored, q and the weights sums of
-// e4m3 terms.
+// A list belongs to a row and a key/value head.  Operands, weights and their precision are those
+// of paged_attn.hip: K and V are operand A as stored, q (and in bf16 the weights) sums of e4m3
+// terms.  An operand has 16 query columns; a head's group seldom fills them, so a unit of work is
+// as many rows that follow one another as do, over the pages that any of them lists, each page read
+// and multiplied once.
+//
+// Two kernels.  attend_chosen: few units, or single tokens, whose pages come from memory: four
+// waves to a unit, and workgroups where units are too few.  attend_alone: many units of rows that
+// share pages in the L2: a wave to a unit, codes by way of LDS.
+//
+// Measured, 32 query and 8 key/value heads of 128 in bf16: one token over 64 of 2047 pages 11.7 us (17
+// MB), 128 tokens over 32 pages each 171 us (5.45 TB/s; a copy reaches 5.2); 2048 rows of a prompt
+// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 67 to 75 us between cards (256 TFLOP/s of what the rows
+// ask for; the vector units are busy for three quarters of a wave's time).
 #include <algorithm>
 #include <type_traits>
 
@@ -64,10 +74,11 @@ FVSR_DEV int limit_of(const Args& a, const Unit& u, int i) {
 FVSR_DEV int pages_of(int limit) { return (limit + kPage - 1) / kPage; }
 
 // The lists of a unit's rows, joined: columns, and which rows list them.
-constexpr int kEntries = 1024;
+constexpr int kShared = 1024, kAlone = 256;  // entries at most
+template <int N>
 struct Lists {
-  int column[kEntries];    // as listed, row by row; kNone where a row does not see it
-  uint32_t rows[kEntries];  // 0: a row before it lists the same
+  int column[N];     // as listed, row by row; kNone where a row does not see it
+  uint32_t rows[N];  // 0: a row before it lists the same
   int falls;
 };
 constexpr int kNone = INT32_MAX;
@@ -75,22 +86,23 @@ constexpr int kNone = INT32_MAX;
 // Rows of one sequence that stand together want much the same pages.  A page that several
 // rows list is read and multiplied once for all of them.  Rising lists (as select_pages gives
 // them) are searched for each other's columns; if one of them is not, each entry stands for itself.
-FVSR_DEV void join_lists(Lists& l, const Args& a, const Unit& u) {
+template <int THREADS, int N>
+FVSR_DEV void join_lists(Lists<N>& l, const Args& a, const Unit& u) {
   const int total = u.n * a.top, H = (int)a.c.heads;
   if (threadIdx.x == 0) l.falls = 0;
-  for (int e = threadIdx.x; e < total; e += kThreads) {
+  for (int e = threadIdx.x; e < total; e += THREADS) {
     const int i = e / a.top;
     const int c = a.columns[((int64_t)(u.row + i) * H + u.h) * a.top + e % a.top];
     l.column[e] = c >= 0 && c < pages_of(limit_of(a, u, i)) ? c : kNone;
   }
   __syncthreads();
   bool falls = false;
-  for (int e = threadIdx.x; e < total; e += kThreads)
+  for (int e = threadIdx.x; e < total; e += THREADS)
     falls |= e % a.top > 0 && l.column[e] != kNone && l.column[e - 1] >= l.column[e];
   if (falls) l.falls = 1;
   __syncthreads();
   const bool search = l.falls == 0;
-  for (int e = threadIdx.x; e < total; e += kThreads) {
+  for (int e = threadIdx.x; e < total; e += THREADS) {
     const int i = e / a.top, c = l.column[e];
     uint32_t rows = c == kNone ? 0 : 1u << i;
     if (search && rows)
@@ -113,6 +125,40 @@ FVSR_DEV void join_lists(Lists& l, const Args& a, const Unit& u) {
     l.rows[e] = rows;
   }
   __syncthreads();
+}
+
+// Weights of fp16 queries are halves (11 bits): V's codes become halves as well, exactly, 8 of
+// them in 4 instructions, which is less work than a weight's three e4m3 terms and their products (2048
+// rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128: 144 and 152).
+FVSR_DEV void halves4(float a, float b, float c, float d, uint32_t (&w)[2], float& sum) {
+  const v2h x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
+  const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
+  sum = __builtin_amdgcn_fdot2(x, one, sum, false);
+  sum = __builtin_amdgcn_fdot2(y, one, sum, false);
+  w[0] = __builtin_bit_cast(uint32_t, x), w[1] = __builtin_bit_cast(uint32_t, y);
+}
+// V's codes times weights: v[4 h + i] is tokens 64 h + 16 g + 4 i .., p[h][2 i] and p[h][2 i + 1]
+// are their weights.
+FVSR_DEV v4f times(const v8i& v, const v8i (&p)[2]) {
+  typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  v4f r = {};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      v4i a, b;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int x = v[4 * h + i + k];
+        a[2 * k] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+        a[2 * k + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
+        b[2 * k] = p[h][2 * (i + k)], b[2 * k + 1] = p[h][2 * (i + k) + 1];
+      }
+      r = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
+                                                 __builtin_bit_cast(v8h, b), r, 0, 0, 0);
+    }
+  return r;
 }
 
 // One wave's share of a unit: lane (r, g) = (l % 16, l / 16) has positions 16 g .. and 64 + 16 g
@@ -177,49 +223,29 @@ struct Queries {
     clear();
   }
 
-  // A page, of which this lane's query sees the first `seen` tokens; `part`: some query of the
-  // wave does not see all of it.  Hidden tokens weigh 0, which a NaN among V's codes would not
-  // survive: CAREFUL takes NaN codes out of the product and counts them where they are seen.
-  template <bool CAREFUL>
-  __device__ __forceinline__ void page(const uint8_t* kp, int k_off, const uint8_t* vp, int v_off,
-                                       int ks, int vs, bool part, int seen, int g,
-                                       float scale_log2) {
-    // (Opaque, so that no sums with them are kept in registers from page to page.)
-    asm volatile("" : "+v"(k_off), "+v"(v_off));
-    kp += k_off, vp += v_off;
-    const auto k_tile = [&](int t) {
-      const uint8_t* x = kp + ((t >> 2) * 64 + (t & 3) * 4) * D;
-      const u32x4_t y = *(const u32x4_t*)x;
-      return ::join(y, D == 128 ? *(const u32x4_t*)(x + 64) : y);
-    };
-    const auto v_tile = [&](int d) {
-      const uint8_t* x = vp + d * 16 * kPage;
-      return ::join(*(const u32x4_t*)x, *(const u32x4_t*)(x + 64));
-    };
-    // (CAREFUL is rare, and keeps no more registers than it needs: operands one by one.)
-    v8i kf[8], vf[DT16];
-    if constexpr (!CAREFUL) {
-#pragma unroll
-      for (int t = 0; t < 8; ++t) kf[t] = k_tile(t);
-#pragma unroll
-      for (int d = 0; d < DT16; ++d) vf[d] = v_tile(d);
-    }
+  // A page, of which this lane's query sees the first `seen` tokens; `cut`: some query of the
+  // wave sees a part of it only, otherwise each sees all or (seen <= 0) nothing.  k_tile(t) and
+  // v_tile(d) are its operands, k_done() and v_first() are called behind the last of K's and before
+  // the first of V's.  Hidden tokens weigh
+  // 0, which a NaN among their codes would not survive: CAREFUL hides each logit, takes V's
+  // NaN codes out of the product and counts them where they are seen.
+  template <bool CAREFUL, class K, class V, class Done, class First>
+  __device__ __forceinline__ void page(K k_tile, V v_tile, Done k_done, First v_first, int ks,
+                                       int vs, bool cut, int seen, int g, float scale_log2) {
     v4f sc[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      if constexpr (CAREFUL) {
-        asm volatile("" ::: "memory");
-        kf[t] = k_tile(t);
-      }
+      const v8i kf = k_tile(t);
       const v4f z = {};
-      sc[t] = mfma(kf[t], qf[0], z, ks, qs[0]);
+      sc[t] = mfma(kf, qf[0], z, ks, qs[0]);
 #pragma unroll
-      for (int k = 1; k < F; ++k) sc[t] = mfma(kf[t], qf[k], sc[t], ks, qs[k]);
+      for (int k = 1; k < F; ++k) sc[t] = mfma(kf, qf[k], sc[t], ks, qs[k]);
     }
+    k_done();
     // Accumulator (t, j) of lane g is position 64 (t / 4) + 16 g + 4 (t % 4) + j.
     const auto at = [](int t, int j) { return (t >> 2) * 64 + (t & 3) * 4 + j; };
     const int left = seen - 16 * g;
-    if (part) {
+    if (CAREFUL || cut) {
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -233,21 +259,30 @@ struct Queries {
       for (int j = 0; j < 4; ++j) top = fmaxf(top, sc[t][j]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
+    top = seen > 0 ? top : -__builtin_huge_valf();
     int shift;
     weigh(sc, top, scale_log2, m, l, shift, [&](float f) {
 #pragma unroll
       for (int d = 0; d < DT16; ++d) acc[d] *= f;
-    });
-    v8i pf[N];
+    }, seen > 0 ? 0.0f : -__builtin_huge_valf());
+    v8i pf[2];  // bf16: two terms; fp16: pairs of halves, tiles 0 .. 3, then 4 .. 7
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      uint32_t x[N];
-      weights4<N>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
-#pragma unroll
-      for (int k = 0; k < N; ++k) pf[k][t] = (int)x[k];
+      uint32_t x[2];
+      if constexpr (DT == FVSR_DT_F16) {
+        halves4(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
+        pf[t >> 2][2 * (t & 3)] = (int)x[0], pf[t >> 2][2 * (t & 3) + 1] = (int)x[1];
+      } else {
+        weights4<2>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
+        pf[0][t] = (int)x[0], pf[1][t] = (int)x[1];
+      }
     }
     l += __builtin_ldexpf(sum, shift);
+    const float by = DT != FVSR_DT_F16 ? 0.0f
+                     : vs == 255 && !CAREFUL
+                         ? __builtin_nanf("")
+                         : __builtin_ldexpf(1.0f, shift + (vs == 255 ? 0 : vs - 127));
     v8i ones;
     if constexpr (CAREFUL) {
 #pragma unroll
@@ -258,49 +293,100 @@ struct Queries {
           if (at(t, j) < left) ones[t] |= 0x38 << (8 * j);
       }
     }
+    v_first();
 #pragma unroll
     for (int d = 0; d < DT16; ++d) {
+      v8i vf = v_tile(d);
       if constexpr (CAREFUL) {
-        asm volatile("" ::: "memory");
-        vf[d] = v_tile(d);
         if (vs == 255)  // a page of NaN
 #pragma unroll
-          for (int i = 0; i < 8; ++i) vf[d][i] = 0x7f7f7f7f;
-        const v8i nans = take_nan(vf[d]);
+          for (int i = 0; i < 8; ++i) vf[i] = 0x7f7f7f7f;
+        const v8i nans = take_nan(vf);
         const v4f z = {};
         const v4f n = mfma(nans, ones, z, 127, 127);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (n[j] > 0.0f) acc[d][j] = __builtin_nanf("");
       }
+      if constexpr (DT == FVSR_DT_F16) {
+        acc[d] += times(vf, pf) * by;
+      } else {
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        acc[d] = mfma(vf[d], pf[k], acc[d], CAREFUL && vs == 255 ? 127 : vs, e8m0(shift - 5 * k));
+        for (int k = 0; k < 2; ++k)
+          acc[d] = mfma(vf, pf[k], acc[d], CAREFUL && vs == 255 ? 127 : vs, e8m0(shift - 5 * k));
+      }
     }
+  }
+
+  // The same with operands straight from memory: all at once, or (CAREFUL, which is rare and keeps
+  // no more registers than it needs) one by one.
+  template <bool CAREFUL>
+  __device__ __forceinline__ void page_from(const uint8_t* kp, int k_off, const uint8_t* vp,
+                                            int v_off, int ks, int vs, bool cut, int seen, int g,
+                                            float scale_log2) {
+    // (Opaque, so that no sums with them are kept in registers from page to page.)
+    asm volatile("" : "+v"(k_off), "+v"(v_off));
+    kp += k_off, vp += v_off;
+    const auto k_load = [&](int t) {
+      const uint8_t* x = kp + ((t >> 2) * 64 + (t & 3) * 4) * D;
+      const u32x4_t y = *(const u32x4_t*)x;
+      return ::join(y, D == 128 ? *(const u32x4_t*)(x + 64) : y);
+    };
+    const auto v_load = [&](int d) {
+      const uint8_t* x = vp + d * 16 * kPage;
+      return ::join(*(const u32x4_t*)x, *(const u32x4_t*)(x + 64));
+    };
+    const auto nothing = [] {};
+    if constexpr (CAREFUL) {
+      const auto apart = [](auto load) {
+        return [load](int i) {
+          asm volatile("" ::: "memory");
+          return load(i);
+        };
+      };
+      page<true>(apart(k_load), apart(v_load), nothing, nothing, ks, vs, cut, seen, g, scale_log2);
+    } else {
+      v8i kf[8], vf[DT16];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) kf[t] = k_load(t);
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) vf[d] = v_load(d);
+      page<false>([&](int t) { return kf[t]; }, [&](int d) { return vf[d]; }, nothing, nothing, ks, vs,
+                  cut, seen, g, scale_log2);
+    }
+  }
+
+  // Whether O has a NaN (or an infinity), which may come from a token that its query does not see.
+  __device__ __forceinline__ bool broken() const {
+    float any = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) any += acc[d][j] * 0.0f;
+    return __ballot(any != any) != 0;
   }
 };
 
 // A workgroup's waves take the pages of a unit in turn (of all that its splits have, every
-// splits * 4th) and add what they have.  GROUP: several rows to a unit, row i's queries in
+// splits * WAVES-th) and add what they have.  GROUP: several rows to a unit, row i's queries in
 // columns i * group and on.
 template <int DT, int D, bool GROUP>
-__global__ __launch_bounds__(kThreads, 2) void attend_chosen(Args a) {
-  constexpr int P = D + 4, C = D / 8;
-  __shared__ __attribute__((aligned(16))) float lds_o[4 * 16 * P];
-  __shared__ float lds_ml[4][16][2];
-  __shared__ std::conditional_t<GROUP, Lists, int> lists;
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void attend_chosen(Args a) {
+  constexpr int P = D + 4, C = D / 8, WAVES = kThreads / 64;
+  __shared__ __attribute__((aligned(16))) float lds_o[WAVES * 16 * P];
+  __shared__ float lds_ml[WAVES][16][2];
+  __shared__ std::conditional_t<GROUP, Lists<kShared>, int> lists;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Unit u;
   if (!unit_of(a, xcd_order(blockIdx.x, gridDim.x), u)) return;
-  if constexpr (GROUP) join_lists(lists, a, u);
+  if constexpr (GROUP) join_lists<kThreads>(lists, a, u);
   const int mine = GROUP ? min(col / a.group, u.n - 1) : 0;  // this lane's row of the unit
   const int head = GROUP ? col % a.group : min(u.q0 + col, a.group - 1);
   const int limit = limit_of(a, u, mine), least = limit_of(a, u, 0);
   const int32_t* const list = a.columns + ((int64_t)u.row * H + u.h) * a.top;
   const int32_t* const table = a.c.table + (int64_t)u.s.b * a.c.table_stride;
-  const uint32_t all = (1u << u.n) - 1;
-  const int total = u.n * a.top, turn = u.split * 4 + wave, turns = a.splits * 4;
+  const int total = u.n * a.top, turn = u.split * WAVES + wave, turns = a.splits * WAVES;
   // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4.
   const int k_off = (16 * (col >> 2) + (col & 3)) * D + 16 * g;
   const int v_off = col * kPage + 16 * g;
@@ -346,40 +432,32 @@ __global__ __launch_bounds__(kThreads, 2) void attend_chosen(Args a) {
         const bool sees = !GROUP || (who >> mine & 1) != 0;
         const int64_t at = ((int64_t)page * H + u.h) * kPage * D;
         const int s = __builtin_amdgcn_readlane(scales, i);
-        w.template page<careful>((const uint8_t*)a.c.k + at, k_off, (const uint8_t*)a.c.v + at,
-                                 v_off, s & 255, s >> 8,
-                                 (GROUP && who != all) || from + kPage > least,
-                                 sees ? limit - from : 0, g, a.scale_log2);
+        w.template page_from<careful>((const uint8_t*)a.c.k + at, k_off, (const uint8_t*)a.c.v + at,
+                                      v_off, s & 255, s >> 8,
+                                 from + kPage > least, sees ? limit - from : 0, g, a.scale_log2);
       }
     }
   };
   pages(std::false_type{});
-  // A NaN may come from a token that its query does not see.
-  float any = 0.0f;
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) any += w.acc[d][j] * 0.0f;
-  if (__ballot(any != any) != 0) {
+  if (w.broken()) {
     w.clear();
     pages(std::true_type{});
   }
   float l = w.l + __shfl_xor(w.l, 16);
   l += __shfl_xor(l, 32);
-
+  const int used = GROUP ? u.n * a.group : min(16, a.group - u.q0);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) *(v4f*)&lds_o[(wave * 16 + col) * P + d * 16 + 4 * g] = w.acc[d];
   if (g == 0) lds_ml[wave][col][0] = w.m, lds_ml[wave][col][1] = l;
   __syncthreads();
   const int d0 = threadIdx.x % C * 8;
-  const int used = GROUP ? u.n * a.group : min(16, a.group - u.q0);
-  for (int i = threadIdx.x / C; i < used; i += kThreads / C) {
+  for (int i = threadIdx.x / C; i < used; i += 64 * WAVES / C) {
     float top = lds_ml[0][i][0];
 #pragma unroll
-    for (int v = 1; v < 4; ++v) top = fmaxf(top, lds_ml[v][i][0]);
+    for (int v = 1; v < WAVES; ++v) top = fmaxf(top, lds_ml[v][i][0]);
     float o[8] = {}, sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < WAVES; ++v) {
       const float f = __builtin_amdgcn_exp2f(lds_ml[v][i][0] - top);
       sum += f * lds_ml[v][i][1];
       const v4f x = *(const v4f*)&lds_o[(v * 16 + i) * P + d0];
@@ -407,6 +485,178 @@ __global__ __launch_bounds__(kThreads, 2) void attend_chosen(Args a) {
   }
 }
 
+// Many units: one a wave (a workgroup of its own).  Straight loads of an operand touch a cache
+// line for each of their 16 rows, four times what its bytes need, and that, not the bytes, is what
+// bounds them where pages come from the L2.  Here a page's codes go to LDS in whole lines, K and V
+// each on its way while the wave computes with the other, and nobody waits for another wave.
+//
+// 16-byte pieces of LDS rows are swapped about so that the 16 lanes that read a piece of 16
+// rows touch every bank once: rows of a K operand differ in token bits 0, 1, 4 and 5
+// (128-byte rows: bit 0 is the bank half, 64-byte rows: bits 0-1 the quarter), those of V in dim
+// bits 0-3.
+template <int D>
+FVSR_DEV int k_swap(int key) {
+  return D == 128 ? ((key >> 1) & 1) | ((key >> 3) & 6) : (key >> 4) & 3;
+}
+FVSR_DEV int v_swap(int d) { return (d >> 1) & 7; }
+
+// 4 KB from `from` to LDS at `to`: the 16 bytes at from + 1024 i + off[i] of each lane go to to +
+// 1024 i, lane by lane.  (Written out: the compiler, which cannot tell K's loads from V's, would wait
+// for all of them before any read.  It is the callers who wait; the loads have no registers
+// that could be read too early.  The offset counts for both addresses.  Nothing else here uses m0.)
+FVSR_DEV void fetch(const uint8_t* to, const uint8_t* from, const int (&off)[4]) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(const uint8_t LDS_AS*)to;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %5\n\t"
+      "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+      "global_load_lds_dwordx4 %4, %5 offset:3072"
+      :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "v"(off[2]),
+      "v"(off[3]), "s"(from) : "memory");
+}
+// Until at most N of them are on their way.
+template <int N>
+FVSR_DEV void wait_for() {
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
+struct Visit {
+  int id, column;
+  uint32_t what;  // scales of K and V, and (16 bits) the rows that list it
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(64, D == 64 ? 2 : 1) void attend_alone(Args a) {
+  constexpr int KR = D / 16;                 // pieces of a K row
+  constexpr int SEG = kPage * D / 1024;      // of 64 pieces
+  __shared__ __attribute__((aligned(1024))) uint8_t kl[kPage * D], vl[kPage * D];
+  __shared__ Visit visits[kAlone];
+  // The lists lie where K will: eight workgroups (64 dims) or four then share a CU.
+  static_assert(sizeof(Lists<kAlone>) <= sizeof(kl), "lists outgrow K's codes");
+  Lists<kAlone>& lists = *(Lists<kAlone>*)kl;
+  const int lane = threadIdx.x, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
+  Unit u;
+  if (!unit_of(a, xcd_order(blockIdx.x, gridDim.x), u)) return;
+  join_lists<64>(lists, a, u);
+  const int mine = min(col / (a.parts > 1 ? 16 : a.group), u.n - 1);
+  const int head = a.parts > 1 ? min(u.q0 + col, a.group - 1) : col % a.group;
+  const int limit = limit_of(a, u, mine), least = limit_of(a, u, 0);
+  const int32_t* const table = a.c.table + (int64_t)u.s.b * a.c.table_stride;
+  Queries<DT, D> w;
+  w.load(a.q + (int64_t)(u.row + mine) * a.q_ts + (int64_t)(u.h * a.group + head) * a.q_hs, g);
+  int n = 0, wrong = 0;
+  for (int e0 = 0; e0 < u.n * a.top; e0 += 64) {
+    const int e = e0 + lane;
+    const int c = e < u.n * a.top ? lists.column[e] : kNone;
+    const uint32_t rows = c != kNone ? lists.rows[e] : 0;
+    const int id = rows ? table[c] : -1;
+    const bool good = id >= 0 && id < a.c.pages;
+    for (uint64_t bad = __ballot(rows && !good); bad; bad &= bad - 1)
+      wrong |= __builtin_amdgcn_readlane(rows, __builtin_ctzll(bad));
+    const uint64_t there = __ballot(good);
+    if (good) {
+      const int64_t ph = (int64_t)id * H + u.h;
+      visits[n + __popcll(there & ((1ull << lane) - 1))] =
+          Visit{id, c,
+                ((const uint8_t*)a.c.k_scale)[ph] |
+                    (uint32_t)((const uint8_t*)a.c.v_scale)[ph] << 8 | rows << 16};
+    }
+    n += __popcll(there);
+  }
+  __syncthreads();
+  const auto visit = [&](int i) {
+    const Visit& v = visits[i];
+    return Visit{__builtin_amdgcn_readfirstlane(v.id), __builtin_amdgcn_readfirstlane(v.column),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)v.what)};
+  };
+  const auto seen_of = [&](const Visit& v) {  // tokens of the page that this lane's query sees
+    return (v.what >> (16 + mine) & 1) != 0 ? limit - v.column * kPage : 0;
+  };
+  const auto codes = [&](const void* p, const Visit& v) {
+    return (const uint8_t*)p + ((int64_t)v.id * H + u.h) * kPage * D;
+  };
+  // What a lane fetches of segment s belongs where it lands: row s * 64 / KR + lane / KR, piece
+  // lane % KR, holds the piece with that number and the row's swap.
+  const auto fetch_k = [&](const Visit& v) {
+    const uint8_t* from = codes(a.c.k, v);
+#pragma unroll
+    for (int s = 0; s < SEG; s += 4) {
+      int off[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        off[i] = lane / KR * D +
+                 ((lane % KR) ^ k_swap<D>((s + i) * (64 / KR) + lane / KR)) * 16;
+      fetch(kl + s * 1024, from + s * 1024, off);
+    }
+  };
+  const auto fetch_v = [&](const Visit& v) {
+    const uint8_t* from = codes(a.c.v, v);
+#pragma unroll
+    for (int s = 0; s < SEG; s += 4) {
+      int off[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        off[i] = lane / 8 * kPage + ((lane % 8) ^ v_swap((s + i) * 8 + lane / 8)) * 16;
+      fetch(vl + s * 1024, from + s * 1024, off);
+    }
+  };
+  // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4.
+  const auto k_tile = [&](int t) {
+    const int key = 64 * (t >> 2) + 16 * (col >> 2) + 4 * (t & 3) + (col & 3);
+    const uint8_t* row = kl + key * D;
+    const u32x4_t x = *(const u32x4_t*)(row + (g ^ k_swap<D>(key)) * 16);
+    return ::join(x, D == 128 ? *(const u32x4_t*)(row + ((g + 4) ^ k_swap<D>(key)) * 16) : x);
+  };
+  const auto v_tile = [&](int d) {
+    const int dim = d * 16 + col;
+    const uint8_t* row = vl + dim * kPage;
+    return ::join(*(const u32x4_t*)(row + (g ^ v_swap(dim)) * 16),
+                  *(const u32x4_t*)(row + ((g + 4) ^ v_swap(dim)) * 16));
+  };
+  if (n > 0) {
+    Visit cur = visit(0);
+    fetch_k(cur);
+    fetch_v(cur);
+    for (int i = 0; i < n; ++i) {
+      const Visit next = visit(min(i + 1, n - 1));  // (the last one again: no branch)
+      const uint32_t what = cur.what;
+      wait_for<SEG>();  // K is there, V may be on its way
+      w.template page<false>(k_tile, v_tile, [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's operands are read
+        fetch_k(next);
+      }, [&] {
+        wait_for<SEG>();  // V is there, the next K may be on its way
+      }, what & 255, what >> 8 & 255, (cur.column + 1) * kPage > least, seen_of(cur), g,
+          a.scale_log2);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V's
+      fetch_v(next);
+      cur = next;
+    }
+    wait_for<0>();  // no load may land in an LDS that the next workgroup has
+  }
+  if (w.broken()) {
+    w.clear();
+    const int k_off = (16 * (col >> 2) + (col & 3)) * D + 16 * g, v_off = col * kPage + 16 * g;
+    for (int i = 0; i < n; ++i) {
+      const Visit v = visit(i);
+      w.template page_from<true>(codes(a.c.k, v), k_off, codes(a.c.v, v), v_off, v.what & 255,
+                                 v.what >> 8 & 255, true, seen_of(v), g, a.scale_log2);
+    }
+  }
+  float l = w.l + __shfl_xor(w.l, 16);
+  l += __shfl_xor(l, 32);
+  if (wrong >> mine & 1) l = __builtin_nanf("");  // no such page: the rows that list it are NaN
+  if (col >= (a.parts > 1 ? min(16, a.group - u.q0) : u.n * a.group)) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = a.out + (int64_t)(u.row + mine) * a.o_ts + (u.h * a.group + head) * a.o_hs + 4 * g;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d)
+    *(u32x2_t*)(op + d * 16) = u32x2_t{pack2<DT>(w.acc[d][0] * inv, w.acc[d][1] * inv),
+                                       pack2<DT>(w.acc[d][2] * inv, w.acc[d][3] * inv)};
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void join_chosen(Args a) {
   const int64_t row = blockIdx.x, rows = (int64_t)a.T * a.q_heads;
@@ -416,11 +666,12 @@ __global__ __launch_bounds__(kThreads) void join_chosen(Args a) {
                   a.out + row / a.q_heads * a.o_ts + row % a.q_heads * a.o_hs);
 }
 
-// How a call is cut up: a function of its sizes only.
+// How a call is cut up: a function of its sizes (and the CUs) only.
 struct Plan {
-  int rows;             // of a unit
+  int rows;              // of a unit
   int64_t tiles, units;  // of rows, over all sequences; with heads and operands of 16 queries
   int parts, splits;
+  bool alone;            // attend_alone: one wave to a unit
   int64_t floats(int64_t T, int64_t q_heads, int64_t D) const {
     return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
   }
@@ -428,14 +679,26 @@ struct Plan {
 
 Plan plan_selected(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, int64_t top) {
   Plan p{};
-  const int64_t cus = 256, B = c->sequences, group = q_heads / c->heads;
+  const int64_t cus = cu_count(), B = c->sequences, group = q_heads / c->heads;
   const int64_t each = c->cu ? (T > B ? T : 1) : T / B;  // rows of a sequence at most
-  p.rows = (int)std::max<int64_t>(
-      1, std::min<int64_t>({16 / std::min<int64_t>(group, 16), each,
-                            kEntries / std::max<int64_t>(top, 1)}));
+  const auto cut = [&](int64_t entries) {
+    p.rows = (int)std::max<int64_t>(
+        1, std::min<int64_t>({16 / std::min<int64_t>(group, 16), each,
+                              entries / std::max<int64_t>(top, 1)}));
+    p.tiles = c->cu ? T / p.rows + B + 1 : B * ((T / B + p.rows - 1) / p.rows);
+    p.units = p.tiles * c->heads * p.parts;
+  };
   p.parts = (int)((group + 15) / 16);
-  p.tiles = c->cu ? T / p.rows + B + 1 : B * ((T / B + p.rows - 1) / p.rows);
-  p.units = p.tiles * c->heads * p.parts;
+  p.splits = 1;
+  cut(kAlone);
+  // A wave to a unit where rows of a sequence follow one another (their pages come from the L2)
+  // and there are units for the CUs' SIMDs.  (us alone / shared at 256 units 49 / 37, 512 units of
+  // 64 dims 44 / 30, of 128 dims 59 / 63, 768 120 / 156, 1024 50 / 65, 2048 of 64 dims 75 / 106, of 128
+  // 129 / 213.)
+  p.alone = each > 1 && top <= kAlone && p.units * 2 >= cus * 5;
+  if (p.alone) return p;
+  cut(kShared);
+  // Two workgroups to a CU, each with a page for every wave.
   p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 2 * cus / p.units),
                                      std::max<int64_t>(1, top / 4), kMaxSplits});
   return p;
@@ -443,7 +706,11 @@ Plan plan_selected(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, int64_t t
 
 template <int DT, int D>
 void launch(const Args& a, const Plan& p, hipStream_t st) {
-  const dim3 block(kThreads), grid((unsigned)(p.units * p.splits));
+  const dim3 grid((unsigned)(p.units * p.splits)), block(kThreads);
+  if (p.alone) {
+    hipLaunchKernelGGL((attend_alone<DT, D>), grid, dim3(64), 0, st, a);
+    return;
+  }
   if (p.rows > 1)
     hipLaunchKernelGGL((attend_chosen<DT, D, true>), grid, block, 0, st, a);
   else
