@@ -12,6 +12,7 @@
 // pages a row reads does not hang on the order of a sum, and equal scores are equal.  Only
 // full pages need one: the page that holds a row's own position is always read.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_pages.h"
 
@@ -133,10 +134,16 @@ __global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// select_kernel: a workgroup takes up to `tt` rows of a sequence and a head.  First its waves
-// share out the pages, 16 at a time: products of 16 rows (a row's group padded to a power
-// of two) and 16 pages; a row's largest goes to LDS as a key.  Then its waves share out the rows:
-// a bisection over the keys finds the one that just makes the list.
+// select_kernel: a workgroup takes up to `tt` rows of a sequence and a head.  First its waves share
+// out the pages, 16 at a time: products of 16 rows (a row's group padded to a power of two) and
+// 16 pages; a row's largest goes to LDS as a key.  Then its waves share out the rows, and a bisection
+// over the keys finds the one that just makes the list.
+//
+// Bound by instructions, not bytes: 4096 rows x 32 / 8 heads over some 500 pages take 45 us, 36 MB
+// would take 7.  Of those 30 go to q's integers and the scores (13 instructions a row's group and
+// page), 15 to the choice (some 200 vector and 200 scalar ones a row and head).  One row's is a chain of
+// lengths, ids, means and choice: 6 us over 157 pages, 11 over 938, 17 over 1953; 64 rows over up to
+// 1016 pages each 16.6.
 //
 // Operands of v_mfma_i32_16x16x64_i8: lane (r, g) = (l % 16, l / 16) holds bytes 16 g .. of row r;
 // accumulator j of lane (c, g) is row 4 g + j (a query) of column c (a page).
@@ -148,134 +155,232 @@ struct SelectArgs {
   const uint16_t* q;
   int64_t q_ts, q_hs;
   int32_t* out;
-  int T, group, top, first, recent, f16;
+  int T, group, top, first, recent;
   int tt, tiles, width;  // rows of a tile; tiles of all sequences; keys of a row in LDS
 };
 
 constexpr int kLow = -(1 << 30);  // key of a page without a mean: below any other
 constexpr int kNever = INT32_MIN;
 
-// dot * 2^scale as an integer that orders like it: sign and magnitude of a float of 9
-// exponent and 20 fraction bits (|dot| < 2^21 has no more).
-FVSR_DEV int key_of(int dot, int scale) {
-  const uint32_t bits = __float_as_uint((float)abs(dot)) >> 3;
-  const int key = (int)(bits + ((uint32_t)scale << 20));
-  return dot == 0 ? 0 : dot < 0 ? -key : key;
+// dot * 2^scale as an integer that orders like it: sign and magnitude of a float of 9 exponent
+// and 20 fraction bits (|dot| < 2^21 has no more).  scale20: the scale's byte << 20.
+FVSR_DEV int key_of(int dot, int scale20) {
+  const uint32_t bits = __float_as_uint((float)dot);
+  const int sign = dot >> 31;
+  return dot == 0 ? 0 : (((int)(bits << 1 >> 4) + scale20) ^ sign) - sign;
 }
 
-FVSR_DEV float q_at(uint32_t pair, int odd, int f16) {
-  const uint16_t u = (uint16_t)(odd ? pair >> 16 : pair & 0xffff);
-  return f16 ? (float)__builtin_bit_cast(_Float16, u) : bf2f(u);
+// A wave's largest value, in a scalar register (DPP moves: no LDS round trips).
+FVSR_DEV int wave_largest(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false));  // row_half_mirror
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, false));  // row_mirror
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
-// What `n` waves that work on one row tell one another.
-struct Told {
-  int count[2][4], gt[4], eq[4], top[4], low[4];
-};
-
-// The list of a row that sees the columns 0 .. seen - 1, more than `top` of them.
-template <int WAVES>
-FVSR_DEV void pick(const SelectArgs& a, const int* keys, int seen, int wave, Told& told,
-                   int32_t* out) {
-  constexpr int R = 8;
-  const int lane = threadIdx.x & 63;
-  const int share = WAVES == 1 ? seen : (seen + 64 * WAVES - 1) / (64 * WAVES) * 64;
-  const int c0 = min(seen, wave * share), c1 = min(seen, c0 + share);
-  const int need = a.top - a.first - a.recent, end = seen - a.recent;
-  const auto key_at = [&](int c) { return c >= a.first && c < min(end, c1) ? keys[c] : kNever; };
-  int key[R], top = kNever;
-#pragma unroll
-  for (int i = 0; i < R; ++i) top = max(top, key[i] = key_at(c0 + i * 64 + lane));
-  for (int c = c0 + R * 64; c < c1; c += 64) top = max(top, key_at(c + lane));
-  // Every lane's largest is at least `low`: with 64 of them (or more) one bound of the search.
-  int low = top;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    top = max(top, __shfl_xor(top, d));
-    low = min(low, __shfl_xor(low, d));
-  }
-  if (WAVES > 1) {
-    if (lane == 0) told.top[wave] = top, told.low[wave] = low;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = max(top, told.top[w]), low = min(low, told.low[w]);
-  }
-  top = __builtin_amdgcn_readfirstlane(top);
-  low = __builtin_amdgcn_readfirstlane(low);
-  int turn = 0;
-  const auto count = [&](int at) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) n += __popcll(__ballot(key[i] >= at));
-    for (int c = c0 + R * 64; c < c1; c += 64) n += __popcll(__ballot(key_at(c + lane) >= at));
-    if (WAVES > 1) {
-      if (lane == 0) told.count[turn & 1][wave] = n;
-      __syncthreads();
-      n = 0;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) n += told.count[turn & 1][w];
-      ++turn;
+// A value that just `need` of some keys reach (exact), or the largest that more do, which some
+// share; at least `need` of them reach lo.  Bit by bit, in as few scalar instructions as can be.
+template <class Count>
+FVSR_DEV int reached(Count count, int need, int lo, int top, bool& exact) {
+  for (int bit = 1 << (31 - __builtin_clz(max(top - lo, 1))); bit > 0; bit >>= 1) {
+    const int n = count(lo + bit);
+    lo = n >= need ? lo + bit : lo;
+    if (n == need) {
+      exact = true;
+      return lo;
     }
-    return __builtin_amdgcn_readfirstlane(n);
+  }
+  exact = false;
+  return lo;
+}
+
+FVSR_DEV int before(uint64_t set, int from) {  // lanes of `set` below this one, and `from`
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)set, from));
+}
+
+// A bound that `need` of a wave's keys reach, and not many more: what `need` of the largest keys of
+// 64 lanes (few are needed) or of 256 groups of them reach.  (Keys order like floats: it is
+// seldom further down than a few powers of two.)
+FVSR_DEV int bound_of(const int (&group)[4], int need) {
+  const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
+  const int top = wave_largest(mine), near = max(top - (3 << 20), kLow);
+  const auto find = [&](auto reach) {
+    bool exact;
+    const bool fits = reach(near) >= need;
+    if (!fits && reach(kLow) < need) return kLow;
+    return reached(reach, need, fits ? near : kLow, top, exact);
   };
-  // At least `need` keys are >= lo, fewer are >= hi; `above` of them.
-  int lo = need <= 64 * WAVES && low > kLow ? low : kLow, hi = top + 1, above = 0;
-  int ties = need;
-  if (need > 0) {
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2, n = count(mid);
-      if (n == need) {  // no tie to break: all above mid - 1
-        lo = mid - 1, above = need;
-        break;
-      }
-      if (n > need)
-        lo = mid;
-      else
-        hi = mid, above = n;
-    }
-    ties = need - above;
-  } else {
-    lo = top;  // none above
-    ties = 0;
-  }
-  // Columns in the list: those always there, keys above lo, the first `ties` at lo.
-  const auto sure = [&](int c) { return c < c1 && (c < a.first || c >= end); };
-  int at = 0, left = ties;
-  if (WAVES > 1) {
-    int gt = 0, eq = 0;
-    for (int c = c0; c < c1; c += 64) {
-      const int k = key_at(c + lane);
-      gt += __popcll(__ballot(sure(c + lane) || k > lo));
-      eq += __popcll(__ballot(k == lo));
-    }
-    if (lane == 0) told.gt[wave] = gt, told.eq[wave] = eq;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      if (w < wave) {
-        const int took = min(left, told.eq[w]);
-        at += told.gt[w] + took, left -= took;
-      }
-  }
-  const uint64_t below = (1ull << lane) - 1;
-  for (int c = c0; c < c1; c += 64) {
-    const int k = key_at(c + lane);
-    const bool tie = k == lo;
-    const uint64_t eq = __ballot(tie);
-    const bool in = sure(c + lane) || k > lo || (tie && __popcll(eq & below) < left);
-    const uint64_t all = __ballot(in);
-    if (in) out[at + __popcll(all & below)] = c + lane;
-    at += __popcll(all);
-    left -= min(left, __popcll(eq));
-  }
+  if (need <= 16) return find([&](int at) { return (int)__popcll(__ballot(mine >= at)); });
+  return find([&](int at) {
+    return (int)(__popcll(__ballot(group[0] >= at)) + __popcll(__ballot(group[1] >= at)) +
+                 __popcll(__ballot(group[2] >= at)) + __popcll(__ballot(group[3] >= at)));
+  });
 }
 
-template <int D, int GP, int M>
+// A wave takes the `need` largest of n > need keys in LDS, of equal ones the first, and gives
+// their places, rising, to emit(place, rank).  R: keys of a lane in registers; the others are read
+// each time.  (Up to R * 64 keys are read whatever n is, in LDS and without a use.)
+template <int R, class Emit>
+FVSR_DEV void choose(const int* keys, int n, int need, Emit emit) {
+  const int lane = threadIdx.x & 63;
+  keys += lane;
+  const auto key_at = [&](int i) { return i + lane < n ? keys[i] : kNever; };
+  int key[R], group[4] = {kNever, kNever, kNever, kNever};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int k = keys[i * 64];
+    key[i] = i * 64 + lane < n ? k : kNever;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) group[i % 4] = max(group[i % 4], key[i]);
+  for (int i = R * 64; i < n; i += 64) group[0] = max(group[0], key_at(i));
+  const auto count = [&](int at) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) c += __popcll(__ballot(key[i] >= at));
+    for (int i = R * 64; i < n; i += 64) c += __popcll(__ballot(key_at(i) >= at));
+    return c;
+  };
+  // Chosen: keys above lo, and the first `left` of those at it.
+  int lo = bound_of(group, need), left = 0, reach = count(lo);
+  if (reach > need + 4) {
+    bool exact;
+    const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
+    lo = reached(count, need, lo, wave_largest(mine), exact);
+    reach = exact ? need : count(lo);
+  }
+  // A few too many reach it: past the least of them, until it is those, or a tie.
+  while (reach > need) {
+    int least = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < R; ++i) least = min(least, key[i] >= lo ? key[i] : INT32_MAX);
+    for (int i = R * 64; i < n; i += 64) {
+      const int k = key_at(i);
+      least = min(least, k >= lo ? k : INT32_MAX);
+    }
+    least = ~wave_largest(~least);
+    const int above = count(least + 1);
+    if (above < need) {
+      lo = least, left = need - above;
+      break;
+    }
+    lo = least + 1, reach = above;
+  }
+  if (left == 0) --lo;
+  int at = 0;
+  const auto put = [&](int i, int k) {
+    bool in = k > lo;
+    if (left > 0) {
+      const uint64_t eq = __ballot(k == lo);
+      in |= (k == lo) & (before(eq, 0) < left);
+      left -= min(left, __popcll(eq));
+    }
+    const uint64_t all = __ballot(in);
+    if (all == 0) return;
+    if (in) emit(i + lane, before(all, at));
+    at += __popcll(all);
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) put(i * 64, key[i]);
+  for (int i = R * 64; i < n; i += 64) put(i, key_at(i));
+}
+
+// A row that has its workgroup to itself: every wave keeps those of its share of the keys that
+// reach the best bound that any of them found, and one wave chooses among what is left.
+constexpr int kLeft = 256;
+struct Sieve {
+  int bound[4], count[4];
+  int key[kLeft], place[kLeft];
+};
+template <class Emit>
+FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s, Emit emit) {
+  if (n <= kLeft) {
+    if (wave == 0) choose<kLeft / 64>(keys, n, need, emit);
+    return;
+  }
+  const int lane = threadIdx.x & 63, share = (n + 255) / 256 * 64;
+  const int i0 = wave * share + lane, i1 = min(n, (wave + 1) * share);
+  int group[4] = {kNever, kNever, kNever, kNever};
+  for (int i = i0; i < i1; i += 256)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      group[g] = max(group[g], i + g * 64 < i1 ? keys[i + g * 64] : kNever);
+  const int bound = bound_of(group, need);
+  if (lane == 0) s.bound[wave] = bound;
+  __syncthreads();
+  const int lo = __builtin_amdgcn_readfirstlane(
+      max(max(s.bound[0], s.bound[1]), max(s.bound[2], s.bound[3])));
+  int c = 0;
+  for (int i = i0; i < i1 + lane; i += 64)  // (whole waves)
+    c += __popcll(__ballot(i < i1 && keys[min(i, n - 1)] >= lo));
+  if (lane == 0) s.count[wave] = c;
+  __syncthreads();
+  int at = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w == wave) at = total;
+    total += s.count[w];
+  }
+  at = __builtin_amdgcn_readfirstlane(at), total = __builtin_amdgcn_readfirstlane(total);
+  if (total > kLeft) {  // (more than a wave's lanes are wanted, or many tie)
+    if (wave == 0) choose<16>(keys, n, need, emit);
+    return;
+  }
+  for (int i = i0; i < i1 + lane; i += 64) {
+    const int k = i < i1 ? keys[i] : kNever;
+    const uint64_t in = __ballot(k >= lo);
+    if (k >= lo) {
+      const int to = before(in, at);
+      s.key[to] = k, s.place[to] = i;
+    }
+    at += __popcll(in);
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  if (total == need) {
+    for (int i = lane; i < need; i += 64) emit(s.place[i], i);
+    return;
+  }
+  choose<kLeft / 64>(s.key, total, need, [&](int i, int rank) { emit(s.place[i], rank); });
+}
+
+// A row's 16 channels at 64 w + 16 g, w < W, of one query.
+template <int W>
+struct Channels {
+  u32x4_t raw[W][2];
+  FVSR_DEV void load(Channels& c, const uint16_t* q) {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      c.raw[w][0] = *(const u32x4_t*)(q + 64 * w), c.raw[w][1] = *(const u32x4_t*)(q + 64 * w + 8);
+  }
+  // The largest magnitude's bits (of two values at once: magnitudes order like their bits).
+  FVSR_DEV uint32_t largest(const Channels& c) {
+    u16x2_t top = {0, 0};
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x = c.raw[w][i >> 2][i & 3] & 0x7fff7fffu;
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x));
+      }
+    return max(top[0], top[1]);
+  }
+};
+template <bool F16>
+FVSR_DEV float half_to_f(uint32_t h) {
+  if (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+  return __uint_as_float(h << 16);
+}
+
+template <int D, int GP, int M, bool F16, int Q = 4>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   constexpr int W = D / 64;
   constexpr int TP = 16 / GP;  // rows of an operand
-  extern __shared__ int keys[];
-  __shared__ Told told;
+  extern __shared__ __attribute__((aligned(16))) int keys[];
+  __shared__ Sieve sieve;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int H = (int)a.c.heads, P = (int)a.c.table_pages, B = (int)a.c.sequences;
@@ -302,150 +407,201 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
     return p < 0 ? 0 : min(p / kPage + 1, P);
   };
   const int most = seen(nt - 1), need = a.top - a.first - a.recent;
-  const int32_t* const table = a.c.table + (int64_t)s.b * a.c.table_stride;
   if (most > a.top && need > 0) {
+    const int32_t* const table = a.c.table + (int64_t)s.b * a.c.table_stride;
     const int chunks = (a.group + 15) / 16;  // (more than one: GP is 16, a row to a tile)
-    const uint16_t* const q0 = a.q + (int64_t)(s.rows.lo + t0) * a.q_ts;
-    const auto row_of = [&](int m, int c) {
+    const uint16_t* const q0 = a.q + (int64_t)(s.rows.lo + t0) * a.q_ts + 16 * g;
+    // Operand m (of rows, or of chunk c + m of one row's group) as integers.
+    const auto load = [&](int m, int c, Channels<W>& x) {
       const int i = chunks == 1 ? min(m * TP + col / GP, nt - 1) : 0;
       const int head = min(chunks == 1 ? col % GP : (c + m) * 16 + col, a.group - 1);
-      return (const u32x4_t*)(q0 + i * a.q_ts + (int64_t)(h * a.group + head) * a.q_hs + 16 * g);
-    };
-    const auto load = [&](int m, int c, u32x4_t(&raw)[W][2]) {
-      const u32x4_t* p = row_of(m, c);
-#pragma unroll
-      for (int w = 0; w < W; ++w) raw[w][0] = p[8 * w], raw[w][1] = p[8 * w + 1];
-    };
-    const auto largest = [&](const u32x4_t(&raw)[W][2]) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          top = max(top, __float_as_uint(q_at(raw[w][i >> 3][(i >> 1) & 3], i & 1, a.f16)) &
-                             0x7fffffffu);
-      return top;
+      Channels<W>::load(x, q0 + i * a.q_ts + (int64_t)(h * a.group + head) * a.q_hs);
     };
     uint32_t top_all = 0;
     if (chunks > 1)
       for (int c = 0; c < chunks; ++c) {
-        u32x4_t raw[W][2];
-        load(0, c, raw);
-        top_all = max(top_all, largest(raw));
+        Channels<W> x;
+        load(0, c, x);
+        top_all = max(top_all, Channels<W>::largest(x));
       }
-    for (int c = 0; c < chunks; c += M) {
+    const auto operand = [&](int m, int c, v4i(&to)[W]) {
+      Channels<W> x;
+      load(m, c, x);
+      uint32_t top = max(top_all, Channels<W>::largest(x));
+      // Over a row's lanes, then over the rows of its group.
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+#pragma unroll
+      for (int d = 1; d < GP; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      // Exponent with the largest <= 127 * 2^e; 0 for all where it is not finite.
+      const uint32_t t = __float_as_uint(half_to_f<F16>(top));
+      const int n = t >= 0x00800000u ? (int)(t >> 23) - 127  // floor of its logarithm
+                    : t != 0         ? -118 - __builtin_clz(t)
+                                     : 0;
+      const int e = __builtin_ldexpf(__uint_as_float(t), -n) > 127.0f / 64 ? n - 5 : n - 6;
+      const bool fine = t < 0x7f800000u;
+      // x * 2^-e + 1.5 * 2^23 has the nearest integer (ties to even) in its low bits: a
+      // product by a power of two, in two steps where one would not hold it, and one rounding.
+      const float f = __builtin_ldexpf(1.0f, min(-e, 100));
+      const float f2 = __builtin_ldexpf(1.0f, -e - min(-e, 100));
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t u = x.raw[w][i >> 1][(i & 1) * 2 + (k >> 1)];
+            const float v = half_to_f<F16>(k & 1 ? u >> 16 : u & 0xffff);
+            r[k] = __float_as_uint(__builtin_fmaf(F16 ? v : v * f2, f, 0x1.8p23f));
+          }
+          const uint32_t lo = __builtin_amdgcn_perm(r[1], r[0], 0x0c0c0400u);
+          const uint32_t hi = __builtin_amdgcn_perm(r[3], r[2], 0x04000c0cu);
+          to[w][i] = fine ? (int)(lo | hi) : 0;
+        }
+    };
+    if (a.c.pages == 0)  // (a pool without pages)
+      for (int i = threadIdx.x; i < nt * a.width; i += kThreads) keys[i] = kLow;
+    for (int c = 0; c < chunks && a.c.pages > 0; c += M) {
       v4i qa[M][W];
+      if constexpr (M == 1) {
+        operand(0, c, qa[0]);
+      } else {
+        // Each wave makes one operand; they change hands where the keys will be (or, with
+        // chunks, behind those).
+        static_assert(M == kThreads / 64, "an operand to each wave");
+        v4i* const shared_q = (v4i*)(keys + (chunks > 1 ? (a.width + 3) / 4 * 4 : 0));
+        v4i own[W];
+        operand(wave, c, own);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        u32x4_t raw[W][2];
-        load(m, c, raw);
-        uint32_t top = max(top_all, largest(raw));
-        // Over a row's lanes, then over the rows of its group.
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        for (int w = 0; w < W; ++w) shared_q[(wave * W + w) * 64 + lane] = own[w];
+        __syncthreads();
 #pragma unroll
-        for (int d = 1; d < GP; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        // Exponent with top <= 127 * 2^e; 0 for all where it is not finite.
-        const float t = __uint_as_float(top);
-        const int x = top >= 0x00800000u ? (int)(top >> 23) - 127  // floor of its logarithm
-                      : top != 0         ? -118 - __builtin_clz(top)
-                                         : 0;
-        const int e = __builtin_ldexpf(t, -x) > 127.0f / 64 ? x - 5 : x - 6;
-        const bool fine = top < 0x7f800000u;
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t word = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int n = 4 * i + k;
-              const float v = q_at(raw[w][n >> 3][(n >> 1) & 3], n & 1, a.f16);
-              const int r = fine ? (int)__builtin_rintf(__builtin_ldexpf(v, -e)) : 0;
-              word |= ((uint32_t)r & 255u) << (8 * k);
-            }
-            qa[m][w][i] = (int)word;
-          }
+          for (int w = 0; w < W; ++w) qa[m][w] = shared_q[(m * W + w) * 64 + lane];
+        __syncthreads();
       }
-      for (int p0 = wave * 16; p0 < most; p0 += kThreads / 64 * 16) {
-        const int p = p0 + col;
-        const int id = p < most ? table[p] : -1;
-        const bool there = id >= 0 && id < a.c.pages;
-        const int64_t ph = (int64_t)(there ? id : 0) * H + h;
-        v4i mb[W];
+      // 16 Q pages at a time, whose means are on their way together; the next ones' ids too.
+      const auto ids = [&](int p0, int(&id)[Q]) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) mb[w] = v4i{};
-        int scale = 255;
-        if (there) {
-#pragma unroll
-          for (int w = 0; w < W; ++w) mb[w] = *(const v4i*)(a.mean + ph * D + 64 * w + 16 * g);
-          scale = a.scale[ph];
+        for (int k = 0; k < Q; ++k) {
+          const int p = p0 + 16 * k + col;
+          const int x = table[min(p, most - 1)];
+          id[k] = p < most ? x : -1;
         }
+      };
+      int id[Q];
+      ids(wave * 16 * Q, id);
+      for (int p0 = wave * 16 * Q; p0 < most; p0 += kThreads / 64 * 16 * Q) {
+        v4i mb[Q][W];
+        int scale[Q];
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-          v4i x = {};
+        for (int k = 0; k < Q; ++k) {
+          const bool there = id[k] >= 0 && id[k] < a.c.pages;
+          const int64_t ph = (int64_t)(there ? id[k] : 0) * H + h;  // (no branch)
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            x = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[m][w], mb[w], x, 0, 0, 0);
-          // The largest over each row's group; x[j] is row 4 g + j of the operand.
-          constexpr int N = GP == 1 ? 4 : GP == 2 ? 2 : 1;  // rows of the tile a lane has
-          if constexpr (GP >= 2) x[0] = max(x[0], x[1]), x[2] = max(x[2], x[3]);
-          if constexpr (GP == 2) x[1] = x[2];
-          if constexpr (GP >= 4) x[0] = max(x[0], x[2]);
-          if constexpr (GP >= 8) x[0] = max(x[0], __shfl_xor(x[0], 16));
-          if constexpr (GP >= 16) x[0] = max(x[0], __shfl_xor(x[0], 32));
-          const int i0 = chunks > 1 ? 0 : m * TP + (GP == 1 ? 4 * g : GP == 2 ? 2 * g
-                                                    : GP == 4 ? g : GP == 8 ? g / 2 : 0);
-          const bool mine = GP <= 4 || (GP == 8 ? (g & 1) == 0 : g == 0);
+          for (int w = 0; w < W; ++w) mb[k][w] = *(const v4i*)(a.mean + ph * D + 64 * w + 16 * g);
+          scale[k] = a.scale[ph] | (there ? 0 : 255);
+        }
+        ids(p0 + kThreads / 64 * 16 * Q, id);
+        // (Bounds only where a tile has fewer rows or the last pages are at hand.)
+        const bool whole = nt >= M * TP && p0 + 16 * Q <= most;
+        const auto score = [&](auto checked) {
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
-            if (!mine || i0 + n >= nt || p >= most) continue;
-            int key = scale == 255 ? kLow : key_of(x[n], scale);
-            int* to = &keys[(i0 + n) * a.width + p];
-            // (One lane has all of a page's chunks, in turn.)
-            if (chunks > 1 && (c + m > 0)) key = max(key, *to);
-            *to = key;
+          for (int k = 0; k < Q; ++k) {
+            const int p = p0 + 16 * k + col, scale20 = scale[k] << 20;
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+              v4i x = {};
+#pragma unroll
+              for (int w = 0; w < W; ++w)
+                x = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[m][w], mb[k][w], x, 0, 0, 0);
+              // The largest over each row's group; x[j] is row 4 g + j of the operand.
+              constexpr int N = GP == 1 ? 4 : GP == 2 ? 2 : 1;  // rows of the tile a lane has
+              if constexpr (GP >= 2) x[0] = max(x[0], x[1]), x[2] = max(x[2], x[3]);
+              if constexpr (GP == 2) x[1] = x[2];
+              if constexpr (GP >= 4) x[0] = max(x[0], x[2]);
+              if constexpr (GP >= 8) x[0] = max(x[0], __shfl_xor(x[0], 16));
+              if constexpr (GP >= 16) x[0] = max(x[0], __shfl_xor(x[0], 32));
+              const int i0 = chunks > 1 ? 0 : m * TP + (GP == 1 ? 4 * g : GP == 2 ? 2 * g
+                                                        : GP == 4 ? g : GP == 8 ? g / 2 : 0);
+              // (Lanes that have the same row write the same.)
+#pragma unroll
+              for (int n = 0; n < N; ++n) {
+                int key = scale[k] == 255 ? kLow : key_of(x[n], scale20);
+                int* to = &keys[(i0 + n) * a.width + p];
+                if (checked && (i0 + n >= nt || p >= most)) continue;
+                // (One lane has all of a page's chunks, in turn.)
+                if (chunks > 1 && (c + m > 0)) key = max(key, *to);
+                *to = key;
+              }
+            }
           }
-        }
+        };
+        if (chunks == 1 && whole)
+          score(std::false_type{});
+        else
+          score(std::true_type{});
       }
     }
     __syncthreads();
   }
-  const auto write = [&](int i, int first, int step, bool together) {
+  const auto list = [&](int i, int first, int step, auto choice) {
     const int v = seen(i);
     int32_t* out = a.out + ((int64_t)(s.rows.lo + t0 + i) * H + h) * a.top;
-    if (v <= a.top)
+    if (v <= a.top) {
       for (int c = first; c < a.top; c += step) out[c] = c < v ? c : -1;
-    else if (together)
-      pick<4>(a, keys + i * a.width, v, wave, told, out);
-    else
-      pick<1>(a, keys + i * a.width, v, 0, told, out);
+      return;
+    }
+    for (int c = first; c < a.first; c += step) out[c] = c;
+    for (int c = first; c < a.recent; c += step) out[a.top - a.recent + c] = v - a.recent + c;
+    if (need > 0)
+      choice(keys + i * a.width + a.first, v - a.first - a.recent,
+             [&](int place, int rank) { out[a.first + rank] = a.first + place; });
   };
-  if (nt == 1)
-    write(0, threadIdx.x, kThreads, true);
-  else
-    for (int i = wave; i < nt; i += kThreads / 64) write(i, lane, 64, false);
+  if (nt == 1) {
+    list(0, threadIdx.x, kThreads, [&](const int* k, int n, auto emit) {
+      choose_alone(k, n, need, wave, sieve, emit);
+    });
+    return;
+  }
+  for (int i = wave; i < nt; i += kThreads / 64)
+    list(i, lane, 64, [&](const int* k, int n, auto emit) {
+      if (most <= 128)
+        choose<2>(k, n, need, emit);
+      else if (most <= 512)
+        choose<8>(k, n, need, emit);
+      else
+        choose<16>(k, n, need, emit);
+    });
 }
 
 constexpr int kLds = 64 << 10;          // of keys, at which two workgroups share a CU
 constexpr int kMaxColumns = 32 << 10;   // one row's keys: 128 KB
 
 template <int D, int GP>
-void launch_select(SelectArgs& a, int grid, bool many, int lds, hipStream_t st) {
+void launch_select(const SelectArgs& a, int grid, bool many, bool f16, int lds, hipStream_t st) {
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, a);
+  };
   if (many)
-    hipLaunchKernelGGL((select_kernel<D, GP, 4>), dim3(grid), dim3(kThreads), lds, st, a);
-  else
-    hipLaunchKernelGGL((select_kernel<D, GP, 1>), dim3(grid), dim3(kThreads), lds, st, a);
+    f16 ? run(select_kernel<D, GP, 4, true>) : run(select_kernel<D, GP, 4, false>);
+  else if (a.c.table_pages <= 256)
+    f16 ? run(select_kernel<D, GP, 1, true>) : run(select_kernel<D, GP, 1, false>);
+  else  // two rounds of memory fewer on the way through many pages
+    f16 ? run(select_kernel<D, GP, 1, true, 8>) : run(select_kernel<D, GP, 1, false, 8>);
 }
 
 template <int D>
-void launch_select(SelectArgs& a, int gp, int grid, bool many, int lds, hipStream_t st) {
+void launch_select(const SelectArgs& a, int gp, int grid, bool many, bool f16, int lds,
+                   hipStream_t st) {
   switch (gp) {
-    case 1: return launch_select<D, 1>(a, grid, many, lds, st);
-    case 2: return launch_select<D, 2>(a, grid, many, lds, st);
-    case 4: return launch_select<D, 4>(a, grid, many, lds, st);
-    case 8: return launch_select<D, 8>(a, grid, many, lds, st);
-    default: return launch_select<D, 16>(a, grid, many, lds, st);
+    case 1: return launch_select<D, 1>(a, grid, many, f16, lds, st);
+    case 2: return launch_select<D, 2>(a, grid, many, f16, lds, st);
+    case 4: return launch_select<D, 4>(a, grid, many, f16, lds, st);
+    case 8: return launch_select<D, 8>(a, grid, many, f16, lds, st);
+    default: return launch_select<D, 16>(a, grid, many, f16, lds, st);
   }
 }
 
@@ -502,7 +658,7 @@ extern "C" int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean,
   a.q = (const uint16_t*)q, a.q_ts = q_tok_stride, a.q_hs = q_head_stride;
   a.out = columns;
   a.T = (int)T, a.group = (int)(q_heads / cache->heads);
-  a.top = (int)top, a.first = (int)first, a.recent = (int)recent, a.f16 = dtype == FVSR_DT_F16;
+  a.top = (int)top, a.first = (int)first, a.recent = (int)recent;
   // (Widths that are odd keep rows' keys off one another's banks.)
   a.width = (int)cache->table_pages | 1;
   int gp = 1;
@@ -516,11 +672,17 @@ extern "C" int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean,
   const int64_t tiles = cache->cu ? T / a.tt + B + 1 : B * ((each + a.tt - 1) / a.tt);
   if (tiles * cache->heads > kMaxBlocks) return FVSR_EUNSUPPORTED;
   a.tiles = (int)tiles;
-  const int grid = (int)(tiles * cache->heads), lds = a.tt * a.width * 4;
+  const int grid = (int)(tiles * cache->heads);
+  // (Up to 512 keys are read behind a row's, 1024 behind a row that is alone.  Operands change hands
+  // behind a chunked row's keys, or in place of them.)
+  const int operands = many ? 4 * (int)cache->head_dim / 64 * 1024 : 0;
+  const int lds = std::max({(a.tt * a.width + (a.width > 512 ? 1024 : 512)) * 4, (a.width + 1024) * 4,
+                            chunked ? (a.width + 3) / 4 * 16 + operands : operands});
   const hipStream_t st = (hipStream_t)stream;
+  const bool f16 = dtype == FVSR_DT_F16;
   if (cache->head_dim == 128)
-    launch_select<128>(a, gp, grid, many, lds, st);
+    launch_select<128>(a, gp, grid, many, f16, lds, st);
   else
-    launch_select<64>(a, gp, grid, many, lds, st);
+    launch_select<64>(a, gp, grid, many, f16, lds, st);
   return fvsr_launch_status();
 }
