@@ -6,8 +6,14 @@
 // back (the gradient) has -t.  The product and its fraction are in 64 bits, so an angle of
 // position 2^31 is still right to 2^-23 of a turn; sine and cosine are fp32, as is all behind them.
 //
-// Bound by bytes: each value is read and written once.  A thread has eight pairs of one token
-// and turns them in every HS-th head, so that an angle is made once for several heads.
+// Bound by bytes: each value is read and written once.  A thread has two 16-byte pieces of one
+// token, at the same place in both halves of the channels that turn, which is whole pairs in either
+// layout and lets lanes read whole lines.  It turns them in every apart-th head, so that an angle is
+// made once for several heads, with the loads of four heads on their way together.
+//
+// Measured: 16384 rows x 32 + 8 heads of 128 in bf16 72 us (4.6 TB/s; a copy reaches 5.2), a head
+// to a thread 89; 16896 x 24 heads of 128, 64 channels turned, fp32 87 us (4.75 TB/s), with interleaved
+// pieces beside one another 104.
 #include <algorithm>
 
 #include "common.h"
@@ -22,23 +28,24 @@ struct Args {
   const int32_t* positions;
   int64_t pos_batch, threads;
   int S, D, turned, back;
-  int heads, slots, turning, step;  // of both; slots of a head, those that turn; heads' stride
+  int slots, turning, apart;  // slots of a head, those that turn; distance of a thread's heads
   float gain;
 };
 
-template <int DT, int V>
-struct Pack {  // V values of type DT as fp32
+// V channels of a type as fp32: 16 bytes of them, or one.
+template <int V>
+struct Pack {
   float v[V];
 };
 template <int DT, int V>
-FVSR_DEV Pack<DT, V> load(const void* p, int64_t i) {
-  Pack<DT, V> r;
+FVSR_DEV Pack<V> load(const void* p, int64_t i) {
+  Pack<V> r;
   if constexpr (V == 1) {
     r.v[0] = ld_elem(p, DT, i);
   } else if constexpr (DT == FVSR_DT_F32) {
-    const f32x4_t a = *(const f32x4_t*)((const float*)p + i), b = *((const f32x4_t*)((const float*)p + i) + 1);
+    const f32x4_t w = *(const f32x4_t*)((const float*)p + i);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) r.v[k] = a[k], r.v[4 + k] = b[k];
+    for (int k = 0; k < 4; ++k) r.v[k] = w[k];
   } else {
     const u32x4_t w = *(const u32x4_t*)((const uint16_t*)p + i);
 #pragma unroll
@@ -56,13 +63,11 @@ FVSR_DEV Pack<DT, V> load(const void* p, int64_t i) {
   return r;
 }
 template <int DT, int V>
-FVSR_DEV void store(void* p, int64_t i, const Pack<DT, V>& r) {
+FVSR_DEV void store(void* p, int64_t i, const Pack<V>& r) {
   if constexpr (V == 1) {
     st_elem(p, DT, i, r.v[0]);
   } else if constexpr (DT == FVSR_DT_F32) {
-    f32x4_t* to = (f32x4_t*)((float*)p + i);
-    to[0] = f32x4_t{r.v[0], r.v[1], r.v[2], r.v[3]};
-    to[1] = f32x4_t{r.v[4], r.v[5], r.v[6], r.v[7]};
+    *(f32x4_t*)((float*)p + i) = f32x4_t{r.v[0], r.v[1], r.v[2], r.v[3]};
   } else {
     u32x4_t w;
 #pragma unroll
@@ -80,51 +85,76 @@ FVSR_DEV void store(void* p, int64_t i, const Pack<DT, V>& r) {
 
 template <int DT, int V, bool HALF>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(Args a) {
+  constexpr int U = 4;
   const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (at >= a.threads) return;
-  const int slot = (int)(at % a.slots);
-  const int64_t group = at / a.slots;
-  const int h0 = (int)(group % a.step);
-  const int64_t row = group / a.step, b = row / a.S;
-  const int s = (int)(row % a.S);
+  // Slots of a head stand beside one another, then heads, then tokens.
+  const uint32_t each = (uint32_t)(a.slots * a.apart);
+  const int64_t row = at <= 0xffffffff ? (uint32_t)at / each : at / each;
+  const uint32_t rest = (uint32_t)(at - row * each);
+  const int h0 = (int)(rest / (uint32_t)a.slots), slot = (int)(rest % (uint32_t)a.slots);
+  const int64_t b = row <= 0x7fffffff ? (uint32_t)row / (uint32_t)a.S : row / a.S;
+  const int s = (int)(row - b * a.S);
   const bool turns = slot < a.turning;
-  // Channels of the slot: V pairs, or 2 V that are copied (the last slot may have V).
-  const int c0 = !turns ? a.turned + (slot - a.turning) * 2 * V : HALF ? slot * V : slot * 2 * V;
-  const int c1 = turns && HALF ? c0 + a.turned / 2 : c0 + V;
+  // The slot's two pieces.  (One channel each: interleaved neighbours.)
+  const bool side = V == 1 && !HALF;
+  const int part = turns ? slot : slot - a.turning, base = turns ? 0 : a.turned;
+  const int c0 = turns && side ? 2 * slot : base + part * V;
+  const int c1 = turns && side ? c0 + 1 : c0 + (turns ? a.turning : a.slots - a.turning) * V;
   const bool both = c1 < a.D;
   float cs[V], sn[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
   if (turns) {
     const double pos = a.positions ? a.positions[b * a.pos_batch + s] : s;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      double t = pos * a.turns[slot * V + i];
+      // Pair i of the slot: (p[i], q[i]), or neighbours in p, then in q.
+      const int pair = HALF || V == 1 ? slot * V + i
+                                      : slot * (V / 2) + i % (V / 2) +
+                                            (i < V / 2 ? 0 : a.turning * (V / 2));
+      double t = pos * a.turns[pair];
       t -= __builtin_rint(t);
       float y, x;
       sincospif((float)(t + t), &y, &x);
       cs[i] = x * a.gain, sn[i] = (a.back ? -y : y) * a.gain;
     }
   }
-  for (int h = h0; h < a.heads; h += a.step) {
-    const bool k = h >= a.x[0].heads;
-    const fvsr_rotary_rows& x = a.x[k];
-    const int64_t hh = h - (k ? a.x[0].heads : 0);
-    const int64_t from = b * x.x_batch + s * x.x_tok + hh * x.x_head;
-    const int64_t to = (row * x.heads + hh) * a.D;
-    Pack<DT, V> p = load<DT, V>(x.x, from + c0), q = p;
-    if (both) q = load<DT, V>(x.x, from + c1);
-    if (turns) {
-      // Pairs (p[i], q[i]), or neighbours in p, then in q.
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float& u = HALF || V == 1 ? p.v[i] : i < V / 2 ? p.v[2 * i] : q.v[2 * i - V];
-        float& v = HALF || V == 1 ? q.v[i] : i < V / 2 ? p.v[2 * i + 1] : q.v[2 * i + 1 - V];
-        const float u0 = u;
-        u = u0 * cs[i] - v * sn[i];
-        v = u0 * sn[i] + v * cs[i];
+  for (int n = 0; n < 2; ++n) {
+    const fvsr_rotary_rows& x = a.x[n];
+    const int heads = (int)x.heads;
+    const int64_t from = b * x.x_batch + s * x.x_tok, to = row * heads * a.D;
+    for (int h1 = h0; h1 < heads; h1 += U * a.apart) {
+      Pack<V> p[U], q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h1 + u * a.apart;
+        if (h >= heads) continue;
+        p[u] = load<DT, V>(x.x, from + h * x.x_head + c0);
+        q[u] = p[u];
+        if (both) q[u] = load<DT, V>(x.x, from + h * x.x_head + c1);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h1 + u * a.apart;
+        if (h >= heads) continue;
+        if (turns) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float& f = HALF || V == 1 ? p[u].v[i] : i < V / 2 ? p[u].v[2 * i] : q[u].v[2 * i - V];
+            float& g = HALF || V == 1 ? q[u].v[i]
+                       : i < V / 2    ? p[u].v[2 * i + 1]
+                                      : q[u].v[2 * i + 1 - V];
+            const float f0 = f;
+            f = f0 * cs[i] - g * sn[i];
+            g = f0 * sn[i] + g * cs[i];
+          }
+        }
+        store<DT, V>(x.y, to + (int64_t)h * a.D + c0, p[u]);
+        if (both) store<DT, V>(x.y, to + (int64_t)h * a.D + c1, q[u]);
       }
     }
-    store<DT, V>(x.y, to + c0, p);
-    if (both) store<DT, V>(x.y, to + c1, q);
   }
 }
 
@@ -138,7 +168,7 @@ void launch(const Args& a, bool half, hipStream_t st) {
 }
 template <int DT>
 void launch(const Args& a, bool vec, bool half, hipStream_t st) {
-  vec ? launch<DT, 8>(a, half, st) : launch<DT, 1>(a, half, st);
+  vec ? launch<DT, DT == FVSR_DT_F32 ? 4 : 8>(a, half, st) : launch<DT, 1>(a, half, st);
 }
 
 }  // namespace
@@ -156,7 +186,7 @@ extern "C" int fvsr_rotary(const fvsr_rotary_rows* q, const fvsr_rotary_rows* k,
   a.x[0] = *q;
   if (k) a.x[1] = *k;
   const int64_t rows = batch * tokens, size = dtype == FVSR_DT_F32 ? 4 : 2;
-  bool vec = turned % 16 == 0 && head_dim % 8 == 0;
+  bool vec = turned % (32 / size) == 0 && head_dim % (16 / size) == 0;
   for (const fvsr_rotary_rows& x : a.x) {
     if (x.heads < 0 || x.heads > (1 << 24)) return FVSR_EINVAL;
     if (x.heads == 0 || rows == 0) continue;
@@ -165,18 +195,20 @@ extern "C" int fvsr_rotary(const fvsr_rotary_rows* q, const fvsr_rotary_rows* k,
     vec = vec && !(((uintptr_t)x.x | (uintptr_t)x.y | (uint64_t)(x.x_batch * size) |
                     (uint64_t)(x.x_tok * size) | (uint64_t)(x.x_head * size)) & 15);
   }
-  a.heads = (int)(a.x[0].heads + a.x[1].heads);
-  if (rows == 0 || a.heads == 0) return FVSR_OK;
+  const int64_t heads = std::max(a.x[0].heads, a.x[1].heads);
+  if (rows == 0 || heads == 0) return FVSR_OK;
   if (turned && (!turns || ((uintptr_t)turns & 7))) return FVSR_EINVAL;
-  const int V = vec ? 8 : 1;
+  const int V = vec ? (int)(16 / size) : 1;
   a.turns = turns, a.positions = positions, a.pos_batch = pos_batch_stride;
   a.S = (int)tokens, a.D = (int)head_dim, a.turned = (int)turned, a.back = back != 0;
   a.turning = (int)(turned / 2 / V);
   a.slots = a.turning + (int)((head_dim - turned + 2 * V - 1) / (2 * V));
   a.gain = gain;
-  a.step = a.heads;
-  if (rows > ((int64_t)1 << 40) / a.slots / a.heads) return FVSR_EUNSUPPORTED;
-  a.threads = rows * a.slots * a.step;
+  if (rows > ((int64_t)1 << 40) / a.slots / heads) return FVSR_EUNSUPPORTED;
+  // Heads of a thread: as many as leave 2^19 threads, two thirds of what the CUs hold, at most 8.
+  const int64_t of = std::min<int64_t>(8, std::max<int64_t>(1, rows * a.slots * heads >> 19));
+  a.apart = (int)((heads + of - 1) / of);
+  a.threads = rows * a.slots * a.apart;
   if (a.threads > kThreads * (int64_t)0xffffff) return FVSR_EUNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   const bool half = pairs == FVSR_PAIRS_HALF;
