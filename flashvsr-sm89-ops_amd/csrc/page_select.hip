@@ -663,7 +663,8 @@ extern "C" int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean,
   a.width = (int)cache->table_pages | 1;
   int gp = 1;
   while (gp < a.group && gp < 16) gp *= 2;
-  const int64_t B = cache->sequences, each = cache->cu ? T : T / B;
+  // Rows of a sequence at most.
+  const int64_t B = cache->sequences, each = cache->cu ? (T > B ? T : 1) : T / B;
   const int64_t fit = std::max<int64_t>(1, kLds / (a.width * 4)), tp = 16 / gp;
   // Four operands of rows share a page's means where there are rows for them and room
   // for their keys.

@@ -117,9 +117,9 @@ def select_pages(q: torch.Tensor, means: PageMeans, page_table: torch.Tensor,
     if dt == _lib.DT_F32:
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
     top, first, recent = int(top), int(first), int(recent)
-    _check(first >= 0 and recent >= 1 and top >= first + recent,
+    _check(first >= 0 and recent >= 1 and first + recent <= top < 1 << 24,
            f"{name}: top {top}, first {first}, recent {recent} (recent at least 1, top at least "
-           "first + recent)")
+           "first + recent and below 2^24)")
     B, P = page_table.shape
     _check(P <= 32768, f"{name}: {P} table columns, 32768 at most")
     _one_device(name, q, *means, page_table, lengths, cu_tokens)

@@ -192,6 +192,16 @@ def test_select_rows(Hq, H, packed):
     check_select(q, random_means(N, H, D), table, lengths, 6, 1, 1, starts(new) if packed else None)
 
 
+@pytest.mark.parametrize("B", [1, 9, 80])
+def test_select_packed_tokens(B):
+    """A token for each of many sequences, packed; some without one, and rows behind the last."""
+    lengths = [(577 * b) % 4000 + 1 for b in range(B)]
+    new = [int(b % 5 != 3) for b in range(B)]
+    table, N = tables(lengths, seed=B)
+    q = torch.randn(B, 4, 64, generator=gen(B)).bfloat16()
+    check_select(q, random_means(N, 2, 64), table, lengths, 7, 1, 1, starts(new))
+
+
 @pytest.mark.parametrize("top,first,recent", [(1, 0, 1), (4, 3, 1), (4, 0, 4), (9, 0, 1), (40, 8, 7),
                                               (200, 1, 1)])
 @pytest.mark.parametrize("n", [1, 21])
@@ -379,6 +389,84 @@ def test_attention_counts(T, Hq, H, D, n, dtype):
                              sm_scale=math.log(2))
     want = S.counted(T, Hq, H, D, table, lengths, cols, most=3)
     assert O.counts_agree(out.cpu(), want)
+
+
+@pytest.mark.parametrize("T,Hq,H,D,dtype", [(5, 4, 1, 64, BF), (30, 10, 2, 128, FP),
+                                            (400, 8, 8, 64, FP), (800, 8, 4, 128, BF)])
+def test_attention_neighbours_of_non_finite_queries(T, Hq, H, D, dtype):
+    """A query with a NaN or an infinity is NaN; the rows and heads beside it are not."""
+    from flashvsr_sm89_ops import selected_attention
+    lengths = [T + 400]
+    table, N = tables(lengths, seed=1)
+    pages = pool(N, H, D, seed=2)
+    cols = random_columns(T, H, 3, lengths, [T], seed=4)
+    q = torch.randn(T, Hq, D, generator=gen(3)).to(dtype)
+    q[1, 0, 3], q[4, Hq - 1, 9] = math.nan, math.inf
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV))
+    bad = torch.isnan(out.cpu()).any(-1)
+    assert bool(bad[1, 0]) and bool(bad[4, Hq - 1]) and int(bad.sum()) == 2
+    rows = torch.cat([torch.arange(5), torch.arange(5, T, 29)])  # (the definition is slow)
+    want, size, logit = S.attended(q, O.from_pages(*pages), table, lengths, torch.where(
+        torch.isin(torch.arange(T), rows)[:, None, None], cols, -1))
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12 + 2.0 ** -11 * logit[..., None]) * size
+    fine = ((out.cpu().double() - want).abs() <= tol + 1e-30) | torch.isnan(want)
+    assert bool(fine[rows].all())
+
+
+@pytest.mark.parametrize("T,Hq,H,D,dtype", [(1, 4, 2, 64, BF), (7, 4, 2, 128, FP), (650, 8, 8, 64, BF)])
+def test_attention_far_logits(T, Hq, H, D, dtype):
+    """Logits up to hundreds, growing from page to page, and rows whose first page comes late: the
+    reference of a row moves while its neighbours' stay.  One channel alone is not zero, so that
+    a logit is a single product and exact; its weight then has the weights' bound alone."""
+    from flashvsr_sm89_ops import selected_attention
+    P = 12
+    lengths = [max(P * 128 - 5, T + 900)]
+    P = -(-lengths[0] // 128)
+    table, N = tables(lengths, seed=1)
+    pages = pool(N, H, D, seed=2)
+    k = torch.zeros(N, H, 128, D)
+    for j in range(P):
+        k[int(table[0, j]), :, :, 0] = float(2 ** (j % 9)) * (-1) ** (j // 9)
+    pages.k.copy_(k.to(torch.float8_e4m3fn))
+    pages.k_scale.view(torch.uint8).fill_(127)
+    q = torch.zeros(T, Hq, D, dtype=dtype)
+    q[..., 0] = torch.tensor([1.0, 2.5, -1.75, 0.25])[torch.arange(T * Hq) % 4].reshape(T, Hq).to(dtype)
+    cols = random_columns(T, H, 4, lengths, [T], seed=4)
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV),
+                             sm_scale=1.0)
+    rows = torch.arange(0, T, 1 if T < 20 else 31)
+    keep = torch.isin(torch.arange(T), rows)[:, None, None]
+    want, size, _ = S.attended(q, O.from_pages(*pages), table, lengths, torch.where(keep, cols, -1),
+                               sm_scale=1.0)
+    # exp2 of a logit in log2 units: its product's fp32 rounding, 2^-24 * 1000 of them, is 2^-14
+    # of a weight, twice that of a quotient.
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -8 + 2.0 ** -12 + 2.0 ** -13) * size
+    assert bool(((out.cpu().double() - want).abs() <= tol + 1e-30)[rows].all())
+
+
+@pytest.mark.parametrize("Hq,H,D,dtype", [(8, 8, 64, BF), (8, 4, 128, FP)])
+def test_attention_many_packed_rows(Hq, H, D, dtype):
+    """Packed chunks and single tokens in one call, a wave to a unit; rows behind the last
+    sequence are zeros, or left alone in `out`."""
+    from flashvsr_sm89_ops import KVPages, selected_attention
+    new, lengths = [300, 0, 1, 417, 2], [300, 128, 900, 1300, 2]
+    T = sum(new) + 3
+    columns = 11
+    table = torch.arange(5 * columns).reshape(5, columns).int()
+    k, v, ks, vs = O.counting_pool(5 * columns, H, D, table, most=3)
+    e4 = torch.float8_e4m3fn
+    pages = KVPages(k.to(DEV).view(e4), v.to(DEV).view(e4), ks.to(DEV).view(E8), vs.to(DEV).view(E8))
+    q = torch.zeros(T, Hq, D, dtype=dtype)
+    q[..., 0] = 1
+    cols = random_columns(T, H, 4, lengths, new, seed=1)
+    args = (q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV), starts(new).to(DEV))
+    out = selected_attention(*args, sm_scale=math.log(2))
+    want = S.counted(T, Hq, H, D, table, lengths, cols, starts(new), most=3)
+    assert O.counts_agree(out.cpu(), want)
+    assert bool((out[-3:] == 0).all())
+    given = torch.full_like(out, 7.0)
+    selected_attention(*args, sm_scale=math.log(2), out=given)
+    assert torch.equal(given[:-3], out[:-3]) and bool((given[-3:] == 7).all())
 
 
 @pytest.mark.parametrize("T", [1, 700])
@@ -577,6 +665,61 @@ def test_graph_and_stream():
         torch.cuda.synchronize()
         for u, v in zip((*want, *a[0], *a[1]), (*got, *b[0], *b[1])):
             assert torch.equal(u.view(torch.uint8), v.view(torch.uint8)), i
+
+
+def test_graph_of_a_chunk():
+    """A chunk's pooling, choice and attention captured, replayed as lengths and pages change."""
+    from flashvsr_sm89_ops import page_means, pool_pages, select_pages, selected_attention
+    H, Hq, D, T = 8, 8, 64, 700
+    table, N = tables([3000])
+    pages = pool(N, H, D)
+    means, t = page_means(pages), table.to(DEV)
+    n = i32([2000]).to(DEV)
+    q = torch.randn(T, Hq, D, device=DEV).half()
+
+    def step():
+        pool_pages(means, pages, t, n)
+        cols = select_pages(q, means, t, n, top=5)
+        return cols, selected_attention(q, pages, t, n, cols)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for i, length in enumerate((2000, 2500, 701, 3000)):
+        n.fill_(length)
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got_now = [x.clone() for x in got]
+        assert all(torch.equal(a, b) for a, b in zip(step(), got_now)), i
+
+
+def test_two_streams():
+    """Calls on two streams at once, each with pieces of its own, give what they give alone."""
+    from flashvsr_sm89_ops import select_pages, selected_attention
+    H, Hq, D = 2, 8, 128
+    table, N = tables([9000, 8000])
+    pages, means = pool(N, H, D), random_means(N, H, D)
+    t, n = table.to(DEV), i32([9000, 8000]).to(DEV)
+    qs = [torch.randn(2, Hq, D, generator=gen(i)).bfloat16().to(DEV) for i in range(2)]
+
+    def step(q):
+        cols = select_pages(q, means, t, n, top=40)
+        return selected_attention(q, pages, t, n, cols)
+    want = [step(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[] for _ in qs]
+    for _ in range(10):
+        for s, q, g in zip(streams, qs, got):
+            with torch.cuda.stream(s):
+                g.append(step(q))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
 
 
 def test_native_and_general_path(monkeypatch):

@@ -249,3 +249,16 @@ def test_on_another_stream():
         out = rotary(y, None, f)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, want)
+
+
+def test_offsets_past_32_bits():
+    """2.2e9 values: rows at the end against the same rows alone."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(128))
+    T, H = 70000, 250
+    x = torch.zeros(T, H, 128, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, H, 128, device=DEV)
+    pos = torch.arange(T, dtype=torch.int32, device=DEV)
+    out = rotary(x, None, f, pos)
+    assert torch.equal(out[-3:], rotary(x[-3:].clone(), None, f, pos[-3:]))
+    assert not bool(out[:5].any())

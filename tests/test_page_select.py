@@ -125,6 +125,7 @@ def test_pool_refuses(change, error):
     (dict(recent=0), ValueError),
     (dict(first=-1), ValueError),
     (dict(first=3), ValueError),
+    (dict(top=1 << 24), ValueError),      # refused before the list is allocated
     (dict(page_table=z(2, 32769, dtype=I32)), ValueError),
 ])
 def test_select_refuses(change, error):
