@@ -28,7 +28,9 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
 
 #include "../../include/fvsr.h"
 
@@ -488,8 +490,82 @@ PyObject* selected_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// rotary(q, k | None, freqs, positions | None, pairs): q or (q, k) turned, or None; a call
-// that is recorded for a gradient goes by the general path.
+// x [.., tokens, heads, channels], three or four dims, channels at unit stride, turned in a new
+// tensor; the second of two may be undefined.  Throws where the library refuses.
+struct Turn {
+  at::Tensor turns, positions;  // (none: undefined)
+  double gain;
+  bool half, back;
+
+  int run(const at::Tensor (&x)[2], at::Tensor (&y)[2]) const {
+    const int64_t d = x[0].dim(), S = x[0].size(d - 3), D = x[0].size(d - 1);
+    fvsr_rotary_rows rows[2] = {};
+    for (int i = 0; i < 2; ++i) {
+      if (!x[i].defined()) continue;
+      y[i] = at::empty(x[i].sizes(), x[i].options());
+      rows[i] = fvsr_rotary_rows{x[i].data_ptr(), y[i].data_ptr(), x[i].size(d - 2),
+                                 d == 4 ? x[i].stride(0) : 0, x[i].stride(d - 3),
+                                 x[i].stride(d - 2)};
+    }
+    return selected.rotary(
+        &rows[0], x[1].defined() ? &rows[1] : nullptr, dtype_code(x[0]),
+        d == 4 ? x[0].size(0) : 1, S, D, 2 * turns.size(0), (const double*)turns.data_ptr(),
+        positions.defined() ? (const int32_t*)positions.data_ptr() : nullptr,
+        positions.defined() && positions.dim() == 2 ? positions.stride(0) : 0, (float)gain,
+        half ? FVSR_PAIRS_HALF : FVSR_PAIRS_INTERLEAVED, back, stream_of(x[0]));
+  }
+};
+
+// The same as a node of a graph.  Its gradient is the rotation back, a node again where a
+// graph of the gradient is asked for.
+struct TurnNode : torch::autograd::Function<TurnNode> {
+  using List = torch::autograd::variable_list;
+  using MaybeTensor = std::optional<at::Tensor>;  // (an undefined tensor is no argument here)
+  static MaybeTensor maybe(const at::Tensor& t) {
+    return t.defined() ? MaybeTensor(t) : std::nullopt;
+  }
+  static List forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                      const MaybeTensor& k, const at::Tensor& turns, const MaybeTensor& positions,
+                      double gain, bool half, bool back) {
+    const at::Tensor pos = positions ? *positions : at::Tensor();
+    const Turn t{turns, pos, gain, half, back};
+    const at::Tensor x[2] = {q, k ? *k : at::Tensor()};
+    at::Tensor y[2];
+    const int rc = t.run(x, y);
+    TORCH_CHECK(rc == FVSR_OK, "rotary failed: ",
+                rc == FVSR_EHIP ? "HIP launch error" : "unsupported shape/stride/alignment",
+                " (status ", rc, ")");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({turns, pos});
+    ctx->saved_data["gain"] = gain;
+    ctx->saved_data["half"] = half;
+    ctx->saved_data["back"] = back;
+    if (!k) return {y[0]};
+    return {y[0], y[1]};
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, List grads) {
+    const auto saved = ctx->get_saved_variables();
+    List out(7);
+    at::Tensor x[2];
+    int at[2], n = 0;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined()) {
+        const at::Tensor& g = grads[i];
+        at[n] = (int)i;
+        // (A gradient may be one value spread over a shape.)
+        x[n++] = g.stride(-1) == 1 || g.size(-1) == 1 ? g : g.contiguous();
+      }
+    if (n == 0) return out;
+    const c10::DeviceGuard guard(x[0].device());
+    const List r = apply(x[0], maybe(x[1]), saved[0], maybe(saved[1]),
+                         ctx->saved_data["gain"].toDouble(), ctx->saved_data["half"].toBool(),
+                         !ctx->saved_data["back"].toBool());
+    for (int i = 0; i < n; ++i) out[at[i]] = r[i];
+    return out;
+  }
+};
+
+// rotary(q, k | None, freqs, positions | None, pairs): q or (q, k) turned, or None
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 5 || !selected.rotary) Py_RETURN_NONE;
@@ -498,8 +574,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Device dev = q->device();
   const int64_t d = q->dim(), D = q->size(d - 1), S = q->size(d - 3);
   const int64_t B = d == 4 ? q->size(0) : 1;
-  const int dt = dtype_code(*q);
-  if (dt < 0 || !is_current(dev) || !optional_on(args[1], dev, k) ||
+  if (dtype_code(*q) < 0 || !is_current(dev) || !optional_on(args[1], dev, k) ||
       !optional_on(args[3], dev, pos) || !PyTuple_Check(args[2]) ||
       PyTuple_GET_SIZE(args[2]) != 2 || !PyUnicode_Check(args[4]))
     Py_RETURN_NONE;
@@ -519,33 +594,32 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
         pos->size(e - 1) != S || pos->stride(e - 1) != 1)
       Py_RETURN_NONE;
   }
-  if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad())))
-    Py_RETURN_NONE;
   const bool half = PyUnicode_CompareWithASCIIString(args[4], "half") == 0;
   if (!half && PyUnicode_CompareWithASCIIString(args[4], "interleaved") != 0) Py_RETURN_NONE;
   const double gain = PyFloat_AsDouble(PyTuple_GET_ITEM(args[2], 1));
   if (gain == -1.0 && PyErr_Occurred()) return nullptr;
   if (modes_active()) Py_RETURN_NONE;
-  const auto rows = [d](const at::Tensor& x, const at::Tensor& y) {
-    return fvsr_rotary_rows{x.data_ptr(), y.data_ptr(),    x.size(d - 2), d == 4 ? x.stride(0) : 0,
-                            x.stride(d - 3), x.stride(d - 2)};
-  };
-  at::Tensor yq = at::empty(q->sizes(), q->options()), yk;
-  if (k) yk = at::empty(k->sizes(), k->options());
-  const fvsr_rotary_rows rq = rows(*q, yq), rk = k ? rows(*k, yk) : fvsr_rotary_rows{};
-  void* st = stream_of(*q);
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = selected.rotary(&rq, k ? &rk : nullptr, dt, B, S, D, 2 * turns->size(0),
-                       (const double*)turns->data_ptr(),
-                       pos ? (const int32_t*)pos->data_ptr() : nullptr,
-                       pos && pos->dim() == 2 ? pos->stride(0) : 0, (float)gain,
-                       half ? FVSR_PAIRS_HALF : FVSR_PAIRS_INTERLEAVED, 0, st);
-  Py_END_ALLOW_THREADS
-  if (rc != FVSR_OK) return not_done(rc, "rotary");
-  PyObject* qo = THPVariable_Wrap(std::move(yq));
+  at::Tensor x[2] = {*q, k ? *k : at::Tensor()}, y[2];
+  if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
+    TurnNode::List r;
+    {
+      pybind11::gil_scoped_release release;
+      r = TurnNode::apply(x[0], TurnNode::maybe(x[1]), *turns,
+                          pos ? TurnNode::MaybeTensor(*pos) : std::nullopt, gain, half, false);
+    }
+    y[0] = r[0];
+    if (k) y[1] = r[1];
+  } else {
+    const Turn t{*turns, pos ? *pos : at::Tensor(), gain, half, false};
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = t.run(x, y);
+    Py_END_ALLOW_THREADS
+    if (rc != FVSR_OK) return not_done(rc, "rotary");
+  }
+  PyObject* qo = THPVariable_Wrap(std::move(y[0]));
   if (!k || !qo) return qo;
-  PyObject* ko = THPVariable_Wrap(std::move(yk));
+  PyObject* ko = THPVariable_Wrap(std::move(y[1]));
   PyObject* r = ko ? PyTuple_Pack(2, qo, ko) : nullptr;
   Py_DECREF(qo);
   Py_XDECREF(ko);

@@ -155,7 +155,7 @@ struct SelectArgs {
   const uint16_t* q;
   int64_t q_ts, q_hs;
   int32_t* out;
-  int T, group, top, first, recent;
+  int T, group, top, first, recent, f16;
   int tt, tiles, width;  // rows of a tile; tiles of all sequences; keys of a row in LDS
 };
 
@@ -326,7 +326,7 @@ FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s,
   }
   at = __builtin_amdgcn_readfirstlane(at), total = __builtin_amdgcn_readfirstlane(total);
   if (total > kLeft) {  // (more than a wave's lanes are wanted, or many tie)
-    if (wave == 0) choose<16>(keys, n, need, emit);
+    if (wave == 0) choose<8>(keys, n, need, emit);
     return;
   }
   for (int i = i0; i < i1 + lane; i += 64) {
@@ -375,7 +375,7 @@ FVSR_DEV float half_to_f(uint32_t h) {
   return __uint_as_float(h << 16);
 }
 
-template <int D, int GP, int M, bool F16, int Q = 4>
+template <int D, int GP, int M, int Q = 4>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   constexpr int W = D / 64;
   constexpr int TP = 16 / GP;  // rows of an operand
@@ -424,7 +424,8 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
         load(0, c, x);
         top_all = max(top_all, Channels<W>::largest(x));
       }
-    const auto operand = [&](int m, int c, v4i(&to)[W]) {
+    const auto operand_of = [&](auto f16, int m, int c, v4i(&to)[W]) {
+      constexpr bool F16 = f16;
       Channels<W> x;
       load(m, c, x);
       uint32_t top = max(top_all, Channels<W>::largest(x));
@@ -459,6 +460,12 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
           const uint32_t hi = __builtin_amdgcn_perm(r[3], r[2], 0x04000c0cu);
           to[w][i] = fine ? (int)(lo | hi) : 0;
         }
+    };
+    const auto operand = [&](int m, int c, v4i(&to)[W]) {
+      if (a.f16)
+        operand_of(std::true_type{}, m, c, to);
+      else
+        operand_of(std::false_type{}, m, c, to);
     };
     if (a.c.pages == 0)  // (a pool without pages)
       for (int i = threadIdx.x; i < nt * a.width; i += kThreads) keys[i] = kLow;
@@ -560,7 +567,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
       choice(keys + i * a.width + a.first, v - a.first - a.recent,
              [&](int place, int rank) { out[a.first + rank] = a.first + place; });
   };
-  if (nt == 1) {
+  if (M == 1 && nt == 1) {
     list(0, threadIdx.x, kThreads, [&](const int* k, int n, auto emit) {
       choose_alone(k, n, need, wave, sieve, emit);
     });
@@ -568,9 +575,9 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   }
   for (int i = wave; i < nt; i += kThreads / 64)
     list(i, lane, 64, [&](const int* k, int n, auto emit) {
-      if (most <= 128)
+      if (M > 1 && most <= 128)
         choose<2>(k, n, need, emit);
-      else if (most <= 512)
+      else if (M == 1 || most <= 512)
         choose<8>(k, n, need, emit);
       else
         choose<16>(k, n, need, emit);
@@ -581,27 +588,27 @@ constexpr int kLds = 64 << 10;          // of keys, at which two workgroups shar
 constexpr int kMaxColumns = 32 << 10;   // one row's keys: 128 KB
 
 template <int D, int GP>
-void launch_select(const SelectArgs& a, int grid, bool many, bool f16, int lds, hipStream_t st) {
+void launch_select(const SelectArgs& a, int grid, bool many, int lds, hipStream_t st) {
   const auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, st, a);
   };
   if (many)
-    f16 ? run(select_kernel<D, GP, 4, true>) : run(select_kernel<D, GP, 4, false>);
+    run(select_kernel<D, GP, 4>);
   else if (a.c.table_pages <= 256)
-    f16 ? run(select_kernel<D, GP, 1, true>) : run(select_kernel<D, GP, 1, false>);
+    run(select_kernel<D, GP, 1>);
   else  // two rounds of memory fewer on the way through many pages
-    f16 ? run(select_kernel<D, GP, 1, true, 8>) : run(select_kernel<D, GP, 1, false, 8>);
+    run(select_kernel<D, GP, 1, 8>);
 }
 
 template <int D>
-void launch_select(const SelectArgs& a, int gp, int grid, bool many, bool f16, int lds,
+void launch_select(const SelectArgs& a, int gp, int grid, bool many, int lds,
                    hipStream_t st) {
   switch (gp) {
-    case 1: return launch_select<D, 1>(a, grid, many, f16, lds, st);
-    case 2: return launch_select<D, 2>(a, grid, many, f16, lds, st);
-    case 4: return launch_select<D, 4>(a, grid, many, f16, lds, st);
-    case 8: return launch_select<D, 8>(a, grid, many, f16, lds, st);
-    default: return launch_select<D, 16>(a, grid, many, f16, lds, st);
+    case 1: return launch_select<D, 1>(a, grid, many, lds, st);
+    case 2: return launch_select<D, 2>(a, grid, many, lds, st);
+    case 4: return launch_select<D, 4>(a, grid, many, lds, st);
+    case 8: return launch_select<D, 8>(a, grid, many, lds, st);
+    default: return launch_select<D, 16>(a, grid, many, lds, st);
   }
 }
 
@@ -659,6 +666,7 @@ extern "C" int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean,
   a.out = columns;
   a.T = (int)T, a.group = (int)(q_heads / cache->heads);
   a.top = (int)top, a.first = (int)first, a.recent = (int)recent;
+  a.f16 = dtype == FVSR_DT_F16;
   // (Widths that are odd keep rows' keys off one another's banks.)
   a.width = (int)cache->table_pages | 1;
   int gp = 1;
@@ -680,10 +688,9 @@ extern "C" int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean,
   const int lds = std::max({(a.tt * a.width + (a.width > 512 ? 1024 : 512)) * 4, (a.width + 1024) * 4,
                             chunked ? (a.width + 3) / 4 * 16 + operands : operands});
   const hipStream_t st = (hipStream_t)stream;
-  const bool f16 = dtype == FVSR_DT_F16;
   if (cache->head_dim == 128)
-    launch_select<128>(a, gp, grid, many, f16, lds, st);
+    launch_select<128>(a, gp, grid, many, lds, st);
   else
-    launch_select<64>(a, gp, grid, many, f16, lds, st);
+    launch_select<64>(a, gp, grid, many, lds, st);
   return fvsr_launch_status();
 }

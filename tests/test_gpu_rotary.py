@@ -137,10 +137,20 @@ def test_nothing():
         assert rotary(torch.empty(shape, device=DEV), None, f).shape == shape
 
 
+@pytest.fixture(params=["native", "general"])
+def path(request, monkeypatch):
+    """Both ways that a call can take on the host."""
+    from flashvsr_sm89_ops import _lib
+    _lib.selected_host()
+    if request.param == "general":
+        monkeypatch.setattr(_lib, "_selected_host", _lib._GeneralPath)
+    return request.param
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pairs", ["half", "interleaved"])
 @pytest.mark.parametrize("D,R", [(128, 128), (64, 32), (24, 20)])
-def test_gradient(dtype, pairs, D, R):
+def test_gradient(dtype, pairs, D, R, path):
     """dq and dk are the rotation back of the gradients, whatever their layout, and q's or k's
     alone where only one is asked for."""
     from flashvsr_sm89_ops import rotary
@@ -163,7 +173,7 @@ def test_gradient(dtype, pairs, D, R):
     assert torch.equal(d4, dk)
 
 
-def test_gradient_of_one_input_and_shared_heads():
+def test_gradient_of_one_input_and_shared_heads(path):
     """k without a gradient; one k spread over heads (a broadcast) gets the sum."""
     from flashvsr_sm89_ops import rotary
     f = on_gpu(freqs_of(64))
@@ -181,7 +191,7 @@ def test_gradient_of_one_input_and_shared_heads():
     assert bool(((d.cpu().double() - want).abs() <= 2.0 ** -20 * g.cpu().abs().sum(1).max()).all())
 
 
-def test_gradient_by_differences():
+def test_gradient_by_differences(path):
     """fp32, the derivative of a random product along a random direction.  The map is linear, so a
     difference over a step of 1 has no error of its own: both sides are sums of 768 products
     that fp32 rounds, 2^-21 of their magnitudes each (the bound above)."""
@@ -197,7 +207,7 @@ def test_gradient_by_differences():
     assert float((slope - (dq.double() * d).sum()).abs()) <= 3 * 2.0 ** -21 * 2 * 1.3 * float(size)
 
 
-def test_second_gradient():
+def test_second_gradient(path):
     from flashvsr_sm89_ops import rotary
     f = on_gpu(freqs_of(64))
     q = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
@@ -208,7 +218,37 @@ def test_second_gradient():
     check(dg[None], w.cpu()[None], freqs_of(64), None, "half")
 
 
-def test_graph_of_forward_and_backward():
+def test_nodes(path):
+    """What a graph holds: no gradient without being asked, outputs of one node, positions changed
+    between the two ways refused, backward on another thread's stream as on the caller's."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    q = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
+    pos = torch.arange(4, dtype=torch.int32, device=DEV)
+    assert not rotary(q.detach(), None, f, pos).requires_grad
+    with torch.no_grad():
+        assert not rotary(q, None, f, pos).requires_grad
+    with torch.inference_mode():
+        rotary(q, None, f, pos)
+    out, k = rotary(q, q.detach(), f, pos)
+    assert out.grad_fn is not None and out.requires_grad and out.is_leaf is False
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out2 = rotary(q, None, f, pos)
+        d2, = torch.autograd.grad(out2, q, torch.ones_like(out2))
+    torch.cuda.current_stream().wait_stream(side)
+    d, = torch.autograd.grad(out, q, torch.ones_like(out), retain_graph=True)
+    assert torch.equal(d, d2)
+    pos += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, q, torch.ones_like(out))
+    empty = torch.empty(0, 2, 64, device=DEV, requires_grad=True)
+    d, = torch.autograd.grad(rotary(empty, None, f).sum(), empty)
+    assert d.shape == empty.shape
+
+
+def test_graph_of_forward_and_backward(path):
     """Captured with leaves of its own, replayed with other inputs between eager steps."""
     from flashvsr_sm89_ops import rotary
     f = on_gpu(freqs_of(128))
