@@ -26,6 +26,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -565,6 +566,15 @@ struct TurnNode : torch::autograd::Function<TurnNode> {
   }
 };
 
+// While a stream captures, a leaf may not have a graph from another stream: the backward pass
+// would wait for that stream inside the capture, which ends the process.
+bool other_graph(const at::Tensor& x) {
+  if (!x.requires_grad() || !x.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
+  const auto at = node ? node->stream() : std::nullopt;
+  return at && at->id() != c10::hip::getCurrentHIPStream(x.device().index()).id();
+}
+
 // rotary(q, k | None, freqs, positions | None, pairs): q or (q, k) turned, or None
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -598,9 +608,15 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!half && PyUnicode_CompareWithASCIIString(args[4], "interleaved") != 0) Py_RETURN_NONE;
   const double gain = PyFloat_AsDouble(PyTuple_GET_ITEM(args[2], 1));
   if (gain == -1.0 && PyErr_Occurred()) return nullptr;
-  if (modes_active()) Py_RETURN_NONE;
+  if (modes_active() || q->_fw_grad(0).defined() || (k && k->_fw_grad(0).defined()))
+    Py_RETURN_NONE;
   at::Tensor x[2] = {*q, k ? *k : at::Tensor()}, y[2];
   if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() ==
+                        c10::hip::CaptureStatus::None ||
+                    !(other_graph(*q) || (k && other_graph(*k))),
+                "rotary: a leaf of a captured step still has a graph from another stream: let "
+                "go of its outputs first, or capture with leaves of its own");
     TurnNode::List r;
     {
       pybind11::gil_scoped_release release;

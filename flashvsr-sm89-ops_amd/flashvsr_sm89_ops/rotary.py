@@ -16,6 +16,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 
@@ -120,7 +121,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
     positions int32, [T] or [S] (the same for all B) or [B, S]; default: 0, 1, ..  Whole turns
     are taken off position * turns in 64 bits; sines, products and sums are fp32, rounded once.
 
-    Differentiable in q and k (any number of times); freqs and positions have no gradient."""
+    Differentiable in q and k (any number of times, backward mode); freqs and positions have no
+    gradient.  A step with its backward pass captures into a graph where its leaves have no
+    graph from another stream left: an earlier step's outputs are let go first."""
     r = (_lib._selected_host or _lib.selected_host()).rotary(q, k, freqs, positions, pairs)
     if r is not None:
         return r
@@ -157,6 +160,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
     _lib.require_gpu(*xs, turns, positions)
     check(all(t is None or t.device == q.device for t in (k, turns, positions)),
           "tensors on several devices")
+    check(all(unpack_dual(x).tangent is None for x in xs), "no forward-mode gradients")
     four = [x if x.dim() == 4 else x[None] for x in xs]
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         ys = _Rotary.apply(turns, float(gain), positions, _PAIRS[pairs], False, *four)

@@ -204,7 +204,7 @@ def test_gradient_by_differences(path):
     dq, = torch.autograd.grad(out, q, w)
     slope = ((rotary(q.detach() + d, None, f, pairs="interleaved") - out.detach()).double() * w).sum()
     size = (w.abs().double() * (q.abs() + d.abs()).double()).sum() + (dq * d).abs().double().sum()
-    assert float((slope - (dq.double() * d).sum()).abs()) <= 3 * 2.0 ** -21 * 2 * 1.3 * float(size)
+    assert float((slope - (dq.double() * d).sum()).detach().abs()) <= 3 * 2.0 ** -21 * 2 * 1.3 * float(size)
 
 
 def test_second_gradient(path):
@@ -275,6 +275,45 @@ def test_graph_of_forward_and_backward(path):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_capture_with_a_live_graph():
+    """Refused before anything is captured; once the outputs are gone the same leaf does."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    q = torch.randn(6, 2, 64, device=DEV, requires_grad=True)
+    g = torch.randn(6, 2, 64, device=DEV)
+    out = rotary(q, None, f)
+    want, = torch.autograd.grad(out, q, g, retain_graph=True)
+    with pytest.raises(RuntimeError, match="graph from another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rotary(q, None, f)
+    with pytest.raises(RuntimeError, match="graph from another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rotary(q.detach(), q, f)
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = rotary(q, q, f)  # (a graph of the same stream is none to refuse)
+        got, = torch.autograd.grad(rotary(q, None, f), q, g)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(first, second)
+
+
+def test_no_forward_mode():
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    q = torch.randn(6, 2, 64, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(ValueError, match="forward-mode"):
+            rotary(dual, None, f)
+        with pytest.raises(ValueError, match="forward-mode"):
+            rotary(q, dual, f)
 
 
 def test_on_another_stream():
