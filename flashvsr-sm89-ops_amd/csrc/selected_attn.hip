@@ -3,8 +3,8 @@
 //   o[q] = sum_k w[k] v[k] / sum_k w[k],  w[k] = exp(sm_scale * q.k) over the tokens up to
 //          q's own position in the pages of its list
 //
-// A list belongs to a row and a key/value head.  Operands, weights and their precision are those
-// of paged_attn.hip: K and V are operand A as stored, q (and in bf16 the weights) sums of e4m3
+// A list belongs to a row and a key/value head.  Operands, bf16 weights and their precision are
+// those of paged_attn.hip: K and V are operand A as stored, q (and in bf16 the weights) sums of e4m3
 // terms.  An operand has 16 query columns; a head's group seldom fills them, so a unit of work is
 // as many rows that follow one another as do, over the pages that any of them lists, each page read
 // and multiplied once.
@@ -127,9 +127,9 @@ FVSR_DEV void join_lists(Lists<N>& l, const Args& a, const Unit& u) {
   __syncthreads();
 }
 
-// Weights of fp16 queries are halves (11 bits): V's codes become halves as well, exactly, 8 of
-// them in 4 instructions, which is less work than a weight's three e4m3 terms and their products (2048
-// rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128: 144 and 152).
+// Weights of fp16 queries are halves (11 bits, 2^-11 of a weight): V's codes become halves as
+// well, exactly, 8 of them in 4 instructions, which is less work than a weight's three e4m3 terms
+// and their products (2048 rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128: 144 and 152).
 FVSR_DEV void halves4(float a, float b, float c, float d, uint32_t (&w)[2], float& sum) {
   const v2h x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
   const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
