@@ -129,7 +129,7 @@ FVSR_DEV void join_lists(Lists<N>& l, const Args& a, const Unit& u) {
 
 // Weights of fp16 queries are halves (11 bits, 2^-11 of a weight): V's codes become halves as
 // well, exactly, 8 of them in 4 instructions, which is less work than a weight's three e4m3 terms
-// and their products (2048 rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128: 144 and 152).
+// and their products (2048 rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128, 119).
 FVSR_DEV void halves4(float a, float b, float c, float d, uint32_t (&w)[2], float& sum) {
   const v2h x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
   const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
@@ -510,11 +510,11 @@ FVSR_DEV void fetch(const uint8_t* to, const uint8_t* from, const int (&off)[4])
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, %5\n\t"
-      "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-      "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-      "global_load_lds_dwordx4 %4, %5 offset:3072"
+      "global_load_lds_dwordx4 %2, %5 offset:%6\n\t"
+      "global_load_lds_dwordx4 %3, %5 offset:%7\n\t"
+      "global_load_lds_dwordx4 %4, %5 offset:%8"
       :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "v"(off[2]),
-      "v"(off[3]), "s"(from) : "memory");
+      "v"(off[3]), "s"(from), "n"(1 << 10), "n"(2 << 10), "n"(3 << 10) : "memory");
 }
 // Until at most N of them are on their way.
 template <int N>
@@ -528,13 +528,19 @@ struct Visit {
 };
 
 template <int DT, int D>
-__global__ __launch_bounds__(64, D == 64 ? 2 : 1) void attend_alone(Args a) {
+__global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
   constexpr int KR = D / 16;                 // pieces of a K row
   constexpr int SEG = kPage * D / 1024;      // of 64 pieces
-  __shared__ __attribute__((aligned(1024))) uint8_t kl[kPage * D], vl[kPage * D];
+  // Codes of 128 dims take one buffer, K and V in turn: two waves to a SIMD, one waiting while the
+  // other works (2048 rows, 32 / 8 heads in bf16, 195 us; a buffer each and one wave 244, but 1024
+  // rows of 12 heads, a unit to a SIMD at most, 126 and 121).  Of 64 dims there is room for both, and
+  // more waves gain nothing (133 us; one buffer, three waves 138).
+  constexpr bool ONE = D == 128;
+  __shared__ __attribute__((aligned(1024))) uint8_t kl[kPage * D * (ONE ? 1 : 2)];
+  uint8_t* const vl = kl + (ONE ? 0 : kPage * D);
   __shared__ Visit visits[kAlone];
-  // The lists lie where K will: eight workgroups (64 dims) or four then share a CU.
-  static_assert(sizeof(Lists<kAlone>) <= sizeof(kl), "lists outgrow K's codes");
+  // The lists lie where K will: eight workgroups then share a CU.
+  static_assert(sizeof(Lists<kAlone>) <= kPage * D, "lists outgrow K's codes");
   Lists<kAlone>& lists = *(Lists<kAlone>*)kl;
   const int lane = threadIdx.x, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
   Unit u;
@@ -618,20 +624,26 @@ __global__ __launch_bounds__(64, D == 64 ? 2 : 1) void attend_alone(Args a) {
   if (n > 0) {
     Visit cur = visit(0);
     fetch_k(cur);
-    fetch_v(cur);
+    if (!ONE) fetch_v(cur);
     for (int i = 0; i < n; ++i) {
       const Visit next = visit(min(i + 1, n - 1));  // (the last one again: no branch)
       const uint32_t what = cur.what;
-      wait_for<SEG>();  // K is there, V may be on its way
+      wait_for<ONE ? 0 : SEG>();  // K is there, V may be on its way
       w.template page<false>(k_tile, v_tile, [&] {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's operands are read
-        fetch_k(next);
+        if constexpr (ONE)
+          fetch_v(cur);
+        else
+          fetch_k(next);
       }, [&] {
-        wait_for<SEG>();  // V is there, the next K may be on its way
+        wait_for<ONE ? 0 : SEG>();  // V is there, the next K may be on its way
       }, what & 255, what >> 8 & 255, (cur.column + 1) * kPage > least, seen_of(cur), g,
           a.scale_log2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V's
-      fetch_v(next);
+      if constexpr (ONE)
+        fetch_k(next);
+      else
+        fetch_v(next);
       cur = next;
     }
     wait_for<0>();  // no load may land in an LDS that the next workgroup has
@@ -693,8 +705,8 @@ Plan plan_selected(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, int64_t t
   cut(kAlone);
   // A wave to a unit where rows of a sequence follow one another (their pages come from the L2)
   // and there are units for the CUs' SIMDs.  (us alone / shared at 256 units 49 / 37, 512 units of
-  // 64 dims 44 / 30, of 128 dims 59 / 63, 768 120 / 156, 1024 50 / 65, 2048 of 64 dims 75 / 106, of 128
-  // 129 / 213.)
+  // 64 dims 44 / 30, of 128 dims 59 / 63, 768 126 / 156, 1024 50 / 65, 2048 of 64 dims 75 / 106, of 128
+  // 104 / 213.)
   p.alone = each > 1 && top <= kAlone && p.units * 2 >= cus * 5;
   if (p.alone) return p;
   cut(kShared);
