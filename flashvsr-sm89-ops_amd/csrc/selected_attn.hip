@@ -608,12 +608,17 @@ __global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
       fetch(vl + s * 1024, from + s * 1024, off);
     }
   };
-  // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4.
+  // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4.  (64 dims stand in
+  // both halves of an operand: they are read twice, which costs less than copies of registers.)
+  const int k_first = 16 * (col >> 2) + (col & 3);
+  int k_again = k_first * D + (g ^ k_swap<D>(k_first)) * 16;
+  asm("" : "+v"(k_again));
   const auto k_tile = [&](int t) {
-    const int key = 64 * (t >> 2) + 16 * (col >> 2) + 4 * (t & 3) + (col & 3);
+    const int key = 64 * (t >> 2) + k_first + 4 * (t & 3);
     const uint8_t* row = kl + key * D;
     const u32x4_t x = *(const u32x4_t*)(row + (g ^ k_swap<D>(key)) * 16);
-    return ::join(x, D == 128 ? *(const u32x4_t*)(row + ((g + 4) ^ k_swap<D>(key)) * 16) : x);
+    return ::join(x, D == 128 ? *(const u32x4_t*)(row + ((g + 4) ^ k_swap<D>(key)) * 16)
+                              : *(const u32x4_t*)(kl + k_again + (key - k_first) * D));
   };
   const auto v_tile = [&](int d) {
     const int dim = d * 16 + col;
