@@ -299,8 +299,12 @@ def test_select_strided_and_nothing():
 # --------------------------------------------------------------------------------------
 
 
-def check_attention(out, q, pages, table, lengths, columns, cu=None, sm_scale=None):
+def check_attention(out, q, pages, table, lengths, columns, cu=None, sm_scale=None, rows=None):
+    """rows: those that are looked at (the definition is slow)."""
     cache = O.from_pages(*pages)
+    if rows is not None:
+        keep = torch.isin(torch.arange(len(columns)), rows)[:, None, None]
+        columns, out = torch.where(keep, columns, -1), torch.where(keep, out.cpu(), 0)
     want, size, logit = S.attended(q, cache, table, lengths, columns, cu, sm_scale)
     dt = q.dtype
     weight = 2.0 ** -8 if dt == BF else 2.0 ** -10
@@ -373,7 +377,8 @@ def test_attention_packed(D, dtype, Hq, H):
 
 @pytest.mark.parametrize("T,Hq,H,D,n,dtype", [
     (1, 2, 2, 128, 300, BF), (1, 4, 1, 64, 64, FP), (3, 8, 2, 128, 40, BF), (600, 8, 8, 64, 5, BF),
-    (1100, 8, 4, 128, 4, FP), (4200, 40, 1, 64, 3, BF)])
+    (1100, 8, 4, 128, 4, FP), (4200, 40, 1, 64, 3, BF), (700, 16, 16, 128, 5, BF),
+    (400, 32, 16, 64, 5, FP), (330, 48, 16, 128, 3, FP), (700, 16, 16, 64, 12, BF)])
 def test_attention_counts(T, Hq, H, D, n, dtype):
     """Over a pool in which attention counts tokens: lists in pieces, a wave to a list; every
     entry of every list shows.  (300 pieces' sums: (4 + 300 / 64) * 2^-24 < 2^-17.)"""
@@ -395,7 +400,8 @@ def test_attention_counts(T, Hq, H, D, n, dtype):
 
 
 @pytest.mark.parametrize("T,Hq,H,D,dtype", [(5, 4, 1, 64, BF), (30, 10, 2, 128, FP),
-                                            (400, 8, 8, 64, FP), (800, 8, 4, 128, BF)])
+                                            (400, 8, 8, 64, FP), (800, 8, 4, 128, BF),
+                                            (700, 16, 16, 128, BF), (400, 32, 16, 64, FP)])
 def test_attention_neighbours_of_non_finite_queries(T, Hq, H, D, dtype):
     """A query with a NaN or an infinity is NaN; the rows and heads beside it are not."""
     from flashvsr_sm89_ops import selected_attention
@@ -416,7 +422,8 @@ def test_attention_neighbours_of_non_finite_queries(T, Hq, H, D, dtype):
     assert bool(fine[rows].all())
 
 
-@pytest.mark.parametrize("T,Hq,H,D,dtype", [(1, 4, 2, 64, BF), (7, 4, 2, 128, FP), (650, 8, 8, 64, BF)])
+@pytest.mark.parametrize("T,Hq,H,D,dtype", [(1, 4, 2, 64, BF), (7, 4, 2, 128, FP), (650, 8, 8, 64, BF),
+                                            (700, 16, 16, 128, FP), (700, 16, 16, 64, BF)])
 def test_attention_far_logits(T, Hq, H, D, dtype):
     """Logits up to hundreds, growing from page to page, and rows whose first page comes late: the
     reference of a row moves while its neighbours' stay.  One channel alone is not zero, so that
@@ -447,9 +454,10 @@ def test_attention_far_logits(T, Hq, H, D, dtype):
     assert bool(((out.cpu().double() - want).abs() <= tol + 1e-30)[rows].all())
 
 
-@pytest.mark.parametrize("Hq,H,D,dtype", [(8, 8, 64, BF), (8, 4, 128, FP)])
+@pytest.mark.parametrize("Hq,H,D,dtype", [(8, 8, 64, BF), (8, 4, 128, FP), (16, 16, 128, BF),
+                                          (32, 16, 64, FP)])
 def test_attention_many_packed_rows(Hq, H, D, dtype):
-    """Packed chunks and single tokens in one call, a wave to a unit; rows behind the last
+    """Packed chunks and single tokens in one call, four waves or one to a unit; rows behind the last
     sequence are zeros, or left alone in `out`."""
     from flashvsr_sm89_ops import KVPages, selected_attention
     new, lengths = [300, 0, 1, 417, 2], [300, 128, 900, 1300, 2]
@@ -472,12 +480,11 @@ def test_attention_many_packed_rows(Hq, H, D, dtype):
     assert torch.equal(given[:-3], out[:-3]) and bool((given[-3:] == 7).all())
 
 
-@pytest.mark.parametrize("T", [1, 700])
-def test_attention_bad_pages_and_hidden_nan(T):
+@pytest.mark.parametrize("T,H,D", [(1, 8, 64), (700, 8, 64), (700, 16, 64), (700, 16, 128)])
+def test_attention_bad_pages_and_hidden_nan(T, H, D):
     """Page ids outside the pool make the rows that list them NaN; what lies behind a row's
     position, and pages that it does not list, may hold NaN."""
     from flashvsr_sm89_ops import selected_attention
-    H, D = 8, 64
     lengths = [T + 300]
     table, N = tables(lengths, seed=1)
     pages = pool(N, H, D, seed=2)
@@ -521,6 +528,32 @@ def test_attention_neighbours_of_nan(Hq, H, D, dtype, where):
     clean = ~torch.isnan(out.cpu()).any(-1).all(-1)
     assert 0 < int(clean.sum()) < T
     check_attention(out, q, pages, table, lengths, cols)
+
+
+@pytest.mark.parametrize("Hq,H,D,dtype", [(16, 16, 128, BF), (16, 16, 64, FP), (32, 16, 128, FP),
+                                          (48, 16, 64, BF)])
+@pytest.mark.parametrize("wild", [False, True])
+@pytest.mark.parametrize("where", ["", "k", "v", "k_scale", "v_scale"])
+def test_attention_many_units(Hq, H, D, dtype, wild, where):
+    """Units enough for a wave each, in lists of any kind, with NaN in some of the pages."""
+    from flashvsr_sm89_ops import selected_attention
+    T, lengths = 700, [1500]
+    table, N = tables(lengths, seed=1)
+    pages = pool(N, H, D, seed=2)
+    for col in (1, 7):
+        page = int(table[0, col])
+        if where in ("k", "v"):
+            getattr(pages, where)[page, :, 5, 3] = math.nan
+        elif where:
+            getattr(pages, where).view(torch.uint8)[page] = 255
+    cols = random_columns(T, H, 4, lengths, [T], seed=4, wild=wild)
+    q = torch.randn(T, Hq, D, generator=gen(3)).to(dtype)
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV))
+    rows = torch.cat([torch.arange(3, T, 37), torch.arange(T - 3, T)])
+    if where:
+        some = torch.isnan(out.cpu()[rows]).any(-1)
+        assert bool(some.any()) and not bool(some.all())
+    check_attention(out, q, pages, table, lengths, cols, rows=rows)
 
 
 def test_attention_nothing():
@@ -670,10 +703,11 @@ def test_graph_and_stream():
             assert torch.equal(u.view(torch.uint8), v.view(torch.uint8)), i
 
 
-def test_graph_of_a_chunk():
+@pytest.mark.parametrize("H,D", [(8, 64), (16, 128)])
+def test_graph_of_a_chunk(H, D):
     """A chunk's pooling, choice and attention captured, replayed as lengths and pages change."""
     from flashvsr_sm89_ops import page_means, pool_pages, select_pages, selected_attention
-    H, Hq, D, T = 8, 8, 64, 700
+    Hq, T = H, 700
     table, N = tables([3000])
     pages = pool(N, H, D)
     means, t = page_means(pages), table.to(DEV)
