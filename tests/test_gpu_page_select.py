@@ -249,14 +249,23 @@ def test_select_special_queries(dtype):
 
 
 @pytest.mark.parametrize("pages,n,top", [(600, 1, 20), (1500, 3, 64), (3000, 1, 500),
-                                         (9000, 2, 33), (32768, 1, 64)])
+                                         (9000, 2, 33), (32768, 1, 64), (600, 40, 20),
+                                         (1100, 30, 64), (600, 33, 300), (140, 70, 40)])
 def test_select_many_pages(pages, n, top):
-    """Columns beyond what registers hold, and the widest table."""
+    """Columns beyond what registers hold, in rows alone and in tiles, and the widest table."""
     lengths = [pages * 128 - 5]
     g = gen(pages)
     table, N = torch.randint(0, 700, (1, pages), generator=g).int(), 700  # pages shared: ties
     q = torch.randn(n, 2, 64, generator=g).bfloat16()
     check_select(q, random_means(N, 1, 64), table, lengths, top, 1, 3)
+
+
+def test_select_many_pages_of_many_heads():
+    """A group past 16 queries over more pages than a wave's registers hold."""
+    lengths, new = [600 * 128 - 9, 700 * 128], [2, 3]
+    table, N = tables(lengths, seed=2)
+    q = torch.randn(sum(new), 20, 64, generator=gen(1)).half()
+    check_select(q, random_means(N, 1, 64), table, lengths, 50, 1, 3, starts(new))
 
 
 def test_select_wide_table():
