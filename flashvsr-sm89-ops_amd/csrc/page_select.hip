@@ -19,6 +19,7 @@
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
@@ -150,11 +151,11 @@ __global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
 // 16 pages; a row's largest goes to LDS as a key.  Then its waves share out the rows, and a bisection
 // over the keys finds the one that just makes the list.
 //
-// Bound by instructions, not bytes: 4096 rows x 32 / 8 heads over some 500 pages take 45 us, 36 MB
-// would take 7.  Of those 30 go to q's integers and the scores (13 instructions a row's group and
-// page), 15 to the choice (some 200 vector and 200 scalar ones a row and head).  One row's is a chain of
-// lengths, ids, means and choice: 6 us over 157 pages, 11 over 938, 17 over 1953; 64 rows over up to
-// 1016 pages each 16.6.
+// Bound by instructions and the chain of one workgroup, not bytes: 4096 rows x 32 / 8 heads over
+// some 500 pages take 40 us, 36 MB would take 7.  Of those 30 go to q's integers and the scores (13
+// instructions a row's group and page), 10 to the choice.  One row's is a chain of lengths, ids,
+// means and choice: 6 us over 157 pages, 11 over 938, 17 over 1953; 64 rows over up to 1016 pages each
+// 16.5.
 //
 // Operands of v_mfma_i32_16x16x64_i8: lane (r, g) = (l % 16, l / 16) holds bytes 16 g .. of row r;
 // accumulator j of lane (c, g) is row 4 g + j (a query) of column c (a page).
@@ -233,9 +234,11 @@ FVSR_DEV int bound_of(const int (&group)[4], int need) {
 
 // A wave takes the `need` largest of n > need keys in LDS, of equal ones the first, and gives
 // their places, rising, to emit(place, rank).  R: keys of a lane in registers; the others are read
-// each time.  (Up to R * 64 keys are read whatever n is, in LDS and without a use.)
+// each time.  (Up to R * 64 keys are read whatever n is, in LDS and without a use.)  Those that
+// reach the first bound are few as a rule: they then go to `few`, one or two to a lane (4096 rows,
+// 13 of 500 pages: 40.2 us, without that 44.8; 2048 rows, 61 of 940: 52.9 and 72.6).
 template <int R, class Emit>
-FVSR_DEV void choose(const int* keys, int n, int need, Emit emit) {
+FVSR_DEV void choose(const int* keys, int n, int need, v2i* few, Emit emit) {
   const int lane = threadIdx.x & 63;
   keys += lane;
   const auto key_at = [&](int i) { return i + lane < n ? keys[i] : kNever; };
@@ -257,6 +260,69 @@ FVSR_DEV void choose(const int* keys, int n, int need, Emit emit) {
   };
   // Chosen: keys above lo, and the first `left` of those at it.
   int lo = bound_of(group, need), left = 0, reach = count(lo);
+  if (R > 2 && reach <= 128) {
+    int at = 0;
+    const auto keep = [&](int i, int k) {
+      const uint64_t set = __ballot(k >= lo);
+      if (k >= lo) few[before(set, at)] = v2i{k, i + lane};
+      at += __popcll(set);
+    };
+#pragma unroll
+    for (int i = 0; i < R; ++i) keep(i * 64, key[i]);
+    for (int i = R * 64; i < n; i += 64) keep(i, key_at(i));
+    __builtin_amdgcn_wave_barrier();  // (a wave's accesses of LDS are in order)
+    const auto choose_few = [&](auto lanes) {
+      constexpr int F = lanes;  // of them to a lane
+      int k[F], place[F], most = kNever;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const v2i x = few[f * 64 + lane];
+        k[f] = f * 64 + lane < reach ? x.x : kNever, place[f] = x.y;
+        most = max(most, k[f]);
+      }
+      const auto of_few = [&](int at) {
+        int c = 0;
+#pragma unroll
+        for (int f = 0; f < F; ++f) c += __popcll(__ballot(k[f] >= at));
+        return c;
+      };
+      if (reach > need + 4) {
+        bool exact;
+        lo = reached(of_few, need, lo, wave_largest(most), exact);
+        reach = exact ? need : of_few(lo);
+      }
+      while (reach > need) {
+        int least = INT32_MAX;
+#pragma unroll
+        for (int f = 0; f < F; ++f) least = min(least, k[f] >= lo ? k[f] : INT32_MAX);
+        least = ~wave_largest(~least);
+        const int above = of_few(least + 1);
+        lo = least, left = need - above;
+        if (left > 0) break;
+        lo = least + 1, left = 0, reach = above;
+      }
+      int at = 0;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        bool in = k[f] >= lo;
+        if (left > 0) {  // the first of those at lo
+          const uint64_t eq = __ballot(k[f] == lo);
+          in = k[f] > lo || (k[f] == lo && before(eq, 0) < left);
+          left = max(left - (int)__popcll(eq), 0);
+          lo += left == 0;
+        }
+        const uint64_t all = __ballot(in);
+        if (in) emit(place[f], before(all, at));
+        at += __popcll(all);
+      }
+    };
+    if (reach <= 64)
+      choose_few(std::integral_constant<int, 1>{});
+    else
+      choose_few(std::integral_constant<int, 2>{});
+    __builtin_amdgcn_wave_barrier();
+    return;
+  }
   if (reach > need + 4) {
     bool exact;
     const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
@@ -307,9 +373,10 @@ struct Sieve {
   int key[kLeft], place[kLeft];
 };
 template <class Emit>
-FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s, Emit emit) {
+FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s, v2i* few,
+                           Emit emit) {
   if (n <= kLeft) {
-    if (wave == 0) choose<kLeft / 64>(keys, n, need, emit);
+    if (wave == 0) choose<kLeft / 64>(keys, n, need, few, emit);
     return;
   }
   const int lane = threadIdx.x & 63, share = (n + 255) / 256 * 64;
@@ -337,7 +404,7 @@ FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s,
   }
   at = __builtin_amdgcn_readfirstlane(at), total = __builtin_amdgcn_readfirstlane(total);
   if (total > kLeft) {  // (more than a wave's lanes are wanted, or many tie)
-    if (wave == 0) choose<8>(keys, n, need, emit);
+    if (wave == 0) choose<8>(keys, n, need, few, emit);
     return;
   }
   for (int i = i0; i < i1 + lane; i += 64) {
@@ -355,7 +422,7 @@ FVSR_DEV void choose_alone(const int* keys, int n, int need, int wave, Sieve& s,
     for (int i = lane; i < need; i += 64) emit(s.place[i], i);
     return;
   }
-  choose<kLeft / 64>(s.key, total, need, [&](int i, int rank) { emit(s.place[i], rank); });
+  choose<kLeft / 64>(s.key, total, need, few, [&](int i, int rank) { emit(s.place[i], rank); });
 }
 
 // A row's 16 channels at 64 w + 16 g, w < W, of one query.
@@ -392,6 +459,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   constexpr int TP = 16 / GP;  // rows of an operand
   extern __shared__ __attribute__((aligned(16))) int keys[];
   __shared__ Sieve sieve;
+  __shared__ v2i few[kThreads / 64][128];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int H = (int)a.c.heads, P = (int)a.c.table_pages, B = (int)a.c.sequences;
@@ -580,18 +648,18 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   };
   if (M == 1 && nt == 1) {
     list(0, threadIdx.x, kThreads, [&](const int* k, int n, auto emit) {
-      choose_alone(k, n, need, wave, sieve, emit);
+      choose_alone(k, n, need, wave, sieve, few[wave], emit);
     });
     return;
   }
   for (int i = wave; i < nt; i += kThreads / 64)
     list(i, lane, 64, [&](const int* k, int n, auto emit) {
       if (M > 1 && most <= 128)
-        choose<2>(k, n, need, emit);
+        choose<2>(k, n, need, few[wave], emit);
       else if (M == 1 || most <= 512)
-        choose<8>(k, n, need, emit);
+        choose<8>(k, n, need, few[wave], emit);
       else
-        choose<16>(k, n, need, emit);
+        choose<16>(k, n, need, few[wave], emit);
     });
 }
 
