@@ -15,8 +15,8 @@
 //
 // Measured, 32 query and 8 key/value heads of 128 in bf16: one token over 64 of 2047 pages 11.7 us (17
 // MB), 128 tokens over 32 pages each 171 us (5.45 TB/s; a copy reaches 5.2); 2048 rows of a prompt
-// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 67 to 75 us between cards (256 TFLOP/s of what the rows
-// ask for; the vector units are busy for three quarters of a wave's time).
+// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 66 to 75 us (257 TFLOP/s of what the rows ask for;
+// 30 us of vector instructions a SIMD, 17 of matrix ones, and some 13 TB/s from the L2).
 #include <algorithm>
 #include <type_traits>
 
