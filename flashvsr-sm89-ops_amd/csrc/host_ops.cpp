@@ -569,10 +569,20 @@ struct TurnNode : torch::autograd::Function<TurnNode> {
 // While a stream captures, a leaf may not have a graph from another stream: the backward pass
 // would wait for that stream inside the capture, which ends the process.
 bool other_graph(const at::Tensor& x) {
-  if (!x.requires_grad() || !x.is_leaf()) return false;
+  if (!x.requires_grad() || !x.is_leaf() ||
+      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+    return false;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
   const auto at = node ? node->stream() : std::nullopt;
   return at && at->id() != c10::hip::getCurrentHIPStream(x.device().index()).id();
+}
+
+// graph_elsewhere(tensor): whether the call in a captured step is to be refused for it
+PyObject* graph_elsewhere(PyObject*, PyObject* o) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(THPVariable_Check(o) && THPVariable_Unpack(o).is_cuda() &&
+                         other_graph(THPVariable_Unpack(o)));
+  END_HANDLE_TH_ERRORS
 }
 
 // rotary(q, k | None, freqs, positions | None, pairs): q or (q, k) turned, or None
@@ -612,11 +622,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   at::Tensor x[2] = {*q, k ? *k : at::Tensor()}, y[2];
   if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() ==
-                        c10::hip::CaptureStatus::None ||
-                    !(other_graph(*q) || (k && other_graph(*k))),
-                "rotary: a leaf of a captured step still has a graph from another stream: let "
-                "go of its outputs first, or capture with leaves of its own");
+    if (other_graph(*q) || (k && other_graph(*k))) Py_RETURN_NONE;  // (refused there)
     TurnNode::List r;
     {
       pybind11::gil_scoped_release release;
@@ -685,6 +691,7 @@ PyMethodDef kMethods[] = {
      "select_pages(q, means, page_table, lengths, cu_tokens, top, first, recent)"},
     {"selected_attention", (PyCFunction)(void*)selected_attention, METH_FASTCALL,
      "selected_attention(q, pages, page_table, lengths, columns, cu_tokens, sm_scale)"},
+    {"graph_elsewhere", graph_elsewhere, METH_O, "graph_elsewhere(tensor)"},
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL,
      "rotary(q, k, freqs, positions, pairs)"},
     {nullptr, nullptr, 0, nullptr}};

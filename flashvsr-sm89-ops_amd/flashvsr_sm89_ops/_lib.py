@@ -132,6 +132,7 @@ class _GeneralPath:
     to the Python path, which reaches the same kernels through ctypes."""
     quantize = gemm = append_kv = paged_attention = staticmethod(lambda *args: None)
     pool_pages = select_pages = selected_attention = rotary = staticmethod(lambda *args: None)
+    graph_elsewhere = staticmethod(lambda tensor: False)  # (not known)
 
 
 _host = None

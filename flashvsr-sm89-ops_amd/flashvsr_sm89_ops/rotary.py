@@ -163,6 +163,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
     check(all(unpack_dual(x).tangent is None for x in xs), "no forward-mode gradients")
     four = [x if x.dim() == 4 else x[None] for x in xs]
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        if any(_lib.host().graph_elsewhere(x) for x in xs):
+            raise RuntimeError(
+                f"{name}: a leaf of a captured step still has a graph from another stream: let go of "
+                "its outputs first, or capture with leaves of its own")
         ys = _Rotary.apply(turns, float(gain), positions, _PAIRS[pairs], False, *four)
     else:
         ys = _launch(four, turns, float(gain), positions, _PAIRS[pairs], False)

@@ -278,7 +278,7 @@ def test_graph_of_forward_and_backward(path):
 
 
 @pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
-def test_capture_with_a_live_graph():
+def test_capture_with_a_live_graph(monkeypatch):
     """Refused before anything is captured; once the outputs are gone the same leaf does."""
     from flashvsr_sm89_ops import rotary
     f = on_gpu(freqs_of(64))
@@ -292,6 +292,12 @@ def test_capture_with_a_live_graph():
     with pytest.raises(RuntimeError, match="graph from another stream"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             rotary(q.detach(), q, f)
+    from flashvsr_sm89_ops import _lib
+    monkeypatch.setattr(_lib, "_selected_host", _lib._GeneralPath)  # by way of Python too
+    with pytest.raises(RuntimeError, match="graph from another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rotary(q.detach(), q, f)
+    monkeypatch.undo()
     del out
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
