@@ -832,7 +832,6 @@ __global__ __launch_bounds__(kThreads) void join_tile(Args a) {
 
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads, 2) void attend_tile(Args a) {
-  constexpr int N = terms(DT);
   // Two pages' K and V: page i of the list in the even or odd ones.  Distinct
   // objects, so that the compiler can tell the loads into one from the reads of
   // another and does not wait for them.

@@ -9,14 +9,14 @@
 // as many rows that follow one another as do, over the pages that any of them lists, each page read
 // and multiplied once.
 //
-// Two kernels.  attend_chosen: few units, or single tokens, whose pages come from memory: four
-// waves to a unit, and workgroups where units are too few.  attend_alone: many units of rows that
-// share pages in the L2: a wave to a unit, codes by way of LDS.
+// Two kernels.  attend_chosen: single tokens, whose pages come from memory, or few units: four
+// waves to a unit, and workgroups where units are too few.  attend_alone: units of rows that stand
+// together: one to four waves to a unit, each on pages of its own by way of LDS.
 //
 // Measured, 32 query and 8 key/value heads of 128 in bf16: one token over 64 of 2047 pages 11.7 us (17
 // MB), 128 tokens over 32 pages each 171 us (5.45 TB/s; a copy reaches 5.2); 2048 rows of a prompt
-// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 66 to 75 us (257 TFLOP/s of what the rows ask for;
-// 30 us of vector instructions a SIMD, 17 of matrix ones, and some 13 TB/s from the L2).
+// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 60.7 us (283 TFLOP/s of what the rows ask for; 30
+// us of vector instructions a SIMD, 17 of matrix ones, and some 14 TB/s from the L2).
 #include <algorithm>
 #include <type_traits>
 
@@ -367,13 +367,61 @@ struct Queries {
   }
 };
 
+// What a workgroup's waves have of a unit's rows, added up and written.
+template <int DT, int D, int WAVES>
+FVSR_DEV void join_waves(const Queries<DT, D>& w, float l, float* lds_o, float (&lds_ml)[WAVES][16][2],
+                         const Args& a, const Unit& u) {
+  constexpr int P = D + 4, C = D / 8;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  const int used = a.parts > 1 ? min(16, a.group - u.q0) : u.n * a.group;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) *(v4f*)&lds_o[(wave * 16 + col) * P + d * 16 + 4 * g] = w.acc[d];
+  if (g == 0) lds_ml[wave][col][0] = w.m, lds_ml[wave][col][1] = l;
+  __syncthreads();
+  const int d0 = threadIdx.x % C * 8;
+  for (int i = threadIdx.x / C; i < used; i += 64 * WAVES / C) {
+    float top = lds_ml[0][i][0];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) top = fmaxf(top, lds_ml[v][i][0]);
+    float o[8] = {}, sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
+      const float f = __builtin_amdgcn_exp2f(lds_ml[v][i][0] - top);
+      sum += f * lds_ml[v][i][1];
+      const v4f x = *(const v4f*)&lds_o[(v * 16 + i) * P + d0];
+      const v4f y = *(const v4f*)&lds_o[(v * 16 + i) * P + d0 + 4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += f * x[j], o[4 + j] += f * y[j];
+    }
+    const int64_t row = u.row + (a.parts > 1 ? 0 : i / a.group);
+    const int oh = u.h * a.group + (a.parts > 1 ? u.q0 + i : i % a.group);
+    if (a.splits == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      u32x2_t* op = (u32x2_t*)(a.out + row * a.o_ts + oh * a.o_hs + d0);
+      op[0] = u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+      op[1] = u32x2_t{pack2<DT>(o[4] * inv, o[5] * inv), pack2<DT>(o[6] * inv, o[7] * inv)};
+    } else {
+      const int64_t pr = (row * a.q_heads + oh) * a.splits + u.split;
+      v4f* po = (v4f*)(a.part + pr * D + d0);
+      po[0] = v4f{o[0], o[1], o[2], o[3]};
+      po[1] = v4f{o[4], o[5], o[6], o[7]};
+      if (d0 == 0) {
+        float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
+        ml[0] = top, ml[1] = sum;
+      }
+    }
+  }
+}
+
 // A workgroup's waves take the pages of a unit in turn (of all that its splits have, every
 // splits * WAVES-th) and add what they have.  GROUP: several rows to a unit, row i's queries in
 // columns i * group and on.
 template <int DT, int D, bool GROUP>
 __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void attend_chosen(Args a) {
-  constexpr int P = D + 4, C = D / 8, WAVES = kThreads / 64;
-  __shared__ __attribute__((aligned(16))) float lds_o[WAVES * 16 * P];
+  constexpr int WAVES = kThreads / 64;
+  __shared__ __attribute__((aligned(16))) float lds_o[WAVES * 16 * (D + 4)];
   __shared__ float lds_ml[WAVES][16][2];
   __shared__ std::conditional_t<GROUP, Lists<kShared>, int> lists;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
@@ -443,52 +491,16 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void attend_chosen(Args 
     w.clear();
     pages(std::true_type{});
   }
-  float l = w.l + __shfl_xor(w.l, 16);
-  l += __shfl_xor(l, 32);
-  const int used = GROUP ? u.n * a.group : min(16, a.group - u.q0);
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d) *(v4f*)&lds_o[(wave * 16 + col) * P + d * 16 + 4 * g] = w.acc[d];
-  if (g == 0) lds_ml[wave][col][0] = w.m, lds_ml[wave][col][1] = l;
-  __syncthreads();
-  const int d0 = threadIdx.x % C * 8;
-  for (int i = threadIdx.x / C; i < used; i += 64 * WAVES / C) {
-    float top = lds_ml[0][i][0];
-#pragma unroll
-    for (int v = 1; v < WAVES; ++v) top = fmaxf(top, lds_ml[v][i][0]);
-    float o[8] = {}, sum = 0.0f;
-#pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-      const float f = __builtin_amdgcn_exp2f(lds_ml[v][i][0] - top);
-      sum += f * lds_ml[v][i][1];
-      const v4f x = *(const v4f*)&lds_o[(v * 16 + i) * P + d0];
-      const v4f y = *(const v4f*)&lds_o[(v * 16 + i) * P + d0 + 4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += f * x[j], o[4 + j] += f * y[j];
-    }
-    const int64_t row = u.row + (GROUP ? i / a.group : 0);
-    const int oh = u.h * a.group + (GROUP ? i % a.group : u.q0 + i);
-    if (a.splits == 1) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      u32x2_t* op = (u32x2_t*)(a.out + row * a.o_ts + oh * a.o_hs + d0);
-      op[0] = u32x2_t{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
-      op[1] = u32x2_t{pack2<DT>(o[4] * inv, o[5] * inv), pack2<DT>(o[6] * inv, o[7] * inv)};
-    } else {
-      const int64_t pr = (row * a.q_heads + oh) * a.splits + u.split;
-      v4f* po = (v4f*)(a.part + pr * D + d0);
-      po[0] = v4f{o[0], o[1], o[2], o[3]};
-      po[1] = v4f{o[4], o[5], o[6], o[7]};
-      if (d0 == 0) {
-        float* ml = a.part + (int64_t)a.T * a.q_heads * a.splits * D + pr * 2;
-        ml[0] = top, ml[1] = sum;
-      }
-    }
-  }
+  join_waves<DT, D, WAVES>(w, w.l, lds_o, lds_ml, a, u);
 }
 
-// Many units: one a wave (a workgroup of its own).  Straight loads of an operand touch a cache
-// line for each of their 16 rows, four times what its bytes need, and that, not the bytes, is what
-// bounds them where pages come from the L2.  Here a page's codes go to LDS in whole lines, K and V
-// each on its way while the wave computes with the other, and nobody waits for another wave.
+// Units of rows that stand together.  Straight loads of an operand touch a cache line for each of
+// their 16 rows, four times what its bytes need, and that, not the bytes, is what bounds them
+// where pages come from the L2.  Here a page's codes go to LDS in whole lines, K and then V into a
+// wave's one buffer (64 dims: 8 KB, 128: 16), and other waves of the SIMD work meanwhile; nobody
+// waits for another wave before the end, where a unit's waves add up what they have of its pages.
+// (2048 rows, 32 / 8 heads of 128 in bf16, a wave to a unit: 200 us; a buffer each for K and V, which
+// leaves a SIMD one wave, 244.)
 //
 // 16-byte pieces of LDS rows are swapped about so that the 16 lanes that read a piece of 16
 // rows touch every bank once: rows of a K operand differ in token bits 0, 1, 4 and 5
@@ -527,25 +539,22 @@ struct Visit {
   uint32_t what;  // scales of K and V, and (16 bits) the rows that list it
 };
 
-template <int DT, int D>
-__global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
+template <int DT, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attend_alone(Args a) {
   constexpr int KR = D / 16;                 // pieces of a K row
   constexpr int SEG = kPage * D / 1024;      // of 64 pieces
-  // Codes of 128 dims take one buffer, K and V in turn: two waves to a SIMD, one waiting while the
-  // other works (2048 rows, 32 / 8 heads in bf16, 195 us; a buffer each and one wave 244, but 1024
-  // rows of 12 heads, a unit to a SIMD at most, 126 and 121).  Of 64 dims there is room for both, and
-  // more waves gain nothing (133 us; one buffer, three waves 138).
-  constexpr bool ONE = D == 128;
-  __shared__ __attribute__((aligned(1024))) uint8_t kl[kPage * D * (ONE ? 1 : 2)];
-  uint8_t* const vl = kl + (ONE ? 0 : kPage * D);
+  constexpr int BUF = kPage * D;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[BUF * WAVES];
+  const int wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  uint8_t* const own = lds + wave * BUF;  // K's codes or V's
   __shared__ Visit visits[kAlone];
-  // The lists lie where K will: eight workgroups then share a CU.
-  static_assert(sizeof(Lists<kAlone>) <= kPage * D, "lists outgrow K's codes");
-  Lists<kAlone>& lists = *(Lists<kAlone>*)kl;
-  const int lane = threadIdx.x, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
+  // The lists lie where codes will.
+  static_assert(sizeof(Lists<kAlone>) <= BUF, "lists outgrow the codes");
+  Lists<kAlone>& lists = *(Lists<kAlone>*)lds;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, H = (int)a.c.heads;
   Unit u;
   if (!unit_of(a, xcd_order(blockIdx.x, gridDim.x), u)) return;
-  join_lists<64>(lists, a, u);
+  join_lists<64 * WAVES>(lists, a, u);
   const int mine = min(col / (a.parts > 1 ? 16 : a.group), u.n - 1);
   const int head = a.parts > 1 ? min(u.q0 + col, a.group - 1) : col % a.group;
   const int limit = limit_of(a, u, mine), least = limit_of(a, u, 0);
@@ -594,7 +603,7 @@ __global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
       for (int i = 0; i < 4; ++i)
         off[i] = lane / KR * D +
                  ((lane % KR) ^ k_swap<D>((s + i) * (64 / KR) + lane / KR)) * 16;
-      fetch(kl + s * 1024, from + s * 1024, off);
+      fetch(own + s * 1024, from + s * 1024, off);
     }
   };
   const auto fetch_v = [&](const Visit& v) {
@@ -605,7 +614,7 @@ __global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         off[i] = lane / 8 * kPage + ((lane % 8) ^ v_swap((s + i) * 8 + lane / 8)) * 16;
-      fetch(vl + s * 1024, from + s * 1024, off);
+      fetch(own + s * 1024, from + s * 1024, off);
     }
   };
   // Row r of K subtile t is key 64 (t / 4) + 16 (r / 4) + 4 (t % 4) + r % 4.  (64 dims stand in
@@ -615,40 +624,31 @@ __global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
   asm("" : "+v"(k_again));
   const auto k_tile = [&](int t) {
     const int key = 64 * (t >> 2) + k_first + 4 * (t & 3);
-    const uint8_t* row = kl + key * D;
+    const uint8_t* row = own + key * D;
     const u32x4_t x = *(const u32x4_t*)(row + (g ^ k_swap<D>(key)) * 16);
     return ::join(x, D == 128 ? *(const u32x4_t*)(row + ((g + 4) ^ k_swap<D>(key)) * 16)
-                              : *(const u32x4_t*)(kl + k_again + (key - k_first) * D));
+                              : *(const u32x4_t*)(own + k_again + (key - k_first) * D));
   };
   const auto v_tile = [&](int d) {
     const int dim = d * 16 + col;
-    const uint8_t* row = vl + dim * kPage;
+    const uint8_t* row = own + dim * kPage;
     return ::join(*(const u32x4_t*)(row + (g ^ v_swap(dim)) * 16),
                   *(const u32x4_t*)(row + ((g + 4) ^ v_swap(dim)) * 16));
   };
-  if (n > 0) {
-    Visit cur = visit(0);
+  if (wave < n) {
+    Visit cur = visit(wave);
     fetch_k(cur);
-    if (!ONE) fetch_v(cur);
-    for (int i = 0; i < n; ++i) {
-      const Visit next = visit(min(i + 1, n - 1));  // (the last one again: no branch)
+    for (int i = wave; i < n; i += WAVES) {
+      const Visit next = visit(i + WAVES < n ? i + WAVES : i);  // (the last one again: no branch)
       const uint32_t what = cur.what;
-      wait_for<ONE ? 0 : SEG>();  // K is there, V may be on its way
+      wait_for<0>();
       w.template page<false>(k_tile, v_tile, [&] {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's operands are read
-        if constexpr (ONE)
-          fetch_v(cur);
-        else
-          fetch_k(next);
-      }, [&] {
-        wait_for<ONE ? 0 : SEG>();  // V is there, the next K may be on its way
-      }, what & 255, what >> 8 & 255, (cur.column + 1) * kPage > least, seen_of(cur), g,
-          a.scale_log2);
+        fetch_v(cur);
+      }, [&] { wait_for<0>(); }, what & 255, what >> 8 & 255, (cur.column + 1) * kPage > least,
+          seen_of(cur), g, a.scale_log2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and V's
-      if constexpr (ONE)
-        fetch_k(next);
-      else
-        fetch_v(next);
+      fetch_k(next);
       cur = next;
     }
     wait_for<0>();  // no load may land in an LDS that the next workgroup has
@@ -656,15 +656,22 @@ __global__ __launch_bounds__(64, 2) void attend_alone(Args a) {
   if (w.broken()) {
     w.clear();
     const int k_off = (16 * (col >> 2) + (col & 3)) * D + 16 * g, v_off = col * kPage + 16 * g;
-    for (int i = 0; i < n; ++i) {
+    for (int i = wave; i < n; i += WAVES) {
       const Visit v = visit(i);
       w.template page_from<true>(codes(a.c.k, v), k_off, codes(a.c.v, v), v_off, v.what & 255,
                                  v.what >> 8 & 255, true, seen_of(v), g, a.scale_log2);
     }
   }
+  if (wrong >> mine & 1) w.l = __builtin_nanf("");  // no such page: the rows that list it are NaN
+  if constexpr (WAVES > 1) {
+    __shared__ float lds_ml[WAVES][16][2];
+    static_assert(16 * (D + 4) * 4 <= BUF, "sums outgrow the codes");
+    __syncthreads();  // (codes are read, and no load is on its way)
+    join_waves<DT, D, WAVES>(w, w.l, (float*)lds, lds_ml, a, u);
+    return;
+  }
   float l = w.l + __shfl_xor(w.l, 16);
   l += __shfl_xor(l, 32);
-  if (wrong >> mine & 1) l = __builtin_nanf("");  // no such page: the rows that list it are NaN
   if (col >= (a.parts > 1 ? min(16, a.group - u.q0) : u.n * a.group)) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* op = a.out + (int64_t)(u.row + mine) * a.o_ts + (u.h * a.group + head) * a.o_hs + 4 * g;
@@ -688,7 +695,7 @@ struct Plan {
   int rows;              // of a unit
   int64_t tiles, units;  // of rows, over all sequences; with heads and operands of 16 queries
   int parts, splits;
-  bool alone;            // attend_alone: one wave to a unit
+  int alone;             // attend_alone: waves to a unit (or 0)
   int64_t floats(int64_t T, int64_t q_heads, int64_t D) const {
     return splits > 1 ? T * q_heads * splits * (D + 2) : 0;
   }
@@ -708,12 +715,16 @@ Plan plan_selected(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, int64_t t
   p.parts = (int)((group + 15) / 16);
   p.splits = 1;
   cut(kAlone);
-  // A wave to a unit where rows of a sequence follow one another (their pages come from the L2)
-  // and there are units for the CUs' SIMDs.  (us alone / shared at 256 units 49 / 37, 512 units of
-  // 64 dims 44 / 30, of 128 dims 59 / 63, 768 126 / 156, 1024 50 / 65, 2048 of 64 dims 75 / 106, of 128
-  // 104 / 213.)
-  p.alone = each > 1 && top <= kAlone && p.units * 2 >= cus * 5;
-  if (p.alone) return p;
+  // Where rows of a sequence follow one another and there are units for half the CUs: as many
+  // waves to a unit, up to four, as all units have room for at a time (LDS holds 16 of 64 dims or 8 of
+  // 128 on a CU).  us with 1, 2 and 4 waves, and by attend_chosen; 64 dims: 128 units 42, 27, 19 and
+  // 20, 512 47, 37, 28 and 31, 1024 54, 45, 41 and 65, 2048 78, 70, 76 and 106; 128 dims: 256 units 57,
+  // 36, 27 and 43, 512 60, 48, 36 and 61, 1024 73, 63, 68, 1400 91, 96, 91, 2048 108, 125, 130 and 213.
+  if (each > 1 && top <= kAlone && p.units * 2 >= cus) {
+    const int64_t room = cus * (c->head_dim == 64 ? 16 : 8) / p.units;
+    p.alone = room >= 4 ? 4 : room >= 2 || c->head_dim == 64 ? 2 : 1;
+    return p;
+  }
   cut(kShared);
   // Two workgroups to a CU, each with a page for every wave.
   p.splits = (int)std::min<int64_t>({std::max<int64_t>(1, 2 * cus / p.units),
@@ -725,7 +736,12 @@ template <int DT, int D>
 void launch(const Args& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.units * p.splits)), block(kThreads);
   if (p.alone) {
-    hipLaunchKernelGGL((attend_alone<DT, D>), grid, dim3(64), 0, st, a);
+    if (p.alone == 4)
+      hipLaunchKernelGGL((attend_alone<DT, D, 4>), grid, dim3(256), 0, st, a);
+    else if (D == 64 || p.alone == 2)
+      hipLaunchKernelGGL((attend_alone<DT, D, 2>), grid, dim3(128), 0, st, a);
+    else
+      hipLaunchKernelGGL((attend_alone<DT, D, D == 64 ? 2 : 1>), grid, dim3(64), 0, st, a);
     return;
   }
   if (p.rows > 1)

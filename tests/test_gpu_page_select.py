@@ -540,11 +540,11 @@ def test_attention_neighbours_of_nan(Hq, H, D, dtype, where):
 
 
 @pytest.mark.parametrize("Hq,H,D,dtype", [(16, 16, 128, BF), (16, 16, 64, FP), (32, 16, 128, FP),
-                                          (48, 16, 64, BF)])
+                                          (48, 16, 64, BF), (8, 8, 128, FP)])
 @pytest.mark.parametrize("wild", [False, True])
 @pytest.mark.parametrize("where", ["", "k", "v", "k_scale", "v_scale"])
 def test_attention_many_units(Hq, H, D, dtype, wild, where):
-    """Units enough for a wave each, in lists of any kind, with NaN in some of the pages."""
+    """Units of one, two or four waves, in lists of any kind, with NaN in some of the pages."""
     from flashvsr_sm89_ops import selected_attention
     T, lengths = 700, [1500]
     table, N = tables(lengths, seed=1)
