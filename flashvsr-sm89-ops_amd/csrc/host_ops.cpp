@@ -492,7 +492,8 @@ PyObject* selected_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // x [.., tokens, heads, channels], three or four dims, channels at unit stride, turned in a new
-// tensor; the second of two may be undefined.  Throws where the library refuses.
+// tensor; the second of two may be undefined.  Returns the library's status; throws where memory
+// runs out, so the GIL is let go of by a guard around it, not by the macros that an exception passes.
 struct Turn {
   at::Tensor turns, positions;  // (none: undefined)
   double gain;
@@ -634,9 +635,10 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   } else {
     const Turn t{*turns, pos ? *pos : at::Tensor(), gain, half, false};
     int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = t.run(x, y);
-    Py_END_ALLOW_THREADS
+    {
+      pybind11::gil_scoped_release release;
+      rc = t.run(x, y);
+    }
     if (rc != FVSR_OK) return not_done(rc, "rotary");
   }
   PyObject* qo = THPVariable_Wrap(std::move(y[0]));

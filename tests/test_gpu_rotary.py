@@ -347,3 +347,17 @@ def test_offsets_past_32_bits():
     out = rotary(x, None, f, pos)
     assert torch.equal(out[-3:], rotary(x[-3:].clone(), None, f, pos[-3:]))
     assert not bool(out[:5].any())
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_out_of_memory(path, grad):
+    """Outputs that memory cannot hold are an exception like any other, and the next call works."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(128))
+    one = torch.ones(1, 1, 128, device=DEV, requires_grad=grad)
+    want = rotary(one, None, f)
+    huge = one.expand(1 << 22, 1 << 10, 128)  # 2 TiB of results
+    for args in ((huge, None), (one.expand(1 << 22, 1, 128), huge)):
+        with pytest.raises(torch.OutOfMemoryError):
+            rotary(*args, f)
+    assert torch.equal(rotary(one, None, f), want)
