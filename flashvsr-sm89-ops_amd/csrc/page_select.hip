@@ -29,13 +29,20 @@ constexpr int kNan = INT32_MIN;
 // pool_kernel: a workgroup per page and head that fills up in this call.  A lane sums 16 channels
 // over some of the tokens; lanes then waves join.  132 pages x 12 heads of 128 (26 MB): 7.0 us
 // (3.7 TB/s; 5.0 at a copy's rate), a chain of lengths, page id, codes, the join and some 250 vector
-// instructions a wave.
+// instructions a wave.  Without a number of rows (T -1) tables may be far wider than the lengths: a
+// sequence's workgroups, some kSpread of all at most, take its pages in turn.  (64 x 4096 columns of 8
+// heads, 64 pages full in each: 54 us, by a workgroup to each column 900, more than a launch holds
+// at 64 x 32768; 64 x 1000 all full, of 64 dims, 742 and 655; half of kSpread 50 and 783, twice 64
+// and 727.)
 // ---------------------------------------------------------------------------
+constexpr int64_t kSpread = 32 << 10;
+constexpr int kMaxColumns = 32 << 10;   // of a table: one row's keys, 128 KB of LDS
+
 struct PoolArgs {
   fvsr_kv_cache c;
   uint8_t *mean, *scale;
   int T;     // rows of the call; -1: every full page of the table
-  int each;  // units of a sequence where that is the same for all (no cu)
+  int each;  // units of a sequence where that is the same for all (no cu, or T -1)
 };
 
 // I * 2^-e, rounded to the nearest, ties to even.
@@ -62,31 +69,12 @@ FVSR_DEV int share(float (&s)[16], int lane) {
   }
 }
 
+// The mean of one page and head, ph of the pool; every wave calls it.
 template <int D>
-__global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
+FVSR_DEV void pool_page(const PoolArgs& a, int64_t ph, int (&sums)[kThreads / 64][D]) {
   constexpr int L = D / 16;            // lanes of a token's row
   constexpr int TOK = kThreads / L;    // tokens of a pass
-  __shared__ int sums[kThreads / 64][D];
-  const int H = (int)a.c.heads, P = (int)a.c.table_pages, B = (int)a.c.sequences;
-  const int h = blockIdx.x % H, unit = blockIdx.x / H;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int b, col;
-  if (a.T >= 0 && a.c.cu) {
-    SeqPart s;
-    const auto filled = [P](int n, int len) {
-      return max(0, min(len / kPage, P) - max(len - n, 0) / kPage);
-    };
-    if (!find_part(a.c.cu, a.c.lengths, B, a.T, unit, false, filled, s)) return;
-    b = s.b, col = max(s.len - s.rows.n, 0) / kPage + s.part;
-  } else {
-    b = unit / a.each;
-    const int len = max(a.c.lengths[b], 0);
-    col = unit % a.each + (a.T < 0 ? 0 : max(len - a.T / B, 0) / kPage);
-    if (col >= min(len / kPage, P)) return;
-  }
-  const int64_t id = a.c.table[b * a.c.table_stride + col];
-  if (id < 0 || id >= a.c.pages) return;
-  const int64_t ph = id * H + h;
   const uint8_t* kp = (const uint8_t*)a.c.k + ph * kPage * D + threadIdx.x * 16;
   u32x4_t w[kPage / TOK];
 #pragma unroll
@@ -143,6 +131,35 @@ __global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
   else
     *mp = (uint8_t)total[0];
   if (lane == 0) a.scale[ph] = (uint8_t)(none ? 255 : e + own + 127);
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
+  // (Of two pages in turn: one's are read while the next one's are made.)
+  __shared__ int sums[2][kThreads / 64][D];
+  const int H = (int)a.c.heads, P = (int)a.c.table_pages, B = (int)a.c.sequences;
+  const int h = blockIdx.x % H, unit = blockIdx.x / H;
+  const int step = a.T < 0 ? a.each : 1;
+  int b, col, end;  // columns col, col + step, .. below end
+  if (a.T >= 0 && a.c.cu) {
+    SeqPart s;
+    const auto filled = [P](int n, int len) {
+      return max(0, min(len / kPage, P) - max(len - n, 0) / kPage);
+    };
+    if (!find_part(a.c.cu, a.c.lengths, B, a.T, unit, false, filled, s)) return;
+    b = s.b, col = max(s.len - s.rows.n, 0) / kPage + s.part, end = col + 1;
+  } else {
+    b = unit / a.each;
+    const int len = max(a.c.lengths[b], 0);
+    col = unit % a.each + (a.T < 0 ? 0 : max(len - a.T / B, 0) / kPage);
+    end = min(len / kPage, P);
+    if (a.T >= 0) end = min(end, col + 1);
+  }
+  for (int buf = 0; col < end; col += step) {
+    const int64_t id = a.c.table[b * a.c.table_stride + col];
+    if (id >= 0 && id < a.c.pages) pool_page<D>(a, id * H + h, sums[buf]), buf ^= 1;
+    if (end - col <= step) return;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -664,7 +681,6 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
 }
 
 constexpr int kLds = 64 << 10;          // of keys, at which two workgroups share a CU
-constexpr int kMaxColumns = 32 << 10;   // one row's keys: 128 KB
 
 template <int D, int GP>
 void launch_select(const SelectArgs& a, int grid, bool many, int lds, hipStream_t st) {
@@ -707,8 +723,11 @@ extern "C" int fvsr_pool_pages(const fvsr_kv_cache* cache, void* mean, void* mea
   a.c = *cache;
   a.mean = (uint8_t*)mean, a.scale = (uint8_t*)mean_scale;
   a.T = (int)T;
+  // (Any table that fvsr_select_pages takes.)
+  if (T < 0 && P > kMaxColumns && B * P > kMaxBlocks) return FVSR_EUNSUPPORTED;
   // Pages that n rows can fill: one more than whole pages of them; packed, over any counts.
-  a.each = (int)(T < 0 ? P : std::min(P, (T / B + kPage - 1) / kPage));
+  const int64_t turns = std::max<int64_t>(1, kSpread / B / cache->heads);
+  a.each = (int)std::min(P, T < 0 ? turns : (T / B + kPage - 1) / kPage);
   const int64_t units = T >= 0 && cache->cu ? (T + B * (kPage - 1)) / kPage : B * a.each;
   if (units > kMaxBlocks || units * cache->heads > kMaxBlocks) return FVSR_EUNSUPPORTED;
   if (units == 0) return FVSR_OK;

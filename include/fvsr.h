@@ -534,7 +534,8 @@ int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_str
  *   scale  the least 2^e, e >= -127, with every |mean| at most 127 * 2^e
  *   mean   the nearest integers to mean / scale, ties to even
  * A NaN among a head's codes, or as its scale, gives scale NaN (byte 255) and zeros.  Of the cache
- * v and its scales are not read.  Page ids outside the pool are passed over.
+ * v and its scales are not read.  Page ids outside the pool are passed over.  T -1 takes tables of up to
+ * 32768 columns for all sequences that a launch holds (sequences * heads < 2^24).
  */
 int fvsr_pool_pages(const fvsr_kv_cache* cache, void* mean, void* mean_scale, int64_t T,
                     void* stream);

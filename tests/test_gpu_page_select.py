@@ -154,6 +154,36 @@ def test_pool_outside():
     assert torch.equal(means.mean, random_means(4, 2, 64).mean)
 
 
+@pytest.mark.parametrize("B,H,P", [(64, 8, 32768), (300, 30, 8192), (2, 3, 32768), (1, 2, 40000)])
+def test_pool_wide_tables(B, H, P):
+    """Every full page of tables far wider than most lengths, with a sequence that fills its row, ids
+    outside the pool among them: the same means as from a table of the pool's pages."""
+    from flashvsr_sm89_ops import page_means, pool_pages
+    N, D = 60, 64
+    pages = pool(N, H, D, seed=2)
+    g = gen(P)
+    lengths = torch.randint(0, 700, (B,), generator=g).int()
+    lengths[B // 2], lengths[B - 1] = P * 128, 2 ** 31 - 1
+    table = torch.randint(-1, N - 1, (B, P), generator=g).int()
+    table[table == N - 2] = N  # (the last two pages are in no table)
+    table[B // 2] = torch.randint(5, 25, (P,), generator=g).int()
+    table[B - 1, :P - 1] = torch.randint(20, 40, (P - 1,), generator=g).int()
+    table[B - 1, P - 1] = 49
+    want = pool_pages(page_means(pages), pages, torch.arange(N)[None].int().to(DEV),
+                      i32([N * 128]).to(DEV))
+    seen = torch.cat([t[:min(n // 128, P)] for t, n in zip(table, lengths.tolist())])
+    listed = torch.zeros(N, dtype=torch.bool)
+    listed[seen[(seen >= 0) & (seen < N)].long()] = True
+    assert bool(listed[20:25].all()) and bool(listed[49]) and not bool(listed.all())
+    means = random_means(N, H, D, seed=9)
+    mean, scale = means.mean.clone(), means.scale.clone()
+    pool_pages(means, pages, table.to(DEV), lengths.to(DEV))
+    listed = listed.to(DEV)
+    assert torch.equal(means.mean, torch.where(listed[:, None, None], want.mean, mean))
+    got, old, new = (x.view(torch.uint8) for x in (means.scale, scale, want.scale))
+    assert torch.equal(got, torch.where(listed[:, None], new, old))
+
+
 # --------------------------------------------------------------------------------------
 
 
