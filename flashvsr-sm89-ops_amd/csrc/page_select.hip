@@ -711,7 +711,7 @@ void launch_select(const SelectArgs& a, int gp, int grid, bool many, int lds,
 
 extern "C" int fvsr_pool_pages(const fvsr_kv_cache* cache, void* mean, void* mean_scale, int64_t T,
                                void* stream) {
-  const int rc = kv_cache_ok(cache, T < 0 ? 0 : T);
+  const int rc = kv_cache_ok(cache, T < 0 ? 0 : T, false);  // (v is not read: k is checked below)
   if (rc != FVSR_OK) return rc;
   if (T < -1) return FVSR_EINVAL;
   const int64_t B = cache->sequences, P = cache->table_pages;

@@ -285,3 +285,18 @@ def test_definition_of_the_choice():
     assert S.selected(q, mean, scale, table, [P * 128], 3, 1, 1)[0, 0].tolist() == [0, 7, 11]
     assert S.selected(q, mean, scale, table, [0], 3, 1, 1)[0, 0].tolist() == [-1, -1, -1]
     assert S.selected(q, mean, scale, table, [129], 3, 1, 1)[0, 0].tolist() == [0, 1, -1]
+
+
+def test_pool_does_not_ask_for_v():
+    """v and its scales are not read, so they may be missing: with or without a number of rows the
+    first refusal is that of the launch's size."""
+    from flashvsr_sm89_ops import _lib
+    many = (1 << 22) - 1
+    for bad in (dict(v=None, v_scale=None), dict(v=FAKE + 8)):
+        c = cache(sequences=many, heads=8, **bad)
+        assert c_pool(c, T=many) == _lib.FVSR_EUNSUPPORTED
+        assert c_pool(c, T=-1) == _lib.FVSR_EUNSUPPORTED
+        c = cache(sequences=many, heads=8, k=None, **bad)
+        assert c_pool(c, T=many) == _lib.FVSR_EINVAL and c_pool(c, T=-1) == _lib.FVSR_EINVAL
+        c = cache(sequences=many, heads=8, k_scale=None, **bad)
+        assert c_pool(c, T=many) == _lib.FVSR_EINVAL and c_pool(c, T=-1) == _lib.FVSR_EINVAL
