@@ -230,12 +230,22 @@ FVSR_DEV int before(uint64_t set, int from) {  // lanes of `set` below this one,
                                         __builtin_amdgcn_mbcnt_lo((uint32_t)set, from));
 }
 
+// A few powers of two below a key (keys order like floats), kLow at least: also below kNever, the
+// largest key of a wave without any.
+constexpr int kNear = 3 << 20;
+__host__ __device__ constexpr int near_below(int key) {
+  return (key > kLow + kNear ? key : kLow + kNear) - kNear;
+}
+static_assert(near_below(kNever) == kLow && near_below(kLow + 1) == kLow &&
+                  near_below(kLow + kNear + 1) == kLow + 1 && near_below(0) == -kNear,
+              "in the range of an int for every key");
+
 // A bound that `need` of a wave's keys reach, and not many more: what `need` of the largest keys of
 // 64 lanes (few are needed) or of 256 groups of them reach.  (Keys order like floats: it is
-// seldom further down than a few powers of two.)
+// seldom further down than near_below.)
 FVSR_DEV int bound_of(const int (&group)[4], int need) {
   const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
-  const int top = wave_largest(mine), near = max(top - (3 << 20), kLow);
+  const int top = wave_largest(mine), near = near_below(top);
   const auto find = [&](auto reach) {
     bool exact;
     const bool fits = reach(near) >= need;

@@ -290,6 +290,16 @@ def test_select_many_pages(pages, n, top):
     check_select(q, random_means(N, 1, 64), table, lengths, top, 1, 3)
 
 
+@pytest.mark.parametrize("top", [2, 20, 240, 256])
+@pytest.mark.parametrize("pages", [257, 258, 300, 384, 386, 513, 770])
+def test_select_waves_without_keys(pages, top):
+    """A row that has its workgroup to itself, where the last waves' shares of the keys are short or
+    empty."""
+    table, N = tables([pages * 128], seed=1)
+    q = torch.randn(1, 2, 64, generator=gen(pages)).bfloat16()
+    check_select(q, random_means(N, 1, 64), table, [pages * 128], top, 1, 1)
+
+
 def test_select_many_pages_of_many_heads():
     """A group past 16 queries over more pages than a wave's registers hold."""
     lengths, new = [600 * 128 - 9, 700 * 128], [2, 3]
