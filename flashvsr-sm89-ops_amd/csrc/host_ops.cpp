@@ -20,6 +20,8 @@
 #include <Python.h>
 
 #include <cmath>
+#include <unordered_set>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
@@ -30,6 +32,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -518,6 +522,53 @@ struct Turn {
   }
 };
 
+// While a stream captures, a leaf whose gradient is asked for may not have a graph from another
+// stream: the backward pass would wait for that stream inside the capture, which ends the process.
+constexpr const char* kElsewhere =
+    "rotary: a leaf of a captured step still has a graph from another stream: let go of its outputs "
+    "first, or capture with leaves of its own";
+
+bool capturing() {
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
+bool elsewhere(torch::autograd::Node& node) {
+  const auto at = node.stream();
+  return at && at->id() != c10::hip::getCurrentHIPStream(at->device_index()).id();
+}
+
+// At the call: a leaf that it is given.
+bool other_graph(const at::Tensor& x) {
+  if (!x.requires_grad() || !x.is_leaf() || !capturing()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
+  return node && elsewhere(*node);
+}
+
+// In the backward pass, before a gradient is handed on: any leaf that this pass goes on to.
+bool other_graph_behind() {
+  using torch::autograd::Node;
+  const std::shared_ptr<Node> from = torch::autograd::get_current_node();
+  if (!from || !capturing()) return false;
+  const auto* info = torch::autograd::get_current_graph_task_exec_info();  // (empty: all nodes)
+  std::unordered_set<Node*> seen{from.get()};
+  std::vector<Node*> todo{from.get()};
+  while (!todo.empty()) {
+    Node* const node = todo.back();
+    todo.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) && elsewhere(*node)) return true;
+    for (const auto& edge : node->next_edges()) {
+      Node* const next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (info && !info->empty()) {
+        const auto it = info->find(next);
+        if (it == info->end() || !it->second.should_execute()) continue;
+      }
+      todo.push_back(next);
+    }
+  }
+  return false;
+}
+
 // The same as a node of a graph.  Its gradient is the rotation back, a node again where a
 // graph of the gradient is asked for.
 struct TurnNode : torch::autograd::Function<TurnNode> {
@@ -559,6 +610,7 @@ struct TurnNode : torch::autograd::Function<TurnNode> {
       }
     if (n == 0) return out;
     const c10::DeviceGuard guard(x[0].device());
+    TORCH_CHECK(!other_graph_behind(), kElsewhere);
     const List r = apply(x[0], maybe(x[1]), saved[0], maybe(saved[1]),
                          ctx->saved_data["gain"].toDouble(), ctx->saved_data["half"].toBool(),
                          !ctx->saved_data["back"].toBool());
@@ -567,22 +619,18 @@ struct TurnNode : torch::autograd::Function<TurnNode> {
   }
 };
 
-// While a stream captures, a leaf may not have a graph from another stream: the backward pass
-// would wait for that stream inside the capture, which ends the process.
-bool other_graph(const at::Tensor& x) {
-  if (!x.requires_grad() || !x.is_leaf() ||
-      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
-    return false;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
-  const auto at = node ? node->stream() : std::nullopt;
-  return at && at->id() != c10::hip::getCurrentHIPStream(x.device().index()).id();
-}
-
 // graph_elsewhere(tensor): whether the call in a captured step is to be refused for it
 PyObject* graph_elsewhere(PyObject*, PyObject* o) {
   HANDLE_TH_ERRORS
   return PyBool_FromLong(THPVariable_Check(o) && THPVariable_Unpack(o).is_cuda() &&
                          other_graph(THPVariable_Unpack(o)));
+  END_HANDLE_TH_ERRORS
+}
+
+// graph_behind(): whether the node whose backward pass runs is to refuse it
+PyObject* graph_behind(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(other_graph_behind());
   END_HANDLE_TH_ERRORS
 }
 
@@ -694,6 +742,7 @@ PyMethodDef kMethods[] = {
     {"selected_attention", (PyCFunction)(void*)selected_attention, METH_FASTCALL,
      "selected_attention(q, pages, page_table, lengths, columns, cu_tokens, sm_scale)"},
     {"graph_elsewhere", graph_elsewhere, METH_O, "graph_elsewhere(tensor)"},
+    {"graph_behind", graph_behind, METH_NOARGS, "graph_behind()"},
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL,
      "rotary(q, k, freqs, positions, pairs)"},
     {nullptr, nullptr, 0, nullptr}};

@@ -132,7 +132,9 @@ class _GeneralPath:
     to the Python path, which reaches the same kernels through ctypes."""
     quantize = gemm = append_kv = paged_attention = staticmethod(lambda *args: None)
     pool_pages = select_pages = selected_attention = rotary = staticmethod(lambda *args: None)
-    graph_elsewhere = staticmethod(lambda tensor: False)  # (not known)
+    # What leaves a backward pass goes on to is not known here: none is captured.
+    graph_elsewhere = staticmethod(lambda tensor: False)
+    graph_behind = staticmethod(lambda: torch.cuda.is_current_stream_capturing())
 
 
 _host = None

@@ -94,6 +94,10 @@ def _launch(xs, turns, gain, positions, pairs, back):
     return ys
 
 
+_ELSEWHERE = ("rotary: a leaf of a captured step still has a graph from another stream: let go of "
+              "its outputs first, or capture with leaves of its own")
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, turns, gain, positions, pairs, back, *xs):
@@ -103,6 +107,9 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
+        if _lib.host().graph_behind():
+            raise RuntimeError(_ELSEWHERE if _lib.host() is not _lib._GeneralPath else
+                               "rotary: a backward pass is captured with the native extension only")
         turns, positions = ctx.saved_tensors
         gain, pairs, back = ctx.how
         # The transpose of a rotation is the one back; the gain stays.
@@ -123,7 +130,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
 
     Differentiable in q and k (any number of times, backward mode); freqs and positions have no
     gradient.  A step with its backward pass captures into a graph where its leaves have no
-    graph from another stream left: an earlier step's outputs are let go first."""
+    graph from another stream left: an earlier step's outputs are let go first.  Otherwise the
+    backward pass is refused, for leaves further up too, and in a capture so is a call that is given
+    such a leaf itself, unless under no_grad.  Without the native extension no backward pass is
+    captured."""
     r = (_lib._selected_host or _lib.selected_host()).rotary(q, k, freqs, positions, pairs)
     if r is not None:
         return r
@@ -164,9 +174,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
     four = [x if x.dim() == 4 else x[None] for x in xs]
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         if any(_lib.host().graph_elsewhere(x) for x in xs):
-            raise RuntimeError(
-                f"{name}: a leaf of a captured step still has a graph from another stream: let go of "
-                "its outputs first, or capture with leaves of its own")
+            raise RuntimeError(_ELSEWHERE)
         ys = _Rotary.apply(turns, float(gain), positions, _PAIRS[pairs], False, *four)
     else:
         ys = _launch(four, turns, float(gain), positions, _PAIRS[pairs], False)

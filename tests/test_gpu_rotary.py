@@ -361,3 +361,56 @@ def test_out_of_memory(path, grad):
         with pytest.raises(torch.OutOfMemoryError):
             rotary(*args, f)
     assert torch.equal(rotary(one, None, f), want)
+
+
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+def test_capture_with_a_live_graph_further_up(path, monkeypatch):
+    """A leaf behind q and k (a projection's weight, or the rows that they are slices of) with an eager
+    graph from another stream: its gradient is refused inside the capture, the call itself and gradients
+    that stop before it are not."""
+    from flashvsr_sm89_ops import _lib, rotary
+    f = on_gpu(freqs_of(64))
+    x = torch.randn(6, 4, 64, device=DEV, requires_grad=True)
+    g = torch.randn(6, 3, 64, device=DEV)
+
+    def step():
+        y = x * 2
+        return y, *rotary(y[:, :3], y[:, 3:], f)
+    live = step()
+    want_q, want_k = live[1].detach(), live[2].detach()
+    want, = torch.autograd.grad(live[1], x, g, retain_graph=True)
+    for inputs in ((x,), None):
+        with pytest.raises(RuntimeError, match="graph from another stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y, q, k = step()
+                torch.autograd.grad(q, x, g) if inputs else q.backward(g)
+        del y, q, k
+    assert x.grad is None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, q, k = step()
+        dy, = torch.autograd.grad(q, y, g)
+    for _ in range(3):
+        dy.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(2 * dy, want)
+    del live, y, q, k, dy, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, q, k = step()
+        dx, = torch.autograd.grad(q, x, g)
+    for _ in range(3):
+        dx.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
+    del y, q, k, dx, graph
+    monkeypatch.setattr(_lib, "_host", _lib._GeneralPath)  # (leaves are not seen from there)
+    monkeypatch.setattr(_lib, "_selected_host", _lib._GeneralPath)
+    with pytest.raises(RuntimeError, match="native extension"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(step()[1], x, g)
+    dx, = torch.autograd.grad(step()[1], x, g)
+    assert torch.equal(dx, want)
