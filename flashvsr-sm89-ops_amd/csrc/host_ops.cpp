@@ -532,9 +532,15 @@ bool capturing() {
   return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
+// (Streams of the same capture wait for each other as any.  The default stream is in none, and may
+// not be asked.)
 bool elsewhere(torch::autograd::Node& node) {
   const auto at = node.stream();
-  return at && at->id() != c10::hip::getCurrentHIPStream(at->device_index()).id();
+  if (!at || at->id() == c10::hip::getCurrentHIPStream(at->device_index()).id()) return false;
+  const c10::hip::HIPStream other(c10::hip::HIPStream::UNCHECKED, *at);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return !other.stream() || hipStreamIsCapturing(other.stream(), &status) != hipSuccess ||
+         status != hipStreamCaptureStatusActive;
 }
 
 // At the call: a leaf that it is given.

@@ -414,3 +414,37 @@ def test_capture_with_a_live_graph_further_up(path, monkeypatch):
             torch.autograd.grad(step()[1], x, g)
     dx, = torch.autograd.grad(step()[1], x, g)
     assert torch.equal(dx, want)
+
+
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+def test_capture_over_two_streams(path):
+    """A captured step that goes over two streams: a leaf's graph from the other one is of the same
+    capture."""
+    from flashvsr_sm89_ops import rotary
+    f = on_gpu(freqs_of(64))
+    x, g = (torch.randn(6, 3, 64, device=DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+
+    def step(x):
+        leaf = x.detach().requires_grad_()
+        here = torch.cuda.current_stream()
+        first = rotary(leaf, None, f)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            second = rotary(leaf, None, f, pairs="interleaved")
+        here.wait_stream(side)
+        d, = torch.autograd.grad((first, second), leaf, (g, g))
+        return first.detach(), second.detach(), d
+    step(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x)
+    for i in range(3):
+        x.normal_()
+        g.normal_()
+        want = step(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
