@@ -3,11 +3,12 @@
 //   o[q] = sum_k w[k] v[k] / sum_k w[k],  w[k] = exp(sm_scale * q.k) over the tokens up to
 //          q's own position in the pages of its list
 //
-// A list belongs to a row and a key/value head.  Operands, bf16 weights and their precision are
-// those of paged_attn.hip: K and V are operand A as stored, q (and in bf16 the weights) sums of e4m3
-// terms.  An operand has 16 query columns; a head's group seldom fills them, so a unit of work is
-// as many rows that follow one another as do, over the pages that any of them lists, each page read
-// and multiplied once.
+// A list belongs to a row and a key/value head.  Operands, weights and their precision are those of
+// paged_attn.hip: K and V are operand A as stored, q and the weights sums of e4m3 terms.  (fp16 weights
+// as halves alone, 2^-11 of themselves, would take 69 of the 80 us below; halves and what they leave 78, of
+// 128 dims 120 where three terms take 115.)  An operand has 16 query columns; a head's group seldom
+// fills them, so a unit of work is as many rows that follow one another as do, over the pages that any of
+// them lists, each page read and multiplied once.
 //
 // Two kernels.  attend_chosen: single tokens, whose pages come from memory, or few units: four
 // waves to a unit, and workgroups where units are too few.  attend_alone: units of rows that stand
@@ -127,40 +128,6 @@ FVSR_DEV void join_lists(Lists<N>& l, const Args& a, const Unit& u) {
   __syncthreads();
 }
 
-// Weights of fp16 queries are halves (11 bits, 2^-11 of a weight): V's codes become halves as
-// well, exactly, 8 of them in 4 instructions, which is less work than a weight's three e4m3 terms
-// and their products (2048 rows, 16 / 4 heads of 64: 77 us, by terms 90; of 128, 119).
-FVSR_DEV void halves4(float a, float b, float c, float d, uint32_t (&w)[2], float& sum) {
-  const v2h x = {(_Float16)a, (_Float16)b}, y = {(_Float16)c, (_Float16)d};
-  const v2h one = {(_Float16)1.0f, (_Float16)1.0f};
-  sum = __builtin_amdgcn_fdot2(x, one, sum, false);
-  sum = __builtin_amdgcn_fdot2(y, one, sum, false);
-  w[0] = __builtin_bit_cast(uint32_t, x), w[1] = __builtin_bit_cast(uint32_t, y);
-}
-// V's codes times weights: v[4 h + i] is tokens 64 h + 16 g + 4 i .., p[h][2 i] and p[h][2 i + 1]
-// are their weights.
-FVSR_DEV v4f times(const v8i& v, const v8i (&p)[2]) {
-  typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-  typedef int v4i __attribute__((ext_vector_type(4)));
-  v4f r = {};
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      v4i a, b;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int x = v[4 * h + i + k];
-        a[2 * k] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
-        a[2 * k + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
-        b[2 * k] = p[h][2 * (i + k)], b[2 * k + 1] = p[h][2 * (i + k) + 1];
-      }
-      r = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
-                                                 __builtin_bit_cast(v8h, b), r, 0, 0, 0);
-    }
-  return r;
-}
-
 // One wave's share of a unit: lane (r, g) = (l % 16, l / 16) has positions 16 g .. and 64 + 16 g
 // .. of row r of an operand, and accumulators of column r (a query), rows 4 g ...
 template <int DT, int D>
@@ -265,24 +232,16 @@ struct Queries {
 #pragma unroll
       for (int d = 0; d < DT16; ++d) acc[d] *= f;
     }, seen > 0 ? 0.0f : -__builtin_huge_valf());
-    v8i pf[2];  // bf16: two terms; fp16: pairs of halves, tiles 0 .. 3, then 4 .. 7
+    v8i pf[N];
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      uint32_t x[2];
-      if constexpr (DT == FVSR_DT_F16) {
-        halves4(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
-        pf[t >> 2][2 * (t & 3)] = (int)x[0], pf[t >> 2][2 * (t & 3) + 1] = (int)x[1];
-      } else {
-        weights4<2>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
-        pf[0][t] = (int)x[0], pf[1][t] = (int)x[1];
-      }
+      uint32_t x[N];
+      weights4<N>(sc[t][0], sc[t][1], sc[t][2], sc[t][3], x, sum);
+#pragma unroll
+      for (int k = 0; k < N; ++k) pf[k][t] = (int)x[k];
     }
     l += __builtin_ldexpf(sum, shift);
-    const float by = DT != FVSR_DT_F16 ? 0.0f
-                     : vs == 255 && !CAREFUL
-                         ? __builtin_nanf("")
-                         : __builtin_ldexpf(1.0f, shift + (vs == 255 ? 0 : vs - 127));
     v8i ones;
     if constexpr (CAREFUL) {
 #pragma unroll
@@ -308,13 +267,9 @@ struct Queries {
         for (int j = 0; j < 4; ++j)
           if (n[j] > 0.0f) acc[d][j] = __builtin_nanf("");
       }
-      if constexpr (DT == FVSR_DT_F16) {
-        acc[d] += times(vf, pf) * by;
-      } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < N; ++k)
           acc[d] = mfma(vf, pf[k], acc[d], CAREFUL && vs == 255 ? 127 : vs, e8m0(shift - 5 * k));
-      }
     }
   }
 

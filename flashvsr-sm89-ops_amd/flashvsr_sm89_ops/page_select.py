@@ -148,9 +148,8 @@ def selected_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor
     columns int32 [T, heads, n], contiguous: columns of the page table for each row and
     key/value head, in any order.  Entries outside 0 .. p // 128 (p the row's position) are
     passed over; a column that stands twice counts twice.  Everything else as in paged_attention
-    with causal=True: a row that sees nothing is zero, a page id outside the pool makes the rows
-    that read it NaN.  So is the precision, but that the weights of float16 queries are halves,
-    within 2^-11 of themselves."""
+    with causal=True, precision too: a row that sees nothing is zero, a page id outside the pool
+    makes the rows that read it NaN.  There is no gradient: the result asks for none, whatever q does."""
     if out is None:
         r = (_lib._selected_host or _lib.selected_host()).selected_attention(
             q, pages, page_table, lengths, columns, cu_tokens, sm_scale)

@@ -562,7 +562,7 @@ int fvsr_select_pages(const fvsr_kv_cache* cache, const void* mean, const void* 
  * fvsr_paged_attn (causal) over the pages in columns [T, heads, top] alone: row t's queries
  * of key/value head h see the tokens up to their own position in the table columns columns[t][h].
  * Entries outside 0 .. the row's last column are passed over; a column that stands twice counts
- * twice.  Weights of fp16 queries are halves (2^-11 of themselves).  Everything else as there.
+ * twice.  Everything else as there.
  *   workspace  fvsr_selected_attn_workspace_floats(...) floats, 16-byte aligned
  *              (0: NULL is fine), used until the call's kernels have run
  */

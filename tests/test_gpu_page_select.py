@@ -605,6 +605,40 @@ def test_attention_many_units(Hq, H, D, dtype, wild, where):
     check_attention(out, q, pages, table, lengths, cols, rows=rows)
 
 
+@pytest.mark.parametrize("T,Hq,H,D", [(1, 16, 2, 64), (1, 16, 2, 128), (5, 8, 2, 64), (5, 8, 2, 128),
+                                      (700, 8, 8, 64), (700, 16, 16, 64), (700, 8, 8, 128),
+                                      (700, 16, 16, 128), (1100, 16, 16, 128)])
+def test_attention_bits_of_half_weights(T, Hq, H, D):
+    """fp16: a weight is within 2^-12 of itself.  Two tokens count, one with the weight 1 (a power of two,
+    so exact in any terms) and V of -1, one with e^x, x small, and V of 1: o = tanh(x / 2), off by 2^-12
+    e^x / (1 + e^x) where the weight is off by 2^-12 of itself, and half a step of the output.  (x is one
+    product of 11 bits with sm_scale 1; the hidden tokens' logits are -7168, weights of 0; exp2
+    and the sums in fp32 are off by less than 2^-18.)"""
+    from flashvsr_sm89_ops import selected_attention
+    lengths = [T + 200]
+    table, N = tables(lengths, seed=1)
+    pages = pool(N, H, D, seed=2)
+    k = torch.zeros(N, H, 128, D)
+    k[:, :, 0, 0] = 1.0
+    k[:, :, 2:, 1] = -448.0
+    v = torch.ones(N, H, D, 128)
+    v[..., 1] = -1.0
+    pages.k.copy_(k.to(torch.float8_e4m3fn))
+    pages.v.copy_(v.to(torch.float8_e4m3fn))
+    for s in pages[2:]:
+        s.view(torch.uint8).fill_(127)
+    q = torch.zeros(T, Hq, D, dtype=FP)
+    x = 0.001 + 0.01 * torch.rand(T, Hq, generator=gen(3))
+    q[..., 0], q[..., 1] = x.half(), 16.0
+    cols = torch.zeros(T, H, 1, dtype=torch.int32)
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV),
+                             sm_scale=1.0).cpu().double()
+    want = torch.tanh(q[..., :1].double() / 2).expand(T, Hq, D)
+    share = torch.sigmoid(q[..., :1].double())
+    tol = 2.0 ** -12 * share + 2.0 ** -11 * want.abs() + 2.0 ** -18
+    assert bool(((out - want).abs() <= tol).all()), float(((out - want).abs() / tol).max())
+
+
 def test_attention_nothing():
     from flashvsr_sm89_ops import selected_attention
     lengths = [300, 128]
