@@ -5,6 +5,8 @@
 // the pairs (2 i, 2 i + 1) or (i, i + turned / 2); the other channels are copied.  The way
 // back (the gradient) has -t.  The product and its fraction are in 64 bits, so an angle of
 // position 2^31 is still right to 2^-23 of a turn; sine and cosine are fp32, as is all behind them.
+// The angle they are of is fp32 too: for fp32 results what its rounding leaves, d, is made up for by
+// cos(t + d) = cos t - d sin t and sin(t + d) = sin t + d cos t (d^2 < 2^-46).
 //
 // Bound by bytes: each value is read and written once.  A thread has two 16-byte pieces of one
 // token, at the same place in both halves of the channels that turn, which is whole pairs in either
@@ -117,6 +119,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Args a) {
       t -= __builtin_rint(t);
       float y, x;
       sincospif((float)(t + t), &y, &x);
+      if constexpr (DT == FVSR_DT_F32) {
+        const float d = (float)(t + t - (float)(t + t)) * 3.14159265f, x0 = x;
+        x -= d * y, y += d * x0;
+      }
       cs[i] = x * a.gain, sn[i] = (a.back ? -y : y) * a.gain;
     }
   }

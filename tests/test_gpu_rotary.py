@@ -448,3 +448,33 @@ def test_capture_over_two_streams(path):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("D", [64, 66])
+@pytest.mark.parametrize("pos", [1, 1000003])
+@pytest.mark.parametrize("back", [False, True])
+def test_angles_of_fp32(pairs, D, pos, back):
+    """Angles 0.001 to 0.01 turns beside a quarter: the cosine is small, so a rounding of the angle to 24
+    bits, up to 2^-25 half turns, would be far more than steps of its own.  Of (1, 0) and (0, 1): sine and
+    cosine 2 units of the last place, 2^-22 of themselves, one more rounding; products with 1 and 0
+    are exact.  What 64 bits leave of the angle is below 2^-30 turns of 2^-10."""
+    from flashvsr_sm89_ops import RotaryFrequencies, rotary
+    g = gen(D)
+    off = (0.001 + 0.009 * torch.rand(32, generator=g).double()) * (1 - 2 * (torch.arange(32) % 2))
+    turns = (torch.randint(0, 1000, (32,), generator=g) * (pos > 1) + 0.25 + off) / pos
+    f, p = RotaryFrequencies(turns, 1.0), torch.tensor([pos], dtype=torch.int32)
+    x = torch.zeros(1, 1, 2, D)
+    x[0, 0, 0, :32] = 1.0
+    x[0, 0, 1, 32:64] = 1.0
+    if pairs == "interleaved":
+        x[..., :64] = x[..., :64].unflatten(-1, (2, 32)).transpose(-1, -2).flatten(-2)
+    if back:
+        q = torch.zeros_like(x, device=DEV).requires_grad_()
+        got, = torch.autograd.grad(rotary(q, None, on_gpu(f), p.to(DEV), pairs=pairs), q, x.to(DEV))
+    else:
+        got = rotary(x.to(DEV), None, on_gpu(f), p.to(DEV), pairs=pairs)
+    want = S.rotated(x, turns, 1.0, p, pairs, back)
+    tol = 2.0 ** -21 * want.abs() + 2.0 ** -40
+    assert bool(((got.cpu().double() - want).abs() <= tol).all()), \
+        float(((got.cpu().double() - want).abs() / tol).max())
