@@ -290,6 +290,21 @@ def test_select_many_pages(pages, n, top):
     check_select(q, random_means(N, 1, 64), table, lengths, top, 1, 3)
 
 
+@pytest.mark.parametrize("Hq,H", [(3, 3), (4, 2), (8, 2), (8, 1), (16, 1), (20, 1)])
+@pytest.mark.parametrize("D,dtype", [(128, BF), (128, FP), (64, BF)])
+def test_select_groups(Hq, H, D, dtype):
+    """Every width of a group: tokens over long tables, and rows enough for four operands."""
+    lengths, new = [300 * 128, 5, 411 * 128 - 7], [1, 0, 1]
+    table, N = tables(lengths, seed=1)
+    q = (2 * torch.randn(3, Hq, D, generator=gen(Hq))).to(dtype)
+    check_select(q[:2], random_means(N, H, D), table, lengths, 30, 1, 2, starts(new))
+    check_select(q, random_means(N, H, D), table, lengths, 30, 1, 2)
+    lengths = [20 * 128 + 40, 3000]
+    table, N = tables(lengths, seed=1)
+    q = (2 * torch.randn(70, Hq, D, generator=gen(Hq))).to(dtype)
+    check_select(q, random_means(N, H, D), table, lengths, 6, 1, 1)
+
+
 @pytest.mark.parametrize("top", [2, 20, 240, 256])
 @pytest.mark.parametrize("pages", [257, 258, 300, 384, 386, 513, 770])
 def test_select_waves_without_keys(pages, top):
@@ -446,6 +461,58 @@ def test_attention_counts(T, Hq, H, D, n, dtype):
                              sm_scale=math.log(2))
     want = S.counted(T, Hq, H, D, table, lengths, cols, most=3)
     assert O.counts_agree(out.cpu(), want)
+
+
+def listed(T, H, n, columns, kind, seed):
+    """[T, H, n] columns: those of neighbouring rows are disjoint as far as the columns go, rising or
+    not, or any, some twice and some that no row sees."""
+    if kind == "any":
+        return torch.randint(-3, columns + 3, (T, H, n), generator=gen(seed)).int()
+    t, h = torch.arange(T)[:, None, None], torch.arange(H)[None, :, None]
+    c = ((t * n + 3 * h + torch.arange(n)) % columns).sort(-1).values
+    return (c if kind == "rising" else c.flip(-1)).int().contiguous()
+
+
+@pytest.mark.parametrize("kind", ["rising", "falling", "any"])
+@pytest.mark.parametrize("T,Hq,H,D,n,dtype", [
+    (7, 4, 4, 64, 255, BF), (7, 4, 4, 64, 256, FP), (7, 4, 2, 128, 257, BF), (7, 8, 2, 64, 512, BF),
+    (7, 2, 2, 64, 1023, BF), (7, 4, 2, 64, 1024, FP), (7, 4, 2, 64, 1025, BF), (3, 20, 1, 64, 1025, BF),
+    (9, 16, 16, 64, 255, BF), (9, 16, 16, 128, 256, BF), (9, 16, 16, 64, 256, FP), (9, 16, 16, 64, 257, FP),
+    (40, 16, 16, 128, 64, BF), (40, 16, 16, 64, 64, FP), (100, 16, 16, 64, 24, BF), (70, 32, 16, 64, 32, BF),
+    (90, 16, 16, 64, 43, BF), (45, 16, 16, 64, 128, BF), (45, 32, 16, 128, 129, FP)])
+def test_attention_long_lists(T, Hq, H, D, n, dtype, kind):
+    """Several rows whose lists, at the sizes where a unit gets a row fewer or the lists leave LDS, and
+    disjoint lists that fill every entry it holds."""
+    from flashvsr_sm89_ops import KVPages, selected_attention
+    columns = max(n, 270 if n <= 128 else 0) + 2
+    lengths = [columns * 128 - 5 - T // 2]
+    table = torch.arange(columns)[None].int()
+    k, v, ks, vs = O.counting_pool(columns, H, D, table, most=2)
+    e4 = torch.float8_e4m3fn
+    pages = KVPages(k.to(DEV).view(e4), v.to(DEV).view(e4), ks.to(DEV).view(E8), vs.to(DEV).view(E8))
+    q = torch.zeros(T, Hq, D, dtype=dtype)
+    q[..., 0] = 1
+    cols = listed(T, H, n, columns, kind, seed=n)
+    out = selected_attention(q.to(DEV), pages, table.to(DEV), i32(lengths).to(DEV), cols.to(DEV),
+                             sm_scale=math.log(2))
+    want = S.counted(T, Hq, H, D, table, lengths, cols, most=2)
+    assert O.counts_agree(out.cpu(), want)
+
+
+@pytest.mark.parametrize("T,Hq,H", [(1100, 16, 16), (530, 32, 8)])
+def test_attention_units_of_a_wave(T, Hq, H):
+    """bf16, heads of 128, more units than two waves of each have room for: a wave to a unit."""
+    test_attention_counts(T, Hq, H, 128, 5, BF)
+    test_attention_neighbours_of_non_finite_queries(T, Hq, H, 128, BF)
+    test_attention_far_logits(T, Hq, H, 128, BF)
+    if Hq == H:
+        test_attention_bad_pages_and_hidden_nan(T, H, 128)
+
+
+@pytest.mark.parametrize("where", ["", "k", "v", "k_scale", "v_scale"])
+@pytest.mark.parametrize("wild", [False, True])
+def test_attention_units_of_a_wave_with_nan(where, wild):
+    test_attention_many_units(32, 32, 128, BF, wild, where)
 
 
 @pytest.mark.parametrize("T,Hq,H,D,dtype", [(5, 4, 1, 64, BF), (30, 10, 2, 128, FP),
