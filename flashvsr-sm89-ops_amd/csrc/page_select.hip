@@ -242,7 +242,9 @@ static_assert(near_below(kNever) == kLow && near_below(kLow + 1) == kLow &&
 
 // A bound that `need` of a wave's keys reach, and not many more: what `need` of the largest keys of
 // 64 lanes (few are needed) or of 256 groups of them reach.  (Keys order like floats: it is
-// seldom further down than near_below.)
+// seldom further down than near_below.)  Lanes are fewer counts (13 of 500 pages for 4096 rows: 42.2 us, by
+// groups 42.5; of 300 for one 7.7 and 8.0) and find no bound for many (61 of 1953: 16.6 us by groups,
+// 43.3).
 FVSR_DEV int bound_of(const int (&group)[4], int need) {
   const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
   const int top = wave_largest(mine), near = near_below(top);
@@ -313,6 +315,8 @@ FVSR_DEV void choose(const int* keys, int n, int need, v2i* few, Emit emit) {
         for (int f = 0; f < F; ++f) c += __popcll(__ballot(k[f] >= at));
         return c;
       };
+      // (By bisection while there are some to drop, then the least one by one: 4096 rows 42.2 us, by
+      // bisection alone 43.5; 61 of 954 pages for 2048 rows 51.2, up to 16 one by one 55.5.)
       if (reach > need + 4) {
         bool exact;
         lo = reached(of_few, need, lo, wave_largest(most), exact);
@@ -480,10 +484,13 @@ FVSR_DEV float half_to_f(uint32_t h) {
   return __uint_as_float(h << 16);
 }
 
-template <int D, int GP, int M, int Q = 4>
+template <int D, int GP, int M>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   constexpr int W = D / 64;
   constexpr int TP = 16 / GP;  // rows of an operand
+  // Groups of 16 pages at a time.  (8 in tables of more than 256 columns: 256 single tokens over up to
+  // 60000 26.4 us, with 4 22.8; one over 300 pages 7.5 and 7.8, over 600 and 1953 the same.)
+  constexpr int Q = 4;
   extern __shared__ __attribute__((aligned(16))) int keys[];
   __shared__ Sieve sieve;
   __shared__ v2i few[kThreads / 64][128];
@@ -699,10 +706,8 @@ void launch_select(const SelectArgs& a, int grid, bool many, int lds, hipStream_
   };
   if (many)
     run(select_kernel<D, GP, 4>);
-  else if (a.c.table_pages <= 256)
+  else
     run(select_kernel<D, GP, 1>);
-  else  // two rounds of memory fewer on the way through many pages
-    run(select_kernel<D, GP, 1, 8>);
 }
 
 template <int D>
