@@ -1,7 +1,7 @@
 // Host side of the calls whose kernels are shorter than their Python path:
 // those an FP8 linear makes (quantisation and GEMM) and those of a paged cache's
-// step (append, attention, the choice of pages, rotary positions), as a CPython extension: argument checks, output
-// allocation and the C ABI call in one crossing.  Through Python checks, torch.empty
+// step (append, attention, the choice of pages, rotary positions), as a CPython extension:
+// argument checks, output allocation and the C ABI call in one crossing.  Through Python checks, torch.empty
 // and ctypes a call costs the host 10-13 us (a paged cache's 20-40), more than a
 // kernel on a few hundred rows takes; here 5.3
 // (GEMM) and 5.6 us (quantisation), of which the launch is about half.  An
@@ -35,7 +35,6 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/utils/pybind.h>
 
 #include "../../include/fvsr.h"
 
@@ -47,6 +46,16 @@ struct Abi {
   decltype(&fvsr_fp8_gemm) fp8_gemm;
   decltype(&fvsr_gemm_amax_parts) gemm_amax_parts;
 } abi{};
+
+// Lets go of the GIL until the end of the block, also where an exception ends it: allocations
+// and the address of a tensor without memory (a transform's) throw, and the Python error that
+// becomes of that is set with the GIL held.
+class WithoutGil {
+  PyThreadState* const state_ = PyEval_SaveThread();
+
+ public:
+  ~WithoutGil() { PyEval_RestoreThread(state_); }
+};
 
 // The tensor behind a Python argument, or nullptr if it is not a plain tensor
 // (or parameter) on a GPU.
@@ -104,10 +113,11 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (wn > 0) ws = at::empty({wn}, f32);
   void* st = stream_of(*x);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = abi.quant_fp8_dt(x->data_ptr(), dt, M, K, x->stride(0), mode, gelu, q.data_ptr(),
-                        (float*)s.data_ptr(), wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = abi.quant_fp8_dt(x->data_ptr(), dt, M, K, x->stride(0), mode, gelu, q.data_ptr(),
+                          (float*)s.data_ptr(), wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, gelu ? "fused_gelu_quant_fp8" : "quantize_fp8");
   PyObject* qo = THPVariable_Wrap(std::move(q));
   PyObject* so = qo ? THPVariable_Wrap(std::move(s)) : nullptr;
@@ -150,15 +160,16 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   at::Tensor out = at::empty({M, N}, x.options().dtype(at::kBFloat16));
   void* st = stream_of(x);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = abi.fp8_gemm(x.data_ptr(), x.stride(0), (const float*)s.data_ptr(),
-                    ns == M && M != 1 ? FVSR_SCALE_ROW : FVSR_SCALE_TENSOR, w.data_ptr(),
-                    w.stride(0), (const float*)wsc.data_ptr(),
-                    nw == N && N != 1 ? FVSR_SCALE_ROW : FVSR_SCALE_TENSOR,
-                    t[4] ? t[4]->data_ptr() : nullptr, out.data_ptr(), N, M, N, K,
-                    t[5] ? FVSR_EPI_ROWMAX : FVSR_EPI_BIAS,
-                    t[5] ? (float*)t[5]->data_ptr() : nullptr, nullptr, nullptr, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = abi.fp8_gemm(x.data_ptr(), x.stride(0), (const float*)s.data_ptr(),
+                      ns == M && M != 1 ? FVSR_SCALE_ROW : FVSR_SCALE_TENSOR, w.data_ptr(),
+                      w.stride(0), (const float*)wsc.data_ptr(),
+                      nw == N && N != 1 ? FVSR_SCALE_ROW : FVSR_SCALE_TENSOR,
+                      t[4] ? t[4]->data_ptr() : nullptr, out.data_ptr(), N, M, N, K,
+                      t[5] ? FVSR_EPI_ROWMAX : FVSR_EPI_BIAS,
+                      t[5] ? (float*)t[5]->data_ptr() : nullptr, nullptr, nullptr, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "fp8_gemm");
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -297,16 +308,17 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (wn > 0) ws = at::empty({wn}, k->options().dtype(at::kFloat));
   void* st = stream_of(*k);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = paged.append(&c, k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0),
-                    v->stride(1), q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0,
-                    q ? q->stride(1) : 0, Hq, q ? out.data_ptr() : nullptr, dt, T,
-                    kw ? kw->data_ptr() : nullptr, kn, qw ? qw->data_ptr() : nullptr, qn,
-                    kw ? dtype_code(*kw) : qw ? dtype_code(*qw) : 0, (float)eps,
-                    f ? (const float*)f->data_ptr() : nullptr, rows,
-                    pos ? (const int32_t*)pos->data_ptr() : nullptr,
-                    wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = paged.append(&c, k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0),
+                      v->stride(1), q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0,
+                      q ? q->stride(1) : 0, Hq, q ? out.data_ptr() : nullptr, dt, T,
+                      kw ? kw->data_ptr() : nullptr, kn, qw ? qw->data_ptr() : nullptr, qn,
+                      kw ? dtype_code(*kw) : qw ? dtype_code(*qw) : 0, (float)eps,
+                      f ? (const float*)f->data_ptr() : nullptr, rows,
+                      pos ? (const int32_t*)pos->data_ptr() : nullptr,
+                      wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "append_kv");
   if (!q) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(out));
@@ -351,11 +363,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (wn > 0) ws = at::empty({wn}, q->options().dtype(at::kFloat));
   void* st = stream_of(*q);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = paged.attn(&c, q->data_ptr(), q->stride(0), q->stride(1), Hq, out.data_ptr(), out.stride(0),
-                  out.stride(1), dt, T, causal, keep ? (const uint8_t*)keep->data_ptr() : nullptr,
-                  nq, nk, (float)scale, 1, wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = paged.attn(&c, q->data_ptr(), q->stride(0), q->stride(1), Hq, out.data_ptr(),
+                    out.stride(0), out.stride(1), dt, T, causal,
+                    keep ? (const uint8_t*)keep->data_ptr() : nullptr, nq, nk, (float)scale, 1,
+                    wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "paged_attention");
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -416,9 +430,10 @@ PyObject* pool_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   void* st = stream_of(*t);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = selected.pool(&c, mean->data_ptr(), scale->data_ptr(), T, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = selected.pool(&c, mean->data_ptr(), scale->data_ptr(), T, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "pool_pages");
   Py_INCREF(args[0]);
   return args[0];
@@ -447,10 +462,11 @@ PyObject* select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
   at::Tensor out = at::empty({T, c.heads, top}, q->options().dtype(at::kInt));
   void* st = stream_of(*q);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = selected.select(&c, mean->data_ptr(), scale->data_ptr(), q->data_ptr(), q->stride(0),
-                       q->stride(1), Hq, dt, T, top, first, recent, (int32_t*)out.data_ptr(), st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = selected.select(&c, mean->data_ptr(), scale->data_ptr(), q->data_ptr(), q->stride(0),
+                         q->stride(1), Hq, dt, T, top, first, recent, (int32_t*)out.data_ptr(), st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "select_pages");
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -485,11 +501,12 @@ PyObject* selected_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (wn > 0) ws = at::empty({wn}, q->options().dtype(at::kFloat));
   void* st = stream_of(*q);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = selected.attn(&c, q->data_ptr(), q->stride(0), q->stride(1), Hq, out.data_ptr(),
-                     out.stride(0), out.stride(1), dt, T, (const int32_t*)cols->data_ptr(), top,
-                     (float)scale, 1, wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
-  Py_END_ALLOW_THREADS
+  {
+    const WithoutGil released;
+    rc = selected.attn(&c, q->data_ptr(), q->stride(0), q->stride(1), Hq, out.data_ptr(),
+                       out.stride(0), out.stride(1), dt, T, (const int32_t*)cols->data_ptr(), top,
+                       (float)scale, 1, wn > 0 ? (float*)ws.data_ptr() : nullptr, wn, st);
+  }
   if (rc != FVSR_OK) return not_done(rc, "selected_attention");
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -497,7 +514,7 @@ PyObject* selected_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // x [.., tokens, heads, channels], three or four dims, channels at unit stride, turned in a new
 // tensor; the second of two may be undefined.  Returns the library's status; throws where memory
-// runs out, so the GIL is let go of by a guard around it, not by the macros that an exception passes.
+// runs out.
 struct Turn {
   at::Tensor turns, positions;  // (none: undefined)
   double gain;
@@ -525,8 +542,8 @@ struct Turn {
 // While a stream captures, a leaf whose gradient is asked for may not have a graph from another
 // stream: the backward pass would wait for that stream inside the capture, which ends the process.
 constexpr const char* kElsewhere =
-    "rotary: a leaf of a captured step still has a graph from another stream: let go of its outputs "
-    "first, or capture with leaves of its own";
+    "rotary: a leaf of a captured step still has a graph from another stream: let go of its "
+    "outputs first, or capture with leaves of its own";
 
 bool capturing() {
   return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
@@ -680,7 +697,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (other_graph(*q) || (k && other_graph(*k))) Py_RETURN_NONE;  // (refused there)
     TurnNode::List r;
     {
-      pybind11::gil_scoped_release release;
+      const WithoutGil released;
       r = TurnNode::apply(x[0], TurnNode::maybe(x[1]), *turns,
                           pos ? TurnNode::MaybeTensor(*pos) : std::nullopt, gain, half, false);
     }
@@ -690,7 +707,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Turn t{*turns, pos ? *pos : at::Tensor(), gain, half, false};
     int rc;
     {
-      pybind11::gil_scoped_release release;
+      const WithoutGil released;
       rc = t.run(x, y);
     }
     if (rc != FVSR_OK) return not_done(rc, "rotary");

@@ -200,3 +200,46 @@ def test_streams():
         side.synchronize()
         _same(got, (x8, s))
         _same(g, h)
+
+
+def test_tensors_without_memory_are_an_exception():
+    """A transform's tensors have no address: each call raises, whichever argument it is, and the next
+    one works.  (The address is asked for while the GIL is let go of.)"""
+    import flashvsr_sm89_ops as fv
+    e8 = torch.float8_e8m0fnu
+    x = torch.randn(4, 2, 64, device=DEV).bfloat16()
+    w = torch.randn(64, device=DEV).bfloat16()
+    pages = fv.kv_pages(4, 2, 64, device=DEV)
+    means = fv.page_means(pages)
+    table = torch.arange(2, dtype=torch.int32, device=DEV)[None]
+    n = torch.full((1,), 200, dtype=torch.int32, device=DEV)
+    cols = torch.zeros(4, 2, 1, dtype=torch.int32, device=DEV)
+    keep = torch.ones(2, 1, 2, dtype=torch.bool, device=DEV)
+    x8, s = fv.quantize_fp8(x[:, 0], per_token=True)
+    w8, ws = fv.quantize_weight_fp8(torch.randn(96, 64, device=DEV).bfloat16(), per_channel=True)
+    pos = torch.arange(4, dtype=torch.int32, device=DEV)
+    f = fv.rotary_frequencies(64)
+    calls = [
+        (x[:, 0], lambda t: fv.quantize_fp8(t, per_token=True)),
+        (x[:, 0], lambda t: fv.fused_gelu_quant_fp8(t)),
+        (s, lambda t: fv.fp8_gemm(x8, t, w8, ws)),
+        (ws, lambda t: fv.fp8_gemm(x8, s, w8, t)),
+        (x, lambda t: fv.append_kv(pages, x, t, table, n)),
+        (w, lambda t: fv.append_kv(pages, x, x, table, n, k_weight=t)),
+        (keep, lambda t: fv.paged_attention(x, pages, table, n, keep=t)),
+        (means.scale.view(torch.uint8), lambda t: fv.pool_pages(
+            fv.PageMeans(means.mean, t.view(e8)), pages, table, n)),
+        (means.scale.view(torch.uint8), lambda t: fv.select_pages(
+            x, fv.PageMeans(means.mean, t.view(e8)), table, n, top=2)),
+        (x, lambda t: fv.select_pages(t, means, table, n, top=2)),
+        (cols, lambda t: fv.selected_attention(x, pages, table, n, t)),
+        (x, lambda t: fv.rotary(t, None, f)),
+        (pos, lambda t: fv.rotary(x, None, f, t)),
+        (f.turns, lambda t: fv.rotary(x, None, fv.RotaryFrequencies(t))),
+    ]
+    for i, (t, call) in enumerate(calls):
+        print("call", i, flush=True)
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            torch.vmap(call)(torch.stack([t, t]))
+        call(t)
+    torch.cuda.synchronize()
