@@ -30,10 +30,10 @@ constexpr int kNan = INT32_MIN;
 // over some of the tokens; lanes then waves join.  132 pages x 12 heads of 128 (26 MB): 7.0 us
 // (3.7 TB/s; 5.0 at a copy's rate), a chain of lengths, page id, codes, the join and some 250 vector
 // instructions a wave.  Without a number of rows (T -1) tables may be far wider than the lengths: a
-// sequence's workgroups, some kSpread of all at most, take its pages in turn.  (64 x 4096 columns of 8
-// heads, 64 pages full in each: 54 us, by a workgroup to each column 900, more than a launch holds
-// at 64 x 32768; 64 x 1000 all full, of 64 dims, 742 and 655; half of kSpread 50 and 783, twice 64
-// and 727.)
+// sequence's workgroups, some kSpread of all at most, take its pages in turn.  (64 x 4096 columns of
+// 8 heads, 64 pages full in each: 86 us, 6.2 TB/s, and 4 full in each of 16 rows 19; by a workgroup to
+// each column 899 and 220, and 64 x 32768 are more than a launch holds.  64 x 1000 all full, of 64
+// dims, 742 and 655.  Half of kSpread: 91, 11 and 782; twice 85, 33 and 729.)
 // ---------------------------------------------------------------------------
 constexpr int64_t kSpread = 32 << 10;
 constexpr int kMaxColumns = 32 << 10;   // of a table: one row's keys, 128 KB of LDS
@@ -169,10 +169,12 @@ __global__ __launch_bounds__(kThreads) void pool_kernel(PoolArgs a) {
 // over the keys finds the one that just makes the list.
 //
 // Bound by instructions and the chain of one workgroup, not bytes: 4096 rows x 32 / 8 heads over
-// some 500 pages take 40 us, 36 MB would take 7.  Of those 30 go to q's integers and the scores (13
+// some 500 pages take 40 us, 36 MB would take 7 and the products 8 (at 2058 TOP/s, what an 8192^3
+// 8-bit product reaches).  Of those 30 go to q's integers and the scores (13
 // instructions a row's group and page), 10 to the choice.  One row's is a chain of lengths, ids,
-// means and choice: 6 us over 157 pages, 11 over 938, 17 over 1953; 64 rows over up to 1016 pages each
-// 16.5.
+// means and choice: 6 us over 157 pages, 11 over 938, 16.5 over 1953; 64 rows over up to 1016
+// pages each 16.7.  A tile's rows are as many as have keys in LDS at the table's width, whatever they see: the
+// 4096 rows take 69 us in a table of 1024 columns, 144 in one of 4096, 856 in one of 32768.
 //
 // Operands of v_mfma_i32_16x16x64_i8: lane (r, g) = (l % 16, l / 16) holds bytes 16 g .. of row r;
 // accumulator j of lane (c, g) is row 4 g + j (a query) of column c (a page).
@@ -242,9 +244,9 @@ static_assert(near_below(kNever) == kLow && near_below(kLow + 1) == kLow &&
 
 // A bound that `need` of a wave's keys reach, and not many more: what `need` of the largest keys of
 // 64 lanes (few are needed) or of 256 groups of them reach.  (Keys order like floats: it is
-// seldom further down than near_below.)  Lanes are fewer counts (13 of 500 pages for 4096 rows: 42.2 us, by
-// groups 42.5; of 300 for one 7.7 and 8.0) and find no bound for many (61 of 1953: 16.6 us by groups,
-// 43.3).
+// seldom further down than near_below.)  Lanes are fewer counts (13 of 500 pages for 4096 rows: 42.2
+// us, by groups 42.5; of 300 for one 7.7 and 8.0) and find no bound for many (61 of 1953: 16.6 us by
+// groups, 43.3).
 FVSR_DEV int bound_of(const int (&group)[4], int need) {
   const int mine = max(max(group[0], group[1]), max(group[2], group[3]));
   const int top = wave_largest(mine), near = near_below(top);

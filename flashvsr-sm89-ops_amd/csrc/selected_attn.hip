@@ -5,10 +5,11 @@
 //
 // A list belongs to a row and a key/value head.  Operands, weights and their precision are those of
 // paged_attn.hip: K and V are operand A as stored, q and the weights sums of e4m3 terms.  (fp16 weights
-// as halves alone, 2^-11 of themselves, would take 69 of the 80 us below; halves and what they leave 78, of
-// 128 dims 120 where three terms take 115.)  An operand has 16 query columns; a head's group seldom
-// fills them, so a unit of work is as many rows that follow one another as do, over the pages that any of
-// them lists, each page read and multiplied once.
+// as halves alone, 2^-11 of themselves, would take 61 of the 74 us below, and of 128 dims 110 of 116;
+// halves and an e4m3 term for what they leave 3 % less than three terms for 64 dims, 4 % more
+// for 128.)  An operand has 16 query columns; a head's group seldom fills them, so a unit of work is as
+// many rows that follow one another as do, over the pages that any of them lists, each page read and
+// multiplied once.
 //
 // Two kernels.  attend_chosen: single tokens, whose pages come from memory, or few units: four
 // waves to a unit, and workgroups where units are too few.  attend_alone: units of rows that stand
@@ -16,8 +17,8 @@
 //
 // Measured, 32 query and 8 key/value heads of 128 in bf16: one token over 64 of 2047 pages 11.7 us (17
 // MB), 128 tokens over 32 pages each 171 us (5.45 TB/s; a copy reaches 5.2); 2048 rows of a prompt
-// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 60.7 us (283 TFLOP/s of what the rows ask for; 30
-// us of vector instructions a SIMD, 17 of matrix ones, and some 14 TB/s from the L2).
+// over 16 of 250 pages, 16 / 4 heads of 64 in fp16, 74 us (233 TFLOP/s of what the rows ask for; 46
+// us of vector instructions a SIMD, 20 of matrix ones, and some 12 TB/s from the L2).
 #include <algorithm>
 #include <type_traits>
 
@@ -672,9 +673,10 @@ Plan plan_selected(const fvsr_kv_cache* c, int64_t T, int64_t q_heads, int64_t t
   cut(kAlone);
   // Where rows of a sequence follow one another and there are units for half the CUs: as many
   // waves to a unit, up to four, as all units have room for at a time (LDS holds 16 of 64 dims or 8 of
-  // 128 on a CU).  us with 1, 2 and 4 waves, and by attend_chosen; 64 dims: 128 units 42, 27, 19 and
-  // 20, 512 47, 37, 28 and 31, 1024 54, 45, 41 and 65, 2048 78, 70, 76 and 106; 128 dims: 256 units 57,
-  // 36, 27 and 43, 512 60, 48, 36 and 61, 1024 73, 63, 68, 1400 91, 96, 91, 2048 108, 125, 130 and 213.
+  // 128 on a CU).  us with 1, 2 and 4 waves, and by attend_chosen, in bf16; 64 dims: 128 units 41,
+  // 26, 19 and 19, 512 46, 37, 25 and 30, 1024 50, 41, 38 and 53, 2048 67, 63, 67 and 88; 128 dims:
+  // 256 units 57, 36, 26 and 42, 512 59, 47, 34 and 62, 1024 69, 57, 62 and 112, 1400 86, 92, 85 and
+  // 154, 2048 99, 113, 116 and 213.  (fp16: up to 25 % more, in the same order.)
   if (each > 1 && top <= kAlone && p.units * 2 >= cus) {
     const int64_t room = cus * (c->head_dim == 64 ? 16 : 8) / p.units;
     p.alone = room >= 4 ? 4 : room >= 2 || c->head_dim == 64 ? 2 : 1;

@@ -62,7 +62,8 @@ def pool_pages(means: PageMeans, pages: KVPages, page_table: torch.Tensor, lengt
     page of the sequences (cu_tokens does not count then).
 
     Per page and head scale is the least power of two, 2^-127 or more, of which every |mean|
-    is at most 127 times, and mean the nearest integers, ties to even: exactly.  A NaN among a
+    is at most 127 times (2^127 for means past that, which are held at 127 of it), and mean the
+    nearest integers, ties to even: exactly.  A NaN among a
     head's codes, or as its scale, gives scale NaN.  Page ids outside the pool are passed
     over."""
     r = (_lib._selected_host or _lib.selected_host()).pool_pages(
@@ -100,7 +101,8 @@ def select_pages(q: torch.Tensor, means: PageMeans, page_table: torch.Tensor,
     power of two for it; products and scores are then exact, whatever else is in the call, and ties
     go to the lower column.  A page whose mean is NaN, or whose id is outside the pool, comes
     behind all others; for a group of queries with an infinity or NaN all other pages tie.  Rows
-    of no sequence get -1.  Tables of up to 32768 columns."""
+    of no sequence get -1.  Tables of up to 32768 columns; of a table far wider than the lengths can
+    be, page_table[:, :n] is faster."""
     r = (_lib._selected_host or _lib.selected_host()).select_pages(
         q, means, page_table, lengths, cu_tokens, top, first, recent)
     if r is not None:

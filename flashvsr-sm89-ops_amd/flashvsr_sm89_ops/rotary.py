@@ -43,7 +43,9 @@ def rotary_frequencies(channels: int, base: float = 10000.0, *, scaling: str | N
                       the slowest is divided by the factor
             "parts"   pairs that turn `fast` times or more over `context` tokens (the old length)
                       stay, those that turn `slow` times or less are divided by the factor,
-                      linear in the turns between
+                      linear in the turns between.  (A model that was trained with another ramp,
+                      such as one linear in i between two rounded pairs, needs its own: a
+                      RotaryFrequencies of `turns` made by hand.)
 
     gain: what q and k are scaled by; by default 0.1 ln(factor) + 1 with "parts", else 1."""
     def need(ok, what):

@@ -531,7 +531,8 @@ int fvsr_paged_attn(const fvsr_kv_cache* cache, const void* q, int64_t q_tok_str
  * aligned) and mean_scale [pages, heads] e8m0 get, for each page of a sequence's table that holds
  * 128 of its tokens now and held fewer before the call's T rows (T -1: each that holds
  * 128, whatever cu says), the mean of its 128 keys:
- *   scale  the least 2^e, e >= -127, with every |mean| at most 127 * 2^e
+ *   scale  the least 2^e, -127 <= e <= 127, with every |mean| at most 127 * 2^e (means past
+ *          127 * 2^127 are held there)
  *   mean   the nearest integers to mean / scale, ties to even
  * A NaN among a head's codes, or as its scale, gives scale NaN (byte 255) and zeros.  Of the cache
  * v and its scales are not read.  Page ids outside the pool are passed over.  T -1 takes tables of up to
