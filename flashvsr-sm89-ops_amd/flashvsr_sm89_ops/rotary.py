@@ -132,7 +132,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, freqs: RotaryFrequencies,
 
     Differentiable in q and k (any number of times, backward mode); freqs and positions have no
     gradient.  A step with its backward pass captures into a graph where its leaves have no
-    graph from another stream left: an earlier step's outputs are let go first.  Otherwise the
+    graph from outside the capture left: an earlier step's outputs are let go first.  Otherwise the
     backward pass is refused, for leaves further up too, and in a capture so is a call that is given
     such a leaf itself, unless under no_grad.  Without the native extension no backward pass is
     captured."""
